@@ -163,6 +163,84 @@ int nvm_paged_attention_noalloc(const void* q, int q_dtype, const void* k_pages,
                                 void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* A bounded cache: sliding window with sinks, key scores, eviction           */
+/* ------------------------------------------------------------------------- */
+/*
+ * nvm_paged_attention with a sliding window and sinks, and with the attention weight that
+ * every cached key receives.  No counterpart in the reference.  Arguments as
+ * nvm_paged_attention, and:
+ *
+ * window, sinks  the query token at position pos = l + context_len - L sees key s only if
+ *                s < sinks or s > pos - window (its own position counts as the first of the
+ *                window); window == 0: no such limit (sinks then changes nothing).  Without
+ *                is_causal the window bounds the past only.  Pages that lie wholly between
+ *                the sinks and the windows of all L tokens are not read and may be unmapped.
+ *                A row that sees no key is zero.
+ * key_mass       NULL, or float32 at key_mass[b*mass_stride_b + h*mass_stride_h + s], s <
+ *                mass_len, h < Hkv.  For s < min(context_len, mass_len):
+ *                  mass = (s < context_len - L ? mass : 0) + sum of the softmax weights of
+ *                  key s over the rows of kv head h (Hq/Hkv heads x L tokens),
+ *                so the newest L tokens start afresh and entries need no clearing when a
+ *                slot gets a new request or a rejected draft is rewound.  Keys outside every
+ *                window and entries past the context keep their value.
+ * A key that no query token of the call sees (past the context, outside every window, on an
+ * unmapped page) has no influence, whatever its K, V and scales hold (NaN and infinities
+ * included).  A key that one query token sees but another does not must hold finite values.
+ * workspace      at least nvm_paged_attention_window_workspace_size(...) bytes, under the
+ *                same rules as nvm_paged_attention's (and it may be the same buffer).
+ */
+int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages,
+                               int kv_dtype, const void* k_scales, const void* v_scales, int scale_dtype,
+                               const int32_t* block_table, const int32_t* context_lens, void* out,
+                               int out_dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D,
+                               int64_t P, int64_t page_size, int64_t max_pages, float scale, int is_causal,
+                               int64_t window, int64_t sinks, float* key_mass, int64_t mass_stride_b,
+                               int64_t mass_stride_h, int64_t mass_len, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Workspace bytes nvm_paged_attention_window needs for these sizes (0 if none). */
+size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D,
+                                                 int64_t page_size, int64_t max_pages, int kv_dtype,
+                                                 int64_t window, int64_t sinks, int with_mass);
+
+/*
+ * nvm_flash_attention with a sliding window and sinks: the token at pos = l + S - L sees key
+ * s only if s < sinks or s > pos - window (window == 0: no such limit), and s <= pos when
+ * is_causal.  No additive mask.  A row that sees no key is zero.
+ */
+int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out,
+                               int out_dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t S,
+                               int64_t D, float scale, int is_causal, int64_t window, int64_t sinks,
+                               void* stream);
+
+/*
+ * Eviction of cached tokens by accumulated attention weight, for a whole batch and in place.
+ * No counterpart in the reference.
+ *
+ * Request b of n = context_lens[b] > budget tokens keeps, separately for every kv head, its
+ * first `sinks` tokens, its last `recent` tokens and, of those between, the budget - sinks -
+ * recent with the largest key_mass (ties: the lowest position; NaN ranks below every number).
+ * The kept tokens' K and V rows (and int8 scales) move in their order to the positions
+ * 0 .. budget-1 of the request's own pages.  A request of n <= budget tokens is unchanged.
+ *   keep_index [B, Hkv, budget] int32: the old position of each kept token, -1 behind them;
+ *   kept, dropped [B] int32: tokens kept and given up.  context_lens is not changed: rewind
+ *     the request by dropped[b] (nvm_paged_rewind), which also frees the pages;
+ *   mass_out: the kept tokens' weights in the same order, zero from there to n, untouched
+ *     from n on; may be key_mass itself (same strides), and must not overlap it otherwise.
+ * The pages from position `sinks` on must belong to this request alone; with page_refcount
+ * ([P] int32, may be NULL) that is checked.  A request with a shared or unmapped page there,
+ * or longer than mass_len or its block-table row, is left as it is (keep_index -1, dropped 0)
+ * and sets *status = NVM_ERR_INVALID_ARGUMENT, which is otherwise left alone.
+ */
+int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, void* v_scales,
+                    int scale_dtype, const int32_t* block_table, const int32_t* context_lens,
+                    const int32_t* page_refcount, const float* key_mass, int64_t mass_stride_b,
+                    int64_t mass_stride_h, int64_t mass_len, float* mass_out, int64_t out_stride_b,
+                    int64_t out_stride_h, int64_t B, int64_t Hkv, int64_t D, int64_t P, int64_t page_size,
+                    int64_t max_pages, int64_t budget, int64_t sinks, int64_t recent, int32_t* keep_index,
+                    int32_t* kept, int32_t* dropped, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Dense flash attention (prefill)                                            */
 /* ------------------------------------------------------------------------- */
 /*

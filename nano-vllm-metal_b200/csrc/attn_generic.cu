@@ -33,9 +33,14 @@ struct GenericPagedParams {
   int64_t B, Hq, Hkv, L, D, P, ps, mp, dense_ctx;
   float scale;
   int causal;
+  int64_t window, sinks;  // kExt only
+  float* lse;             // kExt only, may be NULL
 };
 
-template <int DPL>
+// kExt: the windowed / scored form.  Row l at position pos = l + ctx - L sees key s only if
+// s < sinks or s > pos - window; keys between the sinks and the window are jumped over
+// (virtual index v of the walk -> key v below the sinks, v + gap past them).
+template <int DPL, bool kExt>
 __global__ void __launch_bounds__(kWarps * 32) paged_generic_kernel(GenericPagedParams p) {
   __shared__ float qs[kWarps][32 * DPL];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -48,6 +53,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_generic_kernel(GenericPaged
   const int64_t base_out = row * p.D;
   if (ctx <= 0) {
     for (int64_t d = lane; d < p.D; d += 32) store_dyn(p.out, base_out + d, p.out_dtype, 0.0f);
+    if (kExt && p.lse != nullptr && lane == 0) p.lse[row] = INFINITY;
     return;
   }
   const int64_t cap = p.mp * p.ps;
@@ -56,6 +62,15 @@ __global__ void __launch_bounds__(kWarps * 32) paged_generic_kernel(GenericPaged
   if (p.causal) {
     const int64_t lim = l + ctx - p.L + 1;  // keys [0, lim) are visible
     if (lim < n_keys) n_keys = lim;
+  }
+  int64_t first_win = 0, gap = 0;  // virtual keys [0, first_win) are sinks, the rest lie `gap` further on
+  if (kExt && p.window > 0) {
+    const int64_t lo = l + ctx - p.L - p.window + 1;  // first key inside the row's window
+    if (lo > p.sinks) {
+      first_win = p.sinks < n_keys ? p.sinks : (n_keys > 0 ? n_keys : 0);
+      gap = lo - p.sinks;
+      n_keys = n_keys - gap > first_win ? n_keys - gap : first_win;
+    }
   }
   for (int64_t d = lane; d < 32 * DPL; d += 32) qs[warp][d] = d < p.D ? load_dyn(p.q, row * p.D + d, p.q_dtype) : 0.0f;
   __syncwarp();
@@ -67,9 +82,10 @@ __global__ void __launch_bounds__(kWarps * 32) paged_generic_kernel(GenericPaged
   for (int i = 0; i < DPL; ++i) acc[i] = 0.0f;
 
   for (int64_t j0 = 0; j0 < n_keys; j0 += 32) {
-    const int64_t pos = j0 + lane;
+    int64_t pos = j0 + lane;
     int64_t base = -1;  // element offset / D of this key's row inside the pool
     if (pos < n_keys) {
+      if (kExt && pos >= first_win) pos += gap;
       const int64_t page_idx = pos / p.ps;
       const int64_t pid = p.block_table ? (int64_t)p.block_table[b * p.mp + page_idx] : b;
       if (pid >= 0 && pid < p.P) base = (pid * p.Hkv + kvh) * p.ps + (pos - page_idx * p.ps);
@@ -107,6 +123,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_generic_kernel(GenericPaged
     const int64_t d = lane + 32 * i;
     if (d < p.D) store_dyn(p.out, base_out + d, p.out_dtype, lsum > 0.0f ? acc[i] / lsum : 0.0f);
   }
+  if (kExt && p.lse != nullptr && lane == 0)
+    p.lse[row] = lsum > 0.0f ? m * 1.4426950408889634f + log2f(lsum) : INFINITY;
 }
 
 struct GenericFlashParams {
@@ -193,13 +211,19 @@ int launch_paged_generic(const PagedArgs& a, cudaStream_t s) {
   p.q_dtype = a.q_dtype; p.kv_dtype = a.kv_dtype; p.scale_dtype = a.scale_dtype; p.out_dtype = a.out_dtype;
   p.B = a.B; p.Hq = a.Hq; p.Hkv = a.Hkv; p.L = a.L; p.D = a.D; p.P = a.P; p.ps = a.page_size; p.mp = a.max_pages;
   p.dense_ctx = a.dense_ctx; p.scale = a.scale; p.causal = a.is_causal;
+  p.window = a.window; p.sinks = a.sinks; p.lse = a.lse;
   const int64_t rows = a.B * a.Hq * a.L;
   const dim3 grid((unsigned)((rows + kWarps - 1) / kWarps));
   const int dpl = (int)((a.D + 31) / 32);
-  if (dpl <= 1) paged_generic_kernel<1><<<grid, kWarps * 32, 0, s>>>(p);
-  else if (dpl <= 2) paged_generic_kernel<2><<<grid, kWarps * 32, 0, s>>>(p);
-  else if (dpl <= 4) paged_generic_kernel<4><<<grid, kWarps * 32, 0, s>>>(p);
-  else paged_generic_kernel<8><<<grid, kWarps * 32, 0, s>>>(p);
+  if (paged_is_ext(a)) {
+    if (dpl <= 1) paged_generic_kernel<1, true><<<grid, kWarps * 32, 0, s>>>(p);
+    else if (dpl <= 2) paged_generic_kernel<2, true><<<grid, kWarps * 32, 0, s>>>(p);
+    else if (dpl <= 4) paged_generic_kernel<4, true><<<grid, kWarps * 32, 0, s>>>(p);
+    else paged_generic_kernel<8, true><<<grid, kWarps * 32, 0, s>>>(p);
+  } else if (dpl <= 1) paged_generic_kernel<1, false><<<grid, kWarps * 32, 0, s>>>(p);
+  else if (dpl <= 2) paged_generic_kernel<2, false><<<grid, kWarps * 32, 0, s>>>(p);
+  else if (dpl <= 4) paged_generic_kernel<4, false><<<grid, kWarps * 32, 0, s>>>(p);
+  else paged_generic_kernel<8, false><<<grid, kWarps * 32, 0, s>>>(p);
   return check_cuda(cudaGetLastError(), "paged_attention: generic kernel launch");
 }
 

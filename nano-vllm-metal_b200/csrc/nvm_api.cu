@@ -133,6 +133,27 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
   return NVM_OK;
 }
 
+// Workspace of a windowed / scored call: the attention kernel's own part, then (with key
+// mass) the log-sum-exp of every query row.
+struct WindowWs {
+  size_t lse, total;
+};
+WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, bool with_mass) {
+  auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
+  WindowWs w{};
+  w.lse = al(attn_bytes);
+  w.total = with_mass ? w.lse + al((size_t)(a.B * a.Hq * a.L) * sizeof(float)) : attn_bytes;
+  return w;
+}
+
+int validate_window(int64_t window, int64_t sinks, const char* op) {
+  if (window < 0) return fail(NVM_ERR_INVALID_ARGUMENT, "%s: window must be positive, or 0 for none", op);
+  if (sinks < 0) return fail(NVM_ERR_INVALID_ARGUMENT, "%s: sinks must not be negative", op);
+  if (window > INT32_MAX || sinks > INT32_MAX)
+    return fail(NVM_ERR_UNSUPPORTED, "%s: window and sinks must be below 2^31", op);
+  return NVM_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -265,6 +286,111 @@ int nvm_flash_attention(const void* q, const void* k, const void* v, int dtype, 
   f.out = out; f.out_dtype = out_dtype;
   f.B = B; f.Hq = Hq; f.Hkv = Hkv; f.L = L; f.S = S; f.D = D; f.scale = scale; f.is_causal = is_causal ? 1 : 0;
   return launch_flash_generic(f, s);
+}
+
+size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D,
+                                                 int64_t page_size, int64_t max_pages, int kv_dtype, int64_t window,
+                                                 int64_t sinks, int with_mass) {
+  PagedArgs a{};
+  a.q_dtype = NVM_F32;
+  a.kv_dtype = kv_dtype;
+  a.scale_dtype = NVM_F16;
+  a.out_dtype = NVM_F32;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
+  a.is_causal = 1; a.window = window; a.sinks = sinks;
+  if (validate_paged(a, false) != NVM_OK || validate_window(window, sinks, "paged_attention") != NVM_OK) return 0;
+  return window_ws(a, 0, with_mass != 0).total;
+}
+
+int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages, int kv_dtype,
+                               const void* k_scales, const void* v_scales, int scale_dtype,
+                               const int32_t* block_table, const int32_t* context_lens, void* out, int out_dtype,
+                               int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D, int64_t P,
+                               int64_t page_size, int64_t max_pages, float scale, int is_causal, int64_t window,
+                               int64_t sinks, float* key_mass, int64_t mass_stride_b, int64_t mass_stride_h,
+                               int64_t mass_len, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedArgs a{};
+  a.q = q; a.q_dtype = q_dtype; a.k_pages = k_pages; a.v_pages = v_pages; a.kv_dtype = kv_dtype;
+  a.k_scales = k_scales; a.v_scales = v_scales; a.scale_dtype = scale_dtype;
+  a.block_table = block_table; a.context_lens = context_lens; a.out = out; a.out_dtype = out_dtype;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = P; a.page_size = page_size; a.max_pages = max_pages;
+  a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.window = window; a.sinks = sinks;
+  int st = validate_paged(a, true);
+  if (st != NVM_OK) return st;
+  st = validate_window(window, sinks, "paged_attention");
+  if (st != NVM_OK) return st;
+  if (key_mass != nullptr && (mass_len < 0 || mass_stride_b < 0 || mass_stride_h < 0))
+    return fail(NVM_ERR_INVALID_ARGUMENT, "paged_attention: key_mass sizes must not be negative");
+  if (B == 0) return NVM_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const WindowWs ws = window_ws(a, 0, key_mass != nullptr);
+  if (ws.total > 0 && (workspace == nullptr || workspace_bytes < ws.total))
+    return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
+                workspace_bytes);
+  if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
+  st = launch_paged_generic(a, s);
+  if (st != NVM_OK || key_mass == nullptr) return st;
+  KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
+  return launch_key_mass(a, m, s);
+}
+
+int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,
+                               int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t S, int64_t D, float scale,
+                               int is_causal, int64_t window, int64_t sinks, void* stream) {
+  if (!is_float_dtype(dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: all input arrays must be float32, float16 or bfloat16");
+  if (!is_float_dtype(out_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: output dtype must be floating point");
+  if (B < 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: sizes must be positive");
+  if (Hq % Hkv != 0) return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: num_heads must be divisible by num_kv_heads");
+  if (D > 256) return fail(NVM_ERR_UNSUPPORTED, "flash_attention: E must be <= 256 (got %lld)", (long long)D);
+  if (B * Hq * L > (int64_t)INT32_MAX * 4) return fail(NVM_ERR_UNSUPPORTED, "flash_attention: too many query rows");
+  int st = validate_window(window, sinks, "flash_attention");
+  if (st != NVM_OK) return st;
+  if (B == 0) return NVM_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: null tensor pointer");
+  PagedArgs a{};  // dense K/V [B*Hkv, S, D] viewed as a pool of B pages of size S (page id = b)
+  a.q = q; a.q_dtype = dtype; a.k_pages = k; a.v_pages = v; a.kv_dtype = dtype;
+  a.out = out; a.out_dtype = out_dtype;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = B; a.page_size = S; a.max_pages = 1;
+  a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.dense = 1; a.dense_ctx = S;
+  a.window = window; a.sinks = sinks;
+  return launch_paged_generic(a, static_cast<cudaStream_t>(stream));
+}
+
+int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, void* v_scales, int scale_dtype,
+                    const int32_t* block_table, const int32_t* context_lens, const int32_t* page_refcount,
+                    const float* key_mass, int64_t mass_stride_b, int64_t mass_stride_h, int64_t mass_len,
+                    float* mass_out, int64_t out_stride_b, int64_t out_stride_h, int64_t B, int64_t Hkv, int64_t D,
+                    int64_t P, int64_t page_size, int64_t max_pages, int64_t budget, int64_t sinks, int64_t recent,
+                    int32_t* keep_index, int32_t* kept, int32_t* dropped, int32_t* status, void* stream) {
+  if (!is_float_dtype(kv_dtype) && kv_dtype != NVM_I8)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: pages must be float32, float16, bfloat16 or int8");
+  if (kv_dtype == NVM_I8 && !is_float_dtype(scale_dtype))
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: int8 pages need floating-point key and value scales");
+  if (B < 0 || Hkv <= 0 || D <= 0 || P < 0 || page_size <= 0 || max_pages < 0 || mass_len < 0)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: sizes must be positive");
+  if (mass_stride_b < 0 || mass_stride_h < 0 || out_stride_b < 0 || out_stride_h < 0)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: strides must not be negative");
+  if (budget < 1 || sinks < 0 || recent < 0 || sinks + recent > budget)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: need budget >= 1, sinks >= 0, recent >= 0 and sinks + recent <= budget");
+  if (D > 256) return fail(NVM_ERR_UNSUPPORTED, "evict: head dimension must be <= 256 (got %lld)", (long long)D);
+  if (budget > INT32_MAX || page_size > INT32_MAX || B * Hkv > INT32_MAX)
+    return fail(NVM_ERR_UNSUPPORTED, "evict: budget, page_size and B * Hkv must be below 2^31");
+  if (B == 0) return NVM_OK;
+  if (!k_pages || !v_pages || !block_table || !context_lens || !key_mass || !mass_out || !keep_index || !kept ||
+      !dropped || !status || (kv_dtype == NVM_I8 && (!k_scales || !v_scales)))
+    return fail(NVM_ERR_INVALID_ARGUMENT, "evict: null tensor pointer");
+  EvictArgs a{};
+  a.k_pages = k_pages; a.v_pages = v_pages; a.kv_dtype = kv_dtype; a.k_scales = k_scales; a.v_scales = v_scales;
+  a.scale_dtype = scale_dtype; a.block_table = block_table; a.context_lens = context_lens;
+  a.page_refcount = page_refcount; a.mass = key_mass; a.mass_out = mass_out;
+  a.stride_b = mass_stride_b; a.stride_h = mass_stride_h; a.len = mass_len;
+  a.out_stride_b = out_stride_b; a.out_stride_h = out_stride_h;
+  a.B = B; a.Hkv = Hkv; a.D = D; a.P = P; a.page_size = page_size; a.max_pages = max_pages;
+  a.budget = budget; a.sinks = sinks; a.recent = recent;
+  a.keep_index = keep_index; a.kept = kept; a.dropped = dropped; a.status = status;
+  return launch_evict(a, static_cast<cudaStream_t>(stream));
 }
 
 int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t stride_t, int64_t stride_h,

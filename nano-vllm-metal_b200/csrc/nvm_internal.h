@@ -47,10 +47,48 @@ struct PagedArgs {
   int is_causal;
   int dense;          // 1: dense K/V viewed as one page per sequence (no block table)
   int64_t dense_ctx;  // tokens per sequence when dense
+  // Windowed / scored calls (nvm_paged_attention_window, nvm_flash_attention_window); all
+  // zero otherwise.  A row at position pos = l + ctx - L sees key s only if s < sinks or
+  // s > pos - window (window == 0: no such limit).
+  int64_t window, sinks;
+  float* lse;         // [B*Hq*L] log2 of sum 2^(score * log2 e) of every row (+inf: no key), or NULL
 };
+inline bool paged_is_ext(const PagedArgs& a) { return a.window > 0 || a.lse != nullptr; }
 
 // Generic CUDA-core kernel: any D <= 256, any page_size, F32/F16/BF16/I8 pages.
 int launch_paged_generic(const PagedArgs& a, cudaStream_t s);
+
+// Accumulated attention weight per cached key (key_mass.cu): for the calls' visible keys
+// mass[b, h, s] = (s < ctx - L ? mass[b, h, s] : 0) + sum over the rows of kv head h of
+// 2^(score_log2 - lse[row]); entries at or past min(ctx, mass_len) are left as they are.
+struct KeyMassArgs {
+  float* mass;
+  int64_t stride_b, stride_h, len;
+};
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, cudaStream_t s);
+
+// Eviction by accumulated weight (evict.cu).
+struct EvictArgs {
+  void* k_pages;
+  void* v_pages;
+  int kv_dtype;
+  void* k_scales;
+  void* v_scales;
+  int scale_dtype;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  const int32_t* page_refcount;  // may be NULL
+  const float* mass;
+  float* mass_out;
+  int64_t stride_b, stride_h, len;          // of mass
+  int64_t out_stride_b, out_stride_h;       // of mass_out (same length)
+  int64_t B, Hkv, D, P, page_size, max_pages, budget, sinks, recent;
+  int32_t* keep_index;
+  int32_t* kept;
+  int32_t* dropped;
+  int32_t* status;
+};
+int launch_evict(const EvictArgs& a, cudaStream_t s);
 
 // Generic dense flash attention with the reference's additive-mask semantics.
 struct FlashArgs {

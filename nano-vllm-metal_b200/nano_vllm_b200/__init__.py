@@ -13,6 +13,7 @@ from .layers.attention import (  # noqa: F401
     paged_attention,
     scaled_dot_product_attention_grouped,
 )
+from .cache.evict import EvictResult, evict_tokens  # noqa: F401
 from .cache.kv_cache import BatchingKvCache, TinyKvCache  # noqa: F401
 from .cache.paged import (  # noqa: F401
     DevicePageTable,

@@ -44,6 +44,13 @@ SIGNATURES = {
                                          _I64, _I64, _I64, _I64, _F, _I, _P]),
     "nvm_flash_attention": (_I, [_P, _P, _P, _I, _P, _I64, _I64, _I64, _P, _I, _I64, _I64, _I64, _I64, _I64,
                                  _I64, _F, _I, _P]),
+    "nvm_paged_attention_window": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64,
+                                        _I64, _I64, _I64, _F, _I, _I64, _I64, _P, _I64, _I64, _I64, _P, _SZ, _P]),
+    "nvm_paged_attention_window_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I64, _I64, _I]),
+    "nvm_flash_attention_window": (_I, [_P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I64,
+                                        _I64, _P]),
+    "nvm_paged_evict": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64,
+                             _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "nvm_reshape_and_cache": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I, _P, _P, _I, _P, _I64, _I64, _I64, _I64,
                                    _I64, _P]),
     "nvm_paged_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P]),
@@ -133,6 +140,17 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
+    return ws
+
+
+def private_workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
+    """The cached workspace, except while a CUDA graph is being captured: a graph replays with
+    the addresses it captured, on any stream and beside any other graph, so its calls get a
+    buffer of their own (from the graph's memory pool; the zero fill becomes a graph node)."""
+    if nbytes == 0 or not torch.cuda.is_current_stream_capturing():
+        return workspace(device, nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws[:1 << 20].zero_()
     return ws
 
 

@@ -1,0 +1,100 @@
+"""Eviction of cached tokens by accumulated attention weight.
+
+``paged_attention(..., key_mass=mass)`` adds to ``mass[b, h, s]`` the softmax weight that key
+``s`` gets in every step.  ``evict_tokens`` trims each request that has grown past a budget to
+the tokens that matter: its first ``sinks``, its last ``recent`` and, of the rest, the heaviest,
+chosen separately for every kv head.  Their K/V rows move in order to the front of the request's
+own pages, so attention, append and rewind go on as if the request had always been that short
+(keys carry their rotary positions already; ``positions`` of new tokens stay the caller's).  The
+reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from .. import _native as nv
+from ..layers.attention import _check_rows
+
+__all__ = ["EvictResult", "evict_tokens"]
+
+
+class EvictResult(NamedTuple):
+    keep_index: torch.Tensor  # [B, Hkv, budget] int32: old position of each kept token, -1 behind them
+    kept: torch.Tensor        # [B] int32 tokens kept
+    dropped: torch.Tensor     # [B] int32 tokens given up: what to rewind the request by
+    status: torch.Tensor      # [1] int32, not zero if a request could not be trimmed
+
+
+def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
+                 context_lens: torch.Tensor, key_mass: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0,
+                 key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
+                 page_refcount: torch.Tensor | None = None, mass_out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None) -> EvictResult:
+    """Trim every request of more than ``budget`` tokens to ``budget``, in place.
+
+    key_pages/value_pages ``[P, Hkv, page_size, D]`` (fp32, fp16, bf16, or int8 with
+    ``key_scales``/``value_scales`` ``[P, Hkv, page_size, 1]``), contiguous; block_table
+    ``[B, max_pages]`` and context_lens ``[B]`` int32; key_mass float32 ``[B, Hkv, S]``, last
+    axis contiguous.  Ties go to the lowest position, NaN ranks below every number.  The kept
+    tokens' weights move along (into ``mass_out`` when given, which must not overlap key_mass,
+    else in place) and are zero from there to the old length.
+
+    ``context_lens`` is left alone: rewind each request by ``dropped``
+    (``DevicePageTable.evict`` does both).  The pages from position ``sinks`` on must belong to
+    the request alone; ``page_refcount`` ([P] int32 or longer) makes the kernel check it.  A
+    request with a shared or unmapped page there, or longer than S or its row, is left as it
+    is, with ``dropped`` 0, and sets ``status``.
+    """
+    op = "evict"
+    dev = nv.require_cuda(op, key_pages, value_pages, block_table, context_lens, key_mass, key_scales, value_scales,
+                          page_refcount, mass_out, status)
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != value_pages.dtype:
+        raise RuntimeError(f"{op}: key_pages and value_pages must be [P, Hkv, page_size, D] of one dtype")
+    if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
+        raise RuntimeError(f"{op}: page pools must be contiguous (written in place)")
+    P, Hkv, ps, D = key_pages.shape
+    if block_table.dim() != 2 or context_lens.dim() != 1 or block_table.shape[0] != context_lens.shape[0]:
+        raise RuntimeError(f"{op}: block_table must be [B, max_pages] and context_lens [B]")
+    B = block_table.shape[0]
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise RuntimeError(f"{op}: need budget >= 1, sinks >= 0, recent >= 0 and sinks + recent <= budget")
+    out = key_mass if mass_out is None else mass_out
+    for name, x in (("key_mass", key_mass), ("mass_out", out)):
+        if x.dim() != 3 or tuple(x.shape[:2]) != (B, Hkv) or x.dtype != torch.float32:
+            raise RuntimeError(f"{op}: {name} must be float32 [B, Hkv, S]")
+        _check_rows(f"{op}: {name}", x)
+    if out.shape != key_mass.shape:
+        raise RuntimeError(f"{op}: mass_out must have the shape of key_mass")
+    sdt = nv.NVM_F16
+    if key_pages.dtype == torch.int8:
+        if key_scales is None or value_scales is None:
+            raise RuntimeError(f"{op}: int8 pages need key_scales and value_scales")
+        for s in (key_scales, value_scales):
+            if tuple(s.shape) != (P, Hkv, ps, 1) or not s.is_contiguous() or s.dtype != key_scales.dtype:
+                raise RuntimeError(f"{op}: scales must be contiguous [P, Hkv, page_size, 1] of one dtype")
+        sdt = nv.dtype_code(key_scales.dtype)
+    else:
+        key_scales = value_scales = None
+    if page_refcount is not None and (page_refcount.dtype != torch.int32 or page_refcount.numel() < P or
+                                      not page_refcount.is_contiguous()):
+        raise RuntimeError(f"{op}: page_refcount must be contiguous int32 with an entry per page")
+    if status is None:
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+    elif status.dtype != torch.int32 or status.numel() != 1:
+        raise RuntimeError(f"{op}: status must be one int32")
+    bt = block_table.to(torch.int32).contiguous()
+    cl = context_lens.to(torch.int32).contiguous()
+    keep = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    counts = torch.empty((2, B), dtype=torch.int32, device=dev)
+    kept, dropped = counts[0], counts[1]
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nvm_paged_evict(
+            key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(key_scales),
+            nv.ptr(value_scales), sdt, bt.data_ptr(), cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(),
+            key_mass.stride(0), key_mass.stride(1), key_mass.shape[2], out.data_ptr(), out.stride(0), out.stride(1), B,
+            Hkv, D, P, ps, bt.shape[1], budget, sinks, recent, keep.data_ptr(), kept.data_ptr(), dropped.data_ptr(),
+            status.data_ptr(), nv.stream_ptr(dev)))
+    return EvictResult(keep, kept, dropped, status)

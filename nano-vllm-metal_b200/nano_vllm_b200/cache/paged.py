@@ -342,6 +342,28 @@ class TinyKvPagedCache(TinyKvCache):
         self.page_lens[-1] = new_offset - self.page_size * (target - 1)
         self.offset = new_offset
 
+    def evict(self, key_mass: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0):
+        """Trim this request to ``budget`` tokens by accumulated attention weight (``cache.evict``)
+        and free the pages behind them.  ``key_mass`` [1, H, S] is updated in place.  Returns
+        the ``EvictResult``, or None when the request fits.  Raises if a page that would be
+        rewritten is shared."""
+        from .evict import evict_tokens
+
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise RuntimeError("evict: need budget >= 1, sinks >= 0, recent >= 0 and sinks + recent <= budget")
+        if self.offset <= budget:
+            return None
+        if key_mass.dim() != 3 or key_mass.shape[2] < self.offset:
+            raise RuntimeError(f"evict: key_mass must be [1, H, S] with S >= {self.offset}")
+        for pid in self.page_ids[sinks // self.page_size:]:
+            if self.pool.ref_counts[pid] != 1:
+                raise ValueError(f"evict: page {pid} is shared with another request")
+        pool = self.pool
+        result = evict_tokens(pool.key_pages, pool.value_pages, self.block_table(), self.context_lens(), key_mass, budget,
+                              sinks=sinks, recent=recent, key_scales=pool.key_scales, value_scales=pool.value_scales)
+        self.rewind(self.offset - budget)
+        return result
+
     def release(self) -> None:
         for pid in self.page_ids:
             self.pool.free_page(pid)
@@ -373,6 +395,7 @@ class DevicePageTable:
         self.refcount = torch.zeros(max(capacity, 1), **i32)
         self.last_call = torch.full((max(capacity, 1),), -1, **i32)  # rewind scratch, kept at -1
         self.status = torch.zeros(1, **i32)
+        self.evict_status = torch.zeros(1, **i32)  # not zero once evict has refused a request
 
     def append(self, new_tokens: torch.Tensor, slot_mapping: torch.Tensor | None = None) -> torch.Tensor:
         """new_tokens ``[B]`` int32 on the device; returns int64 slots ``[sum(new_tokens)]``.
@@ -440,7 +463,37 @@ class DevicePageTable:
         """The free stack bottom to top (the next page taken is the last entry)."""
         return self.free_stack[: int(self.free_top.item())].tolist()
 
+    def evict(self, layers, budget: int, *, sinks: int = 0, recent: int = 0) -> list:
+        """Trim every request of more than ``budget`` tokens to ``budget`` (``cache.evict``), in
+        all layers that share this table, and give the freed pages back.
+
+        ``layers``: one ``(key_pages, value_pages, key_mass)`` or ``(key_pages, value_pages,
+        key_scales, value_scales, key_mass)`` per layer; ``key_mass`` is updated in place.
+        Returns one ``EvictResult`` per layer.  A request that shares a page with another
+        (prefix attach) past its sinks stays as it is and makes ``check_status`` raise."""
+        from .evict import evict_tokens
+
+        results = []
+        for layer in layers:
+            if len(layer) not in (3, 5):
+                raise ValueError("evict: a layer is (key_pages, value_pages, key_mass) or (key_pages, value_pages, "
+                                 "key_scales, value_scales, key_mass)")
+            kp, vp, mass = layer[0], layer[1], layer[-1]
+            ks, vs = (layer[2], layer[3]) if len(layer) == 5 else (None, None)
+            if kp.shape[2] != self.page_size or kp.shape[0] > self.refcount.numel():
+                raise ValueError("evict: pages must have the table's page_size and at most its capacity")
+            results.append(evict_tokens(kp, vp, self.block_table, self.context_lens, mass, budget, sinks=sinks,
+                                        recent=recent, key_scales=ks, value_scales=vs,
+                                        page_refcount=self.refcount, status=self.evict_status))
+        if results:
+            self.rewind(results[0].dropped)
+        return results
+
     def check_status(self) -> None:
+        st = int(self.evict_status.item())
+        if st != 0:
+            raise RuntimeError(f"page table: evict refused a request (status {st}: a page shared with another request or "
+                               "unmapped, or more tokens than key_mass holds)")
         st = int(self.status.item())
         if st != 0:
             raise RuntimeError(f"page table: device call failed (status {st}: out of pages, block-table row full, "

@@ -13,7 +13,10 @@ Mirrors ``src/nano_vllm_metal/layers/attention.py`` of nano-vllm-metal:
   plain-torch dense references, used by tests and callers that want them.
 
 Extensions (keyword-only, defaults keep the reference behaviour): ``out_dtype``
-lets the model receive bf16/fp16 directly instead of casting the fp32 result.
+lets the model receive bf16/fp16 directly instead of casting the fp32 result;
+``window`` / ``sinks`` limit every query token to the last ``window`` positions (its own
+included) and the first ``sinks``; ``key_mass`` accumulates the attention weight that
+every cached key receives, by which ``cache.evict`` trims a cache.
 Query tensors are read in their own dtype (fp32, fp16 or bf16); the reference's
 ``query.astype(float32)`` is exact for 16-bit queries, so it is skipped.
 """
@@ -30,6 +33,26 @@ __all__ = [
     "flash_attention",
     "paged_attention",
 ]
+
+
+def _check_window(op: str, window: int | None, sinks: int) -> None:
+    if window is not None and window < 1:
+        raise RuntimeError(f"{op}: window must be at least 1 (None for no window), got {window}")
+    if sinks < 0:
+        raise RuntimeError(f"{op}: sinks must not be negative, got {sinks}")
+
+
+def _check_rows(what: str, x: torch.Tensor) -> None:
+    """x [B, H, S]: rows contiguous along S that do not overlap one another."""
+    B, H, S = x.shape
+    sb, sh, ss = x.stride()
+    ok = S <= 1 or ss == 1
+    if H > 1:
+        ok = ok and sh >= S
+    if B > 1:
+        ok = ok and (sb >= (H - 1) * sh + S or (H > 1 and sh >= (B - 1) * sb + S and sb >= S) or (H == 1 and sb >= S))
+    if not ok:
+        raise RuntimeError(f"{what} must be contiguous along its last axis, its rows apart from one another")
 
 
 def causal_mask(L: int, S: int, dtype: torch.dtype = torch.float32, device=None) -> torch.Tensor:
@@ -64,7 +87,8 @@ def scaled_dot_product_attention_grouped(query, key, value, scale=None, mask=Non
 
 
 def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scale: float | None = None,
-                    mask: torch.Tensor | str | None = None, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                    mask: torch.Tensor | str | None = None, *, out_dtype: torch.dtype | None = None,
+                    window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """Dense flash attention (reference attention.py:103-151).
 
     query ``[..., Hq, L, E]``, key/value ``[B, Hkv, S, E]`` (fp32, fp16 or bf16, all
@@ -72,7 +96,11 @@ def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     ``[..., Hq, L, S]`` that is added to the scaled scores.  Returns ``[..., Hq, L, E]``
     in ``out_dtype`` (default: the query dtype, i.e. fp32 for the reference's fp32
     inputs).
+
+    ``window``: the token at position ``pos = l + S - L`` sees key ``s`` only if ``s < sinks``
+    or ``s > pos - window``; not together with a mask tensor.  A row that sees no key is zero.
     """
+    _check_window("flash_attention", window, sinks)
     factor = scale if scale is not None else 1.0 / (query.shape[-1] ** 0.5)
     *batch_shape, Hq, L, D = query.shape
     _, Hkv, S, _ = key.shape
@@ -88,6 +116,18 @@ def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     is_causal = isinstance(mask, str) and mask == "causal"
     if isinstance(mask, str) and mask != "causal":
         raise NotImplementedError(f"flash_attention: unknown mask {mask!r}")
+    if window is not None:
+        if isinstance(mask, torch.Tensor):
+            raise NotImplementedError("flash_attention: window goes with mask=None or causal only")
+        if q.dim() < 3 or tuple(k.shape) != (B, Hkv, S, D) or v.shape != k.shape:
+            raise RuntimeError("flash_attention: key and value must be [B, Hkv, S, E] with the query's B and E")
+        out = torch.empty((*batch_shape, Hq, L, D), dtype=out_dtype or query.dtype, device=dev)
+        with torch.cuda.device(dev):
+            nv.check(nv.lib().nvm_flash_attention_window(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), nv.dtype_code(q.dtype), out.data_ptr(),
+                nv.dtype_code(out.dtype), B, Hq, Hkv, L, S, D, float(factor), int(is_causal), window, sinks,
+                nv.stream_ptr(dev)))
+        return out
     m = None
     ms = (0, 0, 0)
     if isinstance(mask, torch.Tensor):
@@ -109,14 +149,24 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
                     block_table: torch.Tensor, context_lens: torch.Tensor, page_size: int,
                     key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
                     scale: float | None = None, mask: torch.Tensor | str | None = None, *,
-                    out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+                    out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                    window: int | None = None, sinks: int = 0,
+                    key_mass: torch.Tensor | None = None) -> torch.Tensor:
     """Paged attention over block-paged K/V pools (reference attention.py:154-230).
 
     query ``[B, Hq, L, D]``; key_pages/value_pages ``[P, Hkv, page_size, D]`` (fp32,
     fp16, bf16, or int8 with ``key_scales``/``value_scales`` ``[P, Hkv, page_size, 1]``);
     block_table ``[B, max_pages]`` (-1 padded); context_lens ``[B]`` (tokens of each
     sequence, the new L included).  Returns ``[B, Hq, L, D]`` (fp32 by default).
+
+    ``window``: the query token at position ``pos = l + context_len - L`` sees key ``s`` only if
+    ``s < sinks`` or ``s > pos - window``; pages wholly between are not read.  ``key_mass``
+    (float32 ``[B, Hkv, S]``, last axis contiguous) is updated in place: every key gains the
+    softmax weights it gets from the rows of its kv head, and the newest L keys start at zero,
+    so the buffer needs no clearing between requests; keys at or past S gain nothing.  A row
+    that sees no key is zero, and a key that no row sees has no influence whatever it holds.
     """
+    _check_window("paged_attention", window, sinks)
     if isinstance(mask, torch.Tensor):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
     if mask is not None and mask != "causal":
@@ -156,6 +206,29 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
     L_ = nv.lib()
     kvc = nv.dtype_code(kp.dtype)
+    if window is not None or key_mass is not None:
+        if tuple(out.shape) != (B, Hq, L, D) or not out.is_contiguous() or out.device != dev:
+            raise RuntimeError("paged_attention: out must be a contiguous [B, Hq, L, D] tensor on the query's device")
+        if ps != page_size or (ks is not None and not tuple(ks.shape) == tuple(vs.shape) == (P, Hkv, ps, 1)):
+            raise RuntimeError("paged_attention: pages must be [P, Hkv, page_size, D] and scales [P, Hkv, page_size, 1]")
+        ms = (0, 0, 0)
+        if key_mass is not None:
+            nv.require_cuda("paged_attention", query, key_mass)
+            if key_mass.dim() != 3 or tuple(key_mass.shape[:2]) != (B, Hkv) or key_mass.dtype != torch.float32:
+                raise RuntimeError("paged_attention: key_mass must be float32 [B, Hkv, S]")
+            ms = (*key_mass.stride()[:2], key_mass.shape[2])
+            _check_rows("paged_attention: key_mass", key_mass)
+        w = window or 0
+        ws_bytes = L_.nvm_paged_attention_window_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc, w, sinks,
+                                                                int(key_mass is not None))
+        with torch.cuda.device(dev):
+            ws = nv.private_workspace(dev, ws_bytes)
+            nv.check(L_.nvm_paged_attention_window(
+                q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
+                bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps,
+                bt.shape[1], float(factor), int(mask == "causal"), w, sinks, nv.ptr(key_mass), *ms, nv.ptr(ws),
+                ws_bytes, nv.stream_ptr(dev)))
+        return out
     ws_bytes = L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc)
     ws = nv.workspace(dev, ws_bytes)
     with torch.cuda.device(dev):

@@ -1,0 +1,91 @@
+"""The bounded-cache operators' refusals and host bookkeeping (no GPU needed)."""
+
+import pytest
+import torch
+
+from nano_vllm_b200 import TinyKvPagedCache, TinyKvPagedPool, evict_tokens, flash_attention, paged_attention
+from nano_vllm_b200 import _native as nv
+
+
+def test_window_arguments_are_checked_first():
+    q, k = torch.zeros(1, 4, 1, 64), torch.zeros(1, 2, 8, 64)
+    pages, bt, cl = torch.zeros(2, 2, 16, 64), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for w in (0, -1):
+        with pytest.raises(RuntimeError, match="flash_attention: window must be at least 1"):
+            flash_attention(q, k, k, window=w)
+        with pytest.raises(RuntimeError, match="paged_attention: window must be at least 1"):
+            paged_attention(q, pages, pages, bt, cl, 16, window=w)
+    with pytest.raises(RuntimeError, match="sinks must not be negative"):
+        flash_attention(q, k, k, window=4, sinks=-1)
+    with pytest.raises(RuntimeError, match="sinks must not be negative"):
+        paged_attention(q, pages, pages, bt, cl, 16, window=4, sinks=-2)
+
+
+def test_operators_have_no_cpu_path():
+    q, k = torch.zeros(1, 4, 1, 64), torch.zeros(1, 2, 8, 64)
+    pages, bt, cl = torch.zeros(2, 2, 16, 64), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        flash_attention(q, k, k, window=4)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        paged_attention(q, pages, pages, bt, cl, 16, window=4)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        evict_tokens(pages, pages, bt, cl, torch.zeros(1, 2, 32), 4)
+
+
+def _window_call(**kw):
+    a = dict(B=1, Hq=4, Hkv=2, L=1, D=128, P=4, ps=16, mp=4, window=8, sinks=0, mass=None, sb=0, sh=0, ml=0, kv=2)
+    a.update(kw)
+    return nv.lib().nvm_paged_attention_window(None, 2, None, None, a["kv"], None, None, 1, None, None, None, 0, a["B"],
+                                               a["Hq"], a["Hkv"], a["L"], a["D"], a["P"], a["ps"], a["mp"], 0.1, 1,
+                                               a["window"], a["sinks"], a["mass"], a["sb"], a["sh"], a["ml"], None, 0, None)
+
+
+def test_c_entry_refusals():
+    L = nv.lib()
+    assert _window_call() == -1  # null tensors
+    assert _window_call(B=0) == 0
+    assert _window_call(B=0, window=-1) == -1
+    assert L.nvm_last_error().decode() == "paged_attention: window must be positive, or 0 for none"
+    assert _window_call(B=0, sinks=-1) == -1
+    assert _window_call(B=0, window=1 << 40) == -2
+    assert _window_call(Hq=3) == -1
+    assert _window_call(D=512) == -2
+    args = [None, None, None, 2, None, 0, 1, 4, 2, 8, 8, 64, 0.1, 1]
+    assert L.nvm_flash_attention_window(*args, 4, 0, None) == -1
+    assert L.nvm_flash_attention_window(*args, -4, 0, None) == -1
+
+
+def test_workspace_sizes():
+    size = nv.lib().nvm_paged_attention_window_workspace_size
+    assert size(1, 3, 2, 1, 128, 16, 8, 2, 64, 0, 0) == 0  # refused sizes need none
+    with_mass = size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 1)
+    assert with_mass >= 2 * 32 * 4
+    assert with_mass > size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 0)
+
+
+def test_evict_c_entry_refusals():
+    def call(B=1, D=128, budget=4, sinks=0, recent=0, kv=2, sb=8):
+        return nv.lib().nvm_paged_evict(None, None, kv, None, None, 1, None, None, None, None, sb, 8, 8, None, 8, 8, B, 2, D,
+                                        4, 16, 4, budget, sinks, recent, None, None, None, None, None)
+    assert call() == -1
+    assert call(B=0) == 0
+    for bad in (dict(budget=0), dict(sinks=-1), dict(recent=-1), dict(sinks=3, recent=2), dict(kv=4), dict(sb=-1)):
+        assert call(B=0, **bad) == -1, bad
+    assert call(B=0, D=300) == -2
+
+
+def test_request_cache_evict_checks_on_the_host():
+    pool = TinyKvPagedPool(page_size=4)
+    cache = TinyKvPagedCache(pool)
+    cache.plan_append(10)
+    mass = torch.zeros(1, 2, 16)
+    assert cache.evict(mass, 10) is None and cache.evict(mass, 32, sinks=4) is None
+    for bad in (dict(budget=0), dict(budget=4, sinks=3, recent=2), dict(budget=4, sinks=-1)):
+        with pytest.raises(RuntimeError, match="budget"):
+            cache.evict(mass, **bad)
+    with pytest.raises(RuntimeError, match="key_mass"):
+        cache.evict(torch.zeros(1, 2, 9), 8)
+    pool.incref(cache.page_ids[1])
+    with pytest.raises(ValueError, match="shared"):
+        cache.evict(mass, 8)
+    assert cache.offset == 10 and cache.num_pages == 3
