@@ -133,15 +133,19 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
   return NVM_OK;
 }
 
+// Stands for the log-sum-exp buffer while a call is planned, before its workspace is known.
+float kLseLater;
+
 // Workspace of a windowed / scored call: the attention kernel's own part, then (with key
-// mass) the log-sum-exp of every query row.
+// mass) the log-sum-exp of every query row, behind the ticket region in any case: tickets of
+// other calls that share the workspace must stay zero.
 struct WindowWs {
   size_t lse, total;
 };
 WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, bool with_mass) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   WindowWs w{};
-  w.lse = al(attn_bytes);
+  w.lse = al(attn_bytes > kTicketRegionBytes ? attn_bytes : kTicketRegionBytes);
   w.total = with_mass ? w.lse + al((size_t)(a.B * a.Hq * a.L) * sizeof(float)) : attn_bytes;
   return w;
 }
@@ -299,7 +303,13 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
   a.is_causal = 1; a.window = window; a.sinks = sinks;
   if (validate_paged(a, false) != NVM_OK || validate_window(window, sinks, "paged_attention") != NVM_OK) return 0;
-  return window_ws(a, 0, with_mass != 0).total;
+  if (with_mass) a.lse = &kLseLater;
+  size_t need = 0;
+  if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
+    const MmaPlan plan = plan_paged_mma(a);
+    if (plan.eligible) need = plan.ws_bytes;
+  }
+  return window_ws(a, need, with_mass != 0).total;
 }
 
 int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages, int kv_dtype,
@@ -323,12 +333,15 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
     return fail(NVM_ERR_INVALID_ARGUMENT, "paged_attention: key_mass sizes must not be negative");
   if (B == 0) return NVM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const WindowWs ws = window_ws(a, 0, key_mass != nullptr);
+  if (key_mass != nullptr) a.lse = &kLseLater;
+  MmaPlan plan{};
+  if (!env_flag("NVM_ATTN_FORCE_GENERIC")) plan = plan_paged_mma(a);
+  const WindowWs ws = window_ws(a, plan.eligible ? plan.ws_bytes : 0, key_mass != nullptr);
   if (ws.total > 0 && (workspace == nullptr || workspace_bytes < ws.total))
     return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
                 workspace_bytes);
   if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
-  st = launch_paged_generic(a, s);
+  st = plan.eligible ? launch_paged_mma(a, plan, workspace, s) : launch_paged_generic(a, s);
   if (st != NVM_OK || key_mass == nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
   return launch_key_mass(a, m, s);
@@ -355,7 +368,12 @@ int nvm_flash_attention_window(const void* q, const void* k, const void* v, int 
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = B; a.page_size = S; a.max_pages = 1;
   a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.dense = 1; a.dense_ctx = S;
   a.window = window; a.sinks = sinks;
-  return launch_paged_generic(a, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (window > 0 && dtype != NVM_F32 && !env_flag("NVM_ATTN_FORCE_GENERIC")) {
+    const MmaPlan plan = plan_paged_mma(a);
+    if (plan.eligible && plan.ws_bytes == 0) return launch_paged_mma(a, plan, nullptr, s);
+  }
+  return launch_paged_generic(a, s);
 }
 
 int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, void* v_scales, int scale_dtype,

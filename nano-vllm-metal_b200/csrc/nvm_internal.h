@@ -124,6 +124,7 @@ struct MmaPlan {
 };
 MmaPlan plan_paged_mma(const PagedArgs& a);
 int launch_paged_mma(const PagedArgs& a, const MmaPlan& plan, void* workspace, cudaStream_t s);
+int launch_paged_mma_window(const PagedArgs& a, const MmaPlan& plan, void* workspace, cudaStream_t s);
 
 // tcgen05 / TMEM causal prefill (dense or paged) for 16-bit Q/K/V, D == 128.
 // tcgen05/TMEM kernel (flash_sm100.cu): prefill (>= 64 query rows per head) and grouped

@@ -59,7 +59,7 @@ def test_workspace_sizes():
     size = nv.lib().nvm_paged_attention_window_workspace_size
     assert size(1, 3, 2, 1, 128, 16, 8, 2, 64, 0, 0) == 0  # refused sizes need none
     with_mass = size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 1)
-    assert with_mass >= 2 * 32 * 4
+    assert with_mass >= (1 << 20) + 2 * 32 * 4  # the first MiB holds tickets that stay zero
     assert with_mass > size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 0)
 
 
