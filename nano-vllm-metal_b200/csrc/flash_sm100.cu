@@ -22,6 +22,11 @@
 //              S = Q K^T (N=64) and O += P V (A = P from TMEM, N=128) as tcgen05.mma
 //              kind::f16 with fp32 accumulate from one thread, and signals completion
 //              with tcgen05.commit on mbarriers.
+// kExt instances take a sliding window with sinks (a row at position pos sees key s only if
+// s < sinks or s > pos - window), paged context of any page size that 16 divides, and leave
+// every row's log-sum-exp.  The 64-key tiles between the sinks and a row tile's windows are
+// jumped over by renumbering (virtual tile v is tile v below the sinks' last tile and tile
+// v + skip past it), so rings, phases and chunks run unchanged.
 // Every mbarrier wait is bounded; on expiry the CTA records an error, lets its own
 // copies and MMAs land (bounded), frees TMEM and returns.
 #include <type_traits>
@@ -98,6 +103,8 @@ struct Sm100Params {
   int* counters;
   float2* part_ml;  // [n_units][n_chunks][rows_real]
   float* part_o;    // [n_units][n_chunks][rows_real][kD]
+  int64_t window, sinks;  // kExt: window == 0 for none
+  float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
 };
 
 // Pairs q (keys 2q, 2q+1 of a 64-key tile) whose exponentials run on the FMA pipe.
@@ -113,8 +120,18 @@ struct Item {
   int64_t c, u, n, b, kvh, r0, rows, ctx, ctx_limit, l_first, t_begin, n_chunks_unit;
   int n_tiles;  // 64-key tiles of this item (0: no keys; still produces zero rows when valid)
   bool valid;   // false: a chunk past the unit's last key (nothing to do)
+  // kExt: virtual tiles from sink_tiles on lie `skip` tiles further; keys in [sinks, first)
+  // and keys >= end are seen by no row of the tile
+  int sink_tiles, skip;
+  int64_t first, end;
 };
 
+template <bool kExt>
+__device__ __forceinline__ int64_t tile_of(const Item& it, int64_t v) {
+  return kExt && v >= it.sink_tiles ? v + it.skip : v;
+}
+
+template <bool kExt>
 __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) {
   Item it;
   // Chunk-major, last chunk first: a chunk c >= 1 exists only for long units and is then
@@ -152,7 +169,22 @@ __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) 
     if (lim < need) need = lim;
   }
   if (it.ctx <= 0 || need < 0) need = 0;
-  const int64_t n_tiles_unit = (need + kBN - 1) / kBN;
+  int64_t n_tiles_unit = (need + kBN - 1) / kBN;
+  if constexpr (kExt) {
+    it.sink_tiles = INT32_MAX;
+    it.skip = 0;
+    it.first = 0;
+    it.end = need;
+    if (p.window > 0) {
+      it.first = it.l_first + it.ctx - p.L - p.window + 1;
+      const int64_t st = (p.sinks + kBN - 1) / kBN;
+      if (it.first > 0 && it.first / kBN > st && st < n_tiles_unit) {
+        it.sink_tiles = (int)st;
+        it.skip = (int)(it.first / kBN - st);
+        n_tiles_unit = n_tiles_unit - it.skip > st ? n_tiles_unit - it.skip : st;
+      }
+    }
+  }
   it.n_chunks_unit = n_tiles_unit > 0 ? (int64_t)((uint32_t)(n_tiles_unit + p.ct - 1) / (uint32_t)p.ct) : 1;
   it.valid = it.c < it.n_chunks_unit;
   it.t_begin = it.c * p.ct;
@@ -165,7 +197,7 @@ __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) 
 // when there is one, else blockIdx.x + k * gridDim.x).  Rings and mbarrier phases run on
 // per-CTA tile counters, so the next item's Q load, K/V loads and first S overlap the
 // previous item's last tiles and epilogue.
-template <typename T>
+template <typename T, bool kExt>
 __global__ void __launch_bounds__(kThreads, 2)
     flash_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -230,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     *abort_flag = 0;
     fence_mbar_init();
     if (p.stage_out && (int64_t)blockIdx.x < p.n_items) {
-      const Item it0 = decode_item(p, blockIdx.x);
+      const Item it0 = decode_item<kExt>(p, blockIdx.x);
       if (it0.valid && it0.n_tiles > 0) {
         mbar_arrive_expect_tx(q_full, kQBytes);
         tma_load_3d(sQ, &tm_q, 0, (int)it0.r0, (int)it0.n, q_full);
@@ -250,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tO = tmem + 2 * kBN;
-  constexpr int kPagesPerTile = kBN / 16;  // paged path: page_size == 16
+  constexpr int kPagesPerTile = kBN / 16;  // 16-token groups; paged without kExt: page_size == 16
+  const uint32_t gpp = kExt ? (uint32_t)(p.ps >> 4) : 1u;  // groups per page
 
   // consumers of the item ring: slot k & 3 of the k-th published item
   auto read_item = [&](int k, bool arrive) -> int64_t {
@@ -262,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   // the unit's fewest keys seen by a row: bf16 P is split into hi + lo below split_below
   auto split_of = [&](const Item& it) -> bool {
-    const int64_t min_keys = p.causal ? (it.l_first + it.ctx - p.L + 1) : it.ctx_limit;
+    int64_t min_keys = p.causal ? (it.l_first + it.ctx - p.L + 1) : it.ctx_limit;
+    if (kExt && p.window > 0 && p.window < min_keys) min_keys = p.window;
     return kSplit && min_keys < p.split_below;
   };
 
@@ -309,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           item = -1;
           break;
         }
-        it = decode_item(p, item);
+        it = decode_item<kExt>(p, item);
         if (it.valid) break;
       }
       if (leader) {
@@ -336,7 +370,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       // Paged: the page ids of 8 tiles (32 pages) sit one per lane and are loaded one
       // block ahead; holes and pages past the table read as page P (TMA fills zeros).
       auto load_ids = [&](int blk) -> int {
-        const int pidx = (int)(it.t_begin * kPagesPerTile) + blk * 32 + lane;
+        int pidx = (int)(it.t_begin * kPagesPerTile) + blk * 32 + lane;
+        if constexpr (kExt) {
+          const uint32_t group = (uint32_t)tile_of<true>(it, pidx / kPagesPerTile) * kPagesPerTile + (pidx % kPagesPerTile);
+          pidx = (int)(group / gpp);
+        }
         const int id = pidx < (int)p.mp ? bt_row[pidx] : -1;
         return (id < 0 || id >= (int)p.P) ? (int)p.P : id;
       };
@@ -355,14 +393,19 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (leader) {
           mbar_arrive_expect_tx(full, kTileBytes);
           if (p.dense) {
-            const int key0 = (int)((it.t_begin + t) * kBN);
+            const int key0 = (int)(tile_of<kExt>(it, it.t_begin + t) * kBN);
             tma_load_4d(dst, tm, 0, key0, kvh_i, b_i, full);
             tma_load_4d(dst + kBN * 128, tm, 64, key0, kvh_i, b_i, full);
           } else {
 #pragma unroll
             for (int g = 0; g < kPagesPerTile; ++g) {
-              tma_load_4d(dst + g * 16 * 128, tm, 0, 0, kvh_i, pid[g], full);
-              tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm, 64, 0, kvh_i, pid[g], full);
+              int slot0 = 0;
+              if constexpr (kExt) {
+                const uint32_t group = (uint32_t)tile_of<true>(it, it.t_begin + t) * kPagesPerTile + g;
+                slot0 = (int)(group % gpp) * 16;
+              }
+              tma_load_4d(dst + g * 16 * 128, tm, 0, slot0, kvh_i, pid[g], full);
+              tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm, 64, slot0, kvh_i, pid[g], full);
             }
           }
         }
@@ -471,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         ok = item == -1;
         break;
       }
-      const Item it = decode_item(p, item);
+      const Item it = decode_item<kExt>(p, item);
       const int n = it.n_tiles;
       if (n == 0) continue;
       const bool split = split_of(it);
@@ -624,6 +667,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     };
+    auto put_lse = [&](const Item& it, float mx, float sum) {
+      if constexpr (kExt) {
+        if (p.lse != nullptr && row < it.rows)
+          p.lse[it.n * p.M_rows + it.r0 + row] = sum > 0.f ? mx + log2f(sum) : INFINITY;
+      }
+    };
     while (ok) {
       const int64_t item = read_item(kq, true);
       ++kq;
@@ -631,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         ok = item == -1;
         break;
       }
-      const Item it = decode_item(p, item);
+      const Item it = decode_item<kExt>(p, item);
       if (!it.valid) continue;
       const int n = it.n_tiles;
       const bool row_ok = row < it.rows;
@@ -642,6 +691,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int x = 0; x < 32; ++x) z[x] = 0.f;
         if (row_ok)
           for (int c0 = 0; c0 < kD; c0 += 32) store32(orow, z, c0, 0.f);
+        put_lse(it, 0.f, 0.f);
         continue;
       }
       const bool split = split_of(it);
@@ -650,12 +700,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       int64_t last_key = it.ctx_limit - 1;
       if (p.causal && lpos + it.ctx - p.L < last_key) last_key = lpos + it.ctx - p.L;
       if (!row_ok) last_key = -1;
+      const int64_t row_lo = kExt && p.window > 0 ? lpos + it.ctx - p.L - p.window + 1 : 0;  // its window's first key
       // Paged: page ids two tiles ahead, lanes 0..3 hold page g = lane of a tile; the
       // hole test happens when the tile is processed, so the load latency is hidden.
       const int32_t* bt_row = p.dense ? nullptr : p.block_table + it.b * p.mp;
       auto load_pid = [&](int t) -> int {
         if (p.dense || lane >= kPagesPerTile || t >= n) return 0;
-        const int pidx = (int)(it.t_begin + t) * kPagesPerTile + lane;
+        int pidx = (int)(it.t_begin + t) * kPagesPerTile + lane;
+        if constexpr (kExt)
+          pidx = (int)(((uint32_t)tile_of<true>(it, it.t_begin + t) * kPagesPerTile + lane) / gpp);
         return pidx < (int)p.mp ? bt_row[pidx] : -1;
       };
       int pid0 = load_pid(0), pid1 = load_pid(1);
@@ -675,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         pid0 = pid1;
         pid1 = load_pid(j + 2);
         tmem_wait_ld();
-        const int64_t key0 = (it.t_begin + j) * kBN;
+        const int64_t key0 = tile_of<kExt>(it, it.t_begin + j) * kBN;
         // Only tiles that cross some row's last visible key (the causal diagonal, the
         // context end, rows past the unit) pay for the mask: one compare per score.
         const int64_t vis64 = last_key - key0;  // in-tile index of the row's last visible key
@@ -683,6 +736,31 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int vis = vis64 < -1 ? -1 : (int)vis64;
 #pragma unroll
           for (int c = 0; c < kBN; ++c) sv[c] = c <= vis ? sv[c] : -INFINITY;
+        }
+        if constexpr (kExt) {  // keys in [sinks, row_lo): only tiles at a window's lower edge hold any
+          const int64_t lo64 = row_lo - key0, sk64 = p.sinks - key0;
+          if (__any_sync(0xffffffffu, p.window > 0 && lo64 > 0 && sk64 < kBN && sk64 < lo64)) {
+            const int lo = p.window > 0 && lo64 > 0 ? (lo64 < kBN ? (int)lo64 : kBN) : 0;
+            const int sk = sk64 > 0 ? (sk64 < kBN ? (int)sk64 : kBN) : 0;
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) sv[c] = c >= sk && c < lo ? -INFINITY : sv[c];
+          }
+          // V of the keys that no row of the tile sees becomes zero before the product reads it
+          // (their weight is zero, but 0 times a NaN or an infinity is not)
+          if (key0 + kBN > it.end || (p.window > 0 && key0 < it.first && key0 + kBN > p.sinks)) {
+            const int vs = g % kVStages;
+            if (!warp_wait(&v_full[vs], (uint32_t)((g / kVStages) & 1))) {
+              ok = false;
+              break;
+            }
+            const int64_t key = key0 + (row & (kBN - 1));
+            if (key >= it.end || (p.window > 0 && key >= p.sinks && key < it.first)) {
+              uint4* d = reinterpret_cast<uint4*>(sV + vs * kTileBytes + (row / kBN) * (kBN * 128) + (row & (kBN - 1)) * 128);
+#pragma unroll
+              for (int x = 0; x < 8; ++x) d[x] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+          }
         }
         if (!p.dense) {  // holes: the 16-token groups of missing pages are masked
           const uint32_t holes =
@@ -800,6 +878,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       ++iw;
       tc_fence_after();
       if (it.n_chunks_unit == 1) {
+        put_lse(it, m, lsum);
         const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
 #pragma unroll 1
         for (int c1 = 0; c1 < kD; c1 += 64) {
@@ -879,6 +958,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
             }
             const float inv = lt > 0.f ? 1.f / lt : 0.f;
+            put_lse(it, mxc, lt);
 #pragma unroll 1
             for (int c0 = 0; c0 < kD; c0 += 32) {
               float acc2[32];
@@ -966,12 +1046,13 @@ __global__ void __launch_bounds__(kThreads, 2)
 // Work list for the persistent grid: every item with work, ordered by tile count, largest
 // first (a counting sort; sizes >= kPlanBins - 1 share the first bin), so the dynamic
 // fetch approximates longest-processing-time-first scheduling.  One CTA.
+template <bool kExt>
 __global__ void __launch_bounds__(1024) sm100_plan_kernel(const Sm100Params p, int* list, int* count) {
   __shared__ int hist[kPlanBins];
   for (int i = threadIdx.x; i < kPlanBins; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   for (int64_t item = threadIdx.x; item < p.n_items; item += blockDim.x) {
-    const Item it = decode_item(p, item);
+    const Item it = decode_item<kExt>(p, item);
     if (!it.valid) continue;
     const int bin = kPlanBins - 1 - (it.n_tiles < kPlanBins - 1 ? it.n_tiles : kPlanBins - 1);
     atomicAdd(&hist[bin], 1);
@@ -1008,7 +1089,7 @@ __global__ void __launch_bounds__(1024) sm100_plan_kernel(const Sm100Params p, i
   }
   __syncthreads();
   for (int64_t item = threadIdx.x; item < p.n_items; item += blockDim.x) {
-    const Item it = decode_item(p, item);
+    const Item it = decode_item<kExt>(p, item);
     if (!it.valid) continue;
     const int bin = kPlanBins - 1 - (it.n_tiles < kPlanBins - 1 ? it.n_tiles : kPlanBins - 1);
     list[atomicAdd(&hist[bin], 1)] = (int)item;
@@ -1016,7 +1097,7 @@ __global__ void __launch_bounds__(1024) sm100_plan_kernel(const Sm100Params p, i
 }
 
 // One opt-in to the dynamic shared memory size per kernel instantiation and device.
-template <typename T>
+template <typename T, bool kExt>
 int launch_typed(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                  const CUtensorMap& to, const Sm100Params& p, cudaStream_t s) {
   static std::mutex mu;
@@ -1026,14 +1107,14 @@ int launch_typed(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const 
   {
     std::lock_guard<std::mutex> lock(mu);
     if (dev < 64 && !(done & (1ull << dev))) {
-      int r = check_cuda(cudaFuncSetAttribute(flash_sm100_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      int r = check_cuda(cudaFuncSetAttribute(flash_sm100_kernel<T, kExt>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               kSmemBytes),
                          "flash_attention: cudaFuncSetAttribute");
       if (r != NVM_OK) return r;
       done |= 1ull << dev;
     }
   }
-  flash_sm100_kernel<T><<<grid, kThreads, kSmemBytes, s>>>(tq, tk, tv, to, p);
+  flash_sm100_kernel<T, kExt><<<grid, kThreads, kSmemBytes, s>>>(tq, tk, tv, to, p);
   return check_cuda(cudaGetLastError(), "flash_attention: sm100 kernel launch");
 }
 
@@ -1068,7 +1149,7 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
   if (!sizing_only && !(a.scale > 0.f)) return plan;  // the softmax takes row maxima before scaling
   if (a.dense) {
     if (a.page_size < kBN) return plan;  // dense boxes are kBN rows
-  } else if (a.page_size != 16) {
+  } else if (a.page_size != 16 && !(paged_is_ext(a) && a.page_size % 16 == 0)) {
     return plan;
   }
   if (a.P <= 0 || a.P >= INT32_MAX || a.B * a.Hq > INT32_MAX) return plan;
@@ -1097,7 +1178,14 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
   plan.n_units = plan.n_outer * plan.n_row_tiles;
   plan.rows_real = plan.M_rows < kBM ? plan.M_rows : kBM;
   const int64_t keys = a.dense ? a.page_size : a.max_pages * a.page_size;
-  const int64_t tiles_max = (keys + kBN - 1) / kBN;
+  int64_t tiles_max = (keys + kBN - 1) / kBN;
+  if (a.window > 0) {
+    // the sinks' tiles and those that the windows of one row tile touch (without the causal
+    // limit every row sees on to the last key)
+    const int64_t span = a.is_causal && a.L > kBM ? kBM : a.L;
+    const int64_t seen = (a.sinks + kBN - 1) / kBN + (a.window + span - 1 + kBN - 1) / kBN + 1;
+    if (seen < tiles_max) tiles_max = seen;
+  }
   if (tiles_max >= INT32_MAX / 2) return plan;
   plan.ct = tiles_max > 0 ? tiles_max : 1;
   plan.n_chunks = 1;
@@ -1166,6 +1254,7 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   p.n_row_tiles = plan.n_row_tiles;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.causal = a.is_causal; p.dense = a.dense; p.box_rows = box_rows;
+  p.window = a.window; p.sinks = a.sinks; p.lse = a.lse;
   p.split_below = env_int("NVM_SM100_SPLIT_BELOW", kSplitBelowKeys);  // tuning: 0 = never, huge = always
   p.grouped = plan.grouped;
   p.g = a.Hq / a.Hkv;
@@ -1203,12 +1292,19 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
     int* count = p.work_counter - 1;
     p.item_list = list;
     p.item_count = count;
-    sm100_plan_kernel<<<1, 1024, 0, s>>>(p, list, count);
+    if (paged_is_ext(a))
+      sm100_plan_kernel<true><<<1, 1024, 0, s>>>(p, list, count);
+    else
+      sm100_plan_kernel<false><<<1, 1024, 0, s>>>(p, list, count);
     const int st2 = check_cuda(cudaGetLastError(), "paged_attention: sm100 plan kernel launch");
     if (st2 != NVM_OK) return st2;
   }
   const dim3 grid((unsigned)ctas);
-  if (a.kv_dtype == NVM_F16) return launch_typed<__half>(grid, tq, tk, tv, to, p, s);
-  return launch_typed<__nv_bfloat16>(grid, tq, tk, tv, to, p, s);
+  if (paged_is_ext(a)) {
+    if (a.kv_dtype == NVM_F16) return launch_typed<__half, true>(grid, tq, tk, tv, to, p, s);
+    return launch_typed<__nv_bfloat16, true>(grid, tq, tk, tv, to, p, s);
+  }
+  if (a.kv_dtype == NVM_F16) return launch_typed<__half, false>(grid, tq, tk, tv, to, p, s);
+  return launch_typed<__nv_bfloat16, false>(grid, tq, tk, tv, to, p, s);
 }
 }  // namespace nvm

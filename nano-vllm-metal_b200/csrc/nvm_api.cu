@@ -306,8 +306,13 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   if (with_mass) a.lse = &kLseLater;
   size_t need = 0;
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
+    // q's dtype is not known here: cover both plans
     const MmaPlan plan = plan_paged_mma(a);
     if (plan.eligible) need = plan.ws_bytes;
+    if (!env_flag("NVM_ATTN_NO_SM100")) {
+      const Sm100Plan sp = plan_sm100(a, true);
+      if (sp.eligible && sp.ws_bytes > need) need = sp.ws_bytes;
+    }
   }
   return window_ws(a, need, with_mass != 0).total;
 }
@@ -334,14 +339,20 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
   if (B == 0) return NVM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (key_mass != nullptr) a.lse = &kLseLater;
+  Sm100Plan sp{};
   MmaPlan plan{};
-  if (!env_flag("NVM_ATTN_FORCE_GENERIC")) plan = plan_paged_mma(a);
-  const WindowWs ws = window_ws(a, plan.eligible ? plan.ws_bytes : 0, key_mass != nullptr);
+  if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
+    if (!env_flag("NVM_ATTN_NO_SM100")) sp = plan_sm100(a, false);
+    if (!sp.eligible) plan = plan_paged_mma(a);
+  }
+  const WindowWs ws = window_ws(a, sp.eligible ? sp.ws_bytes : plan.eligible ? plan.ws_bytes : 0, key_mass != nullptr);
   if (ws.total > 0 && (workspace == nullptr || workspace_bytes < ws.total))
     return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
                 workspace_bytes);
   if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
-  st = plan.eligible ? launch_paged_mma(a, plan, workspace, s) : launch_paged_generic(a, s);
+  st = sp.eligible     ? launch_sm100(a, sp, workspace, s)
+       : plan.eligible ? launch_paged_mma(a, plan, workspace, s)
+                       : launch_paged_generic(a, s);
   if (st != NVM_OK || key_mass == nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
   return launch_key_mass(a, m, s);
@@ -370,6 +381,10 @@ int nvm_flash_attention_window(const void* q, const void* k, const void* v, int 
   a.window = window; a.sinks = sinks;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (window > 0 && dtype != NVM_F32 && !env_flag("NVM_ATTN_FORCE_GENERIC")) {
+    if (!env_flag("NVM_ATTN_NO_SM100")) {
+      const Sm100Plan sp = plan_sm100(a, false);
+      if (sp.eligible && sp.ws_bytes == 0) return launch_sm100(a, sp, nullptr, s);
+    }
     const MmaPlan plan = plan_paged_mma(a);
     if (plan.eligible && plan.ws_bytes == 0) return launch_paged_mma(a, plan, nullptr, s);
   }

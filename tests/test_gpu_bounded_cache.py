@@ -67,6 +67,9 @@ WINDOW_CASES = [
     ([1400, 260], 130, 8, 4, 128, 16, HF, HF, 1, 1),              # a window of one key
     ([900, 100], 70, 4, 4, 64, 32, HF, HF, 128, 4),               # chunk, D = 64
     ([900, 200], 90, 8, 2, 128, 64, I8, HF, 128, 4),              # chunk, int8
+    ([900, 200], 90, 8, 2, 128, 48, BF, BF, 100, 49),             # chunk, pages that a 64-key tile straddles
+    ([700, 150], 150, 8, 2, 128, 128, HF, HF, 129, 4),            # chunk, pages of two tiles
+    ([5000, 300, 4100], 5, 32, 4, 128, 32, BF, BF, 3500, 100),    # verify, several chunks a unit
     ([300, 50], 3, 6, 2, 80, 7, F32, F32, 40, 5),                 # odd head dim and page size, fp32
     ([300, 20], 1, 4, 4, 96, 24, HF, F32, 33, 2),                 # odd head dim, fp32 queries over fp16
 ]
