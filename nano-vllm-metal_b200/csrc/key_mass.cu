@@ -5,10 +5,28 @@
 //   mass[b, h, s] = (s < ctx - L ? mass[b, h, s] : 0) + sum_rows 2^(z[row, s] - lse[row])
 // where z is the scaled score in base 2 and lse[row] = log2 sum_s 2^z[row, s] comes from
 // the attention kernel that ran before on the same stream (+inf for a row without a key,
-// which then gives every key weight 0).  Keys of unmapped pages gain nothing.  No atomics:
-// one warp owns a key, so results do not depend on the order of anything.
+// then gives every key weight 0).  Keys of unmapped pages gain nothing.  No atomics:
+// one thread (or warp) owns a key, so results do not depend on the order of anything.
+//
+// The denominators are known only after all keys, so the scores are needed twice.  Which way
+// is cheaper depends on the rows of a kv head, M = Hq/Hkv * L:
+//  * M <= 8 (decode): the attention kernel keeps its scores in the workspace, 4 M bytes a key
+//    written and read once, next to the 4 D bytes of K and V that it reads anyway (M = 4,
+//    D = 128: 32 bytes next to 512); key_mass_scores_kernel adds them up.
+//  * more rows (verify, chunks, prompts): 2 D bytes a key read again cost less than 8 M bytes
+//    from M = D / 4 = 32 on, and prompts could not keep M x S scores at all:
+//    key_mass_sm100_kernel computes them again on the tensor cores, S^T = K Q^T with the keys
+//    as the 128 lanes of tensor memory, so that a thread owns a key: its sum needs no
+//    exchange between threads and K enters shared memory once per 128 keys.  Bound by the
+//    exponentials (16 a clock and SM) from about 32 rows on.
+//  * everything else (fp32, other head dims): key_mass_generic_kernel.
+#include <cstdlib>
+#include <mutex>
+#include <type_traits>
+
 #include "nvm_common.cuh"
 #include "nvm_internal.h"
+#include "tcgen05.cuh"
 
 namespace nvm {
 namespace {
@@ -70,9 +88,392 @@ __global__ void __launch_bounds__(kGenWarps * 32) key_mass_generic_kernel(MassPa
   }
 }
 
+// Scores kept by the attention kernel: [B*Hkv][v_keys][rows_pad] base-2 scores (-inf where a
+// row does not see the key) on the attention kernel's virtual keys; a thread per key.
+struct ScoreParams {
+  const float* scores;
+  int64_t v_keys;
+  int rows, rows_pad;  // rows_pad: rows rounded up to even
+};
+
+__global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p, const ScoreParams sp) {
+  __shared__ float s_lse[8];
+  const int64_t bh = blockIdx.y, b = bh / p.Hkv, h = bh - b * p.Hkv;
+  if (threadIdx.x < 8) s_lse[threadIdx.x] = (int)threadIdx.x < sp.rows ? p.lse[bh * sp.rows + threadIdx.x] : INFINITY;
+  const int64_t ctx = p.context_lens[b], cap = p.mp * p.ps;
+  const int64_t end = ctx < cap ? ctx : cap;
+  // virtual -> real keys, as the attention kernel numbers its 16-key tiles
+  int64_t tiles = (end + 15) / 16, sink_tiles = tiles, skip = 0;
+  if (p.window > 0) {
+    const int64_t first = ctx - p.L - p.window + 1, st = (p.sinks + 15) / 16;
+    if (first > 0 && first / 16 > st && st < tiles) {
+      sink_tiles = st;
+      skip = first / 16 - st;
+      tiles = tiles - skip > st ? tiles - skip : st;
+    }
+  }
+  __syncthreads();
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (end <= 0 || v >= tiles * 16) return;
+  const int64_t key = v / 16 >= sink_tiles ? v + skip * 16 : v;
+  if (key >= end || key >= p.len) return;
+  const float2* z = reinterpret_cast<const float2*>(sp.scores + (bh * sp.v_keys + v) * sp.rows_pad);
+  float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
+  float sum = key < ctx - p.L ? *m : 0.f;
+  float gain = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (2 * i < sp.rows_pad) {
+      const float2 x = __ldcs(z + i);
+      gain += ex2_ftz(x.x - s_lse[2 * i]) + (2 * i + 1 < sp.rows ? ex2_ftz(x.y - s_lse[2 * i + 1]) : 0.f);
+    }
+  }
+  *m = sum + gain;
+}
+
+// ---------------------------------------------------------------------------
+// tcgen05 recomputation: a CTA per 128 keys of one (sequence, kv head)
+// ---------------------------------------------------------------------------
+constexpr int kMK = 128;        // keys per CTA = tensor-memory lanes
+constexpr int kMR = 128;        // query rows per tile = accumulator columns
+constexpr int kMThreads = 192;  // warps 0-3: exponentials; warp 4: Q copies; warp 5: MMAs
+constexpr int kMCols = 256;     // two accumulators; two CTAs per SM share the 512 columns
+
+template <int D>
+struct MassSmem {
+  static constexpr int kKBytes = kMK * D * 2;
+  static constexpr int kQBytes = kMR * D * 2;
+  static constexpr int kStages = 2;
+  static constexpr int kUsed = kKBytes + kStages * kQBytes + 2 * kMR * 8 + 256;
+  // at least a third of an SM's: a third CTA would only wait for tensor memory
+  static constexpr int kBytes = kUsed > 80 * 1024 ? kUsed : 80 * 1024;
+};
+
+template <typename T, typename KvT, int D>
+__global__ void __launch_bounds__(kMThreads, 2)
+    key_mass_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const MassParams p, int* err) {
+  using S = MassSmem<D>;
+  constexpr int kHalves = D / 64;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) record_error(err, kDevErrSmemAlign);
+    return;
+  }
+  uint8_t* sK = smem;
+  uint8_t* sQ = smem + S::kKBytes;
+  float* s_lse = reinterpret_cast<float*>(sQ + S::kStages * S::kQBytes);  // [2][kMR]
+  int* s_pos = reinterpret_cast<int*>(s_lse + 2 * kMR);                   // [2][kMR]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_pos + 2 * kMR);
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* mma_done = s_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bh = blockIdx.y, b = bh / (int)p.Hkv, h = bh - b * (int)p.Hkv;
+  const int ctx = p.context_lens[b];
+  const int64_t cap = p.mp * p.ps;
+  int64_t end64 = ctx < cap ? ctx : cap;
+  if (p.len < end64) end64 = p.len;
+  const int end = (int)end64;
+  const int k0 = blockIdx.x * kMK;
+  if (k0 >= end) return;
+  // rows (per run) that see some key of the tile
+  const int L = (int)p.L, base_pos = ctx - L;
+  const bool by_head = L >= 64;  // else the g * L rows of the kv head are one run
+  int lo = 0, hi = by_head ? L : (int)(p.g * p.L);
+  if (by_head) {
+    if (p.causal && k0 - base_pos > lo) lo = k0 - base_pos;
+    if (p.window > 0 && k0 >= p.sinks) {  // pos <= key + window - 1 for the tile's last key
+      const int64_t last = (int64_t)k0 + kMK - 1 + p.window - 1 - base_pos;
+      if (last + 1 < hi) hi = last + 1 > 0 ? (int)(last + 1) : 0;
+    }
+  }
+  const int n_rows = hi > lo ? hi - lo : 0;
+  const int per_run = (n_rows + kMR - 1) / kMR;
+  const int runs = by_head ? (int)p.g : 1;
+  const int n_tiles = per_run * runs;
+  auto tile_row = [&](int t) { return (t / per_run) * (by_head ? L : 0) + lo + (t % per_run) * kMR; };
+  auto tile_rows = [&](int t) {
+    const int left = n_rows - (t % per_run) * kMR;
+    return left < kMR ? left : kMR;
+  };
+
+  auto load_q = [&](int t) {
+    const int s = t & 1;
+    mbar_arrive_expect_tx(&q_full[s], S::kQBytes);
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf)
+      tma_load_3d(sQ + s * S::kQBytes + hf * (kMR * 128), &tm_q, hf * 64, tile_row(t), bh, &q_full[s]);
+  };
+  if (threadIdx.x == 4 * 32) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 128);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    for (int t = 0; t < 2 && t < n_tiles; ++t) load_q(t);
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kMCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // K: lane = key for the page lookup, then the warp copies its 32 rows with kLanes lanes a
+  // row into the swizzled K-major layout the MMA reads (row r's 16-byte chunk c of a
+  // 64-element half at r * 128 + ((c ^ (r & 7)) << 4)); int8 becomes T exactly and its scale
+  // multiplies the scores.  Unmapped and out-of-range keys are zero.
+  float kf = p.scale_log2;
+  bool mapped = false;
+  if (warp < 4) {
+    const int key = k0 + (int)threadIdx.x;
+    int64_t row = -1;
+    if (key < end) {
+      const uint32_t page = (uint32_t)key / (uint32_t)p.ps, off = (uint32_t)key - page * (uint32_t)p.ps;
+      const int64_t pid = p.block_table[(int64_t)b * p.mp + page];
+      if (pid >= 0 && pid < p.P) row = (pid * p.Hkv + h) * p.ps + off;
+    }
+    mapped = row >= 0;
+    if (std::is_same<KvT, int8_t>::value && mapped) kf *= load_dyn(p.ks, row, p.scale_dtype);
+    constexpr int kLanes = D * (int)sizeof(KvT) / 16;  // lanes a row, and steps
+    constexpr int kRows = 32 / kLanes;                 // rows a step
+    const int sub = lane / kLanes, c = lane % kLanes;
+    uint4 v[kLanes];
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) {
+      const int64_t src = __shfl_sync(0xffffffffu, row, i * kRows + sub);
+      v[i] = src >= 0 ? __ldcs(reinterpret_cast<const uint4*>(static_cast<const KvT*>(p.k) + src * D) + c)
+                      : make_uint4(0u, 0u, 0u, 0u);
+    }
+    auto put = [&](int r, int ch, uint4 x) {
+      *reinterpret_cast<uint4*>(sK + (ch >> 3) * (kMK * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+    };
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) {
+      const int r = warp * 32 + i * kRows + sub;
+      if constexpr (std::is_same<KvT, int8_t>::value) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const uint32_t pair = w[x >> 1] >> (16 * (x & 1));
+          o[x] = cvt_pack<T>((float)(int8_t)(pair & 0xFF), (float)(int8_t)((pair >> 8) & 0xFF));
+        }
+        put(r, 2 * c, make_uint4(o[0], o[1], o[2], o[3]));
+        put(r, 2 * c + 1, make_uint4(o[4], o[5], o[6], o[7]));
+      } else {
+        put(r, c, v[i]);
+      }
+    }
+    fence_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 4) {
+    // -------------------------------------------------------------- Q copies
+    if (lane == 0) {
+      bool ok = true;
+      int issued = n_tiles < 2 ? n_tiles : 2;
+      for (int t = 2; t < n_tiles; ++t) {
+        if (!mbar_wait(&q_empty[t & 1], (uint32_t)(((t >> 1) & 1) ^ 1)) || *(volatile int*)abort_flag != 0) {
+          ok = false;
+          break;
+        }
+        load_q(t);
+        issued = t + 1;
+      }
+      if (!ok) {
+        record_error(err, kDevErrEmptyWait);
+        *(volatile int*)abort_flag = 1;
+      }
+      for (int s = 0; s < 2 && s < issued; ++s) {  // every copy lands before the CTA exits
+        const int last = s + ((issued - 1 - s) / 2) * 2;
+        if (!mbar_wait(&q_full[s], (uint32_t)((last >> 1) & 1))) record_error(err, kDevErrDrainWait);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    // -------------------------------------------------------------- MMAs
+    const uint32_t id = idesc<T>(false, kMR);
+    const uint64_t dk = smem_desc(smem_u32(sK), 16, 1024), dq = smem_desc(smem_u32(sQ), 16, 1024);
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int s = t & 1;
+      if (!warp_wait(&q_full[s], (uint32_t)((t >> 1) & 1)) ||
+          (t >= 2 && !warp_wait(&s_empty[s], (uint32_t)(((t >> 1) & 1) ^ 1)))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t dqs = dq + (uint64_t)((s * S::kQBytes) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint64_t off = (uint64_t)(((ks >> 2) * (kMR * 128) + (ks & 3) * 32) >> 4);
+        mma_f16_warp(tmem + (uint32_t)(s * kMR), dk + off, dqs + off, id, ks > 0 ? 1u : 0u);
+      }
+      mma_commit_warp(&s_full[s]);
+      mma_commit_warp(&q_empty[s]);
+    }
+    if (!ok && lane == 0) {
+      record_error(err, kDevErrMmaWait);
+      *(volatile int*)abort_flag = 1;
+    }
+    __syncwarp();
+    mma_commit_warp(mma_done);
+  } else {
+    // -------------------------------------------------------------- exponentials
+    const int r = threadIdx.x, key = k0 + r;
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const int k_last = (k0 + kMK < end ? k0 + kMK : end) - 1;
+    const int64_t row_base = (int64_t)bh * p.g * p.L;  // of lse: the kv head's rows are contiguous
+    auto row_lse = [&](int t) -> float {
+      return r < tile_rows(t) ? __ldg(&p.lse[row_base + tile_row(t) + r]) : INFINITY;
+    };
+    float next = n_tiles > 0 ? row_lse(0) : 0.f;
+    float2 acc[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int s = t & 1;
+      const int row0 = tile_row(t), rows = tile_rows(t);
+      const int l = (row0 + r) % L;
+      s_lse[s * kMR + r] = next;
+      s_pos[s * kMR + r] = base_pos + l;
+      if (t + 1 < n_tiles) next = row_lse(t + 1);
+      named_barrier(1, 128);  // also: every thread is done with the buffer of tile t - 2
+      // does every row of the tile see every key of the CTA?
+      const int pos_lo = by_head ? base_pos + row0 % L : base_pos;
+      const int pos_hi = by_head ? pos_lo + rows - 1 : ctx - 1;
+      const bool all = (!p.causal || k_last <= pos_lo) &&
+                       (p.window == 0 || k_last < p.sinks || (int64_t)k0 > (int64_t)pos_hi - p.window);
+      if (!warp_wait(&s_full[s], (uint32_t)((t >> 1) & 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < kMR; c0 += 32) {
+        if (c0 >= rows) break;
+        float sv[32];
+        tmem_ld32(tmem + lane_base + (uint32_t)(s * kMR + c0), sv);
+        tmem_wait_ld();
+        const float* ls = s_lse + s * kMR + c0;
+        if (all) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float4 l4 = *reinterpret_cast<const float4*>(ls + 4 * x);
+            const float2 z0 = __ffma2_rn(make_float2(sv[4 * x], sv[4 * x + 1]), make_float2(kf, kf), make_float2(-l4.x, -l4.y));
+            const float2 z1 = __ffma2_rn(make_float2(sv[4 * x + 2], sv[4 * x + 3]), make_float2(kf, kf), make_float2(-l4.z, -l4.w));
+            acc[(2 * x) & 3] = __fadd2_rn(acc[(2 * x) & 3], make_float2(ex2_ftz(z0.x), ex2_ftz(z0.y)));
+            acc[(2 * x + 1) & 3] = __fadd2_rn(acc[(2 * x + 1) & 3], make_float2(ex2_ftz(z1.x), ex2_ftz(z1.y)));
+          }
+        } else {
+          const int* ps = s_pos + s * kMR + c0;
+          const bool sink = key < p.sinks;
+          const int64_t w = p.window > 0 ? p.window : INT64_MAX / 4;
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const int pos = ps[x];
+            const bool seen = (!p.causal || key <= pos) && (sink || (int64_t)key > (int64_t)pos - w);
+            const float e = seen ? ex2_ftz(fmaf(sv[x], kf, -ls[x])) : 0.f;
+            if (x & 1) acc[(x >> 1) & 3].y += e; else acc[(x >> 1) & 3].x += e;
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&s_empty[s]);
+    }
+    if (!ok && lane == 0) {
+      record_error(err, kDevErrFullWait);
+      *(volatile int*)abort_flag = 1;
+    }
+    if (key < end) {
+      const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+      float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
+      const float old = key < base_pos ? *m : 0.f;
+      *m = old + (mapped ? a01.x + a01.y : 0.f);
+    }
+  }
+
+  if (warp == 5 && lane == 0) {
+    if (!mbar_wait(mma_done, 0)) record_error(err, kDevErrMmaWait);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMCols) : "memory");
+}
+
+template <typename T, typename KvT, int D>
+int launch_mass_sm100(const PagedArgs& a, const MassParams& p, int64_t keys, cudaStream_t s) {
+  using S = MassSmem<D>;
+  auto kern = key_mass_sm100_kernel<T, KvT, D>;
+  static std::mutex mu;
+  static uint64_t done = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 64 || !(done & (1ull << dev))) {
+      const int st = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes),
+                                "paged_attention: key mass cudaFuncSetAttribute");
+      if (st != NVM_OK) return st;
+      if (dev < 64) done |= 1ull << dev;
+    }
+  }
+  const CUtensorMapDataType dt =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t rows = (uint64_t)(p.g * p.L);
+  const uint64_t qd[3] = {(uint64_t)D, rows, (uint64_t)(p.B * p.Hkv)};
+  const uint64_t qs[2] = {D * 2, rows * D * 2};
+  const uint32_t qb[3] = {64u, (uint32_t)kMR, 1u};
+  CUtensorMap tq;
+  const int st = encode_tmap(&tq, dt, 3, a.q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != NVM_OK) return st;
+  const dim3 grid((unsigned)((keys + kMK - 1) / kMK), (unsigned)(a.B * a.Hkv));
+  kern<<<grid, kMThreads, S::kBytes, s>>>(tq, p, device_error_word());
+  return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
+}
+
+template <typename T>
+int launch_mass_typed(const PagedArgs& a, const MassParams& p, int64_t keys, cudaStream_t s) {
+  if (a.kv_dtype == NVM_I8)
+    return a.D == 64 ? launch_mass_sm100<T, int8_t, 64>(a, p, keys, s) : launch_mass_sm100<T, int8_t, 128>(a, p, keys, s);
+  return a.D == 64 ? launch_mass_sm100<T, T, 64>(a, p, keys, s) : launch_mass_sm100<T, T, 128>(a, p, keys, s);
+}
+
+bool force_generic() {
+  const char* v = std::getenv("NVM_ATTN_FORCE_GENERIC");
+  return v != nullptr && v[0] != '\0' && v[0] != '0';
+}
+
+// 16-bit queries over pages of their type or int8; the kernel counts keys, rows and
+// positions in 32 bits.
+bool mass_sm100_eligible(const PagedArgs& a) {
+  if (a.q_dtype != NVM_F16 && a.q_dtype != NVM_BF16) return false;
+  if (a.kv_dtype != a.q_dtype && a.kv_dtype != NVM_I8) return false;
+  if (a.D != 64 && a.D != 128) return false;
+  auto al16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
+  if (!al16(a.q) || !al16(a.k_pages)) return false;
+  const int64_t lim = INT32_MAX / 2;
+  return a.B * a.Hkv <= 65535 && a.Hq / a.Hkv * a.L < lim && a.page_size < lim && a.max_pages * a.page_size < lim;
+}
+
 }  // namespace
 
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, cudaStream_t s) {
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, cudaStream_t s) {
   MassParams p{};
   p.q = a.q; p.k = a.k_pages; p.ks = a.k_scales; p.block_table = a.block_table; p.context_lens = a.context_lens;
   p.lse = a.lse; p.mass = m.mass; p.stride_b = m.stride_b; p.stride_h = m.stride_h; p.len = m.len;
@@ -84,6 +485,14 @@ int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, cudaStream_t s) {
   int64_t keys = a.max_pages * a.page_size;
   if (m.len < keys) keys = m.len;
   if (keys <= 0 || a.B * a.Hkv == 0) return NVM_OK;
+  if (a.scores != nullptr) {
+    ScoreParams sp{a.scores, plan->chunk_tiles * plan->n_chunks * 16, (int)(p.g * p.L), (int)((p.g * p.L + 1) & ~int64_t(1))};
+    const dim3 grid((unsigned)((sp.v_keys + 255) / 256), (unsigned)(a.B * a.Hkv));
+    key_mass_scores_kernel<<<grid, 256, 0, s>>>(p, sp);
+    return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
+  }
+  if (!force_generic() && mass_sm100_eligible(a))
+    return a.q_dtype == NVM_F16 ? launch_mass_typed<__half>(a, p, keys, s) : launch_mass_typed<__nv_bfloat16>(a, p, keys, s);
   int64_t bx = (keys + kGenWarps - 1) / kGenWarps;
   if (bx > 65536) bx = 65536;
   const dim3 grid((unsigned)bx, (unsigned)(a.B * a.Hkv));

@@ -140,13 +140,21 @@ float kLseLater;
 // mass) the log-sum-exp of every query row, behind the ticket region in any case: tickets of
 // other calls that share the workspace must stay zero.
 struct WindowWs {
-  size_t lse, total;
+  size_t lse, scores, total;
 };
-WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, bool with_mass) {
+// Bytes of the scores that the n8 decode tile keeps (key_mass.cu says why), 0 if it does not
+// serve the plan.
+size_t score_bytes(const PagedArgs& a, const MmaPlan& plan) {
+  if (!plan.eligible || plan.nwm != 0) return 0;
+  const int64_t rows = (a.Hq / a.Hkv * a.L + 1) & ~int64_t(1);
+  return (size_t)(plan.n_units * plan.n_chunks * plan.chunk_tiles * 16 * rows) * sizeof(float);
+}
+WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, size_t score_bytes, bool with_mass) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   WindowWs w{};
   w.lse = al(attn_bytes > kTicketRegionBytes ? attn_bytes : kTicketRegionBytes);
-  w.total = with_mass ? w.lse + al((size_t)(a.B * a.Hq * a.L) * sizeof(float)) : attn_bytes;
+  w.scores = w.lse + al((size_t)(a.B * a.Hq * a.L) * sizeof(float));
+  w.total = with_mass ? w.scores + score_bytes : attn_bytes;
   return w;
 }
 
@@ -304,17 +312,18 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   a.is_causal = 1; a.window = window; a.sinks = sinks;
   if (validate_paged(a, false) != NVM_OK || validate_window(window, sinks, "paged_attention") != NVM_OK) return 0;
   if (with_mass) a.lse = &kLseLater;
-  size_t need = 0;
+  size_t need = 0, scores = 0;
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
     // q's dtype is not known here: cover both plans
     const MmaPlan plan = plan_paged_mma(a);
     if (plan.eligible) need = plan.ws_bytes;
+    scores = score_bytes(a, plan);
     if (!env_flag("NVM_ATTN_NO_SM100")) {
       const Sm100Plan sp = plan_sm100(a, true);
       if (sp.eligible && sp.ws_bytes > need) need = sp.ws_bytes;
     }
   }
-  return window_ws(a, need, with_mass != 0).total;
+  return window_ws(a, need, scores, with_mass != 0).total;
 }
 
 int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages, int kv_dtype,
@@ -345,17 +354,20 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
     if (!env_flag("NVM_ATTN_NO_SM100")) sp = plan_sm100(a, false);
     if (!sp.eligible) plan = plan_paged_mma(a);
   }
-  const WindowWs ws = window_ws(a, sp.eligible ? sp.ws_bytes : plan.eligible ? plan.ws_bytes : 0, key_mass != nullptr);
+  const size_t kept = key_mass != nullptr ? score_bytes(a, plan) : 0;
+  const WindowWs ws =
+      window_ws(a, sp.eligible ? sp.ws_bytes : plan.eligible ? plan.ws_bytes : 0, kept, key_mass != nullptr);
   if (ws.total > 0 && (workspace == nullptr || workspace_bytes < ws.total))
     return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
                 workspace_bytes);
   if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
+  if (kept > 0) a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
   st = sp.eligible     ? launch_sm100(a, sp, workspace, s)
        : plan.eligible ? launch_paged_mma(a, plan, workspace, s)
                        : launch_paged_generic(a, s);
   if (st != NVM_OK || key_mass == nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
-  return launch_key_mass(a, m, s);
+  return launch_key_mass(a, m, &plan, s);
 }
 
 int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,

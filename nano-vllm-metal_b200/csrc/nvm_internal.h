@@ -52,6 +52,7 @@ struct PagedArgs {
   // s > pos - window (window == 0: no such limit).
   int64_t window, sinks;
   float* lse;         // [B*Hq*L] log2 of sum 2^(score * log2 e) of every row (+inf: no key), or NULL
+  float* scores;      // n8 tile only: keep every base-2 score, [B*Hkv][virtual keys][rows, even], or NULL
 };
 inline bool paged_is_ext(const PagedArgs& a) { return a.window > 0 || a.lse != nullptr; }
 
@@ -65,7 +66,9 @@ struct KeyMassArgs {
   float* mass;
   int64_t stride_b, stride_h, len;
 };
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, cudaStream_t s);
+struct MmaPlan;
+// plan: the attention kernel's, when a.scores is set.
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, cudaStream_t s);
 
 // Eviction by accumulated weight (evict.cu).
 struct EvictArgs {

@@ -70,6 +70,7 @@ struct MmaParams {
   int cluster;        // the n_chunks CTAs of a unit are one cluster: merge over DSMEM
   int64_t window, sinks;  // kExt: window == 0 for none
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
+  float* scores;          // kExt, n8: keep every score ([units][n_chunks * ct * 16][rows, even]), or null
 };
 
 template <typename KvT, int D, int NWM, int NWK, int NS_ = 0>
@@ -454,6 +455,19 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   };
 
+  // kExt, n8: this lane's two rows' scores of keys r and r + 8 of the chunk's tile i
+  float* score_row = nullptr;
+  const int rows_pad = (int)((p.M + 1) & ~int64_t(1));
+  if constexpr (kExt && C::kN8) {
+    if (p.scores != nullptr && 2 * cq < rows_pad)
+      score_row = p.scores + ((unit * p.n_chunks * p.ct + t_begin) * 16 + r) * rows_pad + 2 * cq;
+  }
+  auto keep_scores = [&](int i, float2 a, float2 b2) {
+    float2* d = reinterpret_cast<float2*>(score_row + (int64_t)i * 16 * rows_pad);
+    d[0] = a;
+    d[4 * rows_pad] = b2;  // 8 keys on
+  };
+
   bool timed_out = false;
   for (int i = wk; i < n_my; i += NWK) {
     const int s = i % NS;
@@ -539,6 +553,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
           }
         }
         sv[e] = v;
+      }
+      if constexpr (kExt) {
+        if (score_row != nullptr) keep_scores(i, make_float2(sv[0], sv[1]), make_float2(sv[2], sv[3]));
       }
       // row max over the 16 keys: two in the thread, the rest across r (lanes xor 4, 8, 16)
       float mxA = fmaxf(sv[0], sv[2]), mxB = fmaxf(sv[1], sv[3]);
@@ -793,6 +810,10 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
         }
       }
           }
+    }
+    else if constexpr (kExt && C::kN8) {  // unmapped page: no row sees its keys
+      if (score_row != nullptr)
+        keep_scores(i, make_float2(-INFINITY, -INFINITY), make_float2(-INFINITY, -INFINITY));
     }
     __syncwarp();
     if constexpr (C::kSelfFeed) {
@@ -1162,7 +1183,7 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.causal = a.is_causal;
   p.cluster = 0;
-  p.window = a.window; p.sinks = a.sinks; p.lse = a.lse;
+  p.window = a.window; p.sinks = a.sinks; p.lse = a.lse; p.scores = a.scores;
   const dim3 grid((unsigned)plan.n_units, (unsigned)plan.n_chunks);
   if (plan.cluster && C::kClusterFits && plan.n_chunks > 1 && plan.n_chunks <= 8) {
     p.cluster = 1;
