@@ -229,8 +229,10 @@ int nvm_flash_attention_window(const void* q, const void* k, const void* v, int 
  *     from n on; may be key_mass itself (same strides), and must not overlap it otherwise.
  * The pages from position `sinks` on must belong to this request alone; with page_refcount
  * ([P] int32, may be NULL) that is checked.  A request with a shared or unmapped page there,
- * or longer than mass_len or its block-table row, is left as it is (keep_index -1, dropped 0)
- * and sets *status = NVM_ERR_INVALID_ARGUMENT, which is otherwise left alone.
+ * or longer than mass_len or its block-table row, is left as it is (keep_index -1, dropped 0).
+ *   refused [B] int32: NVM_ERR_INVALID_ARGUMENT for such a request, NVM_OK for the others;
+ *   status, one int32 or NULL, is set to NVM_ERR_INVALID_ARGUMENT by any of them and is
+ *     otherwise left alone.
  */
 int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, void* v_scales,
                     int scale_dtype, const int32_t* block_table, const int32_t* context_lens,
@@ -238,7 +240,7 @@ int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, 
                     int64_t mass_stride_h, int64_t mass_len, float* mass_out, int64_t out_stride_b,
                     int64_t out_stride_h, int64_t B, int64_t Hkv, int64_t D, int64_t P, int64_t page_size,
                     int64_t max_pages, int64_t budget, int64_t sinks, int64_t recent, int32_t* keep_index,
-                    int32_t* kept, int32_t* dropped, int32_t* status, void* stream);
+                    int32_t* kept, int32_t* dropped, int32_t* refused, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* Dense flash attention (prefill)                                            */

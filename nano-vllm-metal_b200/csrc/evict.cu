@@ -7,21 +7,21 @@
 // slots of the request's own pages; weights behind them become zero.  n <= budget changes
 // nothing.
 //
-// Two kernels.  evict_select: a CTA per (request, kv head) finds the k-th largest weight by
-// radix selection on an order-preserving 32-bit image of the weight (four 8-bit digits),
-// then walks the positions once in order, numbering the kept ones with ballots, and moves
-// the weights.  evict_compact: a CTA per (request, kv head, column slice of K or V).  Slot i
-// receives token keep[i] >= i, so a tile of slots read completely before it is written never
-// overwrites a row that a later tile reads (later tiles read positions at or past their own
-// first slot): in place, no second copy of the cache.  The column slices are independent,
-// which is what spreads one (request, kv head) over several SMs.
+// Two kernels.  evict_select: a CTA per (request, kv head) reads the weights once into
+// registers (up to 32 a thread; longer rows re-read them from L2), finds the k-th largest by
+// radix selection on an order-preserving 32-bit image (four 8-bit digits, shared-memory
+// histograms scanned by one warp), numbers the kept positions with one scan over ballot
+// counts in position order, and moves the weights.  evict_compact: a CTA per (request, kv
+// head, column slice of K or V).  Slot i receives token keep[i] >= i, so a tile of slots that
+// is read completely before it is written never overwrites a row that a later tile reads
+// (those lie at or past their own first slot): in place, no second copy of the cache, and the
+// next tile's rows can be on their way while this one is written.  The column slices are
+// independent, which is what spreads one (request, kv head) over several SMs.
 #include "nvm_common.cuh"
 #include "nvm_internal.h"
 
 namespace nvm {
 namespace {
-
-constexpr int kSelThreads = 1024;
 
 struct EvictParams {
   EvictArgs a;
@@ -29,6 +29,7 @@ struct EvictParams {
   int slice_bytes;      // columns of one CTA
   int n_slices;
   int scale_bytes;      // 0: no scales
+  int page_shift;       // log2 of page_size, -1 if it is no power of two
 };
 
 // Larger weight -> larger image; NaN -> 0, -0 -> the image of +0.
@@ -38,12 +39,171 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams ep) {
-  const EvictArgs& p = ep.a;
-  __shared__ int hist[256];
-  __shared__ int wsum[2][32];
-  __shared__ int s_bad, s_digit, s_rank;
+// Exclusive scan of one int per thread over the CTA (T threads); *total the sum.
+template <int T>
+__device__ __forceinline__ int cta_exclusive_scan(int v, int* wsum, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) wsum[warp] = x;
+  __syncthreads();
+  int w = lane < T / 32 ? wsum[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+  __syncthreads();  // wsum may be reused
+  return before + x - v;
+}
+
+constexpr int kPer = 32;  // weights a thread holds in registers
+
+template <int T>
+struct SelSmem {
+  int hist[256];
+  int cnt[T];             // kept per (stretch, warp) of one sweep
+  int wsum[32];
+  int bad, digit, rank;
+};
+
+// Keeps, of positions [0, n): [0, lo), [hi, n) and the k of [lo, hi) with the largest weight;
+// writes their positions and weights in order.  kHeld: the weights fit in registers.
+template <int T, bool kHeld>
+__device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, float* mout, int32_t* keep, int n, int lo, int hi, int k) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int stretches = (n + T - 1) / T;
+  float w[kPer];  // kHeld: the whole row; else one sweep
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j < stretches) w[j] = j * T + t < n ? mass[j * T + t] : 0.f;
+  }
+  // f(position, weight) over this thread's positions, stretch by stretch
+  auto each = [&](auto&& f) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (j < stretches) f(j * T + t, w[j]);
+    } else {
+      for (int j = 0; j < stretches; ++j) {
+        const int i = j * T + t;
+        f(i, i < n ? __ldcg(mass + i) : 0.f);
+      }
+    }
+  };
+  uint32_t prefix = 0;
+  int rank = k;  // how many weights equal to the threshold are kept
+  if (k > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (t < 256) sm.hist[t] = 0;
+      __syncthreads();
+      each([&](int i, float x) {
+        const uint32_t key = weight_key(x);
+        if (i >= lo && i < hi && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
+          atomicAdd(&sm.hist[(key >> shift) & 255], 1);
+      });
+      __syncthreads();
+      if (warp == 0) {  // lane: digits 255 - 8 lane .. 248 - 8 lane, counted from the top
+        int c[8], sum = 0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum += c[x] = sm.hist[255 - 8 * lane - x];
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        int above = incl - sum;  // weights with a larger digit than this lane's
+        if (above < rank && rank <= incl) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            if (above < rank && rank <= above + c[x]) {
+              sm.digit = 255 - 8 * lane - x;
+              sm.rank = rank - above;
+            }
+            above += c[x];
+          }
+        }
+      }
+      __syncthreads();
+      rank = sm.rank;
+      prefix |= (uint32_t)sm.digit << shift;
+    }
+  }
+  // Number the kept positions in sweeps of 32 stretches: first the weights equal to the
+  // threshold (only the first `rank` stay), then all kept.
+  int kept = 0, eq_seen = 0;
+  for (int s0 = 0; s0 < stretches; s0 += kPer) {
+    uint32_t eqs = 0, take = 0;  // bit j: this thread's position of stretch s0 + j
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (s0 + j >= stretches) break;
+      const int i = (s0 + j) * T + t;
+      if constexpr (!kHeld) w[j] = i < n ? __ldcg(mass + i) : 0.f;
+      if (i < n) {
+        if (i < lo || i >= hi) {
+          take |= 1u << j;
+        } else if (k > 0) {
+          const uint32_t key = weight_key(w[j]);
+          if (key > prefix) take |= 1u << j;
+          if (key == prefix) eqs |= 1u << j;
+        }
+      }
+    }
+    const int in_sweep = stretches - s0 < kPer ? stretches - s0 : kPer;
+    // position order within a sweep: stretch, warp, lane -> entry stretch * (T / 32) + warp
+    auto number = [&](uint32_t bits, int* total, auto&& f) {
+      sm.cnt[t] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (j >= in_sweep) break;
+        const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> j) & 1u);
+        if (lane == 0) sm.cnt[j * (T / 32) + warp] = __popc(bal);
+      }
+      __syncthreads();
+      const int mine = cta_exclusive_scan<T>(sm.cnt[t], sm.wsum, total);
+      sm.cnt[t] = mine;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (j >= in_sweep) break;
+        const uint32_t bal = __ballot_sync(0xffffffffu, (bits >> j) & 1u);
+        if ((bits >> j) & 1u) f(j, sm.cnt[j * (T / 32) + warp] + __popc(bal & ((1u << lane) - 1u)));
+      }
+      __syncthreads();
+    };
+    if (k > 0) {
+      int total;
+      number(eqs, &total, [&](int j, int at) {
+        if (eq_seen + at < rank) take |= 1u << j;
+      });
+      eq_seen += total;
+    }
+    // every weight of this sweep has been read (the scans' barriers): slots below its end
+    // may be overwritten when the weights move in place
+    int total;
+    number(take, &total, [&](int j, int at) {
+      keep[kept + at] = (s0 + j) * T + t;
+      mout[kept + at] = w[j];
+    });
+    kept += total;
+  }
+  for (int i = kept + t; i < n; i += T) mout[i] = 0.f;
+}
+
+template <int T>
+__global__ void __launch_bounds__(T, 1024 / T) evict_select_kernel(const EvictParams ep) {
+  const EvictArgs& p = ep.a;
+  __shared__ SelSmem<T> sm;
+  const int t = threadIdx.x;
   const int64_t b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   const int64_t n64 = p.context_lens[b];
   int32_t* keep = p.keep_index + (int64_t)blockIdx.x * p.budget;
@@ -52,107 +212,45 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
 
   // A request whose tokens would have to move is taken only if its row is sound: every page
   // that holds them mapped, and (with refcounts) owned by this request alone.
-  if (t == 0) s_bad = 0;
+  if (t == 0) sm.bad = 0;
   __syncthreads();
   if (n64 < 0 || n64 > p.len || n64 > p.max_pages * p.page_size) {
-    if (t == 0) s_bad = 1;
+    if (t == 0) sm.bad = 1;
   } else if (n64 > p.budget) {
     const int64_t first = p.sinks / p.page_size, last = (n64 - 1) / p.page_size;
-    for (int64_t i = first + t; i <= last; i += kSelThreads) {
+    for (int64_t i = first + t; i <= last; i += T) {
       const int64_t pid = p.block_table[b * p.max_pages + i];
-      if (pid < 0 || pid >= p.P || (p.page_refcount != nullptr && p.page_refcount[pid] != 1)) s_bad = 1;
+      if (pid < 0 || pid >= p.P || (p.page_refcount != nullptr && p.page_refcount[pid] != 1)) sm.bad = 1;
     }
   }
   __syncthreads();
-  const bool bad = s_bad != 0;
+  const bool bad = sm.bad != 0;
   const int n = bad ? 0 : (int)n64;
   const bool evicts = n > p.budget;
   if (t == 0 && h == 0) {
     p.kept[b] = bad ? (int32_t)n64 : (evicts ? (int32_t)p.budget : n);
     p.dropped[b] = evicts ? n - (int32_t)p.budget : 0;
-    if (bad) *p.status = NVM_ERR_INVALID_ARGUMENT;
+    p.refused[b] = bad ? NVM_ERR_INVALID_ARGUMENT : NVM_OK;
+    if (bad && p.status != nullptr) *p.status = NVM_ERR_INVALID_ARGUMENT;
   }
   if (!evicts) {  // everything stays (or the row is refused: no index, weights as they are)
-    for (int64_t i = t; i < p.budget; i += kSelThreads) keep[i] = i < n ? (int32_t)i : -1;
+    for (int64_t i = t; i < p.budget; i += T) keep[i] = i < n ? (int32_t)i : -1;
     if (mout != mass)
-      for (int64_t i = t; i < n; i += kSelThreads) mout[i] = mass[i];
+      for (int64_t i = t; i < n; i += T) mout[i] = mass[i];
     return;
   }
-
-  // k-th largest of the middle [lo, hi): digits from the top, `rank` counted inside the prefix
-  const int lo = (int)p.sinks, hi = n - (int)p.recent;
-  int rank = (int)(p.budget - p.sinks - p.recent);
-  uint32_t prefix = 0;
-  int above = 0;  // weights larger than the threshold, so far
-  if (rank > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (t < 256) hist[t] = 0;
-      __syncthreads();
-      for (int i = lo + t; i < hi; i += kSelThreads) {
-        const uint32_t key = weight_key(mass[i]);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (t == 0) {
-        int left = rank, d = 255;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        s_digit = d;
-        s_rank = left;
-      }
-      __syncthreads();
-      above += rank - s_rank;
-      rank = s_rank;
-      prefix |= (uint32_t)s_digit << shift;
-      __syncthreads();
-    }
-  }
-  // kept of the middle: every weight above the threshold, and the first `rank` equal ones
-  const bool none = p.budget == p.sinks + p.recent;
-  int out = 0, eq_seen = 0;  // kept / equal so far (all threads hold the same values)
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + t;
-    bool eq = false, take = false;
-    float w = 0.f;
-    if (i < n) {
-      w = mass[i];
-      if (i < lo || i >= hi) {
-        take = true;
-      } else if (!none) {
-        const uint32_t key = weight_key(w);
-        take = key > prefix;
-        eq = key == prefix;
-      }
-    }
-    const uint32_t beq = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) wsum[0][warp] = __popc(beq);
-    __syncthreads();
-    int before = 0, total_eq = 0;
-    for (int w2 = 0; w2 < 32; ++w2) {
-      if (w2 < warp) before += wsum[0][w2];
-      total_eq += wsum[0][w2];
-    }
-    const int my_eq = eq_seen + before + __popc(beq & ((1u << lane) - 1u));
-    if (eq && my_eq < rank) take = true;
-    const uint32_t bt = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) wsum[1][warp] = __popc(bt);
-    __syncthreads();  // every weight of this stretch has been read: they may be overwritten
-    int slot = out, total = 0;
-    for (int w2 = 0; w2 < 32; ++w2) {
-      if (w2 < warp) slot += wsum[1][w2];
-      total += wsum[1][w2];
-    }
-    slot += __popc(bt & ((1u << lane) - 1u));
-    if (take) {
-      keep[slot] = i;
-      mout[slot] = w;
-    }
-    out += total;
-    eq_seen += total_eq;
-    __syncthreads();
-  }
-  for (int64_t i = p.budget + t; i < n; i += kSelThreads) mout[i] = 0.f;
+  const int lo = (int)p.sinks, hi = n - (int)p.recent, k = (int)(p.budget - p.sinks - p.recent);
+  if (n <= kPer * T)
+    select_row<T, true>(sm, mass, mout, keep, n, lo, hi, k);
+  else
+    select_row<T, false>(sm, mass, mout, keep, n, lo, hi, k);
 }
 
+// CTAs of 128 threads, seven to an SM (about 900 threads with 2 x 4 vectors each in flight):
+// 512 (request, head) pairs x K and V are 6.9 CTAs an SM, one even wave.
+constexpr int kCmpThreads = 128;
+
+// Rows of one column slice: threads my_row = threadIdx / per_row of a step, kU steps a tile.
 template <typename V>
 __device__ __forceinline__ void compact_rows(const EvictParams& ep, int64_t b, int64_t h, uint8_t* pool, int64_t row_bytes,
                                              int col0, int cols) {
@@ -161,35 +259,53 @@ __device__ __forceinline__ void compact_rows(const EvictParams& ep, int64_t b, i
   const int per_row = cols / (int)sizeof(V);
   const int rows_par = blockDim.x / per_row;  // rows one step of the CTA covers
   const int my_row = threadIdx.x / per_row, my_col = threadIdx.x % per_row;
+  const bool active = my_row < rows_par;
+  const int budget = (int)p.budget, tile = rows_par * kU;
   const int32_t* keep = p.keep_index + (b * p.Hkv + h) * p.budget;
   const int32_t* table = p.block_table + b * p.max_pages;
   const uint32_t ps = (uint32_t)p.page_size;
+  const int shift = ep.page_shift;
   auto at = [&](uint32_t tok) -> V* {
-    const uint32_t page = tok / ps, off = tok - page * ps;
-    return reinterpret_cast<V*>(pool + (((int64_t)table[page] * p.Hkv + h) * ps + off) * row_bytes + col0) + my_col;
+    const uint32_t page = shift >= 0 ? tok >> shift : tok / ps, off = tok - page * ps;
+    return reinterpret_cast<V*>(pool + (((int64_t)__ldg(table + page) * p.Hkv + h) * ps + off) * row_bytes + col0) + my_col;
   };
-  for (int64_t base = p.sinks; base < p.budget; base += (int64_t)rows_par * kU) {
-    V v[kU];
-    bool mv[kU];
+  // where this thread's rows of the tile at `base` come from (the slot itself: nothing moves)
+  auto sources = [&](int base, int (&src)[kU]) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int64_t i = base + u * rows_par + my_row;
-      mv[u] = false;
-      if (my_row < rows_par && i < p.budget) {
-        const int src = keep[i];
-        mv[u] = src != i;
-        if (mv[u]) v[u] = *at((uint32_t)src);
-      }
+      const int i = base + u * rows_par + my_row;
+      src[u] = active && i < budget ? __ldg(keep + i) : i;
     }
-    __syncthreads();
+  };
+  auto fetch = [&](int base, const int (&src)[kU], V (&v)[kU]) {
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      if (mv[u]) *at((uint32_t)(base + u * rows_par + my_row)) = v[u];
+      if (src[u] != base + u * rows_par + my_row) v[u] = __ldcs(at((uint32_t)src[u]));
+  };
+  int src[kU], src2[kU];
+  V v[kU], v2[kU];
+  sources((int)p.sinks, src);
+  fetch((int)p.sinks, src, v);
+  sources((int)p.sinks + tile, src2);
+  for (int base = (int)p.sinks; base < budget; base += tile) {
+    // the next tile's rows lie past this tile's slots: they can be read before it is written
+    fetch(base + tile, src2, v2);
+    int src3[kU];
+    sources(base + 2 * tile, src3);
+    __syncthreads();  // this tile's rows have been read by every thread
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = base + u * rows_par + my_row;
+      if (src[u] != i) *at((uint32_t)i) = v[u];
+      src[u] = src2[u];
+      src2[u] = src3[u];
+      v[u] = v2[u];
+    }
   }
 }
 
 template <typename V>
-__global__ void __launch_bounds__(256) evict_compact_kernel(const EvictParams ep) {
+__global__ void __launch_bounds__(kCmpThreads, 7) evict_compact_kernel(const EvictParams ep) {
   const EvictArgs& p = ep.a;
   const int64_t b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   if (p.dropped[b] == 0) return;
@@ -215,21 +331,36 @@ int launch_evict(const EvictArgs& a, cudaStream_t s) {
   ep.a = a;
   ep.row_bytes = a.D * (int64_t)dtype_size(a.kv_dtype);
   ep.scale_bytes = a.kv_dtype == NVM_I8 ? (int)dtype_size(a.scale_dtype) : 0;
+  ep.page_shift = -1;
+  for (int x = 0; x < 31; ++x)
+    if (a.page_size == int64_t(1) << x) ep.page_shift = x;
+  // Threads of a selection: the longest row that the sizes allow in registers, 32 weights a
+  // thread, but all 1024 when there are fewer rows than SMs anyway.  A CTA of 1024 fills an
+  // SM's registers: 512 rows of 5000 took 72 us in CTAs of 1024 and 42 us in CTAs of 256.
   const dim3 sel((unsigned)(a.B * a.Hkv));
-  evict_select_kernel<<<sel, kSelThreads, 0, s>>>(ep);
+  const int64_t cap = a.len < a.max_pages * a.page_size ? a.len : a.max_pages * a.page_size;
+  if (cap > 512 * kPer || a.B * a.Hkv <= 148) evict_select_kernel<1024><<<sel, 1024, 0, s>>>(ep);
+  else if (cap > 256 * kPer) evict_select_kernel<512><<<sel, 512, 0, s>>>(ep);
+  else evict_select_kernel<256><<<sel, 256, 0, s>>>(ep);
   int st = check_cuda(cudaGetLastError(), "evict: selection kernel launch");
   if (st != NVM_OK) return st;
   // the widest vector that rows and pools are aligned to
   const uint64_t al = (uint64_t)ep.row_bytes | reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
   const int vec = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : (al & 1) == 0 ? 2 : 1;
-  ep.slice_bytes = 32 * (vec >= 4 ? 4 : 1) * (vec >= 16 ? 4 : 1);
-  if (ep.slice_bytes > ep.row_bytes) ep.slice_bytes = (int)ep.row_bytes;
+  // Columns of one CTA: up to 256 bytes (whole rows of 128 16-bit values), halved while the
+  // CTAs would not fill an even wave: to 64 bytes below six per SM, to 32 below two.
+  int slice = vec >= 16 ? 256 : vec >= 4 ? 128 : 32;
+  if (slice > ep.row_bytes) slice = (int)ep.row_bytes;
+  while (slice > 32 && slice % 2 == 0 && (slice / 2) % vec == 0 &&
+         a.B * a.Hkv * 2 * ((ep.row_bytes + slice - 1) / slice) < (slice > 64 ? 6 : 2) * 148)
+    slice /= 2;
+  ep.slice_bytes = slice;
   ep.n_slices = (int)((ep.row_bytes + ep.slice_bytes - 1) / ep.slice_bytes);
   const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)(2 * ep.n_slices + (ep.scale_bytes ? 2 : 0)));
-  if (vec == 16) evict_compact_kernel<uint4><<<grid, 256, 0, s>>>(ep);
-  else if (vec == 4) evict_compact_kernel<uint32_t><<<grid, 256, 0, s>>>(ep);
-  else if (vec == 2) evict_compact_kernel<uint16_t><<<grid, 256, 0, s>>>(ep);
-  else evict_compact_kernel<uint8_t><<<grid, 256, 0, s>>>(ep);
+  if (vec == 16) evict_compact_kernel<uint4><<<grid, kCmpThreads, 0, s>>>(ep);
+  else if (vec == 4) evict_compact_kernel<uint32_t><<<grid, kCmpThreads, 0, s>>>(ep);
+  else if (vec == 2) evict_compact_kernel<uint16_t><<<grid, kCmpThreads, 0, s>>>(ep);
+  else evict_compact_kernel<uint8_t><<<grid, kCmpThreads, 0, s>>>(ep);
   return check_cuda(cudaGetLastError(), "evict: compaction kernel launch");
 }
 

@@ -17,9 +17,14 @@
 //    from M = D / 4 = 32 on, and prompts could not keep M x S scores at all:
 //    key_mass_sm100_kernel computes them again on the tensor cores, S^T = K Q^T with the keys
 //    as the 128 lanes of tensor memory, so that a thread owns a key: its sum needs no
-//    exchange between threads and K enters shared memory once per 128 keys.  Bound by the
-//    exponentials (16 a clock and SM) from about 32 rows on.
+//    exchange between threads and K enters shared memory once per 128 keys.  With 64 rows a
+//    head or more the heads of a group are spread over the CTAs of a cluster, which add their
+//    sums through distributed shared memory: causal rows make the first keys' CTAs the
+//    longest.  Bound by the exponentials (16 a clock and SM) from about 32 rows on; a quarter
+//    of them is taken from that unit and computed by a polynomial on the FMA pipe.
 //  * everything else (fp32, other head dims): key_mass_generic_kernel.
+#include <cooperative_groups.h>
+
 #include <cstdlib>
 #include <mutex>
 #include <type_traits>
@@ -89,13 +94,16 @@ __global__ void __launch_bounds__(kGenWarps * 32) key_mass_generic_kernel(MassPa
 }
 
 // Scores kept by the attention kernel: [B*Hkv][v_keys][rows_pad] base-2 scores (-inf where a
-// row does not see the key) on the attention kernel's virtual keys; a thread per key.
+// row does not see the key) on the attention kernel's virtual keys; a thread takes
+// kScoreKeys keys, 256 apart, so that enough loads are in flight.
 struct ScoreParams {
   const float* scores;
   int64_t v_keys;
-  int rows, rows_pad;  // rows_pad: rows rounded up to even
+  int rows;  // kRows: rows rounded up to even
 };
+constexpr int kScoreKeys = 4;
 
+template <int kRows>
 __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p, const ScoreParams sp) {
   __shared__ float s_lse[8];
   const int64_t bh = blockIdx.y, b = bh / p.Hkv, h = bh - b * p.Hkv;
@@ -113,22 +121,38 @@ __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p
     }
   }
   __syncthreads();
-  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (end <= 0 || v >= tiles * 16) return;
-  const int64_t key = v / 16 >= sink_tiles ? v + skip * 16 : v;
-  if (key >= end || key >= p.len) return;
-  const float2* z = reinterpret_cast<const float2*>(sp.scores + (bh * sp.v_keys + v) * sp.rows_pad);
-  float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
-  float sum = key < ctx - p.L ? *m : 0.f;
-  float gain = 0.f;
+  const int64_t v0 = (int64_t)blockIdx.x * (256 * kScoreKeys) + threadIdx.x;
+  const int64_t v_end = end > 0 ? tiles * 16 : 0;
+  const float* z = sp.scores + bh * sp.v_keys * kRows;
+  float* mrow = p.mass + b * p.stride_b + h * p.stride_h;
+  float x[kScoreKeys][kRows], old[kScoreKeys];
+  int64_t key[kScoreKeys];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (2 * i < sp.rows_pad) {
-      const float2 x = __ldcs(z + i);
-      gain += ex2_ftz(x.x - s_lse[2 * i]) + (2 * i + 1 < sp.rows ? ex2_ftz(x.y - s_lse[2 * i + 1]) : 0.f);
+  for (int u = 0; u < kScoreKeys; ++u) {  // every load of the thread's keys first
+    const int64_t v = v0 + u * 256;
+    key[u] = v >= v_end ? -1 : v / 16 >= sink_tiles ? v + skip * 16 : v;
+    if (key[u] >= end || key[u] >= p.len) key[u] = -1;
+    if (key[u] < 0) continue;
+    old[u] = key[u] < ctx - p.L ? mrow[key[u]] : 0.f;
+    if constexpr (kRows % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < kRows / 4; ++i)
+        *reinterpret_cast<float4*>(&x[u][4 * i]) = __ldcs(reinterpret_cast<const float4*>(z + v * kRows) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRows / 2; ++i)
+        *reinterpret_cast<float2*>(&x[u][2 * i]) = __ldcs(reinterpret_cast<const float2*>(z + v * kRows) + i);
     }
   }
-  *m = sum + gain;
+#pragma unroll
+  for (int u = 0; u < kScoreKeys; ++u) {
+    if (key[u] < 0) continue;
+    float gain = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (i < sp.rows) gain += ex2_ftz(x[u][i] - s_lse[i]);  // an odd last column holds nothing
+    mrow[key[u]] = old[u] + gain;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -144,14 +168,37 @@ struct MassSmem {
   static constexpr int kKBytes = kMK * D * 2;
   static constexpr int kQBytes = kMR * D * 2;
   static constexpr int kStages = 2;
-  static constexpr int kUsed = kKBytes + kStages * kQBytes + 2 * kMR * 8 + 256;
+  static constexpr int kUsed = kKBytes + kStages * kQBytes + 2 * kMR * 8 + kMK * 4 + 256;
   // at least a third of an SM's: a third CTA would only wait for tensor memory
   static constexpr int kBytes = kUsed > 80 * 1024 ? kUsed : 80 * 1024;
 };
 
+// Of 16 pairs of exponentials, the even pairs 2x with bit x set run on the FMA pipe.
+constexpr uint32_t kPolyMask = 0x55u;
+
+// 2^x for a pair on the FMA pipe: n = round(x) through the 1.5 * 2^23 rounding constant,
+// f = x - n in [-0.5, 0.5] (exact), a degree-5 polynomial for 2^f (near-minimax for relative
+// error by iteratively reweighted least squares: 2.0e-7 in fp32, as ex2.approx), and n added to the
+// exponent field.  Arguments below -125 give 2^-125 instead of a smaller number or zero, so a
+// row without a key (lse = +inf) must not come here.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12582912.0f;
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 f = __ffma2_rn(__fadd2_rn(t, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
+  float2 p = __ffma2_rn(make_float2(0.001327647f, 0.001327647f), f, make_float2(0.009675542f, 0.009675542f));
+  p = __ffma2_rn(p, f, make_float2(0.055507135f, 0.055507135f));
+  p = __ffma2_rn(p, f, make_float2(0.2402212f, 0.2402212f));
+  p = __ffma2_rn(p, f, make_float2(0.69314694f, 0.69314694f));
+  p = __ffma2_rn(p, f, make_float2(1.0000001f, 1.0000001f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <typename T, typename KvT, int D>
 __global__ void __launch_bounds__(kMThreads, 2)
-    key_mass_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const MassParams p, int* err) {
+    key_mass_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const MassParams p, int split, int* err) {
   using S = MassSmem<D>;
   constexpr int kHalves = D / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -163,7 +210,8 @@ __global__ void __launch_bounds__(kMThreads, 2)
   uint8_t* sQ = smem + S::kKBytes;
   float* s_lse = reinterpret_cast<float*>(sQ + S::kStages * S::kQBytes);  // [2][kMR]
   int* s_pos = reinterpret_cast<int*>(s_lse + 2 * kMR);                   // [2][kMR]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_pos + 2 * kMR);
+  float* s_sum = reinterpret_cast<float*>(s_pos + 2 * kMR);               // [kMK]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_sum + kMK);
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;
   uint64_t* s_empty = s_full + 2;
@@ -178,8 +226,8 @@ __global__ void __launch_bounds__(kMThreads, 2)
   int64_t end64 = ctx < cap ? ctx : cap;
   if (p.len < end64) end64 = p.len;
   const int end = (int)end64;
-  const int k0 = blockIdx.x * kMK;
-  if (k0 >= end) return;
+  const int k0 = (int)(blockIdx.x / split) * kMK, part = (int)(blockIdx.x % split);
+  if (k0 >= end) return;  // the whole cluster
   // rows (per run) that see some key of the tile
   const int L = (int)p.L, base_pos = ctx - L;
   const bool by_head = L >= 64;  // else the g * L rows of the kv head are one run
@@ -193,9 +241,9 @@ __global__ void __launch_bounds__(kMThreads, 2)
   }
   const int n_rows = hi > lo ? hi - lo : 0;
   const int per_run = (n_rows + kMR - 1) / kMR;
-  const int runs = by_head ? (int)p.g : 1;
+  const int runs = by_head ? (int)p.g / split : 1;  // this CTA's heads: part * runs ..
   const int n_tiles = per_run * runs;
-  auto tile_row = [&](int t) { return (t / per_run) * (by_head ? L : 0) + lo + (t % per_run) * kMR; };
+  auto tile_row = [&](int t) { return (part * runs + t / per_run) * (by_head ? L : 0) + lo + (t % per_run) * kMR; };
   auto tile_rows = [&](int t) {
     const int left = n_rows - (t % per_run) * kMR;
     return left < kMR ? left : kMR;
@@ -369,13 +417,14 @@ __global__ void __launch_bounds__(kMThreads, 2)
         tmem_ld32(tmem + lane_base + (uint32_t)(s * kMR + c0), sv);
         tmem_wait_ld();
         const float* ls = s_lse + s * kMR + c0;
-        if (all) {
+        if (all && c0 + 32 <= rows) {
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const float4 l4 = *reinterpret_cast<const float4*>(ls + 4 * x);
             const float2 z0 = __ffma2_rn(make_float2(sv[4 * x], sv[4 * x + 1]), make_float2(kf, kf), make_float2(-l4.x, -l4.y));
             const float2 z1 = __ffma2_rn(make_float2(sv[4 * x + 2], sv[4 * x + 3]), make_float2(kf, kf), make_float2(-l4.z, -l4.w));
-            acc[(2 * x) & 3] = __fadd2_rn(acc[(2 * x) & 3], make_float2(ex2_ftz(z0.x), ex2_ftz(z0.y)));
+            const float2 e0 = (kPolyMask >> x) & 1 ? exp2_poly(z0) : make_float2(ex2_ftz(z0.x), ex2_ftz(z0.y));
+            acc[(2 * x) & 3] = __fadd2_rn(acc[(2 * x) & 3], e0);
             acc[(2 * x + 1) & 3] = __fadd2_rn(acc[(2 * x + 1) & 3], make_float2(ex2_ftz(z1.x), ex2_ftz(z1.y)));
           }
         } else {
@@ -398,12 +447,27 @@ __global__ void __launch_bounds__(kMThreads, 2)
       record_error(err, kDevErrFullWait);
       *(volatile int*)abort_flag = 1;
     }
-    if (key < end) {
-      const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+    const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+    const float sum = mapped ? a01.x + a01.y : 0.f;
+    if (split > 1) {
+      s_sum[r] = sum;
+    } else if (key < end) {
       float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
-      const float old = key < base_pos ? *m : 0.f;
-      *m = old + (mapped ? a01.x + a01.y : 0.f);
+      *m = (key < base_pos ? *m : 0.f) + sum;
     }
+  }
+  if (split > 1) {  // the parts' sums, always added in the same order
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int key = k0 + (int)threadIdx.x;
+    if (part == 0 && threadIdx.x < kMK && key < end) {
+      float sum = s_sum[threadIdx.x];
+      for (int x = 1; x < split; ++x) sum += cluster.map_shared_rank(s_sum, x)[threadIdx.x];
+      float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
+      *m = (key < base_pos ? *m : 0.f) + sum;
+    }
+    cluster.sync();  // the sums stay until they have been read
   }
 
   if (warp == 5 && lane == 0) {
@@ -442,9 +506,26 @@ int launch_mass_sm100(const PagedArgs& a, const MassParams& p, int64_t keys, cud
   CUtensorMap tq;
   const int st = encode_tmap(&tq, dt, 3, a.q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != NVM_OK) return st;
-  const dim3 grid((unsigned)((keys + kMK - 1) / kMK), (unsigned)(a.B * a.Hkv));
-  kern<<<grid, kMThreads, S::kBytes, s>>>(tq, p, device_error_word());
-  return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
+  // Heads per cluster: the largest divisor of g up to 8, while the key tiles alone are fewer
+  // than eight waves of two CTAs per SM.
+  int split = 1;
+  const int64_t key_tiles = (keys + kMK - 1) / kMK;
+  if (p.L >= 64 && key_tiles * a.B * a.Hkv < 8 * 2 * 148)
+    for (int x = 2; x <= 8; ++x)
+      if (p.g % x == 0) split = x;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(key_tiles * split), (unsigned)(a.B * a.Hkv));
+  cfg.blockDim = dim3(kMThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, tq, p, split, device_error_word()),
+                    "paged_attention: key mass kernel launch");
 }
 
 template <typename T>
@@ -486,9 +567,13 @@ int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* pla
   if (m.len < keys) keys = m.len;
   if (keys <= 0 || a.B * a.Hkv == 0) return NVM_OK;
   if (a.scores != nullptr) {
-    ScoreParams sp{a.scores, plan->chunk_tiles * plan->n_chunks * 16, (int)(p.g * p.L), (int)((p.g * p.L + 1) & ~int64_t(1))};
-    const dim3 grid((unsigned)((sp.v_keys + 255) / 256), (unsigned)(a.B * a.Hkv));
-    key_mass_scores_kernel<<<grid, 256, 0, s>>>(p, sp);
+    ScoreParams sp{a.scores, plan->chunk_tiles * plan->n_chunks * 16, (int)(p.g * p.L)};
+    const int64_t per = 256 * kScoreKeys;
+    const dim3 grid((unsigned)((sp.v_keys + per - 1) / per), (unsigned)(a.B * a.Hkv));
+    if (sp.rows <= 2) key_mass_scores_kernel<2><<<grid, 256, 0, s>>>(p, sp);
+    else if (sp.rows <= 4) key_mass_scores_kernel<4><<<grid, 256, 0, s>>>(p, sp);
+    else if (sp.rows <= 6) key_mass_scores_kernel<6><<<grid, 256, 0, s>>>(p, sp);
+    else key_mass_scores_kernel<8><<<grid, 256, 0, s>>>(p, sp);
     return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
   }
   if (!force_generic() && mass_sm100_eligible(a))

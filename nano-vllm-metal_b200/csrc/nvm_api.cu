@@ -408,7 +408,8 @@ int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, 
                     const float* key_mass, int64_t mass_stride_b, int64_t mass_stride_h, int64_t mass_len,
                     float* mass_out, int64_t out_stride_b, int64_t out_stride_h, int64_t B, int64_t Hkv, int64_t D,
                     int64_t P, int64_t page_size, int64_t max_pages, int64_t budget, int64_t sinks, int64_t recent,
-                    int32_t* keep_index, int32_t* kept, int32_t* dropped, int32_t* status, void* stream) {
+                    int32_t* keep_index, int32_t* kept, int32_t* dropped, int32_t* refused, int32_t* status,
+                    void* stream) {
   if (!is_float_dtype(kv_dtype) && kv_dtype != NVM_I8)
     return fail(NVM_ERR_INVALID_ARGUMENT, "evict: pages must be float32, float16, bfloat16 or int8");
   if (kv_dtype == NVM_I8 && !is_float_dtype(scale_dtype))
@@ -424,7 +425,7 @@ int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, 
     return fail(NVM_ERR_UNSUPPORTED, "evict: budget, page_size and B * Hkv must be below 2^31");
   if (B == 0) return NVM_OK;
   if (!k_pages || !v_pages || !block_table || !context_lens || !key_mass || !mass_out || !keep_index || !kept ||
-      !dropped || !status || (kv_dtype == NVM_I8 && (!k_scales || !v_scales)))
+      !dropped || !refused || (kv_dtype == NVM_I8 && (!k_scales || !v_scales)))
     return fail(NVM_ERR_INVALID_ARGUMENT, "evict: null tensor pointer");
   EvictArgs a{};
   a.k_pages = k_pages; a.v_pages = v_pages; a.kv_dtype = kv_dtype; a.k_scales = k_scales; a.v_scales = v_scales;
@@ -434,7 +435,7 @@ int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, 
   a.out_stride_b = out_stride_b; a.out_stride_h = out_stride_h;
   a.B = B; a.Hkv = Hkv; a.D = D; a.P = P; a.page_size = page_size; a.max_pages = max_pages;
   a.budget = budget; a.sinks = sinks; a.recent = recent;
-  a.keep_index = keep_index; a.kept = kept; a.dropped = dropped; a.status = status;
+  a.keep_index = keep_index; a.kept = kept; a.dropped = dropped; a.refused = refused; a.status = status;
   return launch_evict(a, static_cast<cudaStream_t>(stream));
 }
 

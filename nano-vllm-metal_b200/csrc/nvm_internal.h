@@ -89,7 +89,8 @@ struct EvictArgs {
   int32_t* keep_index;
   int32_t* kept;
   int32_t* dropped;
-  int32_t* status;
+  int32_t* refused;
+  int32_t* status;  // may be NULL
 };
 int launch_evict(const EvictArgs& a, cudaStream_t s);
 

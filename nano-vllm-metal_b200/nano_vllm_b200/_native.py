@@ -7,6 +7,7 @@ tensors are not on a CUDA device.  The library is built in-tree by
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -18,6 +19,7 @@ LIB_PATH = os.path.join(_HERE, "libnvm_attn.so")
 
 NVM_F32, NVM_F16, NVM_BF16, NVM_I8, NVM_I32, NVM_I64 = 0, 1, 2, 3, 4, 5
 NVM_OK = 0
+NVM_ERR_WORKSPACE = -3
 
 _DTYPE_CODE = {
     torch.float32: NVM_F32,
@@ -50,7 +52,7 @@ SIGNATURES = {
     "nvm_flash_attention_window": (_I, [_P, _P, _P, _I, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I64,
                                         _I64, _P]),
     "nvm_paged_evict": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64,
-                             _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+                             _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P]),
     "nvm_reshape_and_cache": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I, _P, _P, _I, _P, _I64, _I64, _I64, _I64,
                                    _I64, _P]),
     "nvm_paged_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P]),
@@ -122,7 +124,19 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle, without building a torch.cuda.Stream (2 us a call)."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """torch.cuda.device(device), or nothing to do when it is the current device."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return _HERE_ALREADY
+    return torch.cuda.device(device)
 
 
 # Split-K workspace: one zero-filled buffer per (device, stream), grown on demand.
@@ -143,15 +157,28 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     return ws
 
 
-def private_workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
-    """The cached workspace, except while a CUDA graph is being captured: a graph replays with
-    the addresses it captured, on any stream and beside any other graph, so its calls get a
-    buffer of their own (from the graph's memory pool; the zero fill becomes a graph node)."""
-    if nbytes == 0 or not torch.cuda.is_current_stream_capturing():
-        return workspace(device, nbytes)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    ws[:1 << 20].zero_()
-    return ws
+def call_with_workspace(device: torch.device, size, call) -> None:
+    """Run ``call(pointer, nbytes, stream) -> status`` with a workspace of ``size()`` bytes.
+
+    The buffer cached for (device, stream) is offered first, whatever its size: a call that
+    needs more says so before any GPU work, and only then is the size asked for and the buffer
+    grown.  While a CUDA graph is being captured the call gets a buffer of its own instead (from
+    the graph's memory pool; the zero fill of its tickets becomes a graph node): a graph replays
+    with the addresses it captured, on any stream and beside any other graph."""
+    stream = stream_ptr(device)
+    if torch.cuda.is_current_stream_capturing():
+        nbytes = size()
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        if ws is not None:
+            ws[:1 << 20].zero_()
+        check(call(ptr(ws), nbytes, stream))
+        return
+    ws = _workspaces.get((device.index if device.index is not None else torch.cuda.current_device(), stream))
+    status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
+    if status == NVM_ERR_WORKSPACE:
+        nbytes = size()
+        status = call(ptr(workspace(device, nbytes)), nbytes, stream)
+    check(status)
 
 
 def device_error(device: torch.device, clear: bool = True) -> int:

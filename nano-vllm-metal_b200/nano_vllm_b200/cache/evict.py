@@ -25,7 +25,7 @@ class EvictResult(NamedTuple):
     keep_index: torch.Tensor  # [B, Hkv, budget] int32: old position of each kept token, -1 behind them
     kept: torch.Tensor        # [B] int32 tokens kept
     dropped: torch.Tensor     # [B] int32 tokens given up: what to rewind the request by
-    status: torch.Tensor      # [1] int32, not zero if a request could not be trimmed
+    refused: torch.Tensor     # [B] int32, not zero for a request that could not be trimmed
 
 
 def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
@@ -46,7 +46,8 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     (``DevicePageTable.evict`` does both).  The pages from position ``sinks`` on must belong to
     the request alone; ``page_refcount`` ([P] int32 or longer) makes the kernel check it.  A
     request with a shared or unmapped page there, or longer than S or its row, is left as it
-    is, with ``dropped`` 0, and sets ``status``.
+    is, with ``dropped`` 0 and ``refused`` not zero; ``status`` (one int32, optional) is then set
+    too and is never cleared.
     """
     op = "evict"
     dev = nv.require_cuda(op, key_pages, value_pages, block_table, context_lens, key_mass, key_scales, value_scales,
@@ -81,20 +82,17 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     if page_refcount is not None and (page_refcount.dtype != torch.int32 or page_refcount.numel() < P or
                                       not page_refcount.is_contiguous()):
         raise RuntimeError(f"{op}: page_refcount must be contiguous int32 with an entry per page")
-    if status is None:
-        status = torch.zeros(1, dtype=torch.int32, device=dev)
-    elif status.dtype != torch.int32 or status.numel() != 1:
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise RuntimeError(f"{op}: status must be one int32")
     bt = block_table.to(torch.int32).contiguous()
     cl = context_lens.to(torch.int32).contiguous()
     keep = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
-    counts = torch.empty((2, B), dtype=torch.int32, device=dev)
-    kept, dropped = counts[0], counts[1]
-    with torch.cuda.device(dev):
+    kept, dropped, refused = torch.empty((3, B), dtype=torch.int32, device=dev).unbind(0)
+    with nv.on_device(dev):
         nv.check(nv.lib().nvm_paged_evict(
             key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(key_scales),
             nv.ptr(value_scales), sdt, bt.data_ptr(), cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(),
             key_mass.stride(0), key_mass.stride(1), key_mass.shape[2], out.data_ptr(), out.stride(0), out.stride(1), B,
             Hkv, D, P, ps, bt.shape[1], budget, sinks, recent, keep.data_ptr(), kept.data_ptr(), dropped.data_ptr(),
-            status.data_ptr(), nv.stream_ptr(dev)))
-    return EvictResult(keep, kept, dropped, status)
+            refused.data_ptr(), nv.ptr(status), nv.stream_ptr(dev)))
+    return EvictResult(keep, kept, dropped, refused)

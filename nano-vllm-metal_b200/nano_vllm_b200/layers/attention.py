@@ -122,7 +122,7 @@ def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         if q.dim() < 3 or tuple(k.shape) != (B, Hkv, S, D) or v.shape != k.shape:
             raise RuntimeError("flash_attention: key and value must be [B, Hkv, S, E] with the query's B and E")
         out = torch.empty((*batch_shape, Hq, L, D), dtype=out_dtype or query.dtype, device=dev)
-        with torch.cuda.device(dev):
+        with nv.on_device(dev):
             nv.check(nv.lib().nvm_flash_attention_window(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), nv.dtype_code(q.dtype), out.data_ptr(),
                 nv.dtype_code(out.dtype), B, Hq, Hkv, L, S, D, float(factor), int(is_causal), window, sinks,
@@ -219,15 +219,16 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
             ms = (*key_mass.stride()[:2], key_mass.shape[2])
             _check_rows("paged_attention: key_mass", key_mass)
         w = window or 0
-        ws_bytes = L_.nvm_paged_attention_window_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc, w, sinks,
-                                                                int(key_mass is not None))
-        with torch.cuda.device(dev):
-            ws = nv.private_workspace(dev, ws_bytes)
-            nv.check(L_.nvm_paged_attention_window(
-                q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
-                bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps,
-                bt.shape[1], float(factor), int(mask == "causal"), w, sinks, nv.ptr(key_mass), *ms, nv.ptr(ws),
-                ws_bytes, nv.stream_ptr(dev)))
+        MP = bt.shape[1]
+        with nv.on_device(dev):
+            nv.call_with_workspace(
+                dev,
+                lambda: L_.nvm_paged_attention_window_workspace_size(B, Hq, Hkv, L, D, ps, MP, kvc, w, sinks,
+                                                                     int(key_mass is not None)),
+                lambda ws, ws_bytes, stream: L_.nvm_paged_attention_window(
+                    q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
+                    bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps, MP,
+                    factor, mask == "causal", w, sinks, nv.ptr(key_mass), *ms, ws, ws_bytes, stream))
         return out
     ws_bytes = L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc)
     ws = nv.workspace(dev, ws_bytes)

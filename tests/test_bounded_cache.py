@@ -66,7 +66,7 @@ def test_workspace_sizes():
 def test_evict_c_entry_refusals():
     def call(B=1, D=128, budget=4, sinks=0, recent=0, kv=2, sb=8):
         return nv.lib().nvm_paged_evict(None, None, kv, None, None, 1, None, None, None, None, sb, 8, 8, None, 8, 8, B, 2, D,
-                                        4, 16, 4, budget, sinks, recent, None, None, None, None, None)
+                                        4, 16, 4, budget, sinks, recent, None, None, None, None, None, None)
     assert call() == -1
     assert call(B=0) == 0
     for bad in (dict(budget=0), dict(sinks=-1), dict(recent=-1), dict(sinks=3, recent=2), dict(kv=4), dict(sb=-1)):

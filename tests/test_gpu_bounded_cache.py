@@ -297,7 +297,8 @@ EVICT_CASES = [  # ctx, Hkv, D, ps, dtype, budget, sinks, recent, kind
     ([300, 299], 3, 64, 16, HF, 64, 0, 64, "plain"),      # nothing but the recent
     ([2049, 1025, 1024, 1023], 2, 64, 64, HF, 1023, 1, 100, "plain"),
     ([5000, 4096], 2, 128, 16, BF, 2500, 4, 64, "ties"),
-    ([40000], 1, 64, 16, BF, 9000, 4, 64, "plain"),
+    ([40000], 1, 64, 16, BF, 9000, 4, 64, "plain"),        # longer than a CTA holds in registers
+    ([70000, 33000], 1, 64, 16, HF, 40000, 1, 1, "ties"),
 ]
 
 
@@ -316,7 +317,7 @@ def test_evict(case, in_place):
     r = evict_tokens(p["k"], p["v"], p["bt"], p["cl"], gm, budget, sinks=sinks, recent=recent, key_scales=p["ks"],
                      value_scales=p["vs"], mass_out=out)
     assert torch.equal(r.keep_index.cpu(), keep)
-    assert torch.equal(r.kept.cpu(), kept) and torch.equal(r.dropped.cpu(), dropped) and int(r.status) == 0
+    assert torch.equal(r.kept.cpu(), kept) and torch.equal(r.dropped.cpu(), dropped) and not r.refused.any()
     got = gm.cpu() if in_place else out.cpu()
     for b, n in enumerate(ctx):
         assert equal_or_nan(got[b, :, :n], mref[b, :, :n])
@@ -340,13 +341,14 @@ def test_evict_leaves_refused_requests_alone():
     keep, kept, dropped, mref, new, bad = evict_reference(prob, mass, 40, 17, 4, ref)
     assert bad and dropped.tolist() == [60, 0, 0, 0, 60]
     p, gm = to_gpu(prob), mass.cuda()
-    r = evict_tokens(p["k"], p["v"], p["bt"], p["cl"], gm, 40, sinks=17, recent=4, page_refcount=ref.cuda())
-    assert int(r.status) != 0
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    r = evict_tokens(p["k"], p["v"], p["bt"], p["cl"], gm, 40, sinks=17, recent=4, page_refcount=ref.cuda(), status=status)
+    assert int(status) != 0 and (r.refused != 0).tolist() == [False, True, True, False, False]
     assert torch.equal(r.keep_index.cpu(), keep) and torch.equal(r.kept.cpu(), kept) and torch.equal(r.dropped.cpu(), dropped)
     assert torch.equal(gm.cpu(), mref)
     assert torch.equal(p["k"].cpu(), new["k"]) and torch.equal(p["v"].cpu(), new["v"])
     short = evict_tokens(p["k"], p["v"], p["bt"], p["cl"], torch.rand(5, 2, 99).cuda(), 40, sinks=17)  # mass too short
-    assert int(short.status) != 0 and short.dropped.tolist() == [0, 0, 0, 0, 0]
+    assert (short.refused != 0).tolist() == [True, True, True, False, True] and short.dropped.tolist() == [0, 0, 0, 0, 0]
 
 
 def test_evict_on_another_stream_and_captured():
