@@ -29,6 +29,8 @@
 // v + skip past it), so rings, phases and chunks run unchanged.
 // Every mbarrier wait is bounded; on expiry the CTA records an error, lets its own
 // copies and MMAs land (bounded), frees TMEM and returns.
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include <cstdlib>
@@ -105,6 +107,7 @@ struct Sm100Params {
   float* part_o;    // [n_units][n_chunks][rows_real][kD]
   int64_t window, sinks;  // kExt: window == 0 for none
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
+  int cluster;            // kExt: the n_chunks CTAs of a unit are one cluster and merge over DSMEM
 };
 
 // Pairs q (keys 2q, 2q+1 of a 64-key tile) whose exponentials run on the FMA pipe.
@@ -232,6 +235,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   int64_t* item_ring = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars) + 256);  // [4]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // cluster: CTA rank c of a cluster takes chunk c of its unit
+  int64_t first_item = blockIdx.x;
+  if (kExt && p.cluster) {
+    const uint32_t nc = (uint32_t)p.n_chunks, u = blockIdx.x / nc, c = blockIdx.x - u * nc;
+    first_item = (int64_t)(nc - 1 - c) * p.n_units + u;
+  }
+  // cluster: this CTA's rows for the merge, in the K/V ring once the item's MMAs are done:
+  // unnormalised O as fp32 [128][128] (16-byte chunk x of row r at r * 512 + ((x ^ (r & 31)) << 4))
+  // and (m, l) of every row
+  float2* part_ml_s = reinterpret_cast<float2*>(sK + kBM * kD * 4);
   // The producer warp's first lane sets up the barriers; with one item per CTA it then
   // requests that item's Q tile at once, before tensor memory is allocated and the CTA
   // synchronises (the first S waits on this copy).
@@ -262,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     *abort_flag = 0;
     fence_mbar_init();
     if (p.stage_out && (int64_t)blockIdx.x < p.n_items) {
-      const Item it0 = decode_item<kExt>(p, blockIdx.x);
+      const Item it0 = decode_item<kExt>(p, first_item);
       if (it0.valid && it0.n_tiles > 0) {
         mbar_arrive_expect_tx(q_full, kQBytes);
         tma_load_3d(sQ, &tm_q, 0, (int)it0.r0, (int)it0.n, q_full);
@@ -337,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           item = __shfl_sync(0xffffffffu, v, leader_lane);
         } else {
           item = (int64_t)blockIdx.x + (int64_t)n_fetched * gridDim.x;
+          if (kExt && p.cluster) item = n_fetched == 0 ? first_item : p.n_items;
         }
         ++n_fetched;
         if (item >= p.n_items) {
@@ -667,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     };
+    bool merged = false;  // cluster: this CTA's part is in shared memory
     auto put_lse = [&](const Item& it, float mx, float sum) {
       if constexpr (kExt) {
         if (p.lse != nullptr && row < it.rows)
@@ -682,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       const Item it = decode_item<kExt>(p, item);
       if (!it.valid) continue;
+      if (kExt && p.cluster && it.n_tiles == 0) continue;
       const int n = it.n_tiles;
       const bool row_ok = row < it.rows;
       uint8_t* orow = reinterpret_cast<uint8_t*>(p.out) + ((it.n * p.M_rows) + it.r0 + row) * (int64_t)kD * esz;
@@ -877,7 +893,20 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       ++iw;
       tc_fence_after();
-      if (it.n_chunks_unit == 1) {
+      if (kExt && p.cluster) {
+        part_ml_s[row] = make_float2(m, lsum);  // m = -inf: no visible key in this chunk
+#pragma unroll 1
+        for (int c1 = 0; c1 < kD; c1 += 32) {
+          float ov[32];
+          tmem_ld32(tO + lane_base + c1, ov);
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            *reinterpret_cast<float4*>(sK + row * 512 + (((c1 / 4 + x) ^ lane) << 4)) =
+                make_float4(ov[4 * x], ov[4 * x + 1], ov[4 * x + 2], ov[4 * x + 3]);
+        }
+        merged = true;
+      } else if (it.n_chunks_unit == 1) {
         put_lse(it, m, lsum);
         const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
 #pragma unroll 1
@@ -1017,6 +1046,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
+    if (kExt && p.cluster && !merged) part_ml_s[row] = make_float2(-INFINITY, 0.f);
     if (!ok) {
       record_error(p.err, kDevErrFullWait);
       *(volatile int*)abort_flag = 1;
@@ -1032,6 +1062,55 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   if (warp == 5) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+  if constexpr (kExt) {
+    if (p.cluster) {
+      // Every CTA of the unit holds its chunk's rows in shared memory; row r is merged by CTA
+      // r % n_chunks, a warp a row, with log-sum-exp weights in chunk order.
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      const Item it = decode_item<true>(p, first_item);
+      const int nc = (int)p.n_chunks, rank = nc - 1 - (int)((uint32_t)first_item / (uint32_t)p.n_units);
+      for (int r = rank + nc * warp; r < it.rows; r += nc * (kThreads / 32)) {
+        float2 ml[8];
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < 8; ++cc) {
+          if (cc < nc) {
+            ml[cc] = cluster.map_shared_rank(part_ml_s, cc)[r];
+            mx = fmaxf(mx, ml[cc].x);
+          }
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int cc = 0; cc < 8; ++cc) {
+          if (cc < nc && ml[cc].x != -INFINITY) {
+            const float w = exp2f(ml[cc].x - mx);
+            const float4 v = *reinterpret_cast<const float4*>(
+                cluster.map_shared_rank(sK, cc) + r * 512 + ((lane ^ (r & 31)) << 4));
+            sum += ml[cc].y * w;
+            o.x += v.x * w;
+            o.y += v.y * w;
+            o.z += v.z * w;
+            o.w += v.w * w;
+          }
+        }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const int64_t row = it.n * p.M_rows + it.r0 + r;
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (p.out_dtype == NVM_F32)
+          reinterpret_cast<float4*>(p.out)[row * (kD / 4) + lane] = o;
+        else if (p.out_dtype == NVM_BF16)
+          reinterpret_cast<uint2*>(p.out)[row * (kD / 4) + lane] =
+              make_uint2(cvt_pack<__nv_bfloat16>(o.x, o.y), cvt_pack<__nv_bfloat16>(o.z, o.w));
+        else
+          reinterpret_cast<uint2*>(p.out)[row * (kD / 4) + lane] =
+              make_uint2(cvt_pack<__half>(o.x, o.y), cvt_pack<__half>(o.z, o.w));
+        if (p.lse != nullptr && lane == 0) p.lse[row] = sum > 0.f ? mx + log2f(sum) : INFINITY;
+      }
+      cluster.sync();  // the parts stay until they have been read
+    }
   }
   // the last CTA to leave resets the work counter for the next call
   if (threadIdx.x == 0 && p.work_counter != nullptr) {
@@ -1114,6 +1193,21 @@ int launch_typed(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const 
       done |= 1ull << dev;
     }
   }
+  if (kExt && p.cluster) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.n_chunks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, flash_sm100_kernel<T, kExt>, tq, tk, tv, to, p),
+                      "paged_attention: sm100 kernel launch (cluster)");
+  }
   flash_sm100_kernel<T, kExt><<<grid, kThreads, kSmemBytes, s>>>(tq, tk, tv, to, p);
   return check_cuda(cudaGetLastError(), "flash_attention: sm100 kernel launch");
 }
@@ -1133,7 +1227,7 @@ WsOffsets sm100_ws_offsets(const Sm100Plan& plan) {
   w.ml = w.list + al(items * sizeof(int));
   w.o = w.ml;
   w.total = w.ml;
-  if (plan.n_chunks > 1) {
+  if (plan.n_chunks > 1 && !plan.cluster) {
     w.o = w.ml + al(items * (size_t)plan.rows_real * sizeof(float2));
     w.total = w.o + items * (size_t)plan.rows_real * kD * sizeof(float);
   }
@@ -1192,7 +1286,21 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
   // Split-K over keys for grouped paged calls (dense callers pass no workspace): aim at
   // a few CTAs per SM slot if every sequence were max_pages long; units whose context is
   // shorter leave their later chunks empty (those CTAs return at once).
-  if (plan.grouped && !a.dense && plan.n_units <= kMaxTicketUnits) {
+  // Windowed / scored few-token calls with at most 96 tiles a unit: a merge through the
+  // workspace costs more than the tiles it saves (32 requests of 5 tokens under a window of
+  // 1000 keys, 128 units of 18 tiles: one chunk 33 us, two of 9 tiles 37 us, three of 8 and
+  // the work list 64 us).  Up to 8 chunks of a unit form a cluster and merge over distributed
+  // shared memory while all CTAs fit at once; more units than that take one chunk each.
+  if (plan.grouped && paged_is_ext(a) && !a.dense && tiles_max <= 96) {
+    int64_t nc = 2 * 148 / plan.n_units;
+    if (nc > 8) nc = 8;
+    if (nc > tiles_max / 2) nc = tiles_max / 2;
+    if (nc >= 2) {
+      plan.ct = (tiles_max + nc - 1) / nc;
+      plan.n_chunks = (tiles_max + plan.ct - 1) / plan.ct;
+      plan.cluster = plan.n_chunks > 1 ? 1 : 0;
+    }
+  } else if (plan.grouped && !a.dense && plan.n_units <= kMaxTicketUnits) {
     int64_t ct = env_int("NVM_SM100_CHUNK_TILES", 0);
     if (ct <= 0) {
       const int64_t target = 148 * 2 * 4;
@@ -1266,7 +1374,7 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
     p.exit_counter = p.work_counter + 1;
   }
   const WsOffsets wo = sm100_ws_offsets(plan);
-  if (plan.n_chunks > 1) {
+  if (plan.n_chunks > 1 && !plan.cluster) {
     uint8_t* w = static_cast<uint8_t*>(ws);
     p.counters = reinterpret_cast<int*>(w);
     p.part_ml = reinterpret_cast<float2*>(w + wo.ml);
@@ -1278,7 +1386,10 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   // per item (the hardware scheduler balances the heavy-first causal tiles), which lets
   // the epilogue stage O in shared memory for bulk tensor stores.
   int64_t ctas = p.n_items;
-  const int64_t persistent = env_int("NVM_SM100_PERSISTENT", plan.grouped ? 1 : 0);
+  // (a bounded number of tiles leaves nothing to balance: no work list then)
+  const int64_t persistent =
+      plan.cluster ? 0 : env_int("NVM_SM100_PERSISTENT", plan.grouped && !(a.window > 0 && plan.n_chunks == 1) ? 1 : 0);
+  p.cluster = plan.cluster;
   if (persistent != 0) {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -20,8 +20,8 @@
 //    exchange between threads and K enters shared memory once per 128 keys.  With 64 rows a
 //    head or more the heads of a group are spread over the CTAs of a cluster, which add their
 //    sums through distributed shared memory: causal rows make the first keys' CTAs the
-//    longest.  Bound by the exponentials (16 a clock and SM) from about 32 rows on; a quarter
-//    of them is taken from that unit and computed by a polynomial on the FMA pipe.
+//    longest.  Bound by the exponentials (16 a clock and SM) inside the tile loop and by the
+//    start of its CTAs.
 //  * everything else (fp32, other head dims): key_mass_generic_kernel.
 #include <cooperative_groups.h>
 
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p
 // ---------------------------------------------------------------------------
 constexpr int kMK = 128;        // keys per CTA = tensor-memory lanes
 constexpr int kMR = 128;        // query rows per tile = accumulator columns
-constexpr int kMThreads = 192;  // warps 0-3: exponentials; warp 4: Q copies; warp 5: MMAs
+constexpr int kMThreads = 320;  // warps 0-7: exponentials; warp 8: Q copies; warp 9: MMAs
 constexpr int kMCols = 256;     // two accumulators; two CTAs per SM share the 512 columns
 
 template <int D>
@@ -168,12 +168,14 @@ struct MassSmem {
   static constexpr int kKBytes = kMK * D * 2;
   static constexpr int kQBytes = kMR * D * 2;
   static constexpr int kStages = 2;
-  static constexpr int kUsed = kKBytes + kStages * kQBytes + 2 * kMR * 8 + kMK * 4 + 256;
+  static constexpr int kUsed = kKBytes + kStages * kQBytes + 2 * kMR * 8 + 2 * kMK * 4 + 256;
   // at least a third of an SM's: a third CTA would only wait for tensor memory
   static constexpr int kBytes = kUsed > 80 * 1024 ? kUsed : 80 * 1024;
 };
 
-// Of 16 pairs of exponentials, the even pairs 2x with bit x set run on the FMA pipe.
+// Of 16 pairs of exponentials, the even pairs 2x with bit x set run on the FMA pipe: a quarter
+// of them takes 1 % off a scored prompt (with four warps a scheduler the MUFU unit is at 80 %
+// inside the tile loop).
 constexpr uint32_t kPolyMask = 0x55u;
 
 // 2^x for a pair on the FMA pipe: n = round(x) through the 1.5 * 2^23 rounding constant,
@@ -208,10 +210,10 @@ __global__ void __launch_bounds__(kMThreads, 2)
   }
   uint8_t* sK = smem;
   uint8_t* sQ = smem + S::kKBytes;
-  float* s_lse = reinterpret_cast<float*>(sQ + S::kStages * S::kQBytes);  // [2][kMR]
-  int* s_pos = reinterpret_cast<int*>(s_lse + 2 * kMR);                   // [2][kMR]
-  float* s_sum = reinterpret_cast<float*>(s_pos + 2 * kMR);               // [kMK]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_sum + kMK);
+  float* s_nls = reinterpret_cast<float*>(sQ + S::kStages * S::kQBytes);  // [2][kMR] -lse
+  int* s_pos = reinterpret_cast<int*>(s_nls + 2 * kMR);                   // [2][kMR]
+  float* s_sum = reinterpret_cast<float*>(s_pos + 2 * kMR);               // [2][kMK]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_sum + 2 * kMK);
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;
   uint64_t* s_empty = s_full + 2;
@@ -220,13 +222,22 @@ __global__ void __launch_bounds__(kMThreads, 2)
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int bh = blockIdx.y, b = bh / (int)p.Hkv, h = bh - b * (int)p.Hkv;
-  const int ctx = p.context_lens[b];
+  // key tile-major, first keys first: with causal rows these have the most work
+  const int bh = blockIdx.x / split, part = blockIdx.x % split, b = bh / (int)p.Hkv, h = bh - b * (int)p.Hkv;
   const int64_t cap = p.mp * p.ps;
+  const int k0 = (int)blockIdx.y * kMK;
+  // this thread's page, asked for beside the context length, not after it
+  int pid = -1;
+  uint32_t key_off = 0;
+  if (warp < 8 && k0 + (int)(threadIdx.x & 127) < cap) {
+    const uint32_t my_key = (uint32_t)k0 + (threadIdx.x & 127), page = my_key / (uint32_t)p.ps;
+    key_off = my_key - page * (uint32_t)p.ps;
+    pid = __ldg(&p.block_table[(int64_t)b * p.mp + page]);
+  }
+  const int ctx = p.context_lens[b];
   int64_t end64 = ctx < cap ? ctx : cap;
   if (p.len < end64) end64 = p.len;
   const int end = (int)end64;
-  const int k0 = (int)(blockIdx.x / split) * kMK, part = (int)(blockIdx.x % split);
   if (k0 >= end) return;  // the whole cluster
   // rows (per run) that see some key of the tile
   const int L = (int)p.L, base_pos = ctx - L;
@@ -243,20 +254,26 @@ __global__ void __launch_bounds__(kMThreads, 2)
   const int per_run = (n_rows + kMR - 1) / kMR;
   const int runs = by_head ? (int)p.g / split : 1;  // this CTA's heads: part * runs ..
   const int n_tiles = per_run * runs;
-  auto tile_row = [&](int t) { return (part * runs + t / per_run) * (by_head ? L : 0) + lo + (t % per_run) * kMR; };
-  auto tile_rows = [&](int t) {
-    const int left = n_rows - (t % per_run) * kMR;
-    return left < kMR ? left : kMR;
+  // Walk of the tiles in order: run by run, `in` rows into the run.
+  struct Walk {
+    int base, in;  // the run's first row of the kv head; rows of the run before this tile
+  };
+  const Walk first{part * runs * (by_head ? L : 0) + lo, 0};
+  auto step = [&](Walk& w) {
+    w.in += kMR;
+    if (w.in >= n_rows) {
+      w.in = 0;
+      w.base += L;
+    }
   };
 
-  auto load_q = [&](int t) {
-    const int s = t & 1;
+  auto load_q = [&](int s, const Walk& w) {
     mbar_arrive_expect_tx(&q_full[s], S::kQBytes);
 #pragma unroll
     for (int hf = 0; hf < kHalves; ++hf)
-      tma_load_3d(sQ + s * S::kQBytes + hf * (kMR * 128), &tm_q, hf * 64, tile_row(t), bh, &q_full[s]);
+      tma_load_3d(sQ + s * S::kQBytes + hf * (kMR * 128), &tm_q, hf * 64, w.base + w.in, bh, &q_full[s]);
   };
-  if (threadIdx.x == 4 * 32) {
+  if (threadIdx.x == 8 * 32) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -266,37 +283,36 @@ __global__ void __launch_bounds__(kMThreads, 2)
     mbar_init(mma_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    for (int t = 0; t < 2 && t < n_tiles; ++t) load_q(t);
+    Walk w = first;
+    for (int t = 0; t < 2 && t < n_tiles; ++t, step(w)) load_q(t, w);
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kMCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // K: lane = key for the page lookup, then the warp copies its 32 rows with kLanes lanes a
-  // row into the swizzled K-major layout the MMA reads (row r's 16-byte chunk c of a
+  // K: lane = key for the page lookup, then warps w and w + 4 copy their 32 rows with kLanes
+  // lanes a row into the swizzled K-major layout the MMA reads (row r's 16-byte chunk c of a
   // 64-element half at r * 128 + ((c ^ (r & 7)) << 4)); int8 becomes T exactly and its scale
   // multiplies the scores.  Unmapped and out-of-range keys are zero.
   float kf = p.scale_log2;
   bool mapped = false;
-  if (warp < 4) {
-    const int key = k0 + (int)threadIdx.x;
+  if (warp < 8) {
+    const int key = k0 + (int)(threadIdx.x & 127);
     int64_t row = -1;
-    if (key < end) {
-      const uint32_t page = (uint32_t)key / (uint32_t)p.ps, off = (uint32_t)key - page * (uint32_t)p.ps;
-      const int64_t pid = p.block_table[(int64_t)b * p.mp + page];
-      if (pid >= 0 && pid < p.P) row = (pid * p.Hkv + h) * p.ps + off;
-    }
+    if (key < end && pid >= 0 && pid < p.P) row = ((int64_t)pid * p.Hkv + h) * p.ps + key_off;
     mapped = row >= 0;
     if (std::is_same<KvT, int8_t>::value && mapped) kf *= load_dyn(p.ks, row, p.scale_dtype);
     constexpr int kLanes = D * (int)sizeof(KvT) / 16;  // lanes a row, and steps
     constexpr int kRows = 32 / kLanes;                 // rows a step
     const int sub = lane / kLanes, c = lane % kLanes;
-    uint4 v[kLanes];
+    constexpr int kHalf = kLanes / 2;                  // steps of each of the two warps
+    const int i0 = (warp >> 2) * kHalf;
+    uint4 v[kHalf];
 #pragma unroll
-    for (int i = 0; i < kLanes; ++i) {
-      const int64_t src = __shfl_sync(0xffffffffu, row, i * kRows + sub);
+    for (int i = 0; i < kHalf; ++i) {
+      const int64_t src = __shfl_sync(0xffffffffu, row, (i0 + i) * kRows + sub);
       v[i] = src >= 0 ? __ldcs(reinterpret_cast<const uint4*>(static_cast<const KvT*>(p.k) + src * D) + c)
                       : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -304,8 +320,8 @@ __global__ void __launch_bounds__(kMThreads, 2)
       *reinterpret_cast<uint4*>(sK + (ch >> 3) * (kMK * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
     };
 #pragma unroll
-    for (int i = 0; i < kLanes; ++i) {
-      const int r = warp * 32 + i * kRows + sub;
+    for (int i = 0; i < kHalf; ++i) {
+      const int r = (warp & 3) * 32 + (i0 + i) * kRows + sub;
       if constexpr (std::is_same<KvT, int8_t>::value) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
         uint32_t o[8];
@@ -327,17 +343,21 @@ __global__ void __launch_bounds__(kMThreads, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 4) {
+  if (warp == 8) {
     // -------------------------------------------------------------- Q copies
     if (lane == 0) {
       bool ok = true;
       int issued = n_tiles < 2 ? n_tiles : 2;
+      Walk w = first;
+      step(w);
+      step(w);
       for (int t = 2; t < n_tiles; ++t) {
         if (!mbar_wait(&q_empty[t & 1], (uint32_t)(((t >> 1) & 1) ^ 1)) || *(volatile int*)abort_flag != 0) {
           ok = false;
           break;
         }
-        load_q(t);
+        load_q(t & 1, w);
+        step(w);
         issued = t + 1;
       }
       if (!ok) {
@@ -350,7 +370,7 @@ __global__ void __launch_bounds__(kMThreads, 2)
       }
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // -------------------------------------------------------------- MMAs
     const uint32_t id = idesc<T>(false, kMR);
     const uint64_t dk = smem_desc(smem_u32(sK), 16, 1024), dq = smem_desc(smem_u32(sQ), 16, 1024);
@@ -380,28 +400,40 @@ __global__ void __launch_bounds__(kMThreads, 2)
     mma_commit_warp(mma_done);
   } else {
     // -------------------------------------------------------------- exponentials
-    const int r = threadIdx.x, key = k0 + r;
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    // Warps 0-3 take the even tiles, warps 4-7 the odd ones: with two CTAs per SM four warps
+    // a scheduler, which hide the tensor-memory loads and the exponentials' latency.
+    const int wg = warp >> 2, r = threadIdx.x & 127, key = k0 + r;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int k_last = (k0 + kMK < end ? k0 + kMK : end) - 1;
     const int64_t row_base = (int64_t)bh * p.g * p.L;  // of lse: the kv head's rows are contiguous
-    auto row_lse = [&](int t) -> float {
-      return r < tile_rows(t) ? __ldg(&p.lse[row_base + tile_row(t) + r]) : INFINITY;
+    auto row_lse = [&](const Walk& w) -> float {
+      return w.in + r < n_rows ? -__ldg(&p.lse[row_base + w.base + w.in + r]) : -INFINITY;
     };
-    float next = n_tiles > 0 ? row_lse(0) : 0.f;
+    Walk w = first;
+    if (wg) step(w);
+    float next = wg < n_tiles ? row_lse(w) : 0.f;
     float2 acc[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) acc[x] = make_float2(0.f, 0.f);
+    const float2 kf2 = make_float2(kf, kf);
+    const bool sink = key < p.sinks;
     bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
-      const int s = t & 1;
-      const int row0 = tile_row(t), rows = tile_rows(t);
-      const int l = (row0 + r) % L;
-      s_lse[s * kMR + r] = next;
-      s_pos[s * kMR + r] = base_pos + l;
-      if (t + 1 < n_tiles) next = row_lse(t + 1);
-      named_barrier(1, 128);  // also: every thread is done with the buffer of tile t - 2
+    const int s = wg;  // the accumulator of this group's tiles
+    const uint32_t tS = tmem + lane_base + (uint32_t)(s * kMR);
+    float* nls = s_nls + s * kMR;
+    int* ps = s_pos + s * kMR;
+    for (int t = wg; t < n_tiles; t += 2) {
+      const Walk now = w;
+      const int rows = n_rows - now.in < kMR ? n_rows - now.in : kMR;
+      step(w);
+      step(w);
+      named_barrier(1 + wg, 128);  // every thread of the group is done with the buffer's last tile
+      nls[r] = next;
+      if (!by_head) ps[r] = base_pos + (now.in + r) % L;
+      if (t + 2 < n_tiles) next = row_lse(w);
+      named_barrier(1 + wg, 128);
       // does every row of the tile see every key of the CTA?
-      const int pos_lo = by_head ? base_pos + row0 % L : base_pos;
+      const int pos_lo = by_head ? base_pos + lo + now.in : base_pos;
       const int pos_hi = by_head ? pos_lo + rows - 1 : ctx - 1;
       const bool all = (!p.causal || k_last <= pos_lo) &&
                        (p.window == 0 || k_last < p.sinks || (int64_t)k0 > (int64_t)pos_hi - p.window);
@@ -410,32 +442,42 @@ __global__ void __launch_bounds__(kMThreads, 2)
         break;
       }
       tc_fence_after();
+      if (all && rows == kMR) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < kMR; c0 += 32) {
-        if (c0 >= rows) break;
-        float sv[32];
-        tmem_ld32(tmem + lane_base + (uint32_t)(s * kMR + c0), sv);
-        tmem_wait_ld();
-        const float* ls = s_lse + s * kMR + c0;
-        if (all && c0 + 32 <= rows) {
+        for (int c = 0; c < kMR; c += 32) {
+          float v[32];
+          tmem_ld32(tS + (uint32_t)c, v);
+          tmem_wait_ld();
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
-            const float4 l4 = *reinterpret_cast<const float4*>(ls + 4 * x);
-            const float2 z0 = __ffma2_rn(make_float2(sv[4 * x], sv[4 * x + 1]), make_float2(kf, kf), make_float2(-l4.x, -l4.y));
-            const float2 z1 = __ffma2_rn(make_float2(sv[4 * x + 2], sv[4 * x + 3]), make_float2(kf, kf), make_float2(-l4.z, -l4.w));
+            const float4 l4 = *reinterpret_cast<const float4*>(nls + c + 4 * x);
+            const float2 z0 = __ffma2_rn(make_float2(v[4 * x], v[4 * x + 1]), kf2, make_float2(l4.x, l4.y));
+            const float2 z1 = __ffma2_rn(make_float2(v[4 * x + 2], v[4 * x + 3]), kf2, make_float2(l4.z, l4.w));
             const float2 e0 = (kPolyMask >> x) & 1 ? exp2_poly(z0) : make_float2(ex2_ftz(z0.x), ex2_ftz(z0.y));
             acc[(2 * x) & 3] = __fadd2_rn(acc[(2 * x) & 3], e0);
             acc[(2 * x + 1) & 3] = __fadd2_rn(acc[(2 * x + 1) & 3], make_float2(ex2_ftz(z1.x), ex2_ftz(z1.y)));
           }
-        } else {
-          const int* ps = s_pos + s * kMR + c0;
-          const bool sink = key < p.sinks;
-          const int64_t w = p.window > 0 ? p.window : INT64_MAX / 4;
+        }
+      } else {
+        // columns [c_lo, c_hi) of a run see this key; rows of several heads look their position up
+        const int64_t w64 = p.window > 0 && !sink ? p.window : INT64_MAX / 4;
+        const int64_t c_hi64 = (int64_t)key + w64 - pos_lo;
+        const int c_lo = p.causal ? key - pos_lo : INT32_MIN, c_hi = c_hi64 < kMR ? (int)c_hi64 : kMR;
+#pragma unroll 1
+        for (int c0 = 0; c0 < rows; c0 += 32) {
+          float sv[32];
+          tmem_ld32(tS + (uint32_t)c0, sv);
+          tmem_wait_ld();
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
-            const int pos = ps[x];
-            const bool seen = (!p.causal || key <= pos) && (sink || (int64_t)key > (int64_t)pos - w);
-            const float e = seen ? ex2_ftz(fmaf(sv[x], kf, -ls[x])) : 0.f;
+            bool seen;
+            if (by_head) {
+              seen = c0 + x >= c_lo && c0 + x < c_hi;
+            } else {
+              const int pos = ps[c0 + x];
+              seen = (!p.causal || key <= pos) && (int64_t)key > (int64_t)pos - w64;
+            }
+            const float e = seen ? ex2_ftz(fmaf(sv[x], kf, nls[c0 + x])) : 0.f;
             if (x & 1) acc[(x >> 1) & 3].y += e; else acc[(x >> 1) & 3].x += e;
           }
         }
@@ -448,35 +490,31 @@ __global__ void __launch_bounds__(kMThreads, 2)
       *(volatile int*)abort_flag = 1;
     }
     const float2 a01 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
-    const float sum = mapped ? a01.x + a01.y : 0.f;
-    if (split > 1) {
-      s_sum[r] = sum;
-    } else if (key < end) {
-      float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
-      *m = (key < base_pos ? *m : 0.f) + sum;
-    }
+    s_sum[wg * kMK + r] = mapped ? a01.x + a01.y : 0.f;
   }
-  if (split > 1) {  // the parts' sums, always added in the same order
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int key = k0 + (int)threadIdx.x;
-    if (part == 0 && threadIdx.x < kMK && key < end) {
-      float sum = s_sum[threadIdx.x];
-      for (int x = 1; x < split; ++x) sum += cluster.map_shared_rank(s_sum, x)[threadIdx.x];
-      float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
-      *m = (key < base_pos ? *m : 0.f) + sum;
+  // the two groups' and the cluster's sums, always added in the same order
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (split > 1) cluster.sync(); else __syncthreads();
+  const int key = k0 + (int)threadIdx.x;
+  if (part == 0 && threadIdx.x < kMK && key < end) {
+    float sum = s_sum[threadIdx.x] + s_sum[kMK + threadIdx.x];
+    for (int x = 1; x < split; ++x) {
+      const float* other = cluster.map_shared_rank(s_sum, x);
+      sum += other[threadIdx.x] + other[kMK + threadIdx.x];
     }
-    cluster.sync();  // the sums stay until they have been read
+    float* m = p.mass + b * p.stride_b + h * p.stride_h + key;
+    *m = (key < base_pos ? *m : 0.f) + sum;
   }
+  if (split > 1) cluster.sync();  // the sums stay until they have been read
 
-  if (warp == 5 && lane == 0) {
+  if (warp == 9 && lane == 0) {
     if (!mbar_wait(mma_done, 0)) record_error(err, kDevErrMmaWait);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5)
+  if (warp == 9)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMCols) : "memory");
 }
 
@@ -506,15 +544,16 @@ int launch_mass_sm100(const PagedArgs& a, const MassParams& p, int64_t keys, cud
   CUtensorMap tq;
   const int st = encode_tmap(&tq, dt, 3, a.q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != NVM_OK) return st;
-  // Heads per cluster: the largest divisor of g up to 8, while the key tiles alone are fewer
-  // than eight waves of two CTAs per SM.
+  // CTAs per cluster: the smallest divisor of the group's heads that makes three CTAs an SM,
+  // enough to even out the causal rows (2 x 2048 tokens, 32/8 heads: 512 CTAs 174 us with the
+  // attention, 256 CTAs 188 us, 1024 CTAs 182 us, where the start of a CTA weighs more).
   int split = 1;
   const int64_t key_tiles = (keys + kMK - 1) / kMK;
-  if (p.L >= 64 && key_tiles * a.B * a.Hkv < 8 * 2 * 148)
-    for (int x = 2; x <= 8; ++x)
+  if (p.L >= 64)
+    for (int x = 2; x <= 8 && key_tiles * a.B * a.Hkv * split < 3 * 148; ++x)
       if (p.g % x == 0) split = x;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(key_tiles * split), (unsigned)(a.B * a.Hkv));
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * split), (unsigned)key_tiles);
   cfg.blockDim = dim3(kMThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = s;
@@ -549,7 +588,8 @@ bool mass_sm100_eligible(const PagedArgs& a) {
   auto al16 = [](const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; };
   if (!al16(a.q) || !al16(a.k_pages)) return false;
   const int64_t lim = INT32_MAX / 2;
-  return a.B * a.Hkv <= 65535 && a.Hq / a.Hkv * a.L < lim && a.page_size < lim && a.max_pages * a.page_size < lim;
+  return a.B * a.Hq < lim && a.Hq / a.Hkv * a.L < lim && a.page_size < lim && a.max_pages < lim &&
+         a.max_pages * a.page_size < int64_t(65535) * kMK;
 }
 
 }  // namespace

@@ -138,6 +138,7 @@ struct Sm100Plan {
   int grouped;
   int64_t M_rows, n_outer, n_row_tiles, n_units, rows_real, ct, n_chunks;
   size_t ws_bytes;
+  int cluster;  // the chunks of a unit merge inside a thread-block cluster
 };
 // sizing_only: plan from shapes alone (q dtype, pointers and scale unknown), for
 // nvm_paged_attention_workspace_size.

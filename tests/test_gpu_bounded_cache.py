@@ -71,6 +71,8 @@ WINDOW_CASES = [
     ([700, 150], 150, 8, 2, 128, 128, HF, HF, 129, 4),            # chunk, pages of two tiles
     ([5000, 300, 4100], 5, 32, 4, 128, 32, BF, BF, 3500, 100),    # verify, several chunks a unit
     ([300, 50], 3, 6, 2, 80, 7, F32, F32, 40, 5),                 # odd head dim and page size, fp32
+    ([3000, 0, 1], 7, 8, 1, 128, 16, BF, BF, 2000, 9),            # one row tile over eight chunks, empty and tiny contexts
+    ([2500, 1800, 60, 3], 40, 16, 2, 128, 16, HF, HF, 700, 4),    # 320 rows a kv head: several row tiles
     ([300, 20], 1, 4, 4, 96, 24, HF, F32, 33, 2),                 # odd head dim, fp32 queries over fp16
 ]
 
