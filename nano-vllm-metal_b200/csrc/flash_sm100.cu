@@ -24,9 +24,12 @@
 //              with tcgen05.commit on mbarriers.
 // kExt instances take a sliding window with sinks (a row at position pos sees key s only if
 // s < sinks or s > pos - window), paged context of any page size that 16 divides, and leave
-// every row's log-sum-exp.  The 64-key tiles between the sinks and a row tile's windows are
-// jumped over by renumbering (virtual tile v is tile v below the sinks' last tile and tile
-// v + skip past it), so rings, phases and chunks run unchanged.
+// every row's log-sum-exp.  The 16-key groups between the sinks and a row tile's windows are
+// jumped over by renumbering (virtual group v is group v below the sinks' end and group
+// v + skip past it), so rings, phases and chunks run unchanged and one tile of four groups can
+// hold the sinks next to the window's start: a tile of its own for 4 sinks cost 7 % of a
+// prompt under a 1024-key window.  Which tiles need a mask is known per item; the mask of a
+// row is a 64-bit pattern.
 // Every mbarrier wait is bounded; on expiry the CTA records an error, lets its own
 // copies and MMAs land (bounded), frees TMEM and returns.
 #include <cooperative_groups.h>
@@ -123,16 +126,23 @@ struct Item {
   int64_t c, u, n, b, kvh, r0, rows, ctx, ctx_limit, l_first, t_begin, n_chunks_unit;
   int n_tiles;  // 64-key tiles of this item (0: no keys; still produces zero rows when valid)
   bool valid;   // false: a chunk past the unit's last key (nothing to do)
-  // kExt: virtual tiles from sink_tiles on lie `skip` tiles further; keys in [sinks, first)
-  // and keys >= end are seen by no row of the tile
-  int sink_tiles, skip;
-  int64_t first, end;
+  // kExt: virtual 16-key groups from sg on lie `skip` groups further; keys in [sinks, first)
+  // and keys >= end are seen by no row of the tile, keys < all_lo (the sinks aside) and keys
+  // > all_hi not by every row
+  int sg, skip, first, end, all_lo, all_hi;
 };
 
-template <bool kExt>
-__device__ __forceinline__ int64_t tile_of(const Item& it, int64_t v) {
-  return kExt && v >= it.sink_tiles ? v + it.skip : v;
+constexpr int kNoSkip = 1 << 26;       // sg of an item without a gap
+constexpr int64_t kExtKeys = 1 << 30;  // kExt counts keys in 32 bits
+
+__device__ __forceinline__ int group_of(const Item& it, int v) { return v < it.sg ? v : v + it.skip; }
+// the virtual group that holds a key (the first one past the gap for a key inside it)
+__device__ __forceinline__ int vgroup_of(const Item& it, int key) {
+  const int g = key >> 4;
+  return g < it.sg ? g : (g - it.skip > it.sg ? g - it.skip : it.sg);
 }
+// columns 0 .. x of a tile
+__device__ __forceinline__ uint64_t cols_to(int x) { return x < 0 ? 0ull : x >= 63 ? ~0ull : (2ull << x) - 1; }
 
 template <bool kExt>
 __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) {
@@ -174,17 +184,23 @@ __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) 
   if (it.ctx <= 0 || need < 0) need = 0;
   int64_t n_tiles_unit = (need + kBN - 1) / kBN;
   if constexpr (kExt) {
-    it.sink_tiles = INT32_MAX;
+    it.sg = kNoSkip;
     it.skip = 0;
-    it.first = 0;
-    it.end = need;
+    it.first = it.all_lo = 0;
+    it.end = (int)need;
+    const int64_t base = it.ctx - p.L;
+    const int64_t hi = p.causal && it.l_first + base < it.ctx_limit - 1 ? it.l_first + base : it.ctx_limit - 1;
+    it.all_hi = hi < -1 ? -1 : (int)hi;
     if (p.window > 0) {
-      it.first = it.l_first + it.ctx - p.L - p.window + 1;
-      const int64_t st = (p.sinks + kBN - 1) / kBN;
-      if (it.first > 0 && it.first / kBN > st && st < n_tiles_unit) {
-        it.sink_tiles = (int)st;
-        it.skip = (int)(it.first / kBN - st);
-        n_tiles_unit = n_tiles_unit - it.skip > st ? n_tiles_unit - it.skip : st;
+      const int64_t first = it.l_first + base - p.window + 1, all_lo = l_last + base - p.window + 1;
+      it.first = first > 0 ? (int)first : 0;
+      it.all_lo = all_lo > 0 ? (int)all_lo : 0;
+      const int sg = (int)((p.sinks + 15) >> 4), n_groups = (it.end + 15) >> 4;
+      if ((it.first >> 4) > sg && sg < n_groups) {
+        it.sg = sg;
+        it.skip = (it.first >> 4) - sg;
+        const int left = n_groups - it.skip > sg ? n_groups - it.skip : sg;
+        n_tiles_unit = (left + 3) >> 2;
       }
     }
   }
@@ -196,6 +212,14 @@ __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) 
   return it;
 }
 
+// Dense K and V in boxes of one 16-key group, for the tile that joins sinks and window.
+template <bool kExt>
+struct ExtMaps {};
+template <>
+struct ExtMaps<true> {
+  CUtensorMap k16, v16;
+};
+
 // Persistent: each CTA loops over work items (fetched from a counter in the workspace
 // when there is one, else blockIdx.x + k * gridDim.x).  Rings and mbarrier phases run on
 // per-CTA tile counters, so the next item's Q load, K/V loads and first S overlap the
@@ -204,7 +228,7 @@ template <typename T, bool kExt>
 __global__ void __launch_bounds__(kThreads, 2)
     flash_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
-                       const Sm100Params p) {
+                       const __grid_constant__ ExtMaps<kExt> em, const Sm100Params p) {
   constexpr bool kSplit = std::is_same<T, __nv_bfloat16>::value;  // bf16 P = hi + lo
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {  // 128B-swizzled tiles need a 1024-byte aligned base
@@ -298,6 +322,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kPagesPerTile = kBN / 16;  // 16-token groups; paged without kExt: page_size == 16
   const uint32_t gpp = kExt ? (uint32_t)(p.ps >> 4) : 1u;  // groups per page
 
+  // does a tile hold sinks and window keys that are not next to one another
+  auto joins = [&](const Item& it, int vt) { return (it.sg >> 2) == vt && (it.sg & 3) != 0; };
   // consumers of the item ring: slot k & 3 of the k-th published item
   auto read_item = [&](int k, bool arrive) -> int64_t {
     if (!warp_wait(&item_full[k & 3], (k >> 2) & 1)) return -2;
@@ -386,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto load_ids = [&](int blk) -> int {
         int pidx = (int)(it.t_begin * kPagesPerTile) + blk * 32 + lane;
         if constexpr (kExt) {
-          const uint32_t group = (uint32_t)tile_of<true>(it, pidx / kPagesPerTile) * kPagesPerTile + (pidx % kPagesPerTile);
-          pidx = (int)(group / gpp);
+          pidx = group_of(it, pidx);
+          if (gpp != 1) pidx = (int)((uint32_t)pidx / gpp);
         }
         const int id = pidx < (int)p.mp ? bt_row[pidx] : -1;
         return (id < 0 || id >= (int)p.P) ? (int)p.P : id;
@@ -406,8 +432,19 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto issue = [&](const CUtensorMap* tm, uint8_t* dst, uint64_t* full, int t, const int* pid) {
         if (leader) {
           mbar_arrive_expect_tx(full, kTileBytes);
-          if (p.dense) {
-            const int key0 = (int)(tile_of<kExt>(it, it.t_begin + t) * kBN);
+          if (kExt && p.dense && joins(it, (int)it.t_begin + t)) {
+            if constexpr (kExt) {
+              const CUtensorMap* tm16 = tm == &tm_k ? &em.k16 : &em.v16;
+#pragma unroll
+              for (int g = 0; g < kPagesPerTile; ++g) {
+                const int key0 = group_of(it, ((int)it.t_begin + t) * kPagesPerTile + g) * 16;
+                tma_load_4d(dst + g * 16 * 128, tm16, 0, key0, kvh_i, b_i, full);
+                tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm16, 64, key0, kvh_i, b_i, full);
+              }
+            }
+          } else if (p.dense) {
+            int key0 = (int)((it.t_begin + t) * kBN);
+            if constexpr (kExt) key0 = group_of(it, ((int)it.t_begin + t) * kPagesPerTile) * 16;
             tma_load_4d(dst, tm, 0, key0, kvh_i, b_i, full);
             tma_load_4d(dst + kBN * 128, tm, 64, key0, kvh_i, b_i, full);
           } else {
@@ -415,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int g = 0; g < kPagesPerTile; ++g) {
               int slot0 = 0;
               if constexpr (kExt) {
-                const uint32_t group = (uint32_t)tile_of<true>(it, it.t_begin + t) * kPagesPerTile + g;
-                slot0 = (int)(group % gpp) * 16;
+                if (gpp != 1)
+                  slot0 = (int)((uint32_t)group_of(it, ((int)it.t_begin + t) * kPagesPerTile + g) % gpp) * 16;
               }
               tma_load_4d(dst + g * 16 * 128, tm, 0, slot0, kvh_i, pid[g], full);
               tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm, 64, slot0, kvh_i, pid[g], full);
@@ -716,15 +753,32 @@ __global__ void __launch_bounds__(kThreads, 2)
       int64_t last_key = it.ctx_limit - 1;
       if (p.causal && lpos + it.ctx - p.L < last_key) last_key = lpos + it.ctx - p.L;
       if (!row_ok) last_key = -1;
-      const int64_t row_lo = kExt && p.window > 0 ? lpos + it.ctx - p.L - p.window + 1 : 0;  // its window's first key
+      // kExt, virtual tiles of this item: masks are needed in [lo_from, lo_to) and from hi_from
+      // on, zeroed V rows in [lo_from, z_to) and from z_from on
+      int lo_from = 0, lo_to = 0, z_to = 0, hi_from = 0, z_from = 0, row_lo = 0, row_last = 0, sinks = 0;
+      if constexpr (kExt) {
+        row_last = (int)last_key;
+        hi_from = vgroup_of(it, it.all_hi + 1) >> 2;
+        z_from = vgroup_of(it, it.end) >> 2;
+        if (p.window > 0) {
+          sinks = (int)(p.sinks < kExtKeys ? p.sinks : kExtKeys);
+          const int64_t lo = lpos + it.ctx - p.L - p.window + 1;
+          row_lo = lo > 0 ? (int)lo : 0;
+          lo_from = sinks >> 6;
+          if (it.all_lo > sinks) lo_to = (vgroup_of(it, it.all_lo - 1) >> 2) + 1;
+          if (it.first > sinks) z_to = (vgroup_of(it, it.first - 1) >> 2) + 1;
+        }
+      }
       // Paged: page ids two tiles ahead, lanes 0..3 hold page g = lane of a tile; the
       // hole test happens when the tile is processed, so the load latency is hidden.
       const int32_t* bt_row = p.dense ? nullptr : p.block_table + it.b * p.mp;
       auto load_pid = [&](int t) -> int {
         if (p.dense || lane >= kPagesPerTile || t >= n) return 0;
         int pidx = (int)(it.t_begin + t) * kPagesPerTile + lane;
-        if constexpr (kExt)
-          pidx = (int)(((uint32_t)tile_of<true>(it, it.t_begin + t) * kPagesPerTile + lane) / gpp);
+        if constexpr (kExt) {
+          pidx = group_of(it, pidx);
+          if (gpp != 1) pidx = (int)((uint32_t)pidx / gpp);
+        }
         return pidx < (int)p.mp ? bt_row[pidx] : -1;
       };
       int pid0 = load_pid(0), pid1 = load_pid(1);
@@ -744,38 +798,50 @@ __global__ void __launch_bounds__(kThreads, 2)
         pid0 = pid1;
         pid1 = load_pid(j + 2);
         tmem_wait_ld();
-        const int64_t key0 = tile_of<kExt>(it, it.t_begin + j) * kBN;
-        // Only tiles that cross some row's last visible key (the causal diagonal, the
-        // context end, rows past the unit) pay for the mask: one compare per score.
-        const int64_t vis64 = last_key - key0;  // in-tile index of the row's last visible key
-        if (__any_sync(0xffffffffu, vis64 < kBN - 1)) {
-          const int vis = vis64 < -1 ? -1 : (int)vis64;
+        if constexpr (kExt) {
+          const int vt = (int)it.t_begin + j;
+          if ((vt >= lo_from && vt < lo_to) || vt >= hi_from) {
+            // Columns below jc are keys b1 + c, the others b2 + c; the row sees key <= row_last
+            // that is a sink or inside its window.
+            const int b1 = vt * kBN, b2 = b1 + it.skip * 16;
+            const int jc0 = it.sg * 16 - b1, jc = jc0 < 0 ? 0 : jc0 > kBN ? kBN : jc0;
+            auto seen_from = [&](int base) -> uint64_t {
+              return cols_to(row_last - base) & (cols_to(sinks - 1 - base) | ~cols_to(row_lo - 1 - base));
+            };
+            const uint64_t below = cols_to(jc - 1);
+            const uint64_t seen = (seen_from(b1) & below) | (seen_from(b2) & ~below);
+            const uint32_t seen_lo = (uint32_t)seen, seen_hi = (uint32_t)(seen >> 32);
 #pragma unroll
-          for (int c = 0; c < kBN; ++c) sv[c] = c <= vis ? sv[c] : -INFINITY;
-        }
-        if constexpr (kExt) {  // keys in [sinks, row_lo): only tiles at a window's lower edge hold any
-          const int64_t lo64 = row_lo - key0, sk64 = p.sinks - key0;
-          if (__any_sync(0xffffffffu, p.window > 0 && lo64 > 0 && sk64 < kBN && sk64 < lo64)) {
-            const int lo = p.window > 0 && lo64 > 0 ? (lo64 < kBN ? (int)lo64 : kBN) : 0;
-            const int sk = sk64 > 0 ? (sk64 < kBN ? (int)sk64 : kBN) : 0;
+            for (int c = 0; c < 32; ++c) {
+              sv[c] = (seen_lo >> c) & 1u ? sv[c] : -INFINITY;
+              sv[32 + c] = (seen_hi >> c) & 1u ? sv[32 + c] : -INFINITY;
+            }
+            // V of the keys that no row of the tile sees becomes zero before the product reads it
+            // (their weight is zero, but 0 times a NaN or an infinity is not)
+            if (vt < z_to || vt >= z_from) {
+              const int vs = g % kVStages;
+              if (!warp_wait(&v_full[vs], (uint32_t)((g / kVStages) & 1))) {
+                ok = false;
+                break;
+              }
+              const int c = row & (kBN - 1), key = c < jc ? b1 + c : b2 + c;
+              if (key >= it.end || (key >= sinks && key < it.first)) {
+                uint4* d = reinterpret_cast<uint4*>(sV + vs * kTileBytes + (row / kBN) * (kBN * 128) + c * 128);
 #pragma unroll
-            for (int c = 0; c < kBN; ++c) sv[c] = c >= sk && c < lo ? -INFINITY : sv[c];
+                for (int x = 0; x < 8; ++x) d[x] = make_uint4(0u, 0u, 0u, 0u);
+              }
+              fence_async_smem();
+            }
           }
-          // V of the keys that no row of the tile sees becomes zero before the product reads it
-          // (their weight is zero, but 0 times a NaN or an infinity is not)
-          if (key0 + kBN > it.end || (p.window > 0 && key0 < it.first && key0 + kBN > p.sinks)) {
-            const int vs = g % kVStages;
-            if (!warp_wait(&v_full[vs], (uint32_t)((g / kVStages) & 1))) {
-              ok = false;
-              break;
-            }
-            const int64_t key = key0 + (row & (kBN - 1));
-            if (key >= it.end || (p.window > 0 && key >= p.sinks && key < it.first)) {
-              uint4* d = reinterpret_cast<uint4*>(sV + vs * kTileBytes + (row / kBN) * (kBN * 128) + (row & (kBN - 1)) * 128);
+        } else {
+          const int64_t key0 = (it.t_begin + j) * kBN;
+          // Only tiles that cross some row's last visible key (the causal diagonal, the
+          // context end, rows past the unit) pay for the mask: one compare per score.
+          const int64_t vis64 = last_key - key0;  // in-tile index of the row's last visible key
+          if (__any_sync(0xffffffffu, vis64 < kBN - 1)) {
+            const int vis = vis64 < -1 ? -1 : (int)vis64;
 #pragma unroll
-              for (int x = 0; x < 8; ++x) d[x] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_async_smem();
+            for (int c = 0; c < kBN; ++c) sv[c] = c <= vis ? sv[c] : -INFINITY;
           }
         }
         if (!p.dense) {  // holes: the 16-token groups of missing pages are masked
@@ -1178,7 +1244,7 @@ __global__ void __launch_bounds__(1024) sm100_plan_kernel(const Sm100Params p, i
 // One opt-in to the dynamic shared memory size per kernel instantiation and device.
 template <typename T, bool kExt>
 int launch_typed(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                 const CUtensorMap& to, const Sm100Params& p, cudaStream_t s) {
+                 const CUtensorMap& to, const ExtMaps<kExt>& em, const Sm100Params& p, cudaStream_t s) {
   static std::mutex mu;
   static uint64_t done = 0;
   int dev = 0;
@@ -1205,10 +1271,10 @@ int launch_typed(dim3 grid, const CUtensorMap& tq, const CUtensorMap& tk, const 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, flash_sm100_kernel<T, kExt>, tq, tk, tv, to, p),
+    return check_cuda(cudaLaunchKernelEx(&cfg, flash_sm100_kernel<T, kExt>, tq, tk, tv, to, em, p),
                       "paged_attention: sm100 kernel launch (cluster)");
   }
-  flash_sm100_kernel<T, kExt><<<grid, kThreads, kSmemBytes, s>>>(tq, tk, tv, to, p);
+  flash_sm100_kernel<T, kExt><<<grid, kThreads, kSmemBytes, s>>>(tq, tk, tv, to, em, p);
   return check_cuda(cudaGetLastError(), "flash_attention: sm100 kernel launch");
 }
 
@@ -1277,10 +1343,10 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
     // the sinks' tiles and those that the windows of one row tile touch (without the causal
     // limit every row sees on to the last key)
     const int64_t span = a.is_causal && a.L > kBM ? kBM : a.L;
-    const int64_t seen = (a.sinks + kBN - 1) / kBN + (a.window + span - 1 + kBN - 1) / kBN + 1;
-    if (seen < tiles_max) tiles_max = seen;
+    const int64_t groups = (a.sinks + 15) / 16 + (a.window + span - 1 + 15) / 16 + 1;
+    if ((groups + 3) / 4 < tiles_max) tiles_max = (groups + 3) / 4;
   }
-  if (tiles_max >= INT32_MAX / 2) return plan;
+  if (tiles_max >= INT32_MAX / 2 || (paged_is_ext(a) && keys >= kExtKeys)) return plan;
   plan.ct = tiles_max > 0 ? tiles_max : 1;
   plan.n_chunks = 1;
   // Split-K over keys for grouped paged calls (dense callers pass no workspace): aim at
@@ -1412,10 +1478,20 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   }
   const dim3 grid((unsigned)ctas);
   if (paged_is_ext(a)) {
-    if (a.kv_dtype == NVM_F16) return launch_typed<__half, true>(grid, tq, tk, tv, to, p, s);
-    return launch_typed<__nv_bfloat16, true>(grid, tq, tk, tv, to, p, s);
+    ExtMaps<true> em;
+    em.k16 = tk;
+    em.v16 = tv;
+    if (a.dense) {
+      const uint32_t kb16[4] = {64u, 16u, 1u, 1u};
+      st = encode_tmap(&em.k16, dt, 4, a.k_pages, kd, ks, kb16, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (st != NVM_OK) return st;
+      st = encode_tmap(&em.v16, dt, 4, a.v_pages, kd, ks, kb16, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (st != NVM_OK) return st;
+    }
+    if (a.kv_dtype == NVM_F16) return launch_typed<__half, true>(grid, tq, tk, tv, to, em, p, s);
+    return launch_typed<__nv_bfloat16, true>(grid, tq, tk, tv, to, em, p, s);
   }
-  if (a.kv_dtype == NVM_F16) return launch_typed<__half, false>(grid, tq, tk, tv, to, p, s);
-  return launch_typed<__nv_bfloat16, false>(grid, tq, tk, tv, to, p, s);
+  if (a.kv_dtype == NVM_F16) return launch_typed<__half, false>(grid, tq, tk, tv, to, ExtMaps<false>{}, p, s);
+  return launch_typed<__nv_bfloat16, false>(grid, tq, tk, tv, to, ExtMaps<false>{}, p, s);
 }
 }  // namespace nvm
