@@ -1339,6 +1339,7 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
   plan.rows_real = plan.M_rows < kBM ? plan.M_rows : kBM;
   const int64_t keys = a.dense ? a.page_size : a.max_pages * a.page_size;
   int64_t tiles_max = (keys + kBN - 1) / kBN;
+  plan.tiles_full = tiles_max;
   if (a.window > 0) {
     // the sinks' tiles and those that the windows of one row tile touch (without the causal
     // limit every row sees on to the last key)
@@ -1452,9 +1453,13 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   // per item (the hardware scheduler balances the heavy-first causal tiles), which lets
   // the epilogue stage O in shared memory for bulk tensor stores.
   int64_t ctas = p.n_items;
-  // (a bounded number of tiles leaves nothing to balance: no work list then)
+  // Windows that shorten the rows make items short and alike: persistent CTAs then hide each
+  // item's start and end behind the last one's tiles (2 x 4096 tokens under 1024 keys: 198 us
+  // against 226 us), and there is nothing for a work list to balance (a chunk of 512: 113 us
+  // against 119 us with it).
+  const bool short_items = a.window > 0 && plan.tiles_full > plan.ct * plan.n_chunks;
   const int64_t persistent =
-      plan.cluster ? 0 : env_int("NVM_SM100_PERSISTENT", plan.grouped && !(a.window > 0 && plan.n_chunks == 1) ? 1 : 0);
+      plan.cluster ? 0 : env_int("NVM_SM100_PERSISTENT", plan.grouped || short_items ? 1 : 0);
   p.cluster = plan.cluster;
   if (persistent != 0) {
     int dev = 0, sms = 148;
@@ -1464,7 +1469,7 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   p.stage_out = ctas == p.n_items ? 1 : 0;
   p.pv_wait = env_int("NVM_SM100_PV_WAIT", 1) != 0 ? 1 : 0;
   if (p.stage_out) p.work_counter = p.exit_counter = nullptr;  // one item per CTA: item = blockIdx.x
-  if (p.work_counter != nullptr && env_int("NVM_SM100_PLAN", 1) != 0) {
+  if (p.work_counter != nullptr && env_int("NVM_SM100_PLAN", short_items ? 0 : 1) != 0) {
     int* list = reinterpret_cast<int*>(static_cast<uint8_t*>(ws) + wo.list);
     int* count = p.work_counter - 1;
     p.item_list = list;

@@ -138,7 +138,8 @@ struct Sm100Plan {
   int grouped;
   int64_t M_rows, n_outer, n_row_tiles, n_units, rows_real, ct, n_chunks;
   size_t ws_bytes;
-  int cluster;  // the chunks of a unit merge inside a thread-block cluster
+  int cluster;         // the chunks of a unit merge inside a thread-block cluster
+  int64_t tiles_full;  // 64-key tiles of the longest context without a window
 };
 // sizing_only: plan from shapes alone (q dtype, pointers and scale unknown), for
 // nvm_paged_attention_workspace_size.
