@@ -212,7 +212,9 @@ __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) 
   return it;
 }
 
-// Dense K and V in boxes of one 16-key group, for the tile that joins sinks and window.
+// Boxes of one 16-key group: dense K and V [B, Hkv, S, D], for the tile that joins sinks and
+// window; pools as rows [P * Hkv * page_size, D], so that one number per group says where it is
+// (page, head and slot as three coordinates cost the issuing thread 9 % of a prompt).
 template <bool kExt>
 struct ExtMaps {};
 template <>
@@ -320,7 +322,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tO = tmem + 2 * kBN;
   constexpr int kPagesPerTile = kBN / 16;  // 16-token groups; paged without kExt: page_size == 16
-  const uint32_t gpp = kExt ? (uint32_t)(p.ps >> 4) : 1u;  // groups per page
+  // groups per page; a division when it is no power of two
+  const uint32_t gpp = kExt ? (uint32_t)(p.ps >> 4) : 1u;
+  const int gpp_shift = kExt && (gpp & (gpp - 1)) == 0 ? __popc(gpp - 1) : -1;
+  auto page_of = [&](int group) -> int {
+    return gpp_shift >= 0 ? group >> gpp_shift : (int)((uint32_t)group / gpp);
+  };
 
   // does a tile hold sinks and window keys that are not next to one another
   auto joins = [&](const Item& it, int vt) { return (it.sg >> 2) == vt && (it.sg & 3) != 0; };
@@ -412,8 +419,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto load_ids = [&](int blk) -> int {
         int pidx = (int)(it.t_begin * kPagesPerTile) + blk * 32 + lane;
         if constexpr (kExt) {
-          pidx = group_of(it, pidx);
-          if (gpp != 1) pidx = (int)((uint32_t)pidx / gpp);
+          // the row of the group's first token in the pool seen as [P * Hkv * page_size, D]
+          const int group = group_of(it, pidx), page = page_of(group);
+          const int pid = page < (int)p.mp ? bt_row[page] : -1;
+          if (pid < 0 || pid >= (int)p.P) return (int)(p.P * p.Hkv * p.ps);
+          return (pid * (int)p.Hkv + (int)it.kvh) * (int)p.ps + (group - page * (int)gpp) * 16;
         }
         const int id = pidx < (int)p.mp ? bt_row[pidx] : -1;
         return (id < 0 || id >= (int)p.P) ? (int)p.P : id;
@@ -450,13 +460,14 @@ __global__ void __launch_bounds__(kThreads, 2)
           } else {
 #pragma unroll
             for (int g = 0; g < kPagesPerTile; ++g) {
-              int slot0 = 0;
               if constexpr (kExt) {
-                if (gpp != 1)
-                  slot0 = (int)((uint32_t)group_of(it, ((int)it.t_begin + t) * kPagesPerTile + g) % gpp) * 16;
+                const CUtensorMap* tm16 = tm == &tm_k ? &em.k16 : &em.v16;
+                tma_load_2d(dst + g * 16 * 128, tm16, 0, pid[g], full);
+                tma_load_2d(dst + kBN * 128 + g * 16 * 128, tm16, 64, pid[g], full);
+              } else {
+                tma_load_4d(dst + g * 16 * 128, tm, 0, 0, kvh_i, pid[g], full);
+                tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm, 64, 0, kvh_i, pid[g], full);
               }
-              tma_load_4d(dst + g * 16 * 128, tm, 0, slot0, kvh_i, pid[g], full);
-              tma_load_4d(dst + kBN * 128 + g * 16 * 128, tm, 64, slot0, kvh_i, pid[g], full);
             }
           }
         }
@@ -776,8 +787,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (p.dense || lane >= kPagesPerTile || t >= n) return 0;
         int pidx = (int)(it.t_begin + t) * kPagesPerTile + lane;
         if constexpr (kExt) {
-          pidx = group_of(it, pidx);
-          if (gpp != 1) pidx = (int)((uint32_t)pidx / gpp);
+          pidx = page_of(group_of(it, pidx));
         }
         return pidx < (int)p.mp ? bt_row[pidx] : -1;
       };
@@ -1348,6 +1358,8 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
     if ((groups + 3) / 4 < tiles_max) tiles_max = (groups + 3) / 4;
   }
   if (tiles_max >= INT32_MAX / 2 || (paged_is_ext(a) && keys >= kExtKeys)) return plan;
+  // paged kExt loads name a row of the pool in 32 bits
+  if (paged_is_ext(a) && !a.dense && a.P * a.Hkv * a.page_size > INT32_MAX - 64) return plan;
   plan.ct = tiles_max > 0 ? tiles_max : 1;
   plan.n_chunks = 1;
   // Split-K over keys for grouped paged calls (dense callers pass no workspace): aim at
@@ -1491,6 +1503,13 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
       st = encode_tmap(&em.k16, dt, 4, a.k_pages, kd, ks, kb16, CU_TENSOR_MAP_SWIZZLE_128B);
       if (st != NVM_OK) return st;
       st = encode_tmap(&em.v16, dt, 4, a.v_pages, kd, ks, kb16, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (st != NVM_OK) return st;
+    } else {
+      const uint64_t rd[2] = {(uint64_t)kD, (uint64_t)(a.P * a.Hkv * a.page_size)}, rs[1] = {kD * 2};
+      const uint32_t rb[2] = {64u, 16u};
+      st = encode_tmap(&em.k16, dt, 2, a.k_pages, rd, rs, rb, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (st != NVM_OK) return st;
+      st = encode_tmap(&em.v16, dt, 2, a.v_pages, rd, rs, rb, CU_TENSOR_MAP_SWIZZLE_128B);
       if (st != NVM_OK) return st;
     }
     if (a.kv_dtype == NVM_F16) return launch_typed<__half, true>(grid, tq, tk, tv, to, em, p, s);
