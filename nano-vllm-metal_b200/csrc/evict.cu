@@ -9,8 +9,8 @@
 //
 // Two kernels.  evict_select: a CTA per (request, kv head) reads the weights once into
 // registers (up to 32 a thread; longer rows re-read them from L2), finds the k-th largest by
-// radix selection on an order-preserving 32-bit image (four 8-bit digits, shared-memory
-// histograms scanned by one warp), numbers the kept positions with one scan over ballot
+// radix selection on an order-preserving 32-bit image (digits of 11, 11 and 10 bits,
+// shared-memory histograms), numbers the kept positions with one scan over ballot
 // counts in position order, and moves the weights.  evict_compact: a CTA per (request, kv
 // head, column slice of K or V).  Slot i receives token keep[i] >= i, so a tile of slots that
 // is read completely before it is written never overwrites a row that a later tile reads
@@ -64,14 +64,19 @@ __device__ __forceinline__ int cta_exclusive_scan(int v, int* wsum, int* total) 
 }
 
 constexpr int kPer = 32;  // weights a thread holds in registers
+// Digits of 11, 11 and 10 bits: the first one holds the exponent and two bits of the mantissa.
+// With 8-bit digits a row's weights fall into a handful of first bins and their atomics
+// serialise (512 rows of 5000: 42 us against 35 us).
+constexpr int kBins = 2048;
 
 template <int T>
 struct SelSmem {
-  int hist[256];
-  int cnt[T];             // kept per (stretch, warp) of one sweep
+  int hist[kBins];
+  int cnt[T];  // kept per (stretch, warp) of one sweep
   int wsum[32];
-  int bad, digit, rank;
+  int bad, digit, rank, count;
 };
+static_assert(kBins % 1024 == 0, "every thread clears and scans whole bins");
 
 // Keeps, of positions [0, n): [0, lo), [hi, n) and the k of [lo, hi) with the largest weight;
 // writes their positions and weights in order.  kHeld: the weights fit in registers.
@@ -99,41 +104,41 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
     }
   };
   uint32_t prefix = 0;
-  int rank = k;  // how many weights equal to the threshold are kept
+  int rank = k;         // how many weights equal to the threshold are kept ..
+  bool all_eq = true;   // .. all of them
   if (k > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (t < 256) sm.hist[t] = 0;
+    constexpr int kBinsPer = kBins / T;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;  // 11, 11 and 10 bits
+      const uint32_t digits = pass == 2 ? 1023u : 2047u;
+#pragma unroll
+      for (int x = 0; x < kBinsPer; ++x) sm.hist[t + x * T] = 0;
       __syncthreads();
       each([&](int i, float x) {
         const uint32_t key = weight_key(x);
-        if (i >= lo && i < hi && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))))
-          atomicAdd(&sm.hist[(key >> shift) & 255], 1);
+        const bool in = pass == 0 || (key >> (shift + 11 - (pass == 2))) == (prefix >> (shift + 11 - (pass == 2)));
+        if (i >= lo && i < hi && in) atomicAdd(&sm.hist[(key >> shift) & digits], 1);
       });
       __syncthreads();
-      if (warp == 0) {  // lane: digits 255 - 8 lane .. 248 - 8 lane, counted from the top
-        int c[8], sum = 0;
+      // thread t: digits kBins - 1 - kBinsPer t, downwards
+      int c[kBinsPer], sum = 0, total;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sum += c[x] = sm.hist[255 - 8 * lane - x];
-        int incl = sum;
+      for (int x = 0; x < kBinsPer; ++x) sum += c[x] = sm.hist[kBins - 1 - kBinsPer * t - x];
+      int above = cta_exclusive_scan<T>(sum, sm.wsum, &total);  // weights with a larger digit
+      if (above < rank && rank <= above + sum) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        int above = incl - sum;  // weights with a larger digit than this lane's
-        if (above < rank && rank <= incl) {
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            if (above < rank && rank <= above + c[x]) {
-              sm.digit = 255 - 8 * lane - x;
-              sm.rank = rank - above;
-            }
-            above += c[x];
+        for (int x = 0; x < kBinsPer; ++x) {
+          if (above < rank && rank <= above + c[x]) {
+            sm.digit = kBins - 1 - kBinsPer * t - x;
+            sm.rank = rank - above;
+            sm.count = c[x];
           }
+          above += c[x];
         }
       }
       __syncthreads();
       rank = sm.rank;
+      all_eq = rank == sm.count;
       prefix |= (uint32_t)sm.digit << shift;
     }
   }
@@ -152,7 +157,7 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
           take |= 1u << j;
         } else if (k > 0) {
           const uint32_t key = weight_key(w[j]);
-          if (key > prefix) take |= 1u << j;
+          if (key > prefix || (all_eq && key == prefix)) take |= 1u << j;
           if (key == prefix) eqs |= 1u << j;
         }
       }
@@ -180,7 +185,7 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
       }
       __syncthreads();
     };
-    if (k > 0) {
+    if (!all_eq) {
       int total;
       number(eqs, &total, [&](int j, int at) {
         if (eq_seen + at < rank) take |= 1u << j;
@@ -334,13 +339,14 @@ int launch_evict(const EvictArgs& a, cudaStream_t s) {
   ep.page_shift = -1;
   for (int x = 0; x < 31; ++x)
     if (a.page_size == int64_t(1) << x) ep.page_shift = x;
-  // Threads of a selection: the longest row that the sizes allow in registers, 32 weights a
-  // thread, but all 1024 when there are fewer rows than SMs anyway.  A CTA of 1024 fills an
-  // SM's registers: 512 rows of 5000 took 72 us in CTAs of 1024 and 42 us in CTAs of 256.
+  // Threads of a selection: enough to hold the longest row that the sizes allow, 32 weights a
+  // thread; with no more rows than SMs, 8 a thread.  A CTA of 1024 fills an SM's registers:
+  // 512 rows of 5000 took 72 us in CTAs of 1024 and 42 us in CTAs of 256 (8-bit digits).
   const dim3 sel((unsigned)(a.B * a.Hkv));
   const int64_t cap = a.len < a.max_pages * a.page_size ? a.len : a.max_pages * a.page_size;
-  if (cap > 512 * kPer || a.B * a.Hkv <= 148) evict_select_kernel<1024><<<sel, 1024, 0, s>>>(ep);
-  else if (cap > 256 * kPer) evict_select_kernel<512><<<sel, 512, 0, s>>>(ep);
+  const int64_t per = a.B * a.Hkv <= 148 ? 8 : kPer;
+  if (cap > 512 * per) evict_select_kernel<1024><<<sel, 1024, 0, s>>>(ep);
+  else if (cap > 256 * per) evict_select_kernel<512><<<sel, 512, 0, s>>>(ep);
   else evict_select_kernel<256><<<sel, 256, 0, s>>>(ep);
   int st = check_cuda(cudaGetLastError(), "evict: selection kernel launch");
   if (st != NVM_OK) return st;
