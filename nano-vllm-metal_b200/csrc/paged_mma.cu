@@ -225,7 +225,10 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
         if (nc > nc_max) nc = nc_max;
         if (nc < 1) nc = 1;
         int64_t ct1 = (tiles_max + nc - 1) / nc;
-        if (ct1 < 16) ct1 = 16;
+        // Windowed / scored calls with few units: up to eight chunks, one cluster, down to four
+        // tiles each (8 units of 35 tiles: seven chunks of 5 against three of 16).
+        const int64_t least = ext && tiles_max <= 128 ? (tiles_max > 32 ? (tiles_max + 7) / 8 : 4) : 16;
+        if (ct1 < least) ct1 = least;
         if (ct1 <= kOneWaveTiles) {
           ct = ct1;
           one_wave = true;

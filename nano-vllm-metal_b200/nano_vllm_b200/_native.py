@@ -111,8 +111,8 @@ def require_cuda(op: str, *tensors: torch.Tensor) -> torch.device:
         if not t.is_cuda:
             raise RuntimeError(f"{op}: tensors must be on a CUDA device (libnvm_attn has no CPU path)")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, t.get_device()
+        elif t.get_device() != index:
             raise RuntimeError(f"{op}: all tensors must be on the same CUDA device")
     if dev is None:
         raise RuntimeError(f"{op}: no tensor given")

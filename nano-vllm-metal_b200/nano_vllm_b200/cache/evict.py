@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _native as nv
-from ..layers.attention import _check_rows
+from ..layers.attention import _int32_rows, _row_strides
 
 __all__ = ["EvictResult", "evict_tokens"]
 
@@ -50,6 +50,7 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     too and is never cleared.
     """
     op = "evict"
+    out = key_mass if mass_out is None else mass_out
     dev = nv.require_cuda(op, key_pages, value_pages, block_table, context_lens, key_mass, key_scales, value_scales,
                           page_refcount, mass_out, status)
     if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != value_pages.dtype:
@@ -59,18 +60,19 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     P, Hkv, ps, D = key_pages.shape
     if block_table.dim() != 2 or context_lens.dim() != 1 or block_table.shape[0] != context_lens.shape[0]:
         raise RuntimeError(f"{op}: block_table must be [B, max_pages] and context_lens [B]")
-    B = block_table.shape[0]
+    B, MP = block_table.shape
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise RuntimeError(f"{op}: need budget >= 1, sinks >= 0, recent >= 0 and sinks + recent <= budget")
-    out = key_mass if mass_out is None else mass_out
-    for name, x in (("key_mass", key_mass), ("mass_out", out)):
-        if x.dim() != 3 or tuple(x.shape[:2]) != (B, Hkv) or x.dtype != torch.float32:
-            raise RuntimeError(f"{op}: {name} must be float32 [B, Hkv, S]")
-        _check_rows(f"{op}: {name}", x)
-    if out.shape != key_mass.shape:
-        raise RuntimeError(f"{op}: mass_out must have the shape of key_mass")
+    if key_mass.dim() != 3 or key_mass.shape[0] != B or key_mass.shape[1] != Hkv or key_mass.dtype is not torch.float32:
+        raise RuntimeError(f"{op}: key_mass must be float32 [B, Hkv, S]")
+    msb, msh = _row_strides(f"{op}: key_mass", key_mass)
+    osb, osh = msb, msh
+    if mass_out is not None:
+        if mass_out.shape != key_mass.shape or mass_out.dtype is not torch.float32:
+            raise RuntimeError(f"{op}: mass_out must be float32 with the shape of key_mass")
+        osb, osh = _row_strides(f"{op}: mass_out", mass_out)
     sdt = nv.NVM_F16
-    if key_pages.dtype == torch.int8:
+    if key_pages.dtype is torch.int8:
         if key_scales is None or value_scales is None:
             raise RuntimeError(f"{op}: int8 pages need key_scales and value_scales")
         for s in (key_scales, value_scales):
@@ -84,15 +86,13 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
         raise RuntimeError(f"{op}: page_refcount must be contiguous int32 with an entry per page")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise RuntimeError(f"{op}: status must be one int32")
-    bt = block_table.to(torch.int32).contiguous()
-    cl = context_lens.to(torch.int32).contiguous()
+    bt, cl = _int32_rows(block_table), _int32_rows(context_lens)
     keep = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
     kept, dropped, refused = torch.empty((3, B), dtype=torch.int32, device=dev).unbind(0)
     with nv.on_device(dev):
         nv.check(nv.lib().nvm_paged_evict(
             key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(key_scales),
-            nv.ptr(value_scales), sdt, bt.data_ptr(), cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(),
-            key_mass.stride(0), key_mass.stride(1), key_mass.shape[2], out.data_ptr(), out.stride(0), out.stride(1), B,
-            Hkv, D, P, ps, bt.shape[1], budget, sinks, recent, keep.data_ptr(), kept.data_ptr(), dropped.data_ptr(),
-            refused.data_ptr(), nv.ptr(status), nv.stream_ptr(dev)))
+            nv.ptr(value_scales), sdt, bt.data_ptr(), cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(), msb, msh,
+            key_mass.shape[2], out.data_ptr(), osb, osh, B, Hkv, D, P, ps, MP, budget, sinks, recent, keep.data_ptr(),
+            kept.data_ptr(), dropped.data_ptr(), refused.data_ptr(), nv.ptr(status), nv.stream_ptr(dev)))
     return EvictResult(keep, kept, dropped, refused)

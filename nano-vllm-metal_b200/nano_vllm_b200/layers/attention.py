@@ -42,17 +42,21 @@ def _check_window(op: str, window: int | None, sinks: int) -> None:
         raise RuntimeError(f"{op}: sinks must not be negative, got {sinks}")
 
 
-def _check_rows(what: str, x: torch.Tensor) -> None:
-    """x [B, H, S]: rows contiguous along S that do not overlap one another."""
+def _row_strides(what: str, x: torch.Tensor) -> tuple[int, int]:
+    """The first two strides of x [B, H, S], whose rows must be contiguous along S and must not
+    overlap one another."""
     B, H, S = x.shape
+    if x.is_contiguous():
+        return H * S, S
     sb, sh, ss = x.stride()
     ok = S <= 1 or ss == 1
     if H > 1:
         ok = ok and sh >= S
     if B > 1:
-        ok = ok and (sb >= (H - 1) * sh + S or (H > 1 and sh >= (B - 1) * sb + S and sb >= S) or (H == 1 and sb >= S))
+        ok = ok and (sb >= (H - 1) * sh + S or (H > 1 and sh >= (B - 1) * sb + S and sb >= S))
     if not ok:
         raise RuntimeError(f"{what} must be contiguous along its last axis, its rows apart from one another")
+    return sb, sh
 
 
 def causal_mask(L: int, S: int, dtype: torch.dtype = torch.float32, device=None) -> torch.Tensor:
@@ -145,6 +149,75 @@ def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     return out
 
 
+def _int32_rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
+def _paged_attention_window(query, key_pages, value_pages, block_table, context_lens, page_size, key_scales, value_scales,
+                            scale, mask, out_dtype, out, window, sinks, key_mass):
+    """paged_attention with a window or key scores."""
+    op = "paged_attention"
+    _check_window(op, window, sinks)
+    if isinstance(mask, torch.Tensor):
+        raise NotImplementedError("Paged attention only supports mask=None or causal")
+    if mask is not None and mask != "causal":
+        raise NotImplementedError
+    B, Hq, L, D = query.shape
+    P, Hkv, ps, pd = key_pages.shape
+    assert Hq % Hkv == 0
+    dev = nv.require_cuda(op, query, key_pages, value_pages, block_table, context_lens, key_scales, value_scales, key_mass,
+                          out)
+    if key_pages.dtype != value_pages.dtype:
+        raise RuntimeError(f"{op}: key_pages and value_pages must have the same dtype")
+    if key_pages.shape != value_pages.shape:
+        raise RuntimeError(f"{op}: key_pages and value_pages must have the same shape")
+    if pd != D:
+        raise RuntimeError(f"{op}: q and page tensors must have the same head dimension")
+    if ps != page_size:
+        raise RuntimeError(f"{op}: pages must be [P, Hkv, page_size, D]")
+    if block_table.dim() != 2 or context_lens.dim() != 1:
+        raise RuntimeError(f"{op}: block_table must be 2D and context_lens must be 1D")
+    MP = block_table.shape[1]
+    if block_table.shape[0] != B or context_lens.shape[0] != B:
+        raise RuntimeError(f"{op}: q batch size must match block_table batch size")
+    q, kp, vp = query.contiguous(), key_pages.contiguous(), value_pages.contiguous()
+    bt, cl = _int32_rows(block_table), _int32_rows(context_lens)
+    ks = vs = None
+    sdt = nv.NVM_F16
+    if kp.dtype is torch.int8:
+        assert key_scales is not None
+        assert value_scales is not None
+        ks, vs = key_scales.contiguous(), value_scales.contiguous()
+        if tuple(ks.shape) != (P, Hkv, ps, 1) or vs.shape != ks.shape:
+            raise RuntimeError(f"{op}: scales must be [P, Hkv, page_size, 1]")
+        if ks.dtype != vs.dtype:
+            vs = vs.to(ks.dtype)
+        sdt = nv.dtype_code(ks.dtype)
+    mp, msb, msh, ml = None, 0, 0, 0
+    if key_mass is not None:
+        if key_mass.dim() != 3 or key_mass.shape[0] != B or key_mass.shape[1] != Hkv or key_mass.dtype is not torch.float32:
+            raise RuntimeError(f"{op}: key_mass must be float32 [B, Hkv, S]")
+        msb, msh = _row_strides(f"{op}: key_mass", key_mass)
+        mp, ml = key_mass.data_ptr(), key_mass.shape[2]
+    if out is None:
+        out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != (B, Hq, L, D) or not out.is_contiguous():
+        raise RuntimeError(f"{op}: out must be a contiguous [B, Hq, L, D] tensor")
+    factor = scale if scale is not None else 1.0 / (D ** 0.5)
+    lib = nv.lib()
+    kvc = nv.dtype_code(kp.dtype)
+    with nv.on_device(dev):
+        nv.call_with_workspace(
+            dev,
+            lambda: lib.nvm_paged_attention_window_workspace_size(B, Hq, Hkv, L, D, ps, MP, kvc, window or 0, sinks,
+                                                                  int(mp is not None)),
+            lambda ws, ws_bytes, stream: lib.nvm_paged_attention_window(
+                q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
+                bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps, MP,
+                factor, mask == "causal", window or 0, sinks, mp, msb, msh, ml, ws, ws_bytes, stream))
+    return out
+
+
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
                     block_table: torch.Tensor, context_lens: torch.Tensor, page_size: int,
                     key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
@@ -166,7 +239,9 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     so the buffer needs no clearing between requests; keys at or past S gain nothing.  A row
     that sees no key is zero, and a key that no row sees has no influence whatever it holds.
     """
-    _check_window("paged_attention", window, sinks)
+    if window is not None or key_mass is not None or sinks != 0:
+        return _paged_attention_window(query, key_pages, value_pages, block_table, context_lens, page_size, key_scales,
+                                       value_scales, scale, mask, out_dtype, out, window, sinks, key_mass)
     if isinstance(mask, torch.Tensor):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
     if mask is not None and mask != "causal":
@@ -206,30 +281,6 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
     L_ = nv.lib()
     kvc = nv.dtype_code(kp.dtype)
-    if window is not None or key_mass is not None:
-        if tuple(out.shape) != (B, Hq, L, D) or not out.is_contiguous() or out.device != dev:
-            raise RuntimeError("paged_attention: out must be a contiguous [B, Hq, L, D] tensor on the query's device")
-        if ps != page_size or (ks is not None and not tuple(ks.shape) == tuple(vs.shape) == (P, Hkv, ps, 1)):
-            raise RuntimeError("paged_attention: pages must be [P, Hkv, page_size, D] and scales [P, Hkv, page_size, 1]")
-        ms = (0, 0, 0)
-        if key_mass is not None:
-            nv.require_cuda("paged_attention", query, key_mass)
-            if key_mass.dim() != 3 or tuple(key_mass.shape[:2]) != (B, Hkv) or key_mass.dtype != torch.float32:
-                raise RuntimeError("paged_attention: key_mass must be float32 [B, Hkv, S]")
-            ms = (*key_mass.stride()[:2], key_mass.shape[2])
-            _check_rows("paged_attention: key_mass", key_mass)
-        w = window or 0
-        MP = bt.shape[1]
-        with nv.on_device(dev):
-            nv.call_with_workspace(
-                dev,
-                lambda: L_.nvm_paged_attention_window_workspace_size(B, Hq, Hkv, L, D, ps, MP, kvc, w, sinks,
-                                                                     int(key_mass is not None)),
-                lambda ws, ws_bytes, stream: L_.nvm_paged_attention_window(
-                    q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
-                    bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps, MP,
-                    factor, mask == "causal", w, sinks, nv.ptr(key_mass), *ms, ws, ws_bytes, stream))
-        return out
     ws_bytes = L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc)
     ws = nv.workspace(dev, ws_bytes)
     with torch.cuda.device(dev):
