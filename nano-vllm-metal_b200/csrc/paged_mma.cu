@@ -184,6 +184,8 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   if (dense) keys = a.page_size;
   int64_t tiles_max = (keys + 15) / 16;
   const bool ext = paged_is_ext(a);
+  // the windowed kernel counts keys and pool rows in 32 bits
+  if (ext && (keys >= (int64_t(1) << 30) || a.P * a.Hkv * a.page_size > INT32_MAX - 64)) return plan;
   if (a.window > 0) {
     // the sinks' tiles and those that the windows of L tokens touch
     const int64_t seen = (a.sinks + 15) / 16 + (a.window + a.L - 1 + 15) / 16 + 1;

@@ -27,7 +27,10 @@
 //    position pos sees key s only if s < sinks or s > pos - window.  The key tiles between
 //    the sinks and the row block's windows are jumped over by renumbering: virtual tile v is
 //    tile v below the sinks' last tile and tile v + skip past it, so chunks, rings and merges
-//    run on virtual tiles unchanged.  They can leave every row's log-sum-exp.
+//    run on virtual tiles unchanged.  They can leave every row's log-sum-exp.  Their keys are
+//    counted in 32 bits, and a tile is named by one row of the pool seen as [P * Hkv *
+//    page_size, D], worked out with the page ids, so that the warp that copies a tile between
+//    two of its own spends few instructions on it.
 //  * Every mbarrier wait is bounded (nvm::mbar_wait); on expiry the kernel records an
 //    error code, each issuing warp drains what it issued, and the CTA returns.
 #pragma once
@@ -70,6 +73,8 @@ struct MmaParams {
   int cluster;        // the n_chunks CTAs of a unit are one cluster: merge over DSMEM
   int64_t window, sinks;  // kExt: window == 0 for none
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
+  const void* k_scales;   // kExt: int8 pages' scales, copied by row
+  const void* v_scales;
   float* scores;          // kExt, n8: keep every score ([units][n_chunks * ct * 16][rows, even]), or null
 };
 
@@ -138,6 +143,17 @@ __device__ __forceinline__ uint32_t swz(uint32_t tile, int tok, int q) {
   return tile + (uint32_t)((q >> 3) * 2048 + tok * 128 + (((q & 7) ^ (tok & 7)) << 4));
 }
 
+constexpr int64_t kExtLimit = int64_t(1) << 30;  // keys of a kExt call; larger windows and sinks count as this
+
+// Untiled bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into this CTA's
+// shared memory, completing on an mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 template <typename KvT, typename ScaleT, int D, int NWM, int NWK, int NS_, bool kExt>
 __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -145,6 +161,7 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
                      const MmaParams p) {
   using C = Cfg<KvT, D, NWM, NWK, NS_>;
   using MmaT = typename C::MmaT;
+  using Tok = typename std::conditional<kExt, int, int64_t>::type;  // key positions
   constexpr int NS = C::kStages;
   constexpr int NKS = D / 16;  // k-steps of Q K^T
   constexpr int NDT = D / 8;   // n8 tiles of the output
@@ -250,37 +267,40 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     kbias1 = 1152.f * __shfl_sync(0xffffffffu, qs, 4 * (2 * cq + 1));
   }
   // kExt: the row block's tiles, renumbered without the ones no row sees
-  int64_t x_tiles = 0, x_sink_tiles = 0, x_skip = 0, x_first = 0;
-  int64_t x_end = 0;  // keys at or past it are seen by no row of the block
+  int x_tiles = 0, x_sink_tiles = 0, x_skip = 0;
+  int x_first = 0, x_end = 0, x_sinks = 0;  // keys in [x_sinks, x_first) and from x_end on: seen by no row
   if constexpr (kExt) {
     const bool spans = rows_here >= p.L || (int64_t)((uint32_t)row0 % (uint32_t)p.L) + rows_here > p.L;
-    x_end = ctx_limit;
+    int64_t end = ctx_limit;
     if (p.causal) {
       const int64_t lmax = spans ? p.L - 1 : (int64_t)((uint32_t)(row0 + rows_here - 1) % (uint32_t)p.L);
       const int64_t lim = lmax + ctx - p.L + 1;
-      if (lim < x_end) x_end = lim;
+      if (lim < end) end = lim;
     }
-    if (ctx <= 0 || x_end < 0) x_end = 0;
-    x_tiles = (x_end + 15) / 16;
+    x_end = ctx <= 0 || end < 0 ? 0 : (int)end;
+    x_tiles = (x_end + 15) >> 4;
     x_sink_tiles = x_tiles;
     if (p.window > 0) {
       const int64_t lmin = spans ? 0 : (int64_t)((uint32_t)row0 % (uint32_t)p.L);
-      x_first = lmin + ctx - p.L - p.window + 1;  // no row's window reaches below this key
-      const int64_t st = (p.sinks + 15) / 16;
-      if (x_first > 0 && x_first / 16 > st && st < x_tiles) {
+      const int64_t first = lmin + ctx - p.L - p.window + 1;  // no row's window reaches below this key
+      x_first = first > 0 ? (int)first : 0;
+      x_sinks = (int)(p.sinks < kExtLimit ? p.sinks : kExtLimit);
+      const int st = (x_sinks + 15) >> 4;
+      if ((x_first >> 4) > st && st < x_tiles) {
         x_sink_tiles = st;
-        x_skip = x_first / 16 - st;
+        x_skip = (x_first >> 4) - st;
         x_tiles = x_tiles - x_skip > st ? x_tiles - x_skip : st;
       }
     }
   }
-  auto tile_of = [&](int64_t v) -> int64_t { return kExt && v >= x_sink_tiles ? v + x_skip : v; };
+  auto tile_of = [&](int v) -> int { return v >= x_sink_tiles ? v + x_skip : v; };  // kExt
+  const int t0 = (int)t_begin;
   if (warp == (C::kSelfFeed ? 0 : C::kCons) && !(kExt && p.block_table == nullptr)) {
     // The chunk's block-table entries, read together with (not after) the context
     // length: the row holds mp entries, so entries past the context are in bounds and
     // simply never used.  All loads are issued before any is consumed.
     int64_t n_tab = (cap + 15) / 16 - t_begin;
-    if constexpr (kExt) n_tab = x_tiles - t_begin;
+    if constexpr (kExt) n_tab = x_tiles - t0;
     if (n_tab > p.ct) n_tab = p.ct;
     constexpr int kPer = kMaxChunkTiles / 32;
     int64_t pv[kPer];
@@ -289,14 +309,20 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
       const int i = lane + 32 * j;
       pv[j] = -1;
       if (i < n_tab) {
-        const uint32_t tile = (uint32_t)tile_of(t_begin + i);
+        const uint32_t tile = kExt ? (uint32_t)tile_of(t0 + i) : (uint32_t)(t_begin + i);
         pv[j] = p.block_table ? (int64_t)__ldg(&p.block_table[b * p.mp + (tpp == 1 ? tile : tile / tpp)]) : b;
       }
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = lane + 32 * j;
-      if (i < n_tab) tile_pid[i] = (pv[j] >= 0 && pv[j] < p.P) ? (int)pv[j] : -1;
+      if constexpr (kExt) {  // the tile's first row in the pool seen as rows
+        const uint32_t tile = (uint32_t)tile_of(t0 + i), slot = tpp == 1 ? 0 : (tile % tpp) * 16;
+        if (i < n_tab)
+          tile_pid[i] = (pv[j] >= 0 && pv[j] < p.P) ? ((int)pv[j] * (int)hkv + (int)h) * (int)p.ps + (int)slot : -1;
+      } else {
+        if (i < n_tab) tile_pid[i] = (pv[j] >= 0 && pv[j] < p.P) ? (int)pv[j] : -1;
+      }
     }
   }
   __syncthreads();
@@ -321,12 +347,31 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   // One ring stage's loads (tile i of the chunk into stage i % NS), by one thread.
   auto issue_tile = [&](int i) {
     const int s = i % NS;
-    const int pid = kExt && p.block_table == nullptr ? (int)b : tile_pid[i];
+    if constexpr (kExt) {
+      const int row = p.block_table == nullptr ? ((int)b * (int)hkv + (int)h) * (int)p.ps + tile_of(t0 + i) * 16 : tile_pid[i];
+      stage_valid[s] = row >= 0 ? 1 : 0;
+      if (row >= 0) {
+        uint8_t* st = smem + s * C::kStageBytes;
+        mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes + (C::kI8 ? 64 : 0));
+#pragma unroll
+        for (int hb = 0; hb < C::kBoxes; ++hb) {
+          tma_load_2d(st + hb * 2048, &tm_k, hb * C::kBoxElems, row, &full[s]);
+          tma_load_2d(st + C::kTileBytes + hb * 2048, &tm_v, hb * C::kBoxElems, row, &full[s]);
+        }
+        if (C::kI8) {
+          bulk_load(st + 2 * C::kTileBytes, static_cast<const ScaleT*>(p.k_scales) + row, 32, &full[s]);
+          bulk_load(st + 2 * C::kTileBytes + 128, static_cast<const ScaleT*>(p.v_scales) + row, 32, &full[s]);
+        }
+      } else {
+        mbar_arrive(&full[s]);
+      }
+      return;
+    }
+    const int pid = tile_pid[i];
     stage_valid[s] = pid >= 0 ? 1 : 0;
     if (pid >= 0) {
-      const uint32_t tile = (uint32_t)tile_of(t_begin + i);
-      const int slot0 = p.block_table ? (tpp == 1 ? 0 : (int)((tile % tpp) * 16))
-                                      : (int)((tile_of(t_begin + i) * 16) % p.ps);
+      const uint32_t tile = (uint32_t)(t_begin + i);
+      const int slot0 = p.block_table ? (tpp == 1 ? 0 : (int)((tile % tpp) * 16)) : (int)(((t_begin + i) * 16) % p.ps);
       uint8_t* st = smem + s * C::kStageBytes;
       mbar_arrive_expect_tx(&full[s], 2 * C::kTileBytes + (C::kI8 ? 64 : 0));
 #pragma unroll
@@ -393,34 +438,42 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   // ------------------------------------------------------------------ consumers
 
   // Inclusive last visible key of each row (rows past M never mask anything).
-  const int64_t BIG = INT64_MAX / 4;
-  int64_t limA = BIG, limB = BIG;
+  const Tok BIG = kExt ? (Tok)kExtLimit : (Tok)(INT64_MAX / 4);
+  Tok limA = BIG, limB = BIG;
   if (p.causal) {
-    if (sA < p.M) limA = (int64_t)((uint32_t)sA % (uint32_t)p.L) + ctx - p.L;
-    if (sB < p.M) limB = (int64_t)((uint32_t)sB % (uint32_t)p.L) + ctx - p.L;
+    if (sA < p.M) limA = (Tok)((int64_t)((uint32_t)sA % (uint32_t)p.L) + ctx - p.L);
+    if (sB < p.M) limB = (Tok)((int64_t)((uint32_t)sB % (uint32_t)p.L) + ctx - p.L);
+    if constexpr (kExt) {  // a context length past the table's end may be as large as an int
+      limA = limA < BIG ? limA : BIG;
+      limB = limB < BIG ? limB : BIG;
+    }
   }
   // kExt: the first key of each row's window (the sinks aside), and the last of these
-  int64_t loA = -BIG, loB = -BIG, lo_max = -BIG;
+  int loA = 0, loB = 0, lo_max = 0;
   if constexpr (kExt) {
     if (p.window > 0) {
-      if (sA < p.M) loA = (int64_t)((uint32_t)sA % (uint32_t)p.L) + ctx - p.L - p.window + 1;
-      if (sB < p.M) loB = (int64_t)((uint32_t)sB % (uint32_t)p.L) + ctx - p.L - p.window + 1;
+      const int64_t base = ctx - p.L - p.window + 1;
+      const int64_t a = sA < p.M ? (int64_t)((uint32_t)sA % (uint32_t)p.L) + base : 0;
+      const int64_t b2 = sB < p.M ? (int64_t)((uint32_t)sB % (uint32_t)p.L) + base : 0;
+      loA = a > 0 ? (int)a : 0;
+      loB = b2 > 0 ? (int)b2 : 0;
       lo_max = loA > loB ? loA : loB;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_xor_sync(0xffffffffu, lo_max, o);
+        const int x = __shfl_xor_sync(0xffffffffu, lo_max, o);
         lo_max = x > lo_max ? x : lo_max;
       }
     }
   }
   // Keys below `clean` are visible to every real row of this warp: no masking there.
-  int64_t clean = ctx_limit;
+  const Tok ctx_end = (Tok)ctx_limit;
+  Tok clean = ctx_end;
   {
-    int64_t mn = limA < limB ? limA : limB;
+    Tok mn = limA < limB ? limA : limB;
     mn = mn + 1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_xor_sync(0xffffffffu, mn, o);
+      const Tok x = __shfl_xor_sync(0xffffffffu, mn, o);
       mn = x < mn ? x : mn;
     }
     if (mn < clean) clean = mn;
@@ -435,10 +488,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   // zero, but 0 times a NaN or an infinity is not): 16-bit pages the row, int8 pages the scale.
   // Only tiles at an edge of a window or of the context come here.  The warps that share a
   // stage all write the same zeros, each before it reads.
-  auto hide_unseen = [&](uint8_t* st, int64_t tok0) {
-    const int t = lane >> 1;
-    const int64_t tok = tok0 + t;
-    if (tok >= x_end || (p.window > 0 && tok >= p.sinks && tok < x_first)) {
+  auto hide_unseen = [&](uint8_t* st, int tok0) {
+    const int t = lane >> 1, tok = tok0 + t;
+    if (tok >= x_end || (tok >= x_sinks && tok < x_first)) {
       if constexpr (C::kI8) {
         if ((lane & 1) == 0) reinterpret_cast<uint16_t*>(st + 2 * C::kTileBytes + 128)[t] = 0;
       } else {
@@ -478,7 +530,7 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     }
     if (stage_valid[s]) {
       if constexpr (C::kN8) {
-      const int64_t tok0 = tile_of(t_begin + i) * 16;
+      const Tok tok0 = kExt ? (Tok)(tile_of(t0 + i) * 16) : (Tok)((t_begin + i) * 16);
       const uint32_t kt = smem_u32(smem + s * C::kStageBytes);
       const uint32_t vt = kt + C::kTileBytes;
       // S^T = K Q^T (16 keys x 8 rows).  16-bit pages: the k-steps go round-robin into
@@ -537,19 +589,19 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
             sv[e] = sacc[0][e] + sacc[1][e];
         }
       }
-      const bool need_mask = tok0 + 16 > clean || (kExt && tok0 < lo_max && tok0 + 16 > p.sinks);
+      const bool need_mask = tok0 + 16 > clean || (kExt && tok0 < lo_max && tok0 + 16 > x_sinks);
       if constexpr (kExt) {
-        if (need_mask) hide_unseen(smem + s * C::kStageBytes, tok0);
+        if (need_mask) hide_unseen(smem + s * C::kStageBytes, (int)tok0);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v = sv[e] * p.scale_log2;
         if (need_mask) {
-          const int64_t tok = tok0 + r + 8 * (e >> 1);
-          const int64_t lim = (e & 1) ? limB : limA;
-          if (tok >= ctx_limit || tok > lim) v = -INFINITY;
+          const Tok tok = tok0 + r + 8 * (e >> 1);
+          const Tok lim = (e & 1) ? limB : limA;
+          if (tok >= ctx_end || tok > lim) v = -INFINITY;
           if constexpr (kExt) {
-            if (tok >= p.sinks && tok < ((e & 1) ? loB : loA)) v = -INFINITY;
+            if (tok >= x_sinks && tok < ((e & 1) ? loB : loA)) v = -INFINITY;
           }
         }
         sv[e] = v;
@@ -642,7 +694,7 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
         }
       }
       } else {
-      const int64_t tok0 = tile_of(t_begin + i) * 16;
+      const Tok tok0 = kExt ? (Tok)(tile_of(t0 + i) * 16) : (Tok)((t_begin + i) * 16);
       const uint32_t kt = smem_u32(smem + s * C::kStageBytes);
       const uint32_t vt = kt + C::kTileBytes;
       float sc[2][4];
@@ -700,9 +752,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
       }
 
       // scale, mask, online softmax (base 2)
-      const bool need_mask = tok0 + 16 > clean || (kExt && tok0 < lo_max && tok0 + 16 > p.sinks);
+      const bool need_mask = tok0 + 16 > clean || (kExt && tok0 < lo_max && tok0 + 16 > x_sinks);
       if constexpr (kExt) {
-        if (need_mask) hide_unseen(smem + s * C::kStageBytes, tok0);
+        if (need_mask) hide_unseen(smem + s * C::kStageBytes, (int)tok0);
       }
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
@@ -710,11 +762,11 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
         for (int e = 0; e < 4; ++e) {
           float v = sc[nt][e] * p.scale_log2;
           if (need_mask) {
-            const int64_t tok = tok0 + nt * 8 + 2 * cq + (e & 1);
-            const int64_t lim = e < 2 ? limA : limB;
-            if (tok >= ctx_limit || tok > lim) v = -INFINITY;
+            const Tok tok = tok0 + nt * 8 + 2 * cq + (e & 1);
+            const Tok lim = e < 2 ? limA : limB;
+            if (tok >= ctx_end || tok > lim) v = -INFINITY;
             if constexpr (kExt) {
-              if (tok >= p.sinks && tok < (e < 2 ? loA : loB)) v = -INFINITY;
+              if (tok >= x_sinks && tok < (e < 2 ? loA : loB)) v = -INFINITY;
             }
           }
           sc[nt][e] = v;
@@ -1146,11 +1198,14 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   const uint64_t strides[3] = {D * e, (uint64_t)a.page_size * D * e, (uint64_t)(a.Hkv * a.page_size) * D * e};
   const uint32_t box[4] = {(uint32_t)C::kBoxElems, 16u, 1u, 1u};
   CUtensorMap tk, tv, tks, tvs;
-  int st = encode_tmap(&tk, dt, 4, a.k_pages, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t rdims[2] = {(uint64_t)D, (uint64_t)(a.P * a.Hkv * a.page_size)};  // kExt: the pool as rows
+  int st = kExt ? encode_tmap(&tk, dt, 2, a.k_pages, rdims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)
+                : encode_tmap(&tk, dt, 4, a.k_pages, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != NVM_OK) return st;
-  st = encode_tmap(&tv, dt, 4, a.v_pages, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  st = kExt ? encode_tmap(&tv, dt, 2, a.v_pages, rdims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)
+            : encode_tmap(&tv, dt, 4, a.v_pages, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != NVM_OK) return st;
-  if (C::kI8) {
+  if (C::kI8 && !kExt) {
     const CUtensorMapDataType sdt =
         std::is_same<ScaleT, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const uint64_t sdims[3] = {(uint64_t)a.page_size, (uint64_t)a.Hkv, (uint64_t)a.P};
@@ -1184,6 +1239,7 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   p.causal = a.is_causal;
   p.cluster = 0;
   p.window = a.window; p.sinks = a.sinks; p.lse = a.lse; p.scores = a.scores;
+  p.k_scales = a.k_scales; p.v_scales = a.v_scales;
   const dim3 grid((unsigned)plan.n_units, (unsigned)plan.n_chunks);
   if (plan.cluster && C::kClusterFits && plan.n_chunks > 1 && plan.n_chunks <= 8) {
     p.cluster = 1;
