@@ -79,30 +79,32 @@ struct SelSmem {
 static_assert(kBins % 1024 == 0, "every thread clears and scans whole bins");
 
 // Keeps, of positions [0, n): [0, lo), [hi, n) and the k of [lo, hi) with the largest weight;
-// writes their positions and weights in order.  kHeld: the weights fit in registers.
+// writes their positions and weights in order.  kHeld: the weights' images fit in registers,
+// and so are made once (4700 instructions a warp were 2000 too many when every pass made them
+// again); the weights themselves are read a second time when they move.
 template <int T, bool kHeld>
 __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, float* mout, int32_t* keep, int n, int lo, int hi, int k) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int stretches = (n + T - 1) / T;
-  float w[kPer];  // kHeld: the whole row; else one sweep
-  if constexpr (kHeld) {
+  uint32_t img[kPer];    // kHeld: the whole row's; else one sweep's
+  uint32_t middle = 0;   // bit j: this thread's position of the sweep's stretch j is in [lo, hi)
+  auto read_sweep = [&](int s0) {
+    middle = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (j < stretches) w[j] = j * T + t < n ? mass[j * T + t] : 0.f;
-  }
-  // f(position, weight) over this thread's positions, stretch by stretch
-  auto each = [&](auto&& f) {
-    if constexpr (kHeld) {
+    for (int j = 0; j < kPer; ++j) {
+      if (s0 + j >= stretches) break;
+      const int i = (s0 + j) * T + t;
+      img[j] = i < n ? __float_as_uint(__ldcg(mass + i)) : 0u;
+    }
 #pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (j < stretches) f(j * T + t, w[j]);
-    } else {
-      for (int j = 0; j < stretches; ++j) {
-        const int i = j * T + t;
-        f(i, i < n ? __ldcg(mass + i) : 0.f);
-      }
+    for (int j = 0; j < kPer; ++j) {
+      if (s0 + j >= stretches) break;
+      const int i = (s0 + j) * T + t;
+      img[j] = weight_key(__uint_as_float(img[j]));
+      if (i >= lo && i < hi) middle |= 1u << j;
     }
   };
+  if constexpr (kHeld) read_sweep(0);
   uint32_t prefix = 0;
   int rank = k;         // how many weights equal to the threshold are kept ..
   bool all_eq = true;   // .. all of them
@@ -114,11 +116,16 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
 #pragma unroll
       for (int x = 0; x < kBinsPer; ++x) sm.hist[t + x * T] = 0;
       __syncthreads();
-      each([&](int i, float x) {
-        const uint32_t key = weight_key(x);
-        const bool in = pass == 0 || (key >> (shift + 11 - (pass == 2))) == (prefix >> (shift + 11 - (pass == 2)));
-        if (i >= lo && i < hi && in) atomicAdd(&sm.hist[(key >> shift) & digits], 1);
-      });
+      const int up = shift + (pass == 2 ? 10 : 11);
+      for (int s0 = 0; s0 < stretches; s0 += kPer) {
+        if constexpr (!kHeld) read_sweep(s0);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (s0 + j >= stretches) break;
+          if (((middle >> j) & 1u) && (pass == 0 || (img[j] >> up) == (prefix >> up)))
+            atomicAdd(&sm.hist[(img[j] >> shift) & digits], 1);
+        }
+      }
       __syncthreads();
       // thread t: digits kBins - 1 - kBinsPer t, downwards
       int c[kBinsPer], sum = 0, total;
@@ -147,19 +154,15 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
   int kept = 0, eq_seen = 0;
   for (int s0 = 0; s0 < stretches; s0 += kPer) {
     uint32_t eqs = 0, take = 0;  // bit j: this thread's position of stretch s0 + j
+    if constexpr (!kHeld) read_sweep(s0);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if (s0 + j >= stretches) break;
-      const int i = (s0 + j) * T + t;
-      if constexpr (!kHeld) w[j] = i < n ? __ldcg(mass + i) : 0.f;
-      if (i < n) {
-        if (i < lo || i >= hi) {
-          take |= 1u << j;
-        } else if (k > 0) {
-          const uint32_t key = weight_key(w[j]);
-          if (key > prefix || (all_eq && key == prefix)) take |= 1u << j;
-          if (key == prefix) eqs |= 1u << j;
-        }
+      if ((middle >> j) & 1u) {
+        if (k > 0 && (img[j] > prefix || (all_eq && img[j] == prefix))) take |= 1u << j;
+        if (img[j] == prefix) eqs |= 1u << j;
+      } else if ((s0 + j) * T + t < n) {
+        take |= 1u << j;
       }
     }
     const int in_sweep = stretches - s0 < kPer ? stretches - s0 : kPer;
@@ -192,12 +195,17 @@ __device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, fl
       });
       eq_seen += total;
     }
-    // every weight of this sweep has been read (the scans' barriers): slots below its end
-    // may be overwritten when the weights move in place
+    // The kept weights of this sweep, read before the barriers of the numbering: slots below
+    // the sweep's end may be overwritten after it when the weights move in place.
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (s0 + j >= stretches) break;
+      if ((take >> j) & 1u) img[j] = __float_as_uint(__ldcg(mass + (s0 + j) * T + t));
+    }
     int total;
     number(take, &total, [&](int j, int at) {
       keep[kept + at] = (s0 + j) * T + t;
-      mout[kept + at] = w[j];
+      mout[kept + at] = __uint_as_float(img[j]);
     });
     kept += total;
   }
