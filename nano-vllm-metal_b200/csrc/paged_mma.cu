@@ -184,12 +184,16 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   if (dense) keys = a.page_size;
   int64_t tiles_max = (keys + 15) / 16;
   const bool ext = paged_is_ext(a);
+  bool even_units = false;  // a window cuts every unit to the same length
   // the windowed kernel counts keys and pool rows in 32 bits
   if (ext && (keys >= (int64_t(1) << 30) || a.P * a.Hkv * a.page_size > INT32_MAX - 64)) return plan;
   if (a.window > 0) {
     // the sinks' tiles and those that the windows of L tokens touch
     const int64_t seen = (a.sinks + 15) / 16 + (a.window + a.L - 1 + 15) / 16 + 1;
-    if (seen < tiles_max) tiles_max = seen;
+    if (seen < tiles_max) {
+      tiles_max = seen;
+      even_units = true;
+    }
   }
   // the kernel's index arithmetic runs in 32 bits
   if (tiles_max >= INT32_MAX / 2 || M >= INT32_MAX) return plan;
@@ -244,6 +248,18 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
         // config 4's 160 and config 3's 256 are above the floor anyway).
         if (tiles_max >= 1024 && plan.n_units * ((tiles_max + 127) / 128) >= 2 * slots) floor_ct = 128;
         if (ct < floor_ct) ct = floor_ct;
+        // Units that a window makes equally long: the fewest chunks whose last wave is about
+        // half full to nearly full (a last wave just begun costs the most).  Windows of 4096
+        // keys, 8 kv heads, against the sizing above: 40 requests 118 / 133 us, 56: 158 / 174,
+        // 64: 174 / 181, 100: 267 / 276, 128: 351 / 358; 48 and 80 within 2 % either way.
+        for (int64_t nc = 2; even_units && nc <= 7; ++nc) {
+          const int64_t part = (plan.n_units * nc) % slots;
+          const int64_t ct1 = (tiles_max + nc - 1) / nc;
+          if (ct1 <= kMaxChunkTiles && ct1 >= 16 && part * 20 >= slots * 9 && part * 20 <= slots * 19) {
+            ct = ct1;
+            break;
+          }
+        }
       }
     }
     // the longest context split evenly over that many chunks (B = 512 at 1024 tokens:
