@@ -70,7 +70,7 @@ constexpr int64_t kMaxTicketUnits = (int64_t)(kSm100CounterBytes / sizeof(int)) 
 constexpr int kPlanBins = 1024;  // tile-count bins of the plan's counting sort
 
 int64_t env_int(const char* name, int64_t dflt) {
-  const char* v = std::getenv(name);
+  const char* v = env_get(name);
   if (v == nullptr || v[0] == '\0') return dflt;
   return std::atoll(v);
 }

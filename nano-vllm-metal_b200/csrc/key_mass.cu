@@ -575,7 +575,7 @@ int launch_mass_typed(const PagedArgs& a, const MassParams& p, int64_t keys, cud
 }
 
 bool force_generic() {
-  const char* v = std::getenv("NVM_ATTN_FORCE_GENERIC");
+  const char* v = env_get("NVM_ATTN_FORCE_GENERIC");
   return v != nullptr && v[0] != '\0' && v[0] != '0';
 }
 

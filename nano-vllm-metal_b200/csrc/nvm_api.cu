@@ -3,6 +3,7 @@
 // paged_attention.cpp:22-63 and flash_attention.cpp:20-56), kernel selection, the
 // per-device error word and tensor-map encoding.
 #include <cudaTypedefs.h>
+#include <unistd.h>
 
 #include <cstdarg>
 #include <cstdio>
@@ -24,10 +25,20 @@ int* g_err_ptr[64] = {nullptr};
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
 bool env_flag(const char* name) {
-  const char* v = std::getenv(name);
+  const char* v = env_get(name);
   return v != nullptr && v[0] != '\0' && v[0] != '0';
 }
 }  // namespace
+
+thread_local bool t_env_none = false;
+
+const char* env_get(const char* name) { return t_env_none ? nullptr : std::getenv(name); }
+
+EnvScope::EnvScope() {
+  t_env_none = true;
+  for (char** e = environ; e != nullptr && *e != nullptr; ++e)
+    if (std::strncmp(*e, "NVM_", 4) == 0) t_env_none = false;
+}
 
 int fail(int status, const char* fmt, ...) {
   char buf[512];
@@ -303,6 +314,7 @@ int nvm_flash_attention(const void* q, const void* k, const void* v, int dtype, 
 size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D,
                                                  int64_t page_size, int64_t max_pages, int kv_dtype, int64_t window,
                                                  int64_t sinks, int with_mass) {
+  const EnvScope env;
   PagedArgs a{};
   a.q_dtype = NVM_F32;
   a.kv_dtype = kv_dtype;
@@ -333,6 +345,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
                                int64_t page_size, int64_t max_pages, float scale, int is_causal, int64_t window,
                                int64_t sinks, float* key_mass, int64_t mass_stride_b, int64_t mass_stride_h,
                                int64_t mass_len, void* workspace, size_t workspace_bytes, void* stream) {
+  const EnvScope env;
   PagedArgs a{};
   a.q = q; a.q_dtype = q_dtype; a.k_pages = k_pages; a.v_pages = v_pages; a.kv_dtype = kv_dtype;
   a.k_scales = k_scales; a.v_scales = v_scales; a.scale_dtype = scale_dtype;
@@ -373,6 +386,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
 int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,
                                int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t S, int64_t D, float scale,
                                int is_causal, int64_t window, int64_t sinks, void* stream) {
+  const EnvScope env;
   if (!is_float_dtype(dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: all input arrays must be float32, float16 or bfloat16");
   if (!is_float_dtype(out_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "flash_attention: output dtype must be floating point");
   if (B < 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0)

@@ -20,6 +20,16 @@ int* device_error_word();
 
 size_t dtype_size(int dtype);
 
+// The tuning variables are read on every call, a dozen of them, and each getenv walks the whole
+// environment (0.4 us among 130 variables).  While an EnvScope lives on this thread and one walk
+// found no name that begins with NVM_, env_get answers without another.
+extern thread_local bool t_env_none;
+const char* env_get(const char* name);
+struct EnvScope {
+  EnvScope();
+  ~EnvScope() { t_env_none = false; }
+};
+
 // Bytes at the start of every split-K workspace that hold the ticket counters: zero
 // before a call, zero again after a successful one.  paged_mma.cu and flash_sm100.cu
 // lay their counters out inside this region; noalloc.cu clears exactly this much.

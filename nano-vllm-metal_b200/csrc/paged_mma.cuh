@@ -1155,7 +1155,7 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
 }
 
 int64_t env_int(const char* name, int64_t dflt) {
-  const char* v = std::getenv(name);
+  const char* v = env_get(name);
   if (v == nullptr || v[0] == '\0') return dflt;
   return std::atoll(v);
 }

@@ -108,11 +108,12 @@ def require_cuda(op: str, *tensors: torch.Tensor) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()  # -1 on the host
+        if i < 0 or not t.is_cuda:
             raise RuntimeError(f"{op}: tensors must be on a CUDA device (libnvm_attn has no CPU path)")
         if dev is None:
-            dev, index = t.device, t.get_device()
-        elif t.get_device() != index:
+            dev, index = t.device, i
+        elif i != index:
             raise RuntimeError(f"{op}: all tensors must be on the same CUDA device")
     if dev is None:
         raise RuntimeError(f"{op}: no tensor given")
