@@ -186,8 +186,12 @@ int nvm_paged_attention_noalloc(const void* q, int q_dtype, const void* k_pages,
  * A key that no query token of the call sees (past the context, outside every window, on an
  * unmapped page) has no influence, whatever its K, V and scales hold (NaN and infinities
  * included).  A key that one query token sees but another does not must hold finite values.
+ * As in nvm_paged_attention, q enters the tensor-core products in the pages' type (f16 over
+ * int8 pages).
  * workspace      at least nvm_paged_attention_window_workspace_size(...) bytes, under the
- *                same rules as nvm_paged_attention's (and it may be the same buffer).
+ *                same rules as nvm_paged_attention's (and it may be the same buffer).  With
+ *                key_mass and at most eight query rows per kv head it holds 4 bytes a query
+ *                row and key.
  */
 int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages,
                                int kv_dtype, const void* k_scales, const void* v_scales, int scale_dtype,

@@ -52,6 +52,8 @@ struct MassParams {
   float scale_log2;
   int causal;
   int64_t window, sinks;
+  int q_round;      // generic: the 16-bit type in which the attention kernel took q, or NVM_F32
+  int64_t blocks;   // 1-D grids: blocks per (sequence, kv head)
 };
 
 // Any head dim <= 256, page size and dtype: a warp per key, lanes along the query rows.
@@ -59,12 +61,13 @@ constexpr int kGenWarps = 4;
 __global__ void __launch_bounds__(kGenWarps * 32) key_mass_generic_kernel(MassParams p) {
   __shared__ float krow[kGenWarps][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
+  const int64_t bh = blockIdx.x / p.blocks, block = blockIdx.x - bh * p.blocks;
+  const int64_t b = bh / p.Hkv, h = bh % p.Hkv;
   const int64_t ctx = p.context_lens[b];
   const int64_t cap = p.mp * p.ps;
   int64_t end = ctx < cap ? ctx : cap;
   if (p.len < end) end = p.len;
-  for (int64_t s = (int64_t)blockIdx.x * kGenWarps + warp; s < end; s += (int64_t)gridDim.x * kGenWarps) {
+  for (int64_t s = block * kGenWarps + warp; s < end; s += p.blocks * kGenWarps) {
     const int64_t page = s / p.ps, off = s - page * p.ps;
     const int64_t pid = p.block_table[b * p.mp + page];
     float sum = 0.f;
@@ -79,7 +82,12 @@ __global__ void __launch_bounds__(kGenWarps * 32) key_mass_generic_kernel(MassPa
         if (!seen) continue;
         const int64_t row = (b * p.Hq + h * p.g) * p.L + r;
         float dot = 0.f;
-        for (int64_t d = 0; d < p.D; ++d) dot += load_dyn(p.q, row * p.D + d, p.q_dtype) * krow[warp][d];
+        for (int64_t d = 0; d < p.D; ++d) {
+          float x = load_dyn(p.q, row * p.D + d, p.q_dtype);
+          if (p.q_round == NVM_F16) x = __half2float(__float2half_rn(x));
+          if (p.q_round == NVM_BF16) x = __bfloat162float(__float2bfloat16_rn(x));
+          dot += x * krow[warp][d];
+        }
         if (p.kv_dtype == NVM_I8) dot *= ksc;
         sum += exp2f(dot * p.scale_log2 - p.lse[row]);
       }
@@ -106,7 +114,8 @@ constexpr int kScoreKeys = 4;
 template <int kRows>
 __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p, const ScoreParams sp) {
   __shared__ float s_lse[8];
-  const int64_t bh = blockIdx.y, b = bh / p.Hkv, h = bh - b * p.Hkv;
+  const int64_t bh = blockIdx.x / p.blocks, block = blockIdx.x - bh * p.blocks;
+  const int64_t b = bh / p.Hkv, h = bh - b * p.Hkv;
   if (threadIdx.x < 8) s_lse[threadIdx.x] = (int)threadIdx.x < sp.rows ? p.lse[bh * sp.rows + threadIdx.x] : INFINITY;
   const int64_t ctx = p.context_lens[b], cap = p.mp * p.ps;
   const int64_t end = ctx < cap ? ctx : cap;
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p
     }
   }
   __syncthreads();
-  const int64_t v0 = (int64_t)blockIdx.x * (256 * kScoreKeys) + threadIdx.x;
+  const int64_t v0 = block * (256 * kScoreKeys) + threadIdx.x;
   const int64_t v_end = end > 0 ? tiles * 16 : 0;
   const float* z = sp.scores + bh * sp.v_keys * kRows;
   float* mrow = p.mass + b * p.stride_b + h * p.stride_h;
@@ -594,7 +603,7 @@ bool mass_sm100_eligible(const PagedArgs& a) {
 
 }  // namespace
 
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, cudaStream_t s) {
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, bool tensor_cores, cudaStream_t s) {
   MassParams p{};
   p.q = a.q; p.k = a.k_pages; p.ks = a.k_scales; p.block_table = a.block_table; p.context_lens = a.context_lens;
   p.lse = a.lse; p.mass = m.mass; p.stride_b = m.stride_b; p.stride_h = m.stride_h; p.len = m.len;
@@ -609,7 +618,9 @@ int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* pla
   if (a.scores != nullptr) {
     ScoreParams sp{a.scores, plan->chunk_tiles * plan->n_chunks * 16, (int)(p.g * p.L)};
     const int64_t per = 256 * kScoreKeys;
-    const dim3 grid((unsigned)((sp.v_keys + per - 1) / per), (unsigned)(a.B * a.Hkv));
+    p.blocks = (sp.v_keys + per - 1) / per;
+    if (p.blocks * a.B * a.Hkv > INT32_MAX) return fail(NVM_ERR_UNSUPPORTED, "paged_attention: too many keys for key_mass");
+    const dim3 grid((unsigned)(p.blocks * a.B * a.Hkv));
     if (sp.rows <= 2) key_mass_scores_kernel<2><<<grid, 256, 0, s>>>(p, sp);
     else if (sp.rows <= 4) key_mass_scores_kernel<4><<<grid, 256, 0, s>>>(p, sp);
     else if (sp.rows <= 6) key_mass_scores_kernel<6><<<grid, 256, 0, s>>>(p, sp);
@@ -620,7 +631,12 @@ int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* pla
     return a.q_dtype == NVM_F16 ? launch_mass_typed<__half>(a, p, keys, s) : launch_mass_typed<__nv_bfloat16>(a, p, keys, s);
   int64_t bx = (keys + kGenWarps - 1) / kGenWarps;
   if (bx > 65536) bx = 65536;
-  const dim3 grid((unsigned)bx, (unsigned)(a.B * a.Hkv));
+  if (bx * a.B * a.Hkv > INT32_MAX) bx = INT32_MAX / (a.B * a.Hkv);
+  if (bx < 1) return fail(NVM_ERR_UNSUPPORTED, "paged_attention: too many sequences for key_mass");
+  p.blocks = bx;
+  // the tensor-core attention kernels take q in the pages' type (f16 over int8 pages)
+  p.q_round = !tensor_cores ? NVM_F32 : a.kv_dtype == NVM_I8 ? NVM_F16 : a.kv_dtype;
+  const dim3 grid((unsigned)(bx * a.B * a.Hkv));
   key_mass_generic_kernel<<<grid, kGenWarps * 32, 0, s>>>(p);
   return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
 }

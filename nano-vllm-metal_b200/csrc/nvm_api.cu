@@ -380,7 +380,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
                        : launch_paged_generic(a, s);
   if (st != NVM_OK || key_mass == nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
-  return launch_key_mass(a, m, &plan, s);
+  return launch_key_mass(a, m, &plan, sp.eligible || plan.eligible, s);
 }
 
 int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,

@@ -77,8 +77,8 @@ struct KeyMassArgs {
   int64_t stride_b, stride_h, len;
 };
 struct MmaPlan;
-// plan: the attention kernel's, when a.scores is set.
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, cudaStream_t s);
+// plan: the attention kernel's, when a.scores is set; tensor_cores: it was not the generic one.
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, bool tensor_cores, cudaStream_t s);
 
 // Eviction by accumulated weight (evict.cu).
 struct EvictArgs {

@@ -395,7 +395,7 @@ class DevicePageTable:
         self.refcount = torch.zeros(max(capacity, 1), **i32)
         self.last_call = torch.full((max(capacity, 1),), -1, **i32)  # rewind scratch, kept at -1
         self.status = torch.zeros(1, **i32)
-        self.evict_status = torch.zeros(1, **i32)  # not zero once evict has refused a request
+        self.evict_status = torch.zeros(1, **i32)  # not zero if the last evict refused a request
 
     def append(self, new_tokens: torch.Tensor, slot_mapping: torch.Tensor | None = None) -> torch.Tensor:
         """new_tokens ``[B]`` int32 on the device; returns int64 slots ``[sum(new_tokens)]``.
@@ -473,15 +473,20 @@ class DevicePageTable:
         (prefix attach) past its sinks stays as it is and makes ``check_status`` raise."""
         from .evict import evict_tokens
 
-        results = []
-        for layer in layers:
+        layers = [tuple(layer) for layer in layers]
+        for layer in layers:  # all of them before any is touched: every layer has to drop the same tokens
             if len(layer) not in (3, 5):
                 raise ValueError("evict: a layer is (key_pages, value_pages, key_mass) or (key_pages, value_pages, "
                                  "key_scales, value_scales, key_mass)")
+            if layer[0].shape[2] != self.page_size or layer[0].shape[0] > self.refcount.numel():
+                raise ValueError("evict: pages must have the table's page_size and at most its capacity")
+            if layer[0].shape[0] != layers[0][0].shape[0] or layer[-1].shape[2] != layers[0][-1].shape[2]:
+                raise ValueError("evict: all layers need the same number of pages and key_mass entries")
+        self.evict_status.zero_()
+        results = []
+        for layer in layers:
             kp, vp, mass = layer[0], layer[1], layer[-1]
             ks, vs = (layer[2], layer[3]) if len(layer) == 5 else (None, None)
-            if kp.shape[2] != self.page_size or kp.shape[0] > self.refcount.numel():
-                raise ValueError("evict: pages must have the table's page_size and at most its capacity")
             results.append(evict_tokens(kp, vp, self.block_table, self.context_lens, mass, budget, sinks=sinks,
                                         recent=recent, key_scales=ks, value_scales=vs,
                                         page_refcount=self.refcount, status=self.evict_status))

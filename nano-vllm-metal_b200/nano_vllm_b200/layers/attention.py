@@ -36,10 +36,10 @@ __all__ = [
 
 
 def _check_window(op: str, window: int | None, sinks: int) -> None:
-    if window is not None and window < 1:
-        raise RuntimeError(f"{op}: window must be at least 1 (None for no window), got {window}")
-    if sinks < 0:
-        raise RuntimeError(f"{op}: sinks must not be negative, got {sinks}")
+    if window is not None and not 1 <= window < 2 ** 31:
+        raise RuntimeError(f"{op}: window must be at least 1 and below 2^31 (None for no window), got {window}")
+    if not 0 <= sinks < 2 ** 31:
+        raise RuntimeError(f"{op}: sinks must not be negative, nor 2^31 or more, got {sinks}")
 
 
 def _row_strides(what: str, x: torch.Tensor) -> tuple[int, int]:

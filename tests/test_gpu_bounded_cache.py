@@ -146,6 +146,38 @@ def test_key_mass(case, causal, path):
             assert abs(float(total.cpu()) - rows) <= 1e-4 * max(rows, 1) + 2 ** -22 * float(old), (float(total), rows)
 
 
+@pytest.mark.parametrize("L", [1, 3, 70])
+@pytest.mark.parametrize("kv,qd", [(BF, F32), (BF, HF), (I8, F32)])
+def test_key_mass_with_queries_of_another_type(L, kv, qd):
+    prob = make_problem(40 + L, [300, 90], L, 16, 4, 128, 16, kv, qd)
+    taken = dict(prob, q=prob["q"].to(HF if kv == I8 else kv))  # as the tensor cores take it
+    mass = torch.rand(2, 4, 300)
+    ref, terms, mref, merr = paged_reference(taken, 0, 0, mass=mass)
+    p, gm = to_gpu(prob), mass.cuda()
+    got = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], mask="causal", key_mass=gm)
+    assert_within(got, ref, out_bound(ref, terms, 128, kv, F32), "out")
+    assert_within(gm, mref, merr + 1e-30, "mass")
+
+
+def test_more_sequences_than_a_grid_axis_holds(path):
+    B = 9000  # x 8 kv heads: more than 65535 rows of key_mass
+    gen = torch.Generator().manual_seed(6)
+    ctx = torch.randint(0, 20, (B,), generator=gen).tolist()
+    prob = make_problem(7, ctx[:50], 1, 16, 8, 64, 16, BF, width_extra=0)
+    pick = torch.randint(0, 50, (B,), generator=gen)
+    prob = dict(prob, q=prob["q"][pick], bt=prob["bt"][pick], cl=prob["cl"][pick])
+    mass = torch.zeros(B, 8, 32)
+    check = torch.tensor([0, 1, 4500, B - 2, B - 1])
+    small = dict(prob, q=prob["q"][check], bt=prob["bt"][check], cl=prob["cl"][check])
+    ref, terms, mref, merr = paged_reference(small, 0, 0, mass=mass[check])
+    p, gm = to_gpu(prob), mass.cuda()
+    got = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=gm)
+    assert_within(got[check.cuda()], ref, out_bound(ref, terms, 64, BF, F32), "out")
+    assert_within(gm[check.cuda()], mref, merr + 1e-30, "mass")
+    total = gm.double().sum((1, 2)).cpu()
+    assert ((total - 16.0 * (prob["cl"] > 0)).abs() <= 1e-3).all()
+
+
 def test_key_mass_shorter_than_the_context(path):
     prob = make_problem(1, [200, 90], 1, 16, 8, 128, 16, BF)
     mass = torch.rand(2, 8, 100)
@@ -489,10 +521,20 @@ def test_table_evict_refuses_shared_prefix_pages():
     with pytest.raises(RuntimeError, match="evict refused"):
         table.check_status()
     # past the shared pages, request 1 may be trimmed; request 0's own pages 2 and 3 too
-    table.evict_status.zero_()
     table.evict([(pages, vals, mass)], 40, sinks=32, recent=2)
     assert table.context_lens.tolist() == [40, 40]
     table.check_status()
+
+
+def test_table_evict_wants_layers_alike():
+    table = DevicePageTable(1, 4, 16, 8)
+    pages, mass = torch.zeros(8, 2, 16, 64, device="cuda", dtype=BF), torch.zeros(1, 2, 64, device="cuda")
+    table.append(torch.tensor([50], dtype=torch.int32, device="cuda"))
+    for bad in ([(pages, pages, mass), (pages, pages, mass[:, :, :40])], [(pages, pages, mass), (pages[:7], pages[:7], mass)],
+                [(pages, mass)], [(pages.view(4, 2, 32, 64), pages.view(4, 2, 32, 64), mass)]):
+        with pytest.raises(ValueError, match="evict"):
+            table.evict(bad, 20)
+    assert table.context_lens.tolist() == [50]
 
 
 def test_request_cache_evict():
