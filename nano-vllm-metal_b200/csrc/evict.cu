@@ -261,14 +261,16 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_select_kernel(const EvictPa
 
 // CTAs of 128 threads, seven to an SM (about 900 threads with 2 x 4 vectors each in flight):
 // 512 (request, head) pairs x K and V are 6.9 CTAs an SM, one even wave.
+// With no more than four CTAs an SM each has eight vectors a tile instead of four, and the
+// registers for them (512 CTAs of int8 rows: 125 us with the selection against 139 us; 1024
+// CTAs would take two waves, 257 us against 215 us).
 constexpr int kCmpThreads = 128;
 
 // Rows of one column slice: threads my_row = threadIdx / per_row of a step, kU steps a tile.
-template <typename V>
+template <typename V, int kU>
 __device__ __forceinline__ void compact_rows(const EvictParams& ep, int64_t b, int64_t h, uint8_t* pool, int64_t row_bytes,
                                              int col0, int cols) {
   const EvictArgs& p = ep.a;
-  constexpr int kU = 4;  // rows in flight per thread
   const int per_row = cols / (int)sizeof(V);
   const int rows_par = blockDim.x / per_row;  // rows one step of the CTA covers
   const int my_row = threadIdx.x / per_row, my_col = threadIdx.x % per_row;
@@ -317,8 +319,8 @@ __device__ __forceinline__ void compact_rows(const EvictParams& ep, int64_t b, i
   }
 }
 
-template <typename V>
-__global__ void __launch_bounds__(kCmpThreads, 7) evict_compact_kernel(const EvictParams ep) {
+template <typename V, int kU>
+__global__ void __launch_bounds__(kCmpThreads, kU > 4 ? 4 : 7) evict_compact_kernel(const EvictParams ep) {
   const EvictArgs& p = ep.a;
   const int64_t b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   if (p.dropped[b] == 0) return;
@@ -327,13 +329,13 @@ __global__ void __launch_bounds__(kCmpThreads, 7) evict_compact_kernel(const Evi
     uint8_t* pool = static_cast<uint8_t*>(y < ep.n_slices ? p.k_pages : p.v_pages);
     const int sl = y % ep.n_slices, col0 = sl * ep.slice_bytes;
     const int left = (int)ep.row_bytes - col0;
-    compact_rows<V>(ep, b, h, pool, ep.row_bytes, col0, left < ep.slice_bytes ? left : ep.slice_bytes);
+    compact_rows<V, kU>(ep, b, h, pool, ep.row_bytes, col0, left < ep.slice_bytes ? left : ep.slice_bytes);
   } else {
     uint8_t* pool = static_cast<uint8_t*>(y == 2 * ep.n_slices ? p.k_scales : p.v_scales);
     if (ep.scale_bytes == 4)
-      compact_rows<uint32_t>(ep, b, h, pool, 4, 0, 4);
+      compact_rows<uint32_t, kU>(ep, b, h, pool, 4, 0, 4);
     else
-      compact_rows<uint16_t>(ep, b, h, pool, 2, 0, 2);
+      compact_rows<uint16_t, kU>(ep, b, h, pool, 2, 0, 2);
   }
 }
 
@@ -361,20 +363,23 @@ int launch_evict(const EvictArgs& a, cudaStream_t s) {
   // the widest vector that rows and pools are aligned to
   const uint64_t al = (uint64_t)ep.row_bytes | reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
   const int vec = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : (al & 1) == 0 ? 2 : 1;
-  // Columns of one CTA: up to 256 bytes (whole rows of 128 16-bit values), halved while the
-  // CTAs would not fill an even wave: to 64 bytes below six per SM, to 32 below two.
+  // Columns of one CTA: up to 256 bytes (whole rows of 128 16-bit values), halved down to 32 while
+  // the CTAs would be fewer than two per SM.  Narrow slices waste the memory's 64-byte accesses
+  // (512 CTAs of whole 128-byte int8 rows 138 us with the selection, 1024 of half rows 147 us,
+  // 2048 of quarter rows 236 us), but one request needs them (8 heads: 26 us against 43 us).
   int slice = vec >= 16 ? 256 : vec >= 4 ? 128 : 32;
   if (slice > ep.row_bytes) slice = (int)ep.row_bytes;
   while (slice > 32 && slice % 2 == 0 && (slice / 2) % vec == 0 &&
-         a.B * a.Hkv * 2 * ((ep.row_bytes + slice - 1) / slice) < (slice > 64 ? 6 : 2) * 148)
+         a.B * a.Hkv * 2 * ((ep.row_bytes + slice - 1) / slice) < 2 * 148)
     slice /= 2;
   ep.slice_bytes = slice;
   ep.n_slices = (int)((ep.row_bytes + ep.slice_bytes - 1) / ep.slice_bytes);
   const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)(2 * ep.n_slices + (ep.scale_bytes ? 2 : 0)));
-  if (vec == 16) evict_compact_kernel<uint4><<<grid, kCmpThreads, 0, s>>>(ep);
-  else if (vec == 4) evict_compact_kernel<uint32_t><<<grid, kCmpThreads, 0, s>>>(ep);
-  else if (vec == 2) evict_compact_kernel<uint16_t><<<grid, kCmpThreads, 0, s>>>(ep);
-  else evict_compact_kernel<uint8_t><<<grid, kCmpThreads, 0, s>>>(ep);
+  if (vec == 16 && a.B * a.Hkv * 2 * ep.n_slices <= 4 * 148) evict_compact_kernel<uint4, 8><<<grid, kCmpThreads, 0, s>>>(ep);
+  else if (vec == 16) evict_compact_kernel<uint4, 4><<<grid, kCmpThreads, 0, s>>>(ep);
+  else if (vec == 4) evict_compact_kernel<uint32_t, 4><<<grid, kCmpThreads, 0, s>>>(ep);
+  else if (vec == 2) evict_compact_kernel<uint16_t, 4><<<grid, kCmpThreads, 0, s>>>(ep);
+  else evict_compact_kernel<uint8_t, 4><<<grid, kCmpThreads, 0, s>>>(ep);
   return check_cuda(cudaGetLastError(), "evict: compaction kernel launch");
 }
 
