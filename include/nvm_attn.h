@@ -3,8 +3,9 @@
  * nano-vllm-metal: paged-attention decode / multi-query, dense flash attention,
  * the paged KV scatter-write (with int8 quantise-on-write), device-side page
  * allocation for a batch of appends, and the fused per-layer q/k RMSNorm + RoPE +
- * K/V write that precedes every attention call, and the 4-bit (W4A16) matmul of the
- * projections around it.
+ * K/V write that precedes every attention call, the 4-bit (W4A16) matmul of the
+ * projections around it, and what keeps a long generation's cache bounded: a sliding
+ * window with sinks, accumulated attention weights, eviction by them.
  *
  * Conventions shared by every entry point
  *   - All tensor arguments are raw DEVICE pointers to row-major contiguous memory

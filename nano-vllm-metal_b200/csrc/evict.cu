@@ -17,6 +17,9 @@
 // (those lie at or past their own first slot): in place, no second copy of the cache, and the
 // next tile's rows can be on their way while this one is written.  The column slices are
 // independent, which is what spreads one (request, kv head) over several SMs.
+// Measured on a B200: 64 requests of 2.1K-8K tokens to 2048, 8 kv heads, bf16: selection 28 us,
+// compaction 178 us for 1.07 GB read and written (6.0 TB/s); 32 requests to 4000, int8 pages:
+// 20 and 95 us.
 #include "nvm_common.cuh"
 #include "nvm_internal.h"
 

@@ -4,7 +4,8 @@ Drop-in for the reference's ``layers/attention`` operators and ``cache/paged``
 page pools: ``paged_attention``, ``flash_attention``, ``TinyKvPagedPool``,
 ``TinyKvPagedCache``, ``BatchingKvCache`` keep the reference's names and
 signatures (the reference's ``PrefixCache`` runs unchanged over these pools); the
-kernels live in ``libnvm_attn.so`` (C ABI in ``include/nvm_attn.h``).
+kernels live in ``libnvm_attn.so`` (C ABI in ``include/nvm_attn.h``).  A cache is kept bounded
+by ``window`` / ``sinks`` and ``key_mass`` of the attention calls and by ``evict_tokens``.
 """
 
 from .layers.attention import (  # noqa: F401
