@@ -267,6 +267,29 @@ def test_dense_window_unseen_keys_may_hold_anything(path):
     assert torch.equal(flash_attention(q.cuda(), k.cuda(), v.cuda(), mask="causal", window=50, sinks=5), clean)
 
 
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_pages_past_two_to_the_31_elements(L, path):
+    prob = make_problem(50 + L, [700, 90], L, 16, 8, 128, 16, BF)
+    P, big = prob["k"].shape[0], 150000  # 2.5e9 elements a pool
+    mass = torch.rand(2, 8, 700)
+    ref, terms, mref, merr = paged_reference(prob, 300, 4, mass=mass)
+    p, gm = to_gpu(prob), mass.cuda()
+    pools = []
+    for x in ("k", "v"):
+        pool = torch.empty(big, 8, 16, 128, dtype=BF, device="cuda")
+        pool[big - P:] = p[x]
+        pools.append(pool)
+    bt = torch.where(p["bt"] >= 0, p["bt"] + (big - P), p["bt"])
+    got = paged_attention(p["q"], *pools, bt, p["cl"], 16, mask="causal", window=300, sinks=4, key_mass=gm)
+    assert_within(got, ref, out_bound(ref, terms, 128, BF, F32), "out")
+    assert_within(gm, mref, merr + 1e-30, "mass")
+    keep, _, _, eref, new, _ = evict_reference(prob, mass, 200, 4, 20)
+    gm = mass.cuda()
+    r = evict_tokens(*pools, bt, p["cl"], gm, 200, sinks=4, recent=20)
+    assert torch.equal(r.keep_index.cpu(), keep) and torch.equal(gm.cpu(), eref)
+    assert torch.equal(pools[0][big - P:].cpu(), new["k"]) and torch.equal(pools[1][big - P:].cpu(), new["v"])
+
+
 def test_refusals():
     prob = to_gpu(make_problem(1, [40], 1, 8, 4, 128, 16, BF))
     call = lambda **kw: paged_attention(prob["q"], prob["k"], prob["v"], prob["bt"], prob["cl"], 16, mask="causal", **kw)  # noqa: E731
