@@ -12,7 +12,11 @@
 // is cheaper depends on the rows of a kv head, M = Hq/Hkv * L:
 //  * M <= 8 (decode): the attention kernel keeps its scores in the workspace, 4 M bytes a key
 //    written and read once, next to the 4 D bytes of K and V that it reads anyway (M = 4,
-//    D = 128: 32 bytes next to 512); key_mass_scores_kernel adds them up.
+//    D = 128: 32 bytes next to 512).  It weighs them itself when its chunks merge in a cluster
+//    or not at all (paged_mma.cuh); when they merge through the workspace,
+//    key_mass_scores_kernel does: the CTA that ends a long unit would hold its slot and, at the
+//    end, the launch (64 requests of 2K-16K keys: 430 us, against 474 us that way; one request
+//    of 1K keys 18 us on the device, against 16 us the other way).
 //  * more rows (verify, chunks, prompts): 2 D bytes a key read again cost less than 8 M bytes
 //    from M = D / 4 = 32 on, and prompts could not keep M x S scores at all:
 //    key_mass_sm100_kernel computes them again on the tensor cores, S^T = K Q^T with the keys
@@ -24,8 +28,8 @@
 //    start of its CTAs.
 //  * everything else (fp32, other head dims): key_mass_generic_kernel.
 // Measured on a B200 (32/8 heads, bf16): 64 requests of 2K-16K keys 26 us for 74 MB of scores
-// (the whole scored step 430 us, 0.85 of a copy's rate for its K and V); prompts of 2 x 2048
-// tokens 60 us next to 102 us of attention, 570 TFLOP/s of S^T.
+// (the whole scored step 430 us, 0.85 of a copy's rate for its K and V); prompts of 2 x 2048 tokens 60 us next to 102 us of
+// attention, 570 TFLOP/s of S^T.
 #include <cooperative_groups.h>
 
 #include <cstdlib>

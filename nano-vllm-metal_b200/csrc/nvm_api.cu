@@ -374,11 +374,15 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
     return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
                 workspace_bytes);
   if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
-  if (kept > 0) a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
+  if (kept > 0) {
+    a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
+    if (plan.ws_bytes == 0) a.mass = key_mass;  // the attention kernel weighs them too
+    a.mass_sb = mass_stride_b; a.mass_sh = mass_stride_h; a.mass_len = mass_len;
+  }
   st = sp.eligible     ? launch_sm100(a, sp, workspace, s)
        : plan.eligible ? launch_paged_mma(a, plan, workspace, s)
                        : launch_paged_generic(a, s);
-  if (st != NVM_OK || key_mass == nullptr) return st;
+  if (st != NVM_OK || key_mass == nullptr || a.mass != nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
   return launch_key_mass(a, m, &plan, sp.eligible || plan.eligible, s);
 }

@@ -63,6 +63,8 @@ struct PagedArgs {
   int64_t window, sinks;
   float* lse;         // [B*Hq*L] log2 of sum 2^(score * log2 e) of every row (+inf: no key), or NULL
   float* scores;      // n8 tile only: keep every base-2 score, [B*Hkv][virtual keys][rows, even], or NULL
+  float* mass;        // with scores, and no merge through the workspace: add the weights, or NULL
+  int64_t mass_sb, mass_sh, mass_len;
 };
 inline bool paged_is_ext(const PagedArgs& a) { return a.window > 0 || a.lse != nullptr; }
 

@@ -28,7 +28,9 @@
 //    the sinks and the row block's windows are jumped over by renumbering: virtual tile v is
 //    tile v below the sinks' last tile and tile v + skip past it, so chunks, rings and merges
 //    run on virtual tiles unchanged.  They can leave every row's log-sum-exp.  Their keys are
-//    counted in 32 bits, and a tile is named by one row of the pool seen as [P * Hkv *
+//    counted in 32 bits.  On the n8 tile they can keep every score in the workspace and, where
+//    units merge in a cluster or not at all, add the keys' weights to a buffer of the caller's
+//    once the log-sum-exps are known.  A tile is named by one row of the pool seen as [P * Hkv *
 //    page_size, D], worked out with the page ids, so that the warp that copies a tile between
 //    two of its own spends few instructions on it.
 //  * Every mbarrier wait is bounded (nvm::mbar_wait); on expiry the kernel records an
@@ -76,6 +78,8 @@ struct MmaParams {
   const void* k_scales;   // kExt: int8 pages' scales, copied by row
   const void* v_scales;
   float* scores;          // kExt, n8: keep every score ([units][n_chunks * ct * 16][rows, even]), or null
+  float* mass;            // kExt, n8, with scores and no workspace merge: [b * mass_sb + h * mass_sh + key], key < mass_len
+  int64_t mass_sb, mass_sh, mass_len;
 };
 
 template <typename KvT, int D, int NWM, int NWK, int NS_ = 0>
@@ -953,6 +957,44 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   auto put_lse = [&](int rl, float ms, float ls) {
     if (p.lse != nullptr) p.lse[q_row0 + row0 + rl] = ls > 0.f ? ms + log2f(ls) : INFINITY;
   };
+  // The weights of virtual keys [v0, v1), by all consumer threads, after put_lse of every row:
+  // new keys (the last L positions) start at zero, the others gain.
+  auto add_mass = [&](int v0, int v1) {
+    named_barrier(1, NCT);
+    float lse[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lse[i] = i < (int)rows_here ? __ldcg(p.lse + q_row0 + i) : INFINITY;
+    float* mrow = p.mass + b * p.mass_sb + h * p.mass_sh;
+    const float* z = p.scores + unit * p.n_chunks * p.ct * 16 * rows_pad;
+    const int end = (int)(p.mass_len < x_end ? p.mass_len : x_end), first_new = (int)(ctx - p.L);
+    constexpr int kU = 4;  // keys in flight per thread
+    for (int v = v0 + tid; v < v1; v += kU * NCT) {
+      float2 x[kU][4];
+      float old[kU];
+      int key[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int vu = v + u * NCT;
+        key[u] = vu < v1 ? tile_of(vu >> 4) * 16 + (vu & 15) : end;
+        if (key[u] >= end) continue;
+        old[u] = key[u] < first_new ? mrow[key[u]] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * i < rows_pad) x[u][i] = __ldcg(reinterpret_cast<const float2*>(z + (int64_t)vu * rows_pad) + i);
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (key[u] >= end) continue;
+        float gain = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (2 * i < (int)rows_here) gain += ex2_ftz(x[u][i].x - lse[2 * i]);
+          if (2 * i + 1 < (int)rows_here) gain += ex2_ftz(x[u][i].y - lse[2 * i + 1]);
+        }
+        mrow[key[u]] = old[u] + gain;
+      }
+    }
+  };
   if constexpr (C::kClusterFits) {
     if (p.cluster) {
       // Split-K inside a thread-block cluster: the unit's chunks are CTAs 0 .. n_chunks-1
@@ -1025,6 +1067,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
         }
       }
       cluster.sync();
+      if constexpr (kExt) {
+        if (p.mass != nullptr) add_mass(t0 * 16, (t0 + n_my) * 16);  // each CTA its own chunk
+      }
       return;
     }
   }
@@ -1055,7 +1100,12 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
       if (d == 0) p.part_ml[wsrow + rl] = make_float2(ms, ls);
     }
   }
-  if (single) return;
+  if (single) {
+    if constexpr (kExt && C::kN8) {
+      if (p.mass != nullptr) add_mass(0, x_tiles * 16);
+    }
+    return;
+  }
 
   // Split-K: the last CTA of this unit merges every chunk's partial result.
   __threadfence();
@@ -1239,6 +1289,7 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   p.causal = a.is_causal;
   p.cluster = 0;
   p.window = a.window; p.sinks = a.sinks; p.lse = a.lse; p.scores = a.scores;
+  p.mass = a.mass; p.mass_sb = a.mass_sb; p.mass_sh = a.mass_sh; p.mass_len = a.mass_len;
   p.k_scales = a.k_scales; p.v_scales = a.v_scales;
   const dim3 grid((unsigned)plan.n_units, (unsigned)plan.n_chunks);
   if (plan.cluster && C::kClusterFits && plan.n_chunks > 1 && plan.n_chunks <= 8) {
