@@ -87,8 +87,8 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise RuntimeError(f"{op}: status must be one int32")
     bt, cl = _int32_rows(block_table), _int32_rows(context_lens)
-    keep = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
-    kept, dropped, refused = torch.empty((3, B), dtype=torch.int32, device=dev).unbind(0)
+    keep = bt.new_empty((B, Hkv, budget))
+    kept, dropped, refused = bt.new_empty((3, B)).unbind(0)
     with nv.on_device(dev):
         nv.check(nv.lib().nvm_paged_evict(
             key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(key_scales),

@@ -200,7 +200,7 @@ def _paged_attention_window(query, key_pages, value_pages, block_table, context_
         msb, msh = _row_strides(f"{op}: key_mass", key_mass)
         mp, ml = key_mass.data_ptr(), key_mass.shape[2]
     if out is None:
-        out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
+        out = torch.empty_like(q) if out_dtype is q.dtype else q.new_empty((B, Hq, L, D), dtype=out_dtype)
     elif tuple(out.shape) != (B, Hq, L, D) or not out.is_contiguous():
         raise RuntimeError(f"{op}: out must be a contiguous [B, Hq, L, D] tensor")
     factor = scale if scale is not None else 1.0 / (D ** 0.5)
