@@ -30,7 +30,7 @@
 // hold the sinks next to the window's start: a tile of its own for 4 sinks cost 7 % of a
 // prompt under a 1024-key window (2 x 4096 tokens, 32/8 heads: 198 us, 610 TFLOP/s of the pairs
 // seen, bound by the softmax warps' issue).  Which tiles need a mask is known per item; the mask of a
-// row is a 64-bit pattern.
+// row is a pattern of two words, built with a few shifts.
 // Every mbarrier wait is bounded; on expiry the CTA records an error, lets its own
 // copies and MMAs land (bounded), frees TMEM and returns.
 #include <cooperative_groups.h>
@@ -142,8 +142,12 @@ __device__ __forceinline__ int vgroup_of(const Item& it, int key) {
   const int g = key >> 4;
   return g < it.sg ? g : (g - it.skip > it.sg ? g - it.skip : it.sg);
 }
-// columns 0 .. x of a tile
-__device__ __forceinline__ uint64_t cols_to(int x) { return x < 0 ? 0ull : x >= 63 ? ~0ull : (2ull << x) - 1; }
+// bits n .. 31 of a word, for any n (PTX shl gives 0 from 32 on, which C leaves open)
+__device__ __forceinline__ uint32_t bits_from(int n) {
+  uint32_t r;
+  asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(0xffffffffu), "r"(n < 0 ? 0 : n));
+  return r;
+}
 
 template <bool kExt>
 __device__ __forceinline__ Item decode_item(const Sm100Params& p, int64_t item) {
@@ -816,16 +820,23 @@ __global__ void __launch_bounds__(kThreads, 2)
             // that is a sink or inside its window.
             const int b1 = vt * kBN, b2 = b1 + it.skip * 16;
             const int jc0 = it.sg * 16 - b1, jc = jc0 < 0 ? 0 : jc0 > kBN ? kBN : jc0;
-            auto seen_from = [&](int base) -> uint64_t {
-              return cols_to(row_last - base) & (cols_to(sinks - 1 - base) | ~cols_to(row_lo - 1 - base));
+            auto seen_from = [&](int key) -> uint32_t {  // 32 columns from this key on
+              return ~bits_from(row_last + 1 - key) & (~bits_from(sinks - key) | bits_from(row_lo - key));
             };
-            const uint64_t below = cols_to(jc - 1);
-            const uint64_t seen = (seen_from(b1) & below) | (seen_from(b2) & ~below);
-            const uint32_t seen_lo = (uint32_t)seen, seen_hi = (uint32_t)(seen >> 32);
+            const int b = jc == kBN ? b1 : b2;
+            uint32_t seen_lo = seen_from(b), seen_hi = seen_from(b + 32);
+            if (jc > 0 && jc < kBN) {  // the first jc columns are sinks
+              const uint32_t win_lo = bits_from(jc), win_hi = bits_from(jc - 32);
+              seen_lo = (seen_lo & win_lo) | (seen_from(b1) & ~win_lo);
+              seen_hi = (seen_hi & win_hi) | (seen_from(b1 + 32) & ~win_hi);
+            }
+            if (__any_sync(0xffffffffu, seen_lo != 0xffffffffu)) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              sv[c] = (seen_lo >> c) & 1u ? sv[c] : -INFINITY;
-              sv[32 + c] = (seen_hi >> c) & 1u ? sv[32 + c] : -INFINITY;
+              for (int c = 0; c < 32; ++c) sv[c] = (seen_lo >> c) & 1u ? sv[c] : -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, seen_hi != 0xffffffffu)) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) sv[32 + c] = (seen_hi >> c) & 1u ? sv[32 + c] : -INFINITY;
             }
             // V of the keys that no row of the tile sees becomes zero before the product reads it
             // (their weight is zero, but 0 times a NaN or an infinity is not)
@@ -895,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         float2 acc[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[x] = make_float2(0.f, 0.f);
-        if (split) {
+        if (kExt || split) {  // (the branches differ only in kEmuPairs; one copy of the code for kExt)
 #pragma unroll
           for (int q = 0; q < kBN / 2; ++q) {
             const float2 x2 = __ffma2_rn(make_float2(sv[2 * q], sv[2 * q + 1]), sl2v, nmu);
