@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   int* last_flag = abort_flag + 1;
   int64_t* item_ring = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars) + 256);  // [4]
 
+  if (kExt && p.lse != nullptr) pdl_trigger();  // the key scores' kernel follows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // cluster: CTA rank c of a cluster takes chunk c of its unit
   int64_t first_item = blockIdx.x;

@@ -195,6 +195,13 @@ __device__ __forceinline__ void record_error(int* err, int code) {
   if (err != nullptr) atomicCAS(err, 0, code);
 }
 
+// Programmatic dependent launch.  A kernel that calls pdl_trigger lets the next one in the stream
+// take free SM slots once all of its own CTAs run; that one (launched with the programmatic
+// attribute) touches nothing of the first one's results before pdl_wait, which returns when the
+// first one is complete and its memory visible.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Named barrier over `nthreads` threads (a multiple of 32), id 1..15.
 __device__ __forceinline__ void named_barrier(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   int* tile_pid = stage_valid + NS;
   int* s_flag = tile_pid + kMaxChunkTiles;
 
+  if (kExt && p.lse != nullptr && p.scores == nullptr) pdl_trigger();  // the key scores' kernel follows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // 32-bit index arithmetic (the plan bounds units, rows and tiles below 2^31): a 64-bit
   // division costs about a hundred instructions, and these sit in front of the first
