@@ -1383,7 +1383,9 @@ Sm100Plan plan_sm100(const PagedArgs& a, bool sizing_only) {
   // 1000 keys, 128 units of 18 tiles: one chunk 33 us, two of 9 tiles 37 us, three of 8 and
   // the work list 64 us).  Up to 8 chunks of a unit form a cluster and merge over distributed
   // shared memory while all CTAs fit at once; more units than that take one chunk each.
-  if (plan.grouped && paged_is_ext(a) && !a.dense && tiles_max <= 96) {
+  // Prompts have no other way to share a unit's keys (3 x 71 tokens, 64 heads, 2.3K keys: 192
+  // items of 36 tiles each); they and dense calls take it at any length.
+  if (paged_is_ext(a) && (!plan.grouped || a.dense || tiles_max <= 96)) {
     int64_t nc = 2 * 148 / plan.n_units;
     if (nc > 8) nc = 8;
     if (nc > tiles_max / 2) nc = tiles_max / 2;

@@ -176,6 +176,13 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   }
   plan.rows_per_block = plan.nwm == 0 ? 8 : 16 * plan.nwm;
   plan.n_row_blocks = (M + plan.rows_per_block - 1) / plan.rows_per_block;
+  // Under a window a block of rows of one head reaches over that many keys more than the window;
+  // one that spans two heads' ends would walk the windows of all L tokens.
+  plan.head_blocks = 0;
+  if (a.window > 0 && plan.nwm == 4 && a.L >= plan.rows_per_block) {
+    plan.head_blocks = (a.L + plan.rows_per_block - 1) / plan.rows_per_block;
+    plan.n_row_blocks = plan.head_blocks * (a.Hq / a.Hkv);
+  }
   plan.rows_real = M < plan.rows_per_block ? M : plan.rows_per_block;
   plan.n_units = a.B * a.Hkv * plan.n_row_blocks;
   if (plan.n_units > INT32_MAX) return plan;
@@ -189,7 +196,9 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   if (ext && (keys >= (int64_t(1) << 30) || a.P * a.Hkv * a.page_size > INT32_MAX - 64)) return plan;
   if (a.window > 0) {
     // the sinks' tiles and those that the windows of L tokens touch
-    const int64_t seen = (a.sinks + 15) / 16 + (a.window + a.L - 1 + 15) / 16 + 1;
+    // (without the causal limit every row sees on to the last key)
+    const int64_t span = a.is_causal && plan.head_blocks > 0 ? plan.rows_per_block : a.L;
+    const int64_t seen = (a.sinks + 15) / 16 + (a.window + span - 1 + 15) / 16 + 1;
     if (seen < tiles_max) {
       tiles_max = seen;
       even_units = true;

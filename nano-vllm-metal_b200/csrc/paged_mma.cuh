@@ -74,6 +74,8 @@ struct MmaParams {
   int causal;
   int cluster;        // the n_chunks CTAs of a unit are one cluster: merge over DSMEM
   int64_t window, sinks;  // kExt: window == 0 for none
+  int out_vec;            // kExt: out is aligned for four elements at once
+  int64_t nb;             // kExt: row blocks per q head (a block then never spans two), 0: over all g * L rows
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
   const void* k_scales;   // kExt: int8 pages' scales, copied by row
   const void* v_scales;
@@ -196,8 +198,15 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   const int64_t ctx = p.context_lens ? (int64_t)p.context_lens[b] : p.dense_ctx;
   const int64_t cap = p.mp * p.ps;
   const int64_t ctx_limit = ctx < cap ? ctx : cap;
-  const int64_t row0 = rb * C::kRB;
-  const int64_t rows_here = (p.M - row0) < C::kRB ? (p.M - row0) : C::kRB;
+  int64_t row0 = rb * C::kRB, row_end = p.M;
+  if constexpr (kExt) {
+    if (p.nb > 0) {
+      const uint32_t head = (uint32_t)rb / (uint32_t)p.nb, j = (uint32_t)rb - head * (uint32_t)p.nb;
+      row0 = (int64_t)head * p.L + (int64_t)j * C::kRB;
+      row_end = ((int64_t)head + 1) * p.L;
+    }
+  }
+  const int64_t rows_here = (row_end - row0) < C::kRB ? (row_end - row0) : C::kRB;
   const int64_t t_begin = c * p.ct;
 
   if (threadIdx.x == 0) {
@@ -215,8 +224,8 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   const int64_t q_row0 = (b * p.Hq + h * p.g) * p.L;  // flat row of (b, h, m = 0)
   // this thread's two softmax rows (unit-relative): m16 tile rows r, r + 8; n8 tile
   // columns 2 cq, 2 cq + 1.  The n8 tile's Q operand is row r (loaded as "row A").
-  const int64_t mA = C::kN8 ? row0 + r : row0 + wm * 16 + r, mB = C::kN8 ? p.M : mA + 8;
-  const bool vA = mA < p.M, vB = mB < p.M;
+  const int64_t mA = C::kN8 ? row0 + r : row0 + wm * 16 + r, mB = C::kN8 ? row_end : mA + 8;
+  const bool vA = mA < row_end, vB = mB < row_end;
   const int64_t sA = C::kN8 ? row0 + 2 * cq : mA, sB = C::kN8 ? sA + 1 : mB;
   uint32_t qa[NKS][4];
   if (warp < C::kCons) {
@@ -299,6 +308,10 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     }
   }
   auto tile_of = [&](int v) -> int { return v >= x_sink_tiles ? v + x_skip : v; };  // kExt
+  if constexpr (kExt) {  // a chunk past the unit's keys ends here, before any barrier
+    const int chunks = x_tiles > 0 ? (int)((uint32_t)(x_tiles + p.ct - 1) / (uint32_t)p.ct) : 1;
+    if (c >= chunks && !(C::kClusterFits && p.cluster)) return;
+  }
   const int t0 = (int)t_begin;
   if (warp == (C::kSelfFeed ? 0 : C::kCons) && !(kExt && p.block_table == nullptr)) {
     // The chunk's block-table entries, read together with (not after) the context
@@ -446,8 +459,8 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   const Tok BIG = kExt ? (Tok)kExtLimit : (Tok)(INT64_MAX / 4);
   Tok limA = BIG, limB = BIG;
   if (p.causal) {
-    if (sA < p.M) limA = (Tok)((int64_t)((uint32_t)sA % (uint32_t)p.L) + ctx - p.L);
-    if (sB < p.M) limB = (Tok)((int64_t)((uint32_t)sB % (uint32_t)p.L) + ctx - p.L);
+    if (sA < row_end) limA = (Tok)((int64_t)((uint32_t)sA % (uint32_t)p.L) + ctx - p.L);
+    if (sB < row_end) limB = (Tok)((int64_t)((uint32_t)sB % (uint32_t)p.L) + ctx - p.L);
     if constexpr (kExt) {  // a context length past the table's end may be as large as an int
       limA = limA < BIG ? limA : BIG;
       limB = limB < BIG ? limB : BIG;
@@ -458,8 +471,8 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   if constexpr (kExt) {
     if (p.window > 0) {
       const int64_t base = ctx - p.L - p.window + 1;
-      const int64_t a = sA < p.M ? (int64_t)((uint32_t)sA % (uint32_t)p.L) + base : 0;
-      const int64_t b2 = sB < p.M ? (int64_t)((uint32_t)sB % (uint32_t)p.L) + base : 0;
+      const int64_t a = sA < row_end ? (int64_t)((uint32_t)sA % (uint32_t)p.L) + base : 0;
+      const int64_t b2 = sB < row_end ? (int64_t)((uint32_t)sB % (uint32_t)p.L) + base : 0;
       loA = a > 0 ? (int)a : 0;
       loB = b2 > 0 ? (int)b2 : 0;
       lo_max = loA > loB ? loA : loB;
@@ -958,6 +971,49 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   auto put_lse = [&](int rl, float ms, float ls) {
     if (p.lse != nullptr) p.lse[q_row0 + row0 + rl] = ls > 0.f ? ms + log2f(ls) : INFINITY;
   };
+  // kExt: four elements at a time (one element a thread and step made the epilogue of a 64-row
+  // block 3800 of its instructions: a chunk of 927 int8 tokens under 3 keys took 107 us, with blocks inside heads and this 34 us).
+  auto put4 = [&](int rl, int d, float4 o4, float ls) {
+    const float inv = ls > 0.f ? 1.f / ls : 0.f;
+    const int64_t at = (q_row0 + row0 + rl) * D + d;
+    o4 = make_float4(o4.x * inv, o4.y * inv, o4.z * inv, o4.w * inv);
+    if (p.out_vec == 0) {
+      store_dyn(p.out, at, p.out_dtype, o4.x);
+      store_dyn(p.out, at + 1, p.out_dtype, o4.y);
+      store_dyn(p.out, at + 2, p.out_dtype, o4.z);
+      store_dyn(p.out, at + 3, p.out_dtype, o4.w);
+    } else if (p.out_dtype == NVM_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = o4;
+    } else if (p.out_dtype == NVM_BF16) {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+          make_uint2(pack2<__nv_bfloat16>(o4.x, o4.y), pack2<__nv_bfloat16>(o4.z, o4.w));
+    } else {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+          make_uint2(pack2<__half>(o4.x, o4.y), pack2<__half>(o4.z, o4.w));
+    }
+  };
+  // kExt: this CTA's row rl, elements d .. d + 3, over its warps along the keys
+  auto combine4 = [&](int rl, int d, float& ms, float& ls) -> float4 {
+    ms = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NWK; ++w) ms = fmaxf(ms, em[w * C::kRB + rl]);
+    ls = 0.f;
+    float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < NWK; ++w) {
+      const float mw = em[w * C::kRB + rl];
+      if (mw != -INFINITY) {
+        const float f = exp2f(mw - ms);
+        const float4 v = *reinterpret_cast<const float4*>(eo + (w * C::kRB + rl) * D + d);
+        ls += el[w * C::kRB + rl] * f;
+        o4.x += v.x * f;
+        o4.y += v.y * f;
+        o4.z += v.z * f;
+        o4.w += v.w * f;
+      }
+    }
+    return o4;
+  };
   // The weights of virtual keys [v0, v1), by all consumer threads, after put_lse of every row:
   // new keys (the last L positions) start at zero, the others gain.
   auto add_mass = [&](int v0, int v1) {
@@ -1010,7 +1066,15 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
       float2* cb_ml = reinterpret_cast<float2*>(cb_o + C::kRB * D);   // [kRB]
       float* cw = reinterpret_cast<float*>(cb_ml + C::kRB);           // [8][kRB] chunk weights
       float* cwl = cw + 8 * C::kRB;                                   // [kRB]
-      for (int64_t idx = tid; idx < rows_here * D; idx += NCT) {
+      if constexpr (kExt) {
+        for (int g4 = tid; g4 < (int)rows_here * (D / 4); g4 += NCT) {
+          const int rl = g4 / (D / 4), d = (g4 % (D / 4)) * 4;
+          float ms, ls;
+          *reinterpret_cast<float4*>(cb_o + rl * D + d) = combine4(rl, d, ms, ls);
+          if (d == 0) cb_ml[rl] = make_float2(ms, ls);
+        }
+      }
+      for (int64_t idx = tid; !kExt && idx < rows_here * D; idx += NCT) {
         const int rl = (int)(idx / D), d = (int)(idx % D);
         float ms = -INFINITY;
 #pragma unroll
@@ -1062,8 +1126,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
             }
           }
           const float ls = cwl[rl];
+          if constexpr (kExt) put4(rl, d, make_float4(o4[0], o4[1], o4[2], o4[3]), ls);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; !kExt && e < 4; ++e)
             store_dyn(p.out, (q_row0 + row0 + rl) * D + d + e, p.out_dtype, ls > 0.f ? o4[e] / ls : 0.f);
         }
       }
@@ -1076,7 +1141,21 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
   }
   const bool single = n_chunks == 1;
   const int64_t wsrow = (unit * p.n_chunks + c) * p.rows_real;
-  for (int64_t idx = tid; idx < rows_here * D; idx += NCT) {
+  if constexpr (kExt) {
+    for (int g4 = tid; g4 < (int)rows_here * (D / 4); g4 += NCT) {
+      const int rl = g4 / (D / 4), d = (g4 % (D / 4)) * 4;
+      float ms, ls;
+      const float4 o4 = combine4(rl, d, ms, ls);
+      if (single) {
+        put4(rl, d, o4, ls);
+        if (d == 0) put_lse(rl, ms, ls);
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (wsrow + rl) * D + d) = o4;
+        if (d == 0) p.part_ml[wsrow + rl] = make_float2(ms, ls);
+      }
+    }
+  }
+  for (int64_t idx = tid; !kExt && idx < rows_here * D; idx += NCT) {
     const int rl = (int)(idx / D), d = (int)(idx % D);
     float ms = -INFINITY;
 #pragma unroll
@@ -1093,9 +1172,6 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     }
     if (single) {
       store_dyn(p.out, (q_row0 + row0 + rl) * D + d, p.out_dtype, ls > 0.f ? os / ls : 0.f);
-      if constexpr (kExt) {
-        if (d == 0) put_lse(rl, ms, ls);
-      }
     } else {
       p.part_o[(wsrow + rl) * D + d] = os;
       if (d == 0) p.part_ml[wsrow + rl] = make_float2(ms, ls);
@@ -1177,8 +1253,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
         }
       }
       const float ls = wl[rl];
+      if constexpr (kExt) put4(rl, d, make_float4(os[0], os[1], os[2], os[3]), ls);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; !kExt && e < 4; ++e)
         store_dyn(p.out, (q_row0 + row0 + rl) * D + d + e, p.out_dtype, ls > 0.f ? os[e] / ls : 0.f);
     }
     if (tid == 0) p.counters[unit] = 0;
@@ -1289,6 +1366,9 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.causal = a.is_causal;
   p.cluster = 0;
+  const uintptr_t out_align = a.out_dtype == NVM_F32 ? 15 : 7;
+  p.out_vec = (reinterpret_cast<uintptr_t>(a.out) & out_align) == 0 ? 1 : 0;
+  p.nb = plan.head_blocks;
   p.window = a.window; p.sinks = a.sinks; p.lse = a.lse; p.scores = a.scores;
   p.mass = a.mass; p.mass_sb = a.mass_sb; p.mass_sh = a.mass_sh; p.mass_len = a.mass_len;
   p.k_scales = a.k_scales; p.v_scales = a.v_scales;

@@ -73,6 +73,9 @@ WINDOW_CASES = [
     ([300, 50], 3, 6, 2, 80, 7, F32, F32, 40, 5),                 # odd head dim and page size, fp32
     ([3000, 0, 1], 7, 8, 1, 128, 16, BF, BF, 2000, 9),            # one row tile over eight chunks, empty and tiny contexts
     ([2500, 1800, 60, 3], 40, 16, 2, 128, 16, HF, HF, 700, 4),    # 320 rows a kv head: several row tiles
+    ([3000, 900], 191, 8, 4, 128, 16, BF, BF, 2900, 4),           # a chunk whose keys a cluster shares
+    ([900, 300], 300, 4, 1, 128, 128, I8, HF, 3, 0),              # int8 chunk, row blocks within heads of odd length
+    ([500, 64], 64, 4, 2, 64, 16, HF, HF, 20, 1),                 # blocks of exactly one head each
     ([300, 20], 1, 4, 4, 96, 24, HF, F32, 33, 2),                 # odd head dim, fp32 queries over fp16
 ]
 
@@ -187,6 +190,21 @@ def test_key_mass_shorter_than_the_context(path):
     assert_within(gm, mref, merr + 1e-30, "mass")
 
 
+def test_out_at_any_alignment(path):
+    for L in (1, 5, 80):
+        prob = make_problem(12 + L, [300, 90], L, 16, 8, 128, 16, BF)
+        p = to_gpu(prob)
+        ref = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", window=100, out_dtype=BF)
+        exact, terms, _, _ = paged_reference(prob, 100, 0)
+        for shift in (1, 4):
+            store = torch.zeros(ref.numel() + 8, dtype=BF, device="cuda")
+            out = store[shift:shift + ref.numel()].view(ref.shape)
+            got = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", window=100, out=out)
+            assert got is out
+            assert_within(out, exact, out_bound(exact, terms, 128, BF, BF), "out")
+            assert not store[:shift].any() and not store[shift + ref.numel():].any()
+
+
 def test_window_as_long_as_the_context_changes_nothing(path):
     prob = make_problem(2, [500, 77, 1300], 1, 32, 8, 128, 16, BF)
     p = to_gpu(prob)
@@ -236,6 +254,8 @@ DENSE_CASES = [  # B, L, S, Hq, Hkv, D, dtype, window, sinks, causal
     (1, 200, 200, 4, 2, 64, HF, 33, 1, True),
     (1, 70, 150, 4, 2, 128, BF, 40, 2, False),
     (1, 40, 60, 4, 2, 72, F32, 11, 2, True),
+    (1, 90, 2000, 8, 2, 128, BF, 1500, 4, True),     # few rows, many keys: a cluster shares them
+    (1, 20, 900, 8, 2, 128, HF, 800, 4, True),       # the rows of a group in one tile, the same
     (1, 20, 8, 4, 2, 128, BF, 3, 1, True),          # more rows than keys: the first rows see none
 ]
 
