@@ -28,7 +28,7 @@
 // jumped over by renumbering (virtual group v is group v below the sinks' end and group
 // v + skip past it), so rings, phases and chunks run unchanged and one tile of four groups can
 // hold the sinks next to the window's start: a tile of its own for 4 sinks cost 7 % of a
-// prompt under a 1024-key window (2 x 4096 tokens, 32/8 heads: 198 us, 610 TFLOP/s of the pairs
+// prompt under a 1024-key window (2 x 4096 tokens, 32/8 heads: 192 us, 630 TFLOP/s of the pairs
 // seen, bound by the softmax warps' issue).  Which tiles need a mask is known per item; the mask of a
 // row is a pattern of two words, built with a few shifts.
 // Every mbarrier wait is bounded; on expiry the CTA records an error, lets its own

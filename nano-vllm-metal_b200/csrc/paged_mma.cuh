@@ -972,7 +972,8 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     if (p.lse != nullptr) p.lse[q_row0 + row0 + rl] = ls > 0.f ? ms + log2f(ls) : INFINITY;
   };
   // kExt: four elements at a time (one element a thread and step made the epilogue of a 64-row
-  // block 3800 of its instructions: a chunk of 927 int8 tokens under 3 keys took 107 us, with blocks inside heads and this 34 us).
+  // block 3800 of its instructions: a chunk of 927 int8 tokens under a 3-key window took 107 us,
+  // with this and row blocks inside heads 34 us).
   auto put4 = [&](int rl, int d, float4 o4, float ls) {
     const float inv = ls > 0.f ? 1.f / ls : 0.f;
     const int64_t at = (q_row0 + row0 + rl) * D + d;

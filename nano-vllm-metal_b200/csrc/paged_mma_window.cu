@@ -1,7 +1,7 @@
 // paged_mma_window.cu -- instances of the tensor-core paged attention kernel (paged_mma.cuh)
 // with a sliding window, sinks and row log-sum-exps, one per default variant of the plan.
 // Measured on a B200: 64 requests of 4K-16K keys under a window of 4096 with 4 sinks, 32/8 heads,
-// bf16: 173 us, 6.2 TB/s of the keys seen (0.95 of a copy's rate); 48 requests under 2048, 64/8
+// bf16: 170-177 us, 6.1-6.3 TB/s of the keys seen (0.93-0.96 of a copy's rate); 48 requests under 2048, 64/8
 // heads, int8 pages: 59 us, 3.5 TB/s, bound by the int8 tile's instructions as without a window.
 #include "paged_mma.cuh"
 
