@@ -86,7 +86,8 @@ static_assert(kBins % 1024 == 0, "every thread clears and scans whole bins");
 // and so are made once (4700 instructions a warp were 2000 too many when every pass made them
 // again); the weights themselves are read a second time when they move.
 template <int T, bool kHeld>
-__device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, float* mout, int32_t* keep, int n, int lo, int hi, int k) {
+__device__ __forceinline__ void select_row(SelSmem<T>& sm, const float* mass, float* mout, int32_t* keep, int n, int lo,
+                                           int hi, int k) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int stretches = (n + T - 1) / T;
   uint32_t img[kPer];    // kHeld: the whole row's; else one sweep's

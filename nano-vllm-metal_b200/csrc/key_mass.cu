@@ -28,8 +28,8 @@
 //    start of its CTAs.
 //  * everything else (fp32, other head dims): key_mass_generic_kernel.
 // Measured on a B200 (32/8 heads, bf16): 64 requests of 2K-16K keys 26 us for 74 MB of scores
-// (the whole scored step 430 us, 0.85 of a copy's rate for its K and V); prompts of 2 x 2048 tokens 60 us next to 102 us of
-// attention, 570 TFLOP/s of S^T.
+// (the whole scored step 430 us, 0.85 of a copy's rate for its K and V); prompts of 2 x 2048
+// tokens 60 us next to 102 us of attention (570 TFLOP/s of S^T), ten of them behind its last wave.
 #include <cooperative_groups.h>
 
 #include <cstdlib>

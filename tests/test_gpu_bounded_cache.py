@@ -451,9 +451,10 @@ def test_evict_on_another_stream_and_captured():
 # ---------------------------------------------------------------------------
 # graphs, streams, repeatability
 # ---------------------------------------------------------------------------
-def test_two_captured_graphs_replayed_side_by_side():
-    probs = [make_problem(20 + i, [2500, 3100, 1000], 1, 64, 8, 128, 16, BF) for i in range(2)]
-    masses = [torch.rand(3, 8, 3200) for _ in range(2)]
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_two_captured_graphs_replayed_side_by_side(L):
+    probs = [make_problem(20 + i, [2500, 2900, 1000], L, 64 if L == 1 else 16, 8, 128, 16, BF) for i in range(2)]
+    masses = [torch.rand(3, 8, 2900) for _ in range(2)]
     gpu, refs, outs, graphs, gms = [], [], [], [], []
     for prob, mass in zip(probs, masses):
         refs.append(paged_reference(prob, 2000, 4, mass=mass))
@@ -473,6 +474,27 @@ def test_two_captured_graphs_replayed_side_by_side():
             with torch.cuda.stream(s):
                 gm.copy_(mass)
                 graph.replay()
+    torch.cuda.synchronize()
+    for (ref, terms, mref, merr), out, gm in zip(refs, outs, gms):
+        assert_within(out, ref, out_bound(ref, terms, 128, BF, F32), "out")
+        assert_within(gm, mref, merr + 1e-30, "mass")
+
+
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_two_streams_at_once(L):
+    probs = [make_problem(60 + i, [1500, 2900, 700], L, 64 if L == 1 else 16, 8, 128, 16, BF) for i in range(2)]
+    masses = [torch.rand(3, 8, 2900) for _ in range(2)]
+    refs = [paged_reference(p, 0, 0, mass=m) for p, m in zip(probs, masses)]
+    gpu, gms = [to_gpu(p) for p in probs], [m.cuda() for m in masses]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [None, None]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                gms[i].copy_(masses[i])
+                p = gpu[i]
+                outs[i] = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=gms[i])
     torch.cuda.synchronize()
     for (ref, terms, mref, merr), out, gm in zip(refs, outs, gms):
         assert_within(out, ref, out_bound(ref, terms, 128, BF, F32), "out")
