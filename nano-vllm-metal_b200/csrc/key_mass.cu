@@ -111,19 +111,27 @@ __global__ void __launch_bounds__(kGenWarps * 32) key_mass_generic_kernel(MassPa
 // Scores kept by the attention kernel: [B*Hkv][v_keys][rows_pad] base-2 scores (-inf where a
 // row does not see the key) on the attention kernel's virtual keys; a thread takes
 // kScoreKeys keys, 256 apart, so that enough loads are in flight.
+// Where the attention kernel left the units' chunks unmerged (kMerge), every CTA finds its unit's
+// log-sum-exps from the chunks' (m, l), a warp a row, and one more CTA per unit merges the rows.
 struct ScoreParams {
   const float* scores;
-  int64_t v_keys;
+  const float2* part_ml;  // kMerge: [B*Hkv][n_chunks][rows]; else the log-sum-exps are in MassParams::lse
+  const float* part_o;    // [B*Hkv][n_chunks][rows][D]
+  void* out;
+  int out_dtype;
+  int64_t v_keys, n_chunks, ct;
   int rows;  // kRows: rows rounded up to even
 };
 constexpr int kScoreKeys = 4;
 
-template <int kRows>
+// kMerge: two instances, since the merge's registers cost the plain one 18 us of 430.
+template <int kRows, bool kMerge>
 __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p, const ScoreParams sp) {
   __shared__ float s_lse[8];
   const int64_t bh = blockIdx.x / p.blocks, block = blockIdx.x - bh * p.blocks;
   const int64_t b = bh / p.Hkv, h = bh - b * p.Hkv;
-  if (threadIdx.x < 8) s_lse[threadIdx.x] = (int)threadIdx.x < sp.rows ? p.lse[bh * sp.rows + threadIdx.x] : INFINITY;
+  if (!kMerge && threadIdx.x < 8)
+    s_lse[threadIdx.x] = (int)threadIdx.x < sp.rows ? p.lse[bh * sp.rows + threadIdx.x] : INFINITY;
   const int64_t ctx = p.context_lens[b], cap = p.mp * p.ps;
   const int64_t end = ctx < cap ? ctx : cap;
   // virtual -> real keys, as the attention kernel numbers its 16-key tiles
@@ -136,9 +144,67 @@ __global__ void __launch_bounds__(256) key_mass_scores_kernel(const MassParams p
       tiles = tiles - skip > st ? tiles - skip : st;
     }
   }
-  __syncthreads();
-  const int64_t v0 = block * (256 * kScoreKeys) + threadIdx.x;
   const int64_t v_end = end > 0 ? tiles * 16 : 0;
+  const int64_t chunks = kMerge && end > 0 ? (tiles + sp.ct - 1) / sp.ct : 1;
+  const bool merges = kMerge && block == p.blocks - 1;  // the unit's extra CTA
+  if (merges ? chunks <= 1 : block * (256 * kScoreKeys) >= v_end) return;
+  const int64_t part0 = bh * sp.n_chunks * sp.rows;
+  if constexpr (kMerge) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float lse = INFINITY, top = -INFINITY;
+    if (warp < sp.rows) {
+      if (chunks <= 1) {
+        lse = p.lse[bh * sp.rows + warp];
+      } else {
+        for (int64_t c = lane; c < chunks; c += 32) top = fmaxf(top, sp.part_ml[part0 + c * sp.rows + warp].x);
+        top = warp_max(top);
+        float sum = 0.f;
+        for (int64_t c = lane; c < chunks; c += 32) {
+          const float2 ml = sp.part_ml[part0 + c * sp.rows + warp];
+          if (ml.x != -INFINITY) sum += ml.y * exp2f(ml.x - top);
+        }
+        sum = warp_sum(sum);
+        lse = sum > 0.f ? top + log2f(sum) : INFINITY;
+      }
+    }
+    if (lane == 0) s_lse[warp] = lse;
+  }
+  __syncthreads();
+  if (merges) {
+    // out = sum over the chunks of 2^(m - lse) O
+    const int d4 = (int)p.D / 4;
+    for (int i = threadIdx.x; i < sp.rows * d4; i += 256) {
+      const int row = i / d4, d = (i - row * d4) * 4;
+      const float lse = s_lse[row];
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int64_t c0 = 0; c0 < chunks; c0 += 8) {
+        float4 v[8];
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int64_t at = part0 + (c0 + j) * sp.rows + row;
+          w[j] = c0 + j < chunks ? exp2f(sp.part_ml[at].x - lse) : 0.f;
+          v[j] = c0 + j < chunks ? *reinterpret_cast<const float4*>(sp.part_o + at * p.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (w[j] > 0.f) {  // a chunk without a key of this row holds no sum
+            o.x += v[j].x * w[j];
+            o.y += v[j].y * w[j];
+            o.z += v[j].z * w[j];
+            o.w += v[j].w * w[j];
+          }
+        }
+      }
+      const int64_t at = (bh * sp.rows + row) * p.D + d;
+      store_dyn(sp.out, at, sp.out_dtype, o.x);
+      store_dyn(sp.out, at + 1, sp.out_dtype, o.y);
+      store_dyn(sp.out, at + 2, sp.out_dtype, o.z);
+      store_dyn(sp.out, at + 3, sp.out_dtype, o.w);
+    }
+    return;
+  }
+  const int64_t v0 = block * (256 * kScoreKeys) + threadIdx.x;
   const float* z = sp.scores + bh * sp.v_keys * kRows;
   float* mrow = p.mass + b * p.stride_b + h * p.stride_h;
   float x[kScoreKeys][kRows], old[kScoreKeys];
@@ -616,7 +682,8 @@ bool mass_sm100_eligible(const PagedArgs& a) {
 
 }  // namespace
 
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, bool tensor_cores, cudaStream_t s) {
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, const void* ws, bool tensor_cores,
+                    cudaStream_t s) {
   MassParams p{};
   p.q = a.q; p.k = a.k_pages; p.ks = a.k_scales; p.block_table = a.block_table; p.context_lens = a.context_lens;
   p.lse = a.lse; p.mass = m.mass; p.stride_b = m.stride_b; p.stride_h = m.stride_h; p.len = m.len;
@@ -629,15 +696,19 @@ int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* pla
   if (m.len < keys) keys = m.len;
   if (keys <= 0 || a.B * a.Hkv == 0) return NVM_OK;
   if (a.scores != nullptr) {
-    ScoreParams sp{a.scores, plan->chunk_tiles * plan->n_chunks * 16, (int)(p.g * p.L)};
+    const uint8_t* w = static_cast<const uint8_t*>(ws);
+    ScoreParams sp{a.scores, a.defer ? reinterpret_cast<const float2*>(w + mma_ws_ml()) : nullptr,
+                   reinterpret_cast<const float*>(w + mma_ws_o(*plan)), a.out, a.out_dtype,
+                   plan->chunk_tiles * plan->n_chunks * 16, plan->n_chunks, plan->chunk_tiles, (int)(p.g * p.L)};
     const int64_t per = 256 * kScoreKeys;
-    p.blocks = (sp.v_keys + per - 1) / per;
+    p.blocks = (sp.v_keys + per - 1) / per + (a.defer ? 1 : 0);  // one more: the merge
     if (p.blocks * a.B * a.Hkv > INT32_MAX) return fail(NVM_ERR_UNSUPPORTED, "paged_attention: too many keys for key_mass");
     const dim3 grid((unsigned)(p.blocks * a.B * a.Hkv));
-    if (sp.rows <= 2) key_mass_scores_kernel<2><<<grid, 256, 0, s>>>(p, sp);
-    else if (sp.rows <= 4) key_mass_scores_kernel<4><<<grid, 256, 0, s>>>(p, sp);
-    else if (sp.rows <= 6) key_mass_scores_kernel<6><<<grid, 256, 0, s>>>(p, sp);
-    else key_mass_scores_kernel<8><<<grid, 256, 0, s>>>(p, sp);
+    auto kern = a.defer ? key_mass_scores_kernel<8, true> : key_mass_scores_kernel<8, false>;
+    if (sp.rows <= 2) kern = a.defer ? key_mass_scores_kernel<2, true> : key_mass_scores_kernel<2, false>;
+    else if (sp.rows <= 4) kern = a.defer ? key_mass_scores_kernel<4, true> : key_mass_scores_kernel<4, false>;
+    else if (sp.rows <= 6) kern = a.defer ? key_mass_scores_kernel<6, true> : key_mass_scores_kernel<6, false>;
+    kern<<<grid, 256, 0, s>>>(p, sp);
     return check_cuda(cudaGetLastError(), "paged_attention: key mass kernel launch");
   }
   if (!force_generic() && mass_sm100_eligible(a))

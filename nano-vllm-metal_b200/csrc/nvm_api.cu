@@ -147,6 +147,13 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
 // Stands for the log-sum-exp buffer while a call is planned, before its workspace is known.
 float kLseLater;
 
+// Scored decode through the workspace with fewer units than this leaves its merges to the kernel
+// over the scores: the one CTA of 64 threads that ends a unit needs up to 40 us for 60 chunks
+// while most SMs have run dry (4 kv-head units of 16K keys 59 -> 26 us, 32 of 1.3K-10.7K keys
+// 51 -> 38 us).  With many units the merges hide behind the others' keys (512 units: 430 us,
+// against 460 us deferred).
+constexpr int64_t kDeferUnits = 148;
+
 // Workspace of a windowed / scored call: the attention kernel's own part, then (with key
 // mass) the log-sum-exp of every query row, behind the ticket region in any case: tickets of
 // other calls that share the workspace must stay zero.
@@ -376,7 +383,10 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
   if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
   if (kept > 0) {
     a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
-    if (plan.ws_bytes == 0) a.mass = key_mass;  // the attention kernel weighs them too
+    if (plan.ws_bytes == 0)
+      a.mass = key_mass;  // the attention kernel weighs them too
+    else
+      a.defer = plan.n_units < kDeferUnits ? 1 : 0;
     a.mass_sb = mass_stride_b; a.mass_sh = mass_stride_h; a.mass_len = mass_len;
   }
   st = sp.eligible     ? launch_sm100(a, sp, workspace, s)
@@ -384,7 +394,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
                        : launch_paged_generic(a, s);
   if (st != NVM_OK || key_mass == nullptr || a.mass != nullptr) return st;
   KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
-  return launch_key_mass(a, m, &plan, sp.eligible || plan.eligible, s);
+  return launch_key_mass(a, m, &plan, workspace, sp.eligible || plan.eligible, s);
 }
 
 int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,

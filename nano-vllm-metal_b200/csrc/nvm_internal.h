@@ -63,6 +63,7 @@ struct PagedArgs {
   int64_t window, sinks;
   float* lse;         // [B*Hq*L] log2 of sum 2^(score * log2 e) of every row (+inf: no key), or NULL
   float* scores;      // n8 tile only: keep every base-2 score, [B*Hkv][virtual keys][rows, even], or NULL
+  int defer;          // with scores: leave the merge through the workspace to the kernel over the scores
   float* mass;        // with scores, and no merge through the workspace: add the weights, or NULL
   int64_t mass_sb, mass_sh, mass_len;
 };
@@ -79,8 +80,13 @@ struct KeyMassArgs {
   int64_t stride_b, stride_h, len;
 };
 struct MmaPlan;
-// plan: the attention kernel's, when a.scores is set; tensor_cores: it was not the generic one.
-int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, bool tensor_cores, cudaStream_t s);
+// plan, ws: the attention kernel's, when a.scores is set (with a.defer the launch merges its
+// chunks too); tensor_cores: it was not the generic one.
+int launch_key_mass(const PagedArgs& a, const KeyMassArgs& m, const MmaPlan* plan, const void* ws, bool tensor_cores,
+                    cudaStream_t s);
+// Where a plan's partial results lie in its workspace: (m, l) and O of [units][chunks][rows].
+size_t mma_ws_ml();
+size_t mma_ws_o(const MmaPlan& plan);
 
 // Eviction by accumulated weight (evict.cu).
 struct EvictArgs {

@@ -319,6 +319,11 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   return plan;
 }
 
+size_t mma_ws_ml() { return kCounterBytes; }
+size_t mma_ws_o(const MmaPlan& plan) {
+  return kCounterBytes + align256(plan.n_units * plan.n_chunks * plan.rows_real * sizeof(float2));
+}
+
 int launch_paged_mma(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s) {
   if (paged_is_ext(a)) return launch_paged_mma_window(a, plan, ws, s);
   if (a.kv_dtype == NVM_F16) {

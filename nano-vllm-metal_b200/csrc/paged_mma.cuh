@@ -75,6 +75,7 @@ struct MmaParams {
   int cluster;        // the n_chunks CTAs of a unit are one cluster: merge over DSMEM
   int64_t window, sinks;  // kExt: window == 0 for none
   int out_vec;            // kExt: out is aligned for four elements at once
+  int defer;              // kExt: leave the chunks' merge to the kernel over the kept scores
   int64_t nb;             // kExt: row blocks per q head (a block then never spans two), 0: over all g * L rows
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
   const void* k_scales;   // kExt: int8 pages' scales, copied by row
@@ -1185,6 +1186,9 @@ __global__ void __launch_bounds__(Cfg<KvT, D, NWM, NWK, NS_>::kThreads)
     return;
   }
 
+  if constexpr (kExt && C::kN8) {
+    if (p.defer) return;
+  }
   // Split-K: the last CTA of this unit merges every chunk's partial result.
   __threadfence();
   named_barrier(1, NCT);
@@ -1370,6 +1374,7 @@ int launch_cfg(const PagedArgs& a, const MmaPlan& plan, void* ws, cudaStream_t s
   const uintptr_t out_align = a.out_dtype == NVM_F32 ? 15 : 7;
   p.out_vec = (reinterpret_cast<uintptr_t>(a.out) & out_align) == 0 ? 1 : 0;
   p.nb = plan.head_blocks;
+  p.defer = a.defer;
   p.window = a.window; p.sinks = a.sinks; p.lse = a.lse; p.scores = a.scores;
   p.mass = a.mass; p.mass_sb = a.mass_sb; p.mass_sh = a.mass_sh; p.mass_len = a.mass_len;
   p.k_scales = a.k_scales; p.v_scales = a.v_scales;

@@ -108,6 +108,9 @@ SCORED_CASES = [
     ([1, 0, 5], 1, 8, 8, 128, 16, BF, BF),
     ([777, 64, 2100], 1, 32, 8, 128, 16, BF, BF),
     ([5000, 4500], 1, 64, 8, 128, 16, HF, HF),       # several chunks a unit
+    ([9000, 200, 3], 1, 7, 1, 64, 32, BF, BF),       # dozens of chunks, 7 rows, merged by the scores' kernel
+    ([3000, 2600], 2, 8, 2, 128, 128, I8, HF),       # the same for two tokens over int8 pages
+    ([300] * 12 + [4000] * 8, 1, 64, 8, 128, 16, BF, BF),  # more units than SMs, merged by their own CTAs
     ([33, 1000], 1, 28, 4, 64, 32, HF, HF),
     ([600, 1025], 1, 64, 8, 128, 128, I8, HF),
     ([600, 40], 1, 128, 8, 128, 16, BF, BF),         # 16 rows a kv head
