@@ -328,21 +328,24 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   a.scale_dtype = NVM_F16;
   a.out_dtype = NVM_F32;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
-  a.is_causal = 1; a.window = window; a.sinks = sinks;
+  a.window = window; a.sinks = sinks;
   if (validate_paged(a, false) != NVM_OK || validate_window(window, sinks, "paged_attention") != NVM_OK) return 0;
   if (with_mass) a.lse = &kLseLater;
-  size_t need = 0, scores = 0;
-  if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
-    // q's dtype is not known here: cover both plans
+  // q's dtype and the mask are not known here: cover both kernels' plans, and both masks (without
+  // the causal limit the rows of a block see on to the last key, so windows take more chunks)
+  size_t total = window_ws(a, 0, 0, with_mass != 0).total;
+  for (int causal = 0; causal < 2 && !env_flag("NVM_ATTN_FORCE_GENERIC"); ++causal) {
+    a.is_causal = causal;
     const MmaPlan plan = plan_paged_mma(a);
-    if (plan.eligible) need = plan.ws_bytes;
-    scores = score_bytes(a, plan);
+    size_t need = plan.eligible ? plan.ws_bytes : 0;
     if (!env_flag("NVM_ATTN_NO_SM100")) {
       const Sm100Plan sp = plan_sm100(a, true);
       if (sp.eligible && sp.ws_bytes > need) need = sp.ws_bytes;
     }
+    const size_t t = window_ws(a, need, score_bytes(a, plan), with_mass != 0).total;
+    if (t > total) total = t;
   }
-  return window_ws(a, need, scores, with_mass != 0).total;
+  return total;
 }
 
 int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages, int kv_dtype,

@@ -1,5 +1,8 @@
 """The bounded-cache operators' refusals and host bookkeeping (no GPU needed)."""
 
+import random
+import re
+
 import pytest
 import torch
 
@@ -61,6 +64,37 @@ def test_workspace_sizes():
     with_mass = size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 1)
     assert with_mass >= (1 << 20) + 2 * 32 * 4  # the first MiB holds tickets that stay zero
     assert with_mass > size(2, 32, 8, 1, 128, 16, 8, 2, 0, 0, 0)
+
+
+def _window_workspace_required(causal, B, Hq, Hkv, L, D, ps, mp, kv, window, sinks, mass):
+    """What the entry says it needs.  It refuses a missing workspace before any launch; with ``mass`` it always
+    needs one, so the addresses below (any that are aligned) are never used."""
+    L_ = nv.lib()
+    at, q_dtype, scale_dtype = 1 << 20, 1 if kv == 3 else kv, 1
+    st = L_.nvm_paged_attention_window(at, q_dtype, at, at, kv, at, at, scale_dtype, at, at, at, 0, B, Hq, Hkv, L, D, 64, ps, mp,
+                                       0.1, causal, window, sinks, at if mass else None, Hkv * mp * ps, mp * ps, mp * ps, None, 0,
+                                       None)
+    if st != -3:
+        assert not mass
+        return 0
+    return int(re.search(r"workspace of (\d+) bytes", L_.nvm_last_error().decode()).group(1))
+
+
+def test_workspace_size_covers_what_the_call_needs():
+    rng = random.Random(4)
+    shapes = [(1, 8, 8, 512, 64, 16, 64, 2, 64, 0), (2, 8, 8, 1024, 128, 16, 128, 3, 256, 4), (1, 2, 1, 1024, 128, 16, 64, 2, 64, 0)]
+    for _ in range(1500):
+        Hkv = rng.choice([1, 2, 8])
+        shapes.append((rng.randint(1, 40), Hkv * rng.choice([1, 4, 7, 8]), Hkv, int(2 ** rng.uniform(0, 11)), rng.choice([64, 128]),
+                       rng.choice([16, 128]), rng.randint(1, 300), rng.choice([1, 2, 3]),
+                       rng.choice([0, int(2 ** rng.uniform(0, 12))]), rng.choice([0, 4, 100])))
+    size = nv.lib().nvm_paged_attention_window_workspace_size
+    for shape in shapes:
+        # without a workspace to miss, a call of those addresses would reach the GPU, so only where there is none
+        for mass in (0, 1) if not torch.cuda.is_available() else (1,):
+            for causal in (0, 1):
+                need = _window_workspace_required(causal, *shape, mass)
+                assert size(*shape, mass) >= need, (shape, causal, mass, need)
 
 
 def test_evict_c_entry_refusals():

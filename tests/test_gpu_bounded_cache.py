@@ -228,6 +228,29 @@ def test_window_without_causal(path):
         assert_within(got, ref, out_bound(ref, terms, 128, HF, F32), f"L={L}")
 
 
+@pytest.mark.parametrize("case", [([1020], 512, 8, 8, 64, BF, 64, 0, 64), ([1500, 1100], 1024, 8, 8, 128, I8, 256, 4, 128),
+                                  ([1024], 1024, 2, 1, 128, BF, 64, 0, 64)], ids=["d64", "int8", "tcgen05"])
+def test_long_windows_without_causal_find_their_workspace(case):
+    ctx, L, Hq, Hkv, D, kv, window, sinks, mp = case
+    prob = make_problem(L, ctx, L, Hq, Hkv, D, 16, kv)
+    prob["bt"] = torch.nn.functional.pad(prob["bt"], (0, mp - prob["bt"].shape[1]), value=-1)
+    ref, terms, _, _ = paged_reference(prob, window, sinks, causal=False)
+    p = to_gpu(prob)
+    run = lambda: paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], window=window, sinks=sinks)  # noqa: E731
+    fresh = torch.cuda.Stream()  # no earlier call grew this stream's workspace
+    fresh.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(fresh):
+        got = run()
+    fresh.synchronize()
+    assert_within(got, ref, out_bound(ref, terms, D, kv, F32), "out")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert_within(got, ref, out_bound(ref, terms, D, kv, F32), "captured")
+
+
 def test_holes_inside_the_window(path):
     prob = make_problem(9, [400, 200], 1, 16, 8, 128, 16, BF, holes=[(0, 20), (1, 0), (1, 11)])
     ref, terms, mref, merr = paged_reference(prob, 100, 20, mass=torch.zeros(2, 8, 400))
