@@ -20,6 +20,8 @@ from ..layers.attention import _int32_rows, _row_strides
 
 __all__ = ["EvictResult", "evict_tokens"]
 
+_PAGE_DTYPES = (torch.float32, torch.float16, torch.bfloat16, torch.int8)
+
 
 class EvictResult(NamedTuple):
     keep_index: torch.Tensor  # [B, Hkv, budget] int32: old position of each kept token, -1 behind them
@@ -49,11 +51,41 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     is, with ``dropped`` 0 and ``refused`` not zero; ``status`` (one int32, optional) is then set
     too and is never cleared.
     """
+    return plan_evict(key_pages, value_pages, block_table, context_lens, key_mass, budget, sinks, recent, key_scales,
+                      value_scales, page_refcount, mass_out, status).launch()
+
+
+class EvictPlan:
+    """One checked call of ``evict_tokens``: nothing can refuse it any more.  ``args`` are those of
+    nvm_paged_evict up to the stream, ``written`` the page pools and scales that it rewrites, ``mass``
+    the weights that it selects by; ``held`` keeps converted inputs alive until the launch."""
+
+    __slots__ = ("device", "args", "result", "written", "mass", "held")
+
+    def __init__(self, device, args, result, written, mass, held):
+        self.device, self.args, self.result, self.written, self.mass, self.held = device, args, result, written, mass, held
+
+    def launch(self) -> EvictResult:
+        with nv.on_device(self.device):
+            nv.check(nv.lib().nvm_paged_evict(*self.args, nv.stream_ptr(self.device)))
+        return self.result
+
+
+def overlap(tensors) -> bool:
+    """Do any two of these contiguous tensors share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
+def plan_evict(key_pages, value_pages, block_table, context_lens, key_mass, budget, sinks=0, recent=0, key_scales=None,
+               value_scales=None, page_refcount=None, mass_out=None, status=None) -> EvictPlan:
+    """Every check and allocation of ``evict_tokens``, and no launch."""
     op = "evict"
     out = key_mass if mass_out is None else mass_out
     dev = nv.require_cuda(op, key_pages, value_pages, block_table, context_lens, key_mass, key_scales, value_scales,
                           page_refcount, mass_out, status)
-    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != value_pages.dtype:
+    dtype = key_pages.dtype
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or dtype is not value_pages.dtype:
         raise RuntimeError(f"{op}: key_pages and value_pages must be [P, Hkv, page_size, D] of one dtype")
     if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
         raise RuntimeError(f"{op}: page pools must be contiguous (written in place)")
@@ -72,12 +104,18 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
             raise RuntimeError(f"{op}: mass_out must be float32 with the shape of key_mass")
         osb, osh = _row_strides(f"{op}: mass_out", mass_out)
     sdt = nv.NVM_F16
-    if key_pages.dtype is torch.int8:
+    if dtype not in _PAGE_DTYPES:
+        raise RuntimeError(f"{op}: pages must be float32, float16, bfloat16 or int8")
+    if D > 256:
+        raise RuntimeError(f"{op}: head dimension must be <= 256 (got {D})")
+    if dtype is torch.int8:
         if key_scales is None or value_scales is None:
             raise RuntimeError(f"{op}: int8 pages need key_scales and value_scales")
         for s in (key_scales, value_scales):
             if tuple(s.shape) != (P, Hkv, ps, 1) or not s.is_contiguous() or s.dtype != key_scales.dtype:
                 raise RuntimeError(f"{op}: scales must be contiguous [P, Hkv, page_size, 1] of one dtype")
+        if key_scales.dtype not in _PAGE_DTYPES[:3]:
+            raise RuntimeError(f"{op}: int8 pages need floating-point key and value scales")
         sdt = nv.dtype_code(key_scales.dtype)
     else:
         key_scales = value_scales = None
@@ -89,10 +127,12 @@ def evict_tokens(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table
     bt, cl = _int32_rows(block_table), _int32_rows(context_lens)
     keep = bt.new_empty((B, Hkv, budget))
     kept, dropped, refused = bt.new_empty((3, B)).unbind(0)
-    with nv.on_device(dev):
-        nv.check(nv.lib().nvm_paged_evict(
-            key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(key_scales),
-            nv.ptr(value_scales), sdt, bt.data_ptr(), cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(), msb, msh,
-            key_mass.shape[2], out.data_ptr(), osb, osh, B, Hkv, D, P, ps, MP, budget, sinks, recent, keep.data_ptr(),
-            kept.data_ptr(), dropped.data_ptr(), refused.data_ptr(), nv.ptr(status), nv.stream_ptr(dev)))
-    return EvictResult(keep, kept, dropped, refused)
+    kp, vp = key_pages.data_ptr(), value_pages.data_ptr()
+    written = (key_pages, value_pages) if key_scales is None else (key_pages, value_pages, key_scales, value_scales)
+    if abs(kp - vp) < P * Hkv * ps * D * dtype.itemsize or (key_scales is not None and overlap(written)):
+        raise RuntimeError(f"{op}: page pools and scales must not share memory with one another")
+    args = (kp, vp, nv.dtype_code(dtype), nv.ptr(key_scales), nv.ptr(value_scales), sdt, bt.data_ptr(),
+            cl.data_ptr(), nv.ptr(page_refcount), key_mass.data_ptr(), msb, msh, key_mass.shape[2], out.data_ptr(), osb, osh,
+            B, Hkv, D, P, ps, MP, budget, sinks, recent, keep.data_ptr(), kept.data_ptr(), dropped.data_ptr(),
+            refused.data_ptr(), nv.ptr(status))
+    return EvictPlan(dev, args, EvictResult(keep, kept, dropped, refused), written, key_mass, (bt, cl))

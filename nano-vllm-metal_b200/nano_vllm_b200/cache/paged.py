@@ -470,8 +470,10 @@ class DevicePageTable:
         ``layers``: one ``(key_pages, value_pages, key_mass)`` or ``(key_pages, value_pages,
         key_scales, value_scales, key_mass)`` per layer; ``key_mass`` is updated in place.
         Returns one ``EvictResult`` per layer.  A request that shares a page with another
-        (prefix attach) past its sinks stays as it is and makes ``check_status`` raise."""
-        from .evict import evict_tokens
+        (prefix attach) past its sinks stays as it is and makes ``check_status`` raise.  Every
+        layer is checked before any is touched, and no two may share pages, scales or weights:
+        an exception leaves all of them, and the table, as they were."""
+        from .evict import overlap, plan_evict
 
         layers = [tuple(layer) for layer in layers]
         for layer in layers:  # all of them before any is touched: every layer has to drop the same tokens
@@ -482,14 +484,18 @@ class DevicePageTable:
                 raise ValueError("evict: pages must have the table's page_size and at most its capacity")
             if layer[0].shape[0] != layers[0][0].shape[0] or layer[-1].shape[2] != layers[0][-1].shape[2]:
                 raise ValueError("evict: all layers need the same number of pages and key_mass entries")
-        self.evict_status.zero_()
-        results = []
+        plans = []
         for layer in layers:
-            kp, vp, mass = layer[0], layer[1], layer[-1]
             ks, vs = (layer[2], layer[3]) if len(layer) == 5 else (None, None)
-            results.append(evict_tokens(kp, vp, self.block_table, self.context_lens, mass, budget, sinks=sinks,
-                                        recent=recent, key_scales=ks, value_scales=vs,
-                                        page_refcount=self.refcount, status=self.evict_status))
+            plans.append(plan_evict(layer[0], layer[1], self.block_table, self.context_lens, layer[-1], budget, sinks=sinks,
+                                    recent=recent, key_scales=ks, value_scales=vs, page_refcount=self.refcount,
+                                    status=self.evict_status))
+        if overlap([t for plan in plans for t in plan.written]):
+            raise ValueError("evict: layers must not share page pools or scales")
+        if len({plan.mass.data_ptr() for plan in plans if plan.mass.numel()}) < sum(plan.mass.numel() > 0 for plan in plans):
+            raise ValueError("evict: layers must not share key_mass")
+        self.evict_status.zero_()
+        results = [plan.launch() for plan in plans]
         if results:
             self.rewind(results[0].dropped)
         return results

@@ -6,7 +6,7 @@ import re
 import pytest
 import torch
 
-from nano_vllm_b200 import TinyKvPagedCache, TinyKvPagedPool, evict_tokens, flash_attention, paged_attention
+from nano_vllm_b200 import DevicePageTable, TinyKvPagedCache, TinyKvPagedPool, evict_tokens, flash_attention, paged_attention
 from nano_vllm_b200 import _native as nv
 
 
@@ -123,3 +123,56 @@ def test_request_cache_evict_checks_on_the_host():
     with pytest.raises(ValueError, match="shared"):
         cache.evict(mass, 8)
     assert cache.offset == 10 and cache.num_pages == 3
+
+
+def _layer(int8=False, P=8, D=64):
+    dt = torch.int8 if int8 else torch.bfloat16
+    k, v = (torch.zeros(P, 2, 16, D, dtype=dt) for _ in range(2))
+    scales = [torch.zeros(P, 2, 16, 1, dtype=torch.float16) for _ in range(2)] if int8 else []
+    return (k, v, *scales, torch.zeros(1, 2, 64))
+
+
+def _changed(layer, **at):
+    layer = list(layer)
+    for i, x in at.items():
+        layer[int(i[1:])] = x
+    return tuple(layer)
+
+
+def test_table_evict_checks_every_layer_before_it_launches_any(monkeypatch):
+    calls = []
+
+    class Lib:
+        def nvm_paged_evict(self, *args):
+            calls.append(args)
+            return 0
+
+    monkeypatch.setattr(nv, "lib", Lib)
+    monkeypatch.setattr(nv, "require_cuda", lambda op, *t: torch.device("cpu"))
+    monkeypatch.setattr(nv, "stream_ptr", lambda dev: 0)
+    table = DevicePageTable(1, 4, 16, 8, device="cpu")
+    monkeypatch.setattr(table, "rewind", lambda n: calls.append("rewind"))
+    good, other, wide = _layer(), _layer(int8=True), _layer(D=32)
+    assert len(table.evict([good, other, wide], 20)) == 3 and len(calls) == 4 and calls[-1] == "rewind"
+    calls.clear()
+    shared = _layer()
+    for bad in (_changed(_layer(), i2=torch.zeros(1, 2, 64, dtype=torch.float64)),  # weights of another type,
+                _changed(_layer(), i2=torch.zeros(1, 3, 64)),                       # of other heads,
+                _changed(_layer(), i2=torch.zeros(2, 2, 64)),                       # another batch,
+                _changed(_layer(), i2=torch.zeros(1, 2, 128)[:, :, ::2]),           # with gaps between them
+                _layer(int8=True)[:2] + _layer()[2:],                               # 8-bit pages without scales
+                _changed(_layer(int8=True), i2=torch.zeros(8, 2, 16, dtype=torch.float16)),
+                _changed(_layer(), i1=torch.zeros(8, 2, 16, 64, dtype=torch.float16)),  # K and V of two types
+                _changed(_layer(), i0=torch.zeros(8, 2, 64, 16).bfloat16().transpose(2, 3)),
+                _layer(D=300),
+                _changed(_changed(_layer(), i0=torch.zeros(8, 2, 16, 64, dtype=torch.int32)),
+                         i1=torch.zeros(8, 2, 16, 64, dtype=torch.int32)),
+                _changed(_changed(_layer(int8=True), i2=torch.zeros(8, 2, 16, 1, dtype=torch.int32)),
+                         i3=torch.zeros(8, 2, 16, 1, dtype=torch.int32)),
+                _changed(shared, i1=shared[0]),                                     # K is V
+                _changed(_layer(), i0=good[0]),                                     # pages of the other layer
+                _changed(_layer(), i1=good[1]),
+                _changed(_layer(), i2=good[2])):                                    # weights of the other layer
+        with pytest.raises((RuntimeError, ValueError), match="evict"):
+            table.evict([good, bad], 20)
+        assert calls == []

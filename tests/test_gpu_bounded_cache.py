@@ -628,6 +628,23 @@ def test_table_evict_wants_layers_alike():
     assert table.context_lens.tolist() == [50]
 
 
+def test_table_evict_with_a_faulty_layer_touches_none():
+    table = DevicePageTable(1, 4, 16, 8)
+    table.append(torch.tensor([50], dtype=torch.int32, device="cuda"))
+    layers = [(*(torch.randn(8, 2, 16, 64, device="cuda").to(BF) for _ in range(2)), torch.rand(1, 2, 64, device="cuda"))
+              for _ in range(2)]
+    before = [[x.clone() for x in layer] for layer in layers]
+    (k, v, mass), first = layers[1], layers[0]
+    for bad in ((k, v, mass.double()), (k, v, torch.rand(1, 3, 64, device="cuda")), (k, first[1], mass), (k, v, first[2]),
+                (k.to(I8), v.to(I8), mass), (k, v, mass.cpu())):
+        with pytest.raises((RuntimeError, ValueError), match="evict"):
+            table.evict([first, bad], 20)
+        assert table.context_lens.tolist() == [50]
+        assert all(torch.equal(x, y) for layer, old in zip(layers, before) for x, y in zip(layer, old))
+    table.evict(layers, 20)
+    assert table.context_lens.tolist() == [20]
+
+
 def test_request_cache_evict():
     gen = torch.Generator().manual_seed(2)
     pool = TinyKvPagedPool(page_size=16, kv_bits=8)
