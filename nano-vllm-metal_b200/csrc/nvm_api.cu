@@ -98,9 +98,16 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* 
     estride[i] = 1;
     if (i + 1 < rank) gstride[i] = strides_bytes[i];
   }
-  CUresult r = g_encode(map, dt, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode(map, dt, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstride, bdim, estride,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  // A driver call does not bind the device's context to a host thread that has called nothing
+  // yet; the runtime does.
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
   if (r != CUDA_SUCCESS) return fail(NVM_ERR_CUDA, "nvm: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return NVM_OK;
 }

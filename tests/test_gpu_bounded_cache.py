@@ -1,6 +1,7 @@
 """Windowed attention with sinks, attention with key scores, and eviction, against 64 bits."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -525,6 +526,35 @@ def test_two_streams_at_once(L):
     for (ref, terms, mref, merr), out, gm in zip(refs, outs, gms):
         assert_within(out, ref, out_bound(ref, terms, 128, BF, F32), "out")
         assert_within(gm, mref, merr + 1e-30, "mass")
+
+
+@pytest.mark.parametrize("L", [1, 6, 80])
+@pytest.mark.parametrize("kind", ["plain", "window", "dense", "scored"])
+def test_first_call_of_a_thread(L, kind):
+    """A thread's first call to CUDA may be one of the library's."""
+    prob = make_problem(90 + L, [600, 700], L, 16, 8, 128, 16, BF)
+    ref, terms, _, _ = paged_reference(prob, 100 if kind == "window" else 0, 4)
+    p, got, mass = to_gpu(prob), [], torch.zeros(2, 8, 700, device="cuda")
+    dense = torch.randn(2, 8, 300, 128, device="cuda").to(BF)
+    want = flash_attention(p["q"], dense, dense, mask="causal", window=50)
+    torch.cuda.synchronize()
+
+    def run():
+        if kind == "dense":
+            got.append(flash_attention(p["q"], dense, dense, mask="causal", window=50))
+        else:
+            got.append(paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", sinks=4,
+                                       window=100 if kind == "window" else None, key_mass=mass if kind == "scored" else None))
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1, "the call raised"
+    if kind == "dense":
+        assert torch.equal(got[0], want)
+    else:
+        assert_within(got[0], ref, out_bound(ref, terms, 128, BF, F32), "out")
 
 
 @pytest.mark.parametrize("L", [1, 4, 100])
