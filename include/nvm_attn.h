@@ -126,7 +126,9 @@ int nvm_selftest_wait_expiry(int64_t limit_ns, unsigned long long* waited_ns, vo
  *              filled before the first use and every successful call leaves it
  *              zero again, so one workspace serves calls of any shape; the rest
  *              is overwritten by every call.  May be NULL if the size is 0.
- *              Calls that share one workspace must not overlap on the GPU.
+ *              Calls that share one workspace must not overlap on the GPU, nor on the
+ *              host: a call may launch several kernels, so two host threads on one
+ *              stream have to take turns.
  */
 int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const void* v_pages,
                         int kv_dtype, const void* k_scales, const void* v_scales, int scale_dtype,

@@ -145,12 +145,24 @@ def on_device(device: torch.device):
 # the GPU.  A call whose bounded wait expired may leave tickets non-zero, so
 # device_error() re-zeroes every workspace of the device after a non-zero word.
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+# A call that uses the workspace may launch several kernels, the later ones on what the first left
+# there, and ctypes drops the interpreter lock meanwhile: host threads that share a stream take turns.
+_workspace_locks: dict[tuple[int, int], threading.Lock] = {}
+
+
+def _workspace_key(device: torch.device) -> tuple[int, int]:
+    return device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device)
+
+
+def workspace_lock(device: torch.device) -> threading.Lock:
+    """To be held from ``workspace(device, ...)`` until the call that uses it has returned."""
+    return _workspace_locks.setdefault(_workspace_key(device), threading.Lock())
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if nbytes == 0:
         return None
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device))
+    key = _workspace_key(device)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
@@ -163,9 +175,10 @@ def call_with_workspace(device: torch.device, size, call) -> None:
 
     The buffer cached for (device, stream) is offered first, whatever its size: a call that
     needs more says so before any GPU work, and only then is the size asked for and the buffer
-    grown.  While a CUDA graph is being captured the call gets a buffer of its own instead (from
-    the graph's memory pool; the zero fill of its tickets becomes a graph node): a graph replays
-    with the addresses it captured, on any stream and beside any other graph."""
+    grown.  Threads on one stream take turns (0.5 us).  While a CUDA graph is being captured the
+    call gets a buffer of its own instead (from the graph's memory pool; the zero fill of its
+    tickets becomes a graph node): a graph replays with the addresses it captured, on any stream
+    and beside any other graph."""
     stream = stream_ptr(device)
     if torch.cuda.is_current_stream_capturing():
         nbytes = size()
@@ -174,11 +187,13 @@ def call_with_workspace(device: torch.device, size, call) -> None:
             ws[:1 << 20].zero_()
         check(call(ptr(ws), nbytes, stream))
         return
-    ws = _workspaces.get((device.index if device.index is not None else torch.cuda.current_device(), stream))
-    status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
-    if status == NVM_ERR_WORKSPACE:
-        nbytes = size()
-        status = call(ptr(workspace(device, nbytes)), nbytes, stream)
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+    with _workspace_locks.get(key) or workspace_lock(device):
+        ws = _workspaces.get(key)
+        status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
+        if status == NVM_ERR_WORKSPACE:
+            nbytes = size()
+            status = call(ptr(workspace(device, nbytes)), nbytes, stream)
     check(status)
 
 
@@ -194,7 +209,7 @@ def device_error(device: torch.device, clear: bool = True) -> int:
         if word != 0:
             index = device.index if device.index is not None else torch.cuda.current_device()
             torch.cuda.synchronize(device)
-            for (dev_index, _), ws in _workspaces.items():
+            for (dev_index, _), ws in list(_workspaces.items()):
                 if dev_index == index:
                     ws.zero_()
             torch.cuda.synchronize(device)

@@ -282,8 +282,8 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     L_ = nv.lib()
     kvc = nv.dtype_code(kp.dtype)
     ws_bytes = L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc)
-    ws = nv.workspace(dev, ws_bytes)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(dev), nv.workspace_lock(dev):
+        ws = nv.workspace(dev, ws_bytes)
         nv.check(L_.nvm_paged_attention(
             q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
             bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps,

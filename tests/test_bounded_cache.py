@@ -1,7 +1,10 @@
 """The bounded-cache operators' refusals and host bookkeeping (no GPU needed)."""
 
+import contextlib
 import random
 import re
+import threading
+import time
 
 import pytest
 import torch
@@ -176,3 +179,73 @@ def test_table_evict_checks_every_layer_before_it_launches_any(monkeypatch):
         with pytest.raises((RuntimeError, ValueError), match="evict"):
             table.evict([good, bad], 20)
         assert calls == []
+
+
+class _Turns:
+    """Counts how many threads are inside at once."""
+
+    def __init__(self, inside=lambda: time.sleep(0.02)):
+        self.now = self.most = 0
+        self.inside, self.lock = inside, threading.Lock()
+
+    def __call__(self, *args):
+        with self.lock:
+            self.now += 1
+            self.most = max(self.most, self.now)
+        self.inside()
+        with self.lock:
+            self.now -= 1
+        return 0
+
+
+def _in_threads(n, f):
+    failed = []
+
+    def run(i):
+        try:
+            f(i)
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_threads_on_one_stream_take_turns(monkeypatch):
+    """The kernels of a call find what its first one left in the stream's workspace."""
+    dev = torch.device("cuda", 0)
+    streams = {}
+    monkeypatch.setattr(nv, "stream_ptr", lambda d: streams.get(threading.get_ident(), 7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    call = _Turns()
+    _in_threads(4, lambda i: [nv.call_with_workspace(dev, lambda: 0, call) for _ in range(3)])
+    assert call.most == 1
+    both = _Turns(threading.Barrier(2, timeout=20).wait)  # streams of their own: side by side
+
+    def other_stream(i):
+        streams[threading.get_ident()] = 100 + i
+        nv.call_with_workspace(dev, lambda: 0, both)
+
+    _in_threads(2, other_stream)
+    assert both.most == 2
+
+
+def test_threads_on_one_stream_take_turns_without_a_window(monkeypatch):
+    call = _Turns()
+
+    class Lib:
+        nvm_paged_attention = call
+        nvm_paged_attention_workspace_size = staticmethod(lambda *args: 0)
+
+    monkeypatch.setattr(nv, "lib", lambda: Lib)
+    monkeypatch.setattr(nv, "require_cuda", lambda op, *t: torch.device("cuda", 0))
+    monkeypatch.setattr(nv, "stream_ptr", lambda d: 7)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    pages, q = torch.zeros(2, 2, 16, 64), torch.zeros(1, 4, 1, 64)
+    bt, cl = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    _in_threads(4, lambda i: [paged_attention(q, pages, pages, bt, cl, 16, out=torch.zeros_like(q)) for _ in range(3)])
+    assert call.most == 1

@@ -557,6 +557,37 @@ def test_first_call_of_a_thread(L, kind):
         assert_within(got[0], ref, out_bound(ref, terms, 128, BF, F32), "out")
 
 
+@pytest.mark.parametrize("scored", [True, False])
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_two_threads_on_one_stream(L, scored):
+    probs = [make_problem(70 + i, [1500 + 300 * i, 2900, 700], L, 64 if L == 1 else 16, 8, 128, 16, BF) for i in range(2)]
+    masses = [torch.rand(3, 8, 2900) for _ in range(2)]
+    refs = [paged_reference(p, 0, 0, mass=m) for p, m in zip(probs, masses)]
+    gpu, starts = [to_gpu(p) for p in probs], [m.cuda() for m in masses]
+    torch.cuda.synchronize()
+    results = [[], []]
+
+    def run(i):
+        p = gpu[i]
+        for _ in range(100):
+            gm = starts[i].clone() if scored else None
+            results[i].append((paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=gm), gm))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for (ref, terms, mref, merr), got in zip(refs, results):
+        assert len(got) == 100
+        assert all(torch.equal(out, got[0][0]) for out, _ in got)
+        assert_within(got[0][0], ref, out_bound(ref, terms, 128, BF, F32), "out")
+        if scored:
+            assert all(torch.equal(gm, got[0][1]) for _, gm in got)
+            assert_within(got[0][1], mref, merr + 1e-30, "mass")
+
+
 @pytest.mark.parametrize("L", [1, 4, 100])
 def test_results_do_not_depend_on_the_run(L, path):
     prob = make_problem(30 + L, [2300, 1700], L, 16, 2, 128, 16, BF)
