@@ -145,6 +145,9 @@ def on_device(device: torch.device):
 # the GPU.  A call whose bounded wait expired may leave tickets non-zero, so
 # device_error() re-zeroes every workspace of the device after a non-zero word.
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+# Buffers that a CUDA graph captured: kept when a larger call replaces them, as the graph replays
+# with their addresses.
+_captured: dict[int, torch.Tensor] = {}
 # A call that uses the workspace may launch several kernels, the later ones on what the first left
 # there, and ctypes drops the interpreter lock meanwhile: host threads that share a stream take turns.
 _workspace_locks: dict[tuple[int, int], threading.Lock] = {}
@@ -167,6 +170,8 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
+    if torch.cuda.is_current_stream_capturing():
+        _captured[ws.data_ptr()] = ws
     return ws
 
 

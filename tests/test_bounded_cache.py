@@ -5,6 +5,7 @@ import random
 import re
 import threading
 import time
+import weakref
 
 import pytest
 import torch
@@ -249,3 +250,19 @@ def test_threads_on_one_stream_take_turns_without_a_window(monkeypatch):
     bt, cl = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     _in_threads(4, lambda i: [paged_attention(q, pages, pages, bt, cl, 16, out=torch.zeros_like(q)) for _ in range(3)])
     assert call.most == 1
+
+
+def test_a_captured_workspace_outlives_a_larger_call(monkeypatch):
+    """A graph of unwindowed calls replays with the stream's buffer, also after a scored call grew it."""
+    capturing = [True]
+    monkeypatch.setattr(nv, "_workspace_key", lambda d: (0, 123))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(nv, "_workspaces", {})
+    monkeypatch.setattr(nv, "_captured", {}, raising=False)
+    cpu = torch.device("cpu")
+    captured = weakref.ref(nv.workspace(cpu, 1 << 21))
+    capturing[0] = False
+    larger = weakref.ref(nv.workspace(cpu, 1 << 22))
+    assert captured() is not None and nv.workspace(cpu, 1 << 21) is larger()
+    nv.workspace(cpu, 1 << 23)
+    assert larger() is None  # one that no graph holds is given back
