@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kMThreads, 2)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) record_error(err, kDevErrSmemAlign);
+    pdl_wait();
     return;
   }
   uint8_t* sK = smem;
@@ -320,7 +321,12 @@ __global__ void __launch_bounds__(kMThreads, 2)
   int64_t end64 = ctx < cap ? ctx : cap;
   if (p.len < end64) end64 = p.len;
   const int end = (int)end64;
-  if (k0 >= end) return;  // the whole cluster
+  if (k0 >= end) {  // the whole cluster
+    // The next kernel waits for this one alone, so this one ends after the attention kernel also
+    // when no sequence has a key: the first tile's CTAs wait in any case, here or below.
+    if (k0 == 0) pdl_wait();
+    return;
+  }
   // rows (per run) that see some key of the tile
   const int L = (int)p.L, base_pos = ctx - L;
   const bool by_head = L >= 64;  // else the g * L rows of the kv head are one run

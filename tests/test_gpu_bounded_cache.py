@@ -588,6 +588,38 @@ def test_two_threads_on_one_stream(L, scored):
             assert_within(got[0][1], mref, merr + 1e-30, "mass")
 
 
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_a_batch_of_empty_contexts_and_the_next_call(L):
+    """Nothing is attended or scored, and what follows on the stream comes after it, captured too."""
+    empty = to_gpu(make_problem(3, [0, 0, 0], L, 16, 4, 128, 16, BF, spare=40, width_extra=30))
+    prob = make_problem(4, [400, 300], L, 16, 4, 128, 16, BF)
+    mass, mass0 = torch.rand(2, 4, 400), torch.rand(3, 4, 480).cuda()
+    ref, terms, mref, merr = paged_reference(prob, 0, 0, mass=mass)
+    p, gm0, gm = to_gpu(prob), mass0.clone(), mass.cuda()
+    out0, copy = torch.empty(3, 16, L, 128, device="cuda"), torch.empty(3, 16, L, 128, device="cuda")
+
+    def both():
+        paged_attention(empty["q"], empty["k"], empty["v"], empty["bt"], empty["cl"], 16, mask="causal", key_mass=gm0, out=out0)
+        copy.copy_(out0)
+        return paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=gm)
+
+    for _ in range(20):
+        out0.fill_(math.nan), gm.copy_(mass)
+        got = both()
+        assert not copy.any() and torch.equal(gm0, mass0)
+    assert_within(got, ref, out_bound(ref, terms, 128, BF, F32), "out")
+    assert_within(gm, mref, merr + 1e-30, "mass")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for _ in range(20):
+        out0.fill_(math.nan), gm.copy_(mass)
+        graph.replay()
+        assert not copy.any() and torch.equal(gm0, mass0)
+    assert_within(got, ref, out_bound(ref, terms, 128, BF, F32), "captured")
+    assert_within(gm, mref, merr + 1e-30, "mass")
+
+
 @pytest.mark.parametrize("L", [1, 4, 100])
 def test_results_do_not_depend_on_the_run(L, path):
     prob = make_problem(30 + L, [2300, 1700], L, 16, 2, 128, 16, BF)
