@@ -396,7 +396,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
     if (plan.ws_bytes == 0)
       a.mass = key_mass;  // the attention kernel weighs them too
     else
-      a.defer = plan.n_units < kDeferUnits ? 1 : 0;
+      a.defer = plan.n_units < kDeferUnits && mass_len > 0 ? 1 : 0;  // no entries: no kernel over the scores
     a.mass_sb = mass_stride_b; a.mass_sh = mass_stride_h; a.mass_len = mass_len;
   }
   st = sp.eligible     ? launch_sm100(a, sp, workspace, s)

@@ -9,6 +9,7 @@ import torch
 from bounded_reference import (HALF_STEP, assert_within, evict_reference, make_problem, out_bound, paged_reference, to_gpu,
                                visible)
 from nano_vllm_b200 import DevicePageTable, TinyKvPagedCache, TinyKvPagedPool, evict_tokens, flash_attention, paged_attention
+from nano_vllm_b200 import _native as nv
 from nano_vllm_b200 import write_slots
 
 pytestmark = pytest.mark.gpu
@@ -192,6 +193,25 @@ def test_key_mass_shorter_than_the_context(path):
     p, gm = to_gpu(prob), mass.cuda()
     paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=gm)
     assert_within(gm, mref, merr + 1e-30, "mass")
+
+
+@pytest.mark.parametrize("L", [1, 6, 80])
+def test_c_call_with_key_mass_of_no_length(L, path):
+    """A buffer of no entries keeps no score, and the output is written all the same."""
+    ctx, Hq, Hkv, D = [9000, 200, 3], 7 if L == 1 else 8, 1, 64
+    prob = make_problem(2 + L, ctx, L, Hq, Hkv, D, 32, BF)
+    ref, terms, _, _ = paged_reference(prob)
+    p, lib = to_gpu(prob), nv.lib()
+    mp, mass = p["bt"].shape[1], torch.full((8,), 3.0, device="cuda")
+    out = torch.full((3, Hq, L, D), math.nan, device="cuda")
+    need = lib.nvm_paged_attention_window_workspace_size(3, Hq, Hkv, L, D, 32, mp, nv.NVM_BF16, 0, 0, 1)
+    ws = torch.zeros(max(need, 1), dtype=torch.uint8, device="cuda")
+    nv.check(lib.nvm_paged_attention_window(
+        p["q"].data_ptr(), nv.NVM_BF16, p["k"].data_ptr(), p["v"].data_ptr(), nv.NVM_BF16, None, None, nv.NVM_F16,
+        p["bt"].data_ptr(), p["cl"].data_ptr(), out.data_ptr(), nv.NVM_F32, 3, Hq, Hkv, L, D, p["k"].shape[0], 32, mp, D ** -0.5,
+        1, 0, 0, mass.data_ptr(), 0, 0, 0, ws.data_ptr(), need, nv.stream_ptr(out.device)))
+    assert_within(out, ref, out_bound(ref, terms, D, BF, F32), "out")
+    assert (mass == 3).all() and not ws[:min(need, 1 << 20)].any()  # the tickets are zero again
 
 
 def test_out_at_any_alignment(path):
