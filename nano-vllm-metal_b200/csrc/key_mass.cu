@@ -260,15 +260,23 @@ struct MassSmem {
 // inside the tile loop).
 constexpr uint32_t kPolyMask = 0x55u;
 
+// The larger of a score and -125; NaN stays NaN.
+__device__ __forceinline__ float clamp_score(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-125.f));
+  return r;
+}
+
 // 2^x for a pair on the FMA pipe: n = round(x) through the 1.5 * 2^23 rounding constant,
 // f = x - n in [-0.5, 0.5] (exact), a degree-5 polynomial for 2^f (near-minimax for relative
-// error by iteratively reweighted least squares: 2.0e-7 in fp32, as ex2.approx), and n added to the
-// exponent field.  Arguments below -125 give 2^-125 instead of a smaller number or zero, so a
+// error by iteratively reweighted least squares: 2.0e-7 in fp32, as ex2.approx), times 2^n (its
+// exponent field is t's last bits; a product, since adding n to the polynomial's bits would make
+// a number of a NaN).  Arguments below -125 give 2^-125 instead of a smaller number or zero, so a
 // row without a key (lse = +inf) must not come here.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   constexpr float kRound = 12582912.0f;
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
+  x.x = clamp_score(x.x);
+  x.y = clamp_score(x.y);
   const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
   const float2 f = __ffma2_rn(__fadd2_rn(t, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
   float2 p = __ffma2_rn(make_float2(0.001327647f, 0.001327647f), f, make_float2(0.009675542f, 0.009675542f));
@@ -276,8 +284,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   p = __ffma2_rn(p, f, make_float2(0.2402212f, 0.2402212f));
   p = __ffma2_rn(p, f, make_float2(0.69314694f, 0.69314694f));
   p = __ffma2_rn(p, f, make_float2(1.0000001f, 1.0000001f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 
 template <typename T, typename KvT, int D>
@@ -548,10 +556,11 @@ __global__ void __launch_bounds__(kMThreads, 2)
           }
         }
       } else {
-        // columns [c_lo, c_hi) of a run see this key; rows of several heads look their position up
+        // Columns [c_lo, c_hi) of a run see this key (those from `rows` on hold another head's rows);
+        // rows of several heads look their position up.
         const int64_t w64 = p.window > 0 && !sink ? p.window : INT64_MAX / 4;
         const int64_t c_hi64 = (int64_t)key + w64 - pos_lo;
-        const int c_lo = p.causal ? key - pos_lo : INT32_MIN, c_hi = c_hi64 < kMR ? (int)c_hi64 : kMR;
+        const int c_lo = p.causal ? key - pos_lo : INT32_MIN, c_hi = c_hi64 < rows ? (int)c_hi64 : rows;
 #pragma unroll 1
         for (int c0 = 0; c0 < rows; c0 += 32) {
           float sv[32];

@@ -195,6 +195,23 @@ def test_key_mass_shorter_than_the_context(path):
     assert_within(gm, mref, merr + 1e-30, "mass")
 
 
+@pytest.mark.parametrize("L,D,kv", [(1, 128, BF), (6, 128, HF), (256, 128, BF), (256, 64, HF), (256, 128, I8), (30, 64, BF)])
+def test_a_query_row_of_nan_shows_in_every_score_it_makes(L, D, kv, path):
+    ctx, mass = 400, torch.rand(1, 2, 400)
+    for head, row in ((0, 0), (1, L // 3), (2, L // 2 + 1), (3, L - 1), (1, 11), (2, 13), (0, 130), (3, 255)):
+        if row >= L:
+            continue
+        prob = make_problem(50, [ctx], L, 8, 2, D, 16, kv)
+        _, _, mref, merr = paged_reference(prob, mass=mass)
+        prob["q"][0, head, row] = math.nan
+        p, gm = to_gpu(prob), mass.cuda()
+        paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], mask="causal", key_mass=gm)
+        seen = ctx - L + row + 1  # by the NaN row
+        assert gm[0, 0, :seen].isnan().all(), (head, row, int(gm[0, 0, :seen].isnan().sum()))
+        assert_within(gm[0, 0, seen:], mref[0, 0, seen:], merr[0, 0, seen:] + 1e-30, "keys it does not see")
+        assert_within(gm[0, 1], mref[0, 1], merr[0, 1] + 1e-30, "the other kv head")
+
+
 @pytest.mark.parametrize("L", [1, 6, 80])
 def test_c_call_with_key_mass_of_no_length(L, path):
     """A buffer of no entries keeps no score, and the output is written all the same."""
