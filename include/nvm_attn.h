@@ -184,8 +184,11 @@ int nvm_paged_attention_noalloc(const void* q, int q_dtype, const void* k_pages,
  *                  mass = (s < context_len - L ? mass : 0) + sum of the softmax weights of
  *                  key s over the rows of kv head h (Hq/Hkv heads x L tokens),
  *                so the newest L tokens start afresh and entries need no clearing when a
- *                slot gets a new request or a rejected draft is rewound.  Keys outside every
- *                window and entries past the context keep their value.
+ *                slot gets a new request or a rejected draft is rewound.  That holds while
+ *                scored calls append every token of a request: the entries of tokens that
+ *                none of its scored calls appended (an attached prefix, a prompt that was not
+ *                scored) are the caller's to zero.  Keys outside every window and entries past
+ *                the context keep their value.
  * A key that no query token of the call sees (past the context, outside every window, on an
  * unmapped page) has no influence, whatever its K, V and scales hold (NaN and infinities
  * included).  A key that one query token sees but another does not must hold finite values.

@@ -445,14 +445,26 @@ class DevicePageTable:
         fin = result.finished.to(device=self.device, dtype=torch.bool)
         self.rewind(torch.where(fin, self.context_lens, result.rewind.to(device=self.device, dtype=torch.int32)))
 
-    def attach(self, pages: torch.Tensor, count: torch.Tensor) -> None:
+    def attach(self, pages: torch.Tensor, count: torch.Tensor, *, key_mass=()) -> None:
         """``PrefixCache.attach`` on the device (``paged.py:305-328``): fresh request b
         takes the shared full pages ``pages[b, :count[b]]`` (each gains a reference) and
-        starts at length ``count[b] * page_size``."""
+        starts at length ``count[b] * page_size``.
+
+        ``key_mass``: the layers' score buffers (float32 ``[B, H, S]``), whose entries of the
+        attached tokens become zero.  A scored call starts the tokens that it appends itself;
+        these were appended by another request, and their entries are the slot's last tenant's."""
         pg = pages.to(device=self.device, dtype=torch.int32).contiguous()
         ct = count.to(device=self.device, dtype=torch.int32).contiguous()
         if pg.dim() != 2 or pg.shape[0] != self.B or ct.numel() != self.B:
             raise ValueError("attach: pages must be [B, max_prefix] and count [B]")
+        key_mass = list(key_mass)
+        for m in key_mass:
+            if m.dim() != 3 or m.shape[0] != self.B or m.dtype != torch.float32 or m.device != self.context_lens.device:
+                raise ValueError("attach: key_mass must be float32 [B, H, S] on the table's device")
+        if key_mass:  # a request that is not fresh is refused below and keeps its scores
+            start = torch.where(self.context_lens == 0, ct.view(-1) * self.page_size, 0)[:, None, None]
+            for m in key_mass:
+                m.masked_fill_(torch.arange(m.shape[2], device=self.device) < start, 0.0)
         with torch.cuda.device(self.device):
             nv.check(nv.lib().nvm_paged_attach(
                 self.block_table.data_ptr(), self.context_lens.data_ptr(), pg.data_ptr(), ct.data_ptr(),

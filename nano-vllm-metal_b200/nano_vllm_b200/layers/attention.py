@@ -236,8 +236,10 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     ``s < sinks`` or ``s > pos - window``; pages wholly between are not read.  ``key_mass``
     (float32 ``[B, Hkv, S]``, last axis contiguous) is updated in place: every key gains the
     softmax weights it gets from the rows of its kv head, and the newest L keys start at zero,
-    so the buffer needs no clearing between requests; keys at or past S gain nothing.  A row
-    that sees no key is zero, and a key that no row sees has no influence whatever it holds.
+    so the buffer needs no clearing between requests whose tokens scored calls append (zero the
+    entries of others, as ``DevicePageTable.attach`` does for an attached prefix); keys at or past
+    S gain nothing.  A row that sees no key is zero, and a key that no row sees has no influence
+    whatever it holds.
     """
     if window is not None or key_mass is not None or sinks != 0:
         return _paged_attention_window(query, key_pages, value_pages, block_table, context_lens, page_size, key_scales,

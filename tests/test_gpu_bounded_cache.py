@@ -747,6 +747,40 @@ def test_table_evict_refuses_shared_prefix_pages():
     table.check_status()
 
 
+def test_an_attached_prefix_starts_without_scores():
+    """The slot's last tenant left weights (and NaN) behind; the prefix's tokens are scored by the
+    calls that follow alone, and eviction ranks by these."""
+    B, Hq, Hkv, D, ps, layers = 3, 8, 2, 128, 16, 2
+    table = DevicePageTable(B, 8, ps, 32)
+    pools = [torch.randn(32, Hkv, ps, D, device="cuda").to(BF) for _ in range(2)]
+    stale = torch.rand(B, Hkv, 128, device="cuda") * 100
+    stale[2] = math.nan
+    mass = [stale.clone() for _ in range(layers)]
+    table.append(torch.tensor([64, 0, 0], dtype=torch.int32, device="cuda"))
+    prefix = torch.tensor([[0, 0, 0], [0, 1, 2], [0, 1, 2]], dtype=torch.int32)
+    table.attach(prefix, torch.tensor([0, 3, 2], dtype=torch.int32), key_mass=mass)
+    table.check_status()
+    for m in mass:
+        assert torch.equal(m[0], stale[0])  # nothing attached
+        assert not m[1, :, :48].any() and torch.equal(m[1, :, 48:], stale[1, :, 48:])
+        assert not m[2, :, :32].any() and m[2, :, 32:].isnan().all()
+    table.append(torch.tensor([0, 5, 5], dtype=torch.int32, device="cuda"))
+    q = torch.randn(B, Hq, 5, D, device="cuda").to(BF)
+    paged_attention(q, *pools, table.block_table, table.context_lens, ps, mask="causal", key_mass=mass[0])
+    for b, n in ((1, 53), (2, 37)):  # every row's weights sum to one
+        total = mass[0][b, :, :n].double().sum().item()
+        assert abs(total - Hq * 5) <= 1e-4 * Hq * 5
+    # refused: request 0 has tokens, and its scores stay; the table is as it was
+    before, lens = mass[0].clone(), table.context_lens.clone()
+    table.attach(prefix[:, :1].contiguous(), torch.tensor([1, 0, 0], dtype=torch.int32), key_mass=[mass[0]])
+    with pytest.raises(RuntimeError):
+        table.check_status()
+    assert torch.equal(mass[0][0], before[0]) and torch.equal(table.context_lens, lens)
+    for bad in (torch.zeros(2, Hkv, 8, device="cuda"), mass[0].double(), mass[0][0], mass[0].cpu()):
+        with pytest.raises(ValueError, match="attach: key_mass"):
+            table.attach(prefix, torch.zeros(3, dtype=torch.int32), key_mass=[bad])
+
+
 def test_table_evict_wants_layers_alike():
     table = DevicePageTable(1, 4, 16, 8)
     pages, mass = torch.zeros(8, 2, 16, 64, device="cuda", dtype=BF), torch.zeros(1, 2, 64, device="cuda")
