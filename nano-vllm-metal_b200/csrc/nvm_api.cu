@@ -151,6 +151,54 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
   return NVM_OK;
 }
 
+// Sequences of each launch of the mma.sync kernel (but the last) and its plan: all of them, unless
+// their units outnumber the merge tickets.
+int64_t plan_parts(const PagedArgs& a, MmaPlan* plan) {
+  PagedArgs x = a;
+  *plan = plan_paged_mma(x);
+  while (!plan->eligible && plan->max_batch > 0 && plan->max_batch < x.B) {
+    const int64_t parts = (a.B + plan->max_batch - 1) / plan->max_batch;
+    x.B = (a.B + parts - 1) / parts;
+    *plan = plan_paged_mma(x);
+  }
+  return x.B;
+}
+// Sequences b0 .. b0 + n - 1 of a call.
+PagedArgs batch_part(const PagedArgs& a, int64_t b0, int64_t n) {
+  PagedArgs x = a;
+  const int64_t rows = b0 * a.Hq * a.L * a.D;
+  x.B = n;
+  x.q = static_cast<const uint8_t*>(a.q) + rows * (int64_t)dtype_size(a.q_dtype);
+  x.out = static_cast<uint8_t*>(a.out) + rows * (int64_t)dtype_size(a.out_dtype);
+  x.block_table = a.block_table + b0 * a.max_pages;
+  x.context_lens = a.context_lens + b0;
+  return x;
+}
+// The last part's plan differs in its batch: calls f(arguments, plan, first sequence) for every part
+// until one fails.
+template <typename F>
+int each_part(const PagedArgs& a, int64_t n, const MmaPlan& plan, F&& f) {
+  if (n >= a.B) return f(a, plan, (int64_t)0);
+  for (int64_t b0 = 0; b0 < a.B; b0 += n) {
+    const int64_t m = a.B - b0 < n ? a.B - b0 : n;
+    const PagedArgs x = batch_part(a, b0, m);
+    const int st = f(x, m == n ? plan : plan_paged_mma(x), b0);
+    if (st != NVM_OK) return st;
+  }
+  return NVM_OK;
+}
+// Workspace of the mma.sync kernel's part of a call, over its parts.
+size_t parts_ws(const PagedArgs& a, int64_t n, const MmaPlan& plan) {
+  size_t need = plan.eligible ? plan.ws_bytes : 0;
+  PagedArgs x = a;
+  x.B = a.B % n;
+  if (n < a.B && x.B != 0) {
+    const MmaPlan last = plan_paged_mma(x);
+    if (last.eligible && last.ws_bytes > need) need = last.ws_bytes;
+  }
+  return need;
+}
+
 // Stands for the log-sum-exp buffer while a call is planned, before its workspace is known.
 float kLseLater;
 
@@ -181,6 +229,20 @@ WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, size_t score_bytes, bo
   w.scores = w.lse + al((size_t)(a.B * a.Hq * a.L) * sizeof(float));
   w.total = with_mass ? w.scores + score_bytes : attn_bytes;
   return w;
+}
+
+// The same over the parts of a call whose batch the mma.sync kernel takes.
+size_t parts_window_ws(const PagedArgs& a, int64_t n, const MmaPlan& plan, bool with_mass) {
+  PagedArgs x = a;
+  x.B = n;
+  size_t need = window_ws(x, plan.eligible ? plan.ws_bytes : 0, score_bytes(x, plan), with_mass).total;
+  x.B = a.B % n;
+  if (n < a.B && x.B != 0) {
+    const MmaPlan last = plan_paged_mma(x);
+    const size_t t = window_ws(x, last.eligible ? last.ws_bytes : 0, score_bytes(x, last), with_mass).total;
+    if (t > need) need = t;
+  }
+  return need;
 }
 
 int validate_window(int64_t window, int64_t sinks, const char* op) {
@@ -241,8 +303,9 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
   if (env_flag("NVM_ATTN_FORCE_GENERIC")) return 0;
   // q's dtype is not known here: cover the tcgen05 plan (taken when q matches the pages)
   // and the mma.sync plan (taken otherwise).
-  MmaPlan plan = plan_paged_mma(a);
-  size_t need = plan.eligible ? plan.ws_bytes : 0;
+  MmaPlan plan{};
+  const int64_t n = plan_parts(a, &plan);
+  size_t need = n > 0 ? parts_ws(a, n, plan) : 0;
   if (!env_flag("NVM_ATTN_NO_SM100")) {
     const Sm100Plan sp = plan_sm100(a, true);
     if (sp.eligible && sp.ws_bytes > need) need = sp.ws_bytes;
@@ -277,12 +340,16 @@ int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const v
         return launch_sm100(a, sp, workspace, s);
       }
     }
-    MmaPlan plan = plan_paged_mma(a);
+    MmaPlan plan{};
+    const int64_t n = plan_parts(a, &plan);
     if (plan.eligible) {
-      if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes))
-        return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", plan.ws_bytes,
+      const size_t need = parts_ws(a, n, plan);
+      if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", need,
                     workspace_bytes);
-      return launch_paged_mma(a, plan, workspace, s);
+      return each_part(a, n, plan, [&](const PagedArgs& x, const MmaPlan& xp, int64_t) {
+        return xp.eligible ? launch_paged_mma(x, xp, workspace, s) : launch_paged_generic(x, s);
+      });
     }
   }
   return launch_paged_generic(a, s);
@@ -343,13 +410,15 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   size_t total = window_ws(a, 0, 0, with_mass != 0).total;
   for (int causal = 0; causal < 2 && !env_flag("NVM_ATTN_FORCE_GENERIC"); ++causal) {
     a.is_causal = causal;
-    const MmaPlan plan = plan_paged_mma(a);
-    size_t need = plan.eligible ? plan.ws_bytes : 0;
+    size_t t = 0;
     if (!env_flag("NVM_ATTN_NO_SM100")) {
       const Sm100Plan sp = plan_sm100(a, true);
-      if (sp.eligible && sp.ws_bytes > need) need = sp.ws_bytes;
+      if (sp.eligible) t = window_ws(a, sp.ws_bytes, 0, with_mass != 0).total;
     }
-    const size_t t = window_ws(a, need, score_bytes(a, plan), with_mass != 0).total;
+    if (t > total) total = t;
+    MmaPlan plan{};
+    const int64_t n = plan_parts(a, &plan);
+    if (n > 0) t = parts_window_ws(a, n, plan, with_mass != 0);
     if (t > total) total = t;
   }
   return total;
@@ -380,31 +449,37 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
   if (key_mass != nullptr) a.lse = &kLseLater;
   Sm100Plan sp{};
   MmaPlan plan{};
+  int64_t n = B;
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
     if (!env_flag("NVM_ATTN_NO_SM100")) sp = plan_sm100(a, false);
-    if (!sp.eligible) plan = plan_paged_mma(a);
+    if (!sp.eligible) n = plan_parts(a, &plan);
   }
-  const size_t kept = key_mass != nullptr ? score_bytes(a, plan) : 0;
-  const WindowWs ws =
-      window_ws(a, sp.eligible ? sp.ws_bytes : plan.eligible ? plan.ws_bytes : 0, kept, key_mass != nullptr);
-  if (ws.total > 0 && (workspace == nullptr || workspace_bytes < ws.total))
-    return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", ws.total,
-                workspace_bytes);
-  if (key_mass != nullptr) a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
-  if (kept > 0) {
-    a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
-    if (plan.ws_bytes == 0)
-      a.mass = key_mass;  // the attention kernel weighs them too
-    else
-      a.defer = plan.n_units < kDeferUnits && mass_len > 0 ? 1 : 0;  // no entries: no kernel over the scores
-    a.mass_sb = mass_stride_b; a.mass_sh = mass_stride_h; a.mass_len = mass_len;
-  }
-  st = sp.eligible     ? launch_sm100(a, sp, workspace, s)
-       : plan.eligible ? launch_paged_mma(a, plan, workspace, s)
-                       : launch_paged_generic(a, s);
-  if (st != NVM_OK || key_mass == nullptr || a.mass != nullptr) return st;
-  KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
-  return launch_key_mass(a, m, &plan, workspace, sp.eligible || plan.eligible, s);
+  const size_t need = sp.eligible ? window_ws(a, sp.ws_bytes, 0, key_mass != nullptr).total
+                                  : parts_window_ws(a, n, plan, key_mass != nullptr);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", need, workspace_bytes);
+  return each_part(a, n, plan, [&](PagedArgs x, const MmaPlan& xp, int64_t b0) {
+    KeyMassArgs m{key_mass, mass_stride_b, mass_stride_h, mass_len};
+    if (key_mass != nullptr) {
+      m.mass += b0 * mass_stride_b;
+      const size_t kept = score_bytes(x, xp);
+      const WindowWs ws = window_ws(x, sp.eligible ? sp.ws_bytes : xp.eligible ? xp.ws_bytes : 0, kept, true);
+      x.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.lse);
+      if (kept > 0) {
+        x.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.scores);
+        if (xp.ws_bytes == 0)
+          x.mass = m.mass;  // the attention kernel weighs them too
+        else
+          x.defer = xp.n_units < kDeferUnits && mass_len > 0 ? 1 : 0;  // no entries: no kernel over the scores
+        x.mass_sb = mass_stride_b; x.mass_sh = mass_stride_h; x.mass_len = mass_len;
+      }
+    }
+    const int r = sp.eligible   ? launch_sm100(x, sp, workspace, s)
+                  : xp.eligible ? launch_paged_mma(x, xp, workspace, s)
+                                : launch_paged_generic(x, s);
+    if (r != NVM_OK || key_mass == nullptr || x.mass != nullptr) return r;
+    return launch_key_mass(x, m, &xp, workspace, sp.eligible || xp.eligible, s);
+  });
 }
 
 int nvm_flash_attention_window(const void* q, const void* k, const void* v, int dtype, void* out, int out_dtype,

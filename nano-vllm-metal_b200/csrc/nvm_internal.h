@@ -141,6 +141,7 @@ struct MmaPlan {
   int64_t n_chunks;       // max chunks per unit
   int64_t n_units;
   size_t ws_bytes;        // workspace for the split-K combine (0 if n_chunks == 1 or cluster)
+  int64_t max_batch;      // not eligible for more tickets than the workspace has: the largest batch that is, or 0
   int64_t head_blocks;    // windowed calls: row blocks per q head (no block spans two), 0: over all rows
   int cluster;            // 1: a unit's n_chunks CTAs form one thread-block cluster and merge
                           // their partial results over distributed shared memory (no workspace)

@@ -287,6 +287,12 @@ MmaPlan plan_paged_mma(const PagedArgs& a) {
   plan.n_chunks = (tiles_max + ct - 1) / ct;
   if (plan.n_chunks < 1) plan.n_chunks = 1;
   if (plan.n_chunks > 65535) return plan;
+  if (!can_split && !dense && plan.n_chunks > 1) {
+    // A chunk's page table holds kMaxChunkTiles tiles, so longer contexts are cut whatever the
+    // number of units, but there are no tickets for so many: the caller takes the batch in parts.
+    plan.max_batch = kMaxUnits / (a.Hkv * plan.n_row_blocks);
+    return plan;
+  }
   // n8 tile with 2..8 chunks: the chunks of a unit merge inside a thread-block cluster
   // (distributed shared memory) instead of through the workspace, which takes the
   // global-memory round trips of the split-K merge off every unit's critical path.

@@ -101,6 +101,17 @@ def test_workspace_size_covers_what_the_call_needs():
                 assert size(*shape, mass) >= need, (shape, causal, mass, need)
 
 
+def test_more_units_than_merge_tickets_go_in_parts():
+    """257 prompts of 1024 row blocks are 263168 units, the first MiB of the workspace holds 262144 tickets:
+    two launches of at most 129 prompts, in the workspace of one of them."""
+    L_ = nv.lib()
+    base = lambda B: L_.nvm_paged_attention_workspace_size(B, 8, 1, 8192, 64, 16, 545, 2)  # noqa: E731
+    window = lambda B, w=5000: L_.nvm_paged_attention_window_workspace_size(B, 8, 1, 8192, 64, 16, 545, 2, w, 4, 0)  # noqa: E731
+    assert base(257) == base(129) > base(128) > 1 << 20
+    assert window(257) == window(129) > window(128) > 1 << 20
+    assert L_.nvm_paged_attention_workspace_size(2, 8, 1, 262144 * 9, 64, 16, 545, 2) == 0  # too many in one prompt
+
+
 def test_evict_c_entry_refusals():
     def call(B=1, D=128, budget=4, sinks=0, recent=0, kv=2, sb=8):
         return nv.lib().nvm_paged_evict(None, None, kv, None, None, 1, None, None, None, None, sb, 8, 8, None, 8, 8, B, 2, D,

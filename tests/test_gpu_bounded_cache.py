@@ -212,6 +212,27 @@ def test_a_query_row_of_nan_shows_in_every_score_it_makes(L, D, kv, path):
         assert_within(gm[0, 1], mref[0, 1], merr[0, 1] + 1e-30, "the other kv head")
 
 
+@pytest.mark.parametrize("window", [None, 5000])
+def test_more_units_than_merge_tickets(window):
+    """257 prompts of 8192 tokens and 8 heads: 263168 blocks of 64 rows, whose chunks merge in two launches."""
+    B, Hq, L, D, ps, mp = 257, 8, 8192, 64, 16, 545
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(600, 1, ps, D, device="cuda", generator=gen).to(BF) for _ in range(2))
+    q = torch.empty(B, Hq, L, D, device="cuda", dtype=BF).normal_(generator=gen)
+    bt = torch.stack([torch.randperm(600)[:mp] for _ in range(B)]).int()
+    cl = torch.randint(8192, mp * ps + 1, (B,)).int()
+    out = paged_attention(q, k, v, bt.cuda(), cl.cuda(), ps, mask="causal", window=window, sinks=4, out_dtype=BF)
+    pick = [(b, h, r) for b in (0, 1, 127, 128, 129, 130, 255, 256) for h, r in ((0, 0), (3, 4000), (7, L - 1))]
+    b, h, r = (torch.tensor(x) for x in zip(*pick))
+    # a row is a decode call of its own at its position
+    prob = {"q": q[b.cuda(), h.cuda(), r.cuda()].cpu()[:, None, None], "k": k.cpu(), "v": v.cpu(), "ks": None, "vs": None,
+            "bt": bt[b], "cl": cl[b] - L + r.int() + 1, "ps": ps}
+    ref, terms, _, _ = paged_reference(prob, window or 0, 4)
+    assert_within(out[b.cuda(), h.cuda(), r.cuda()][:, None, None], ref, out_bound(ref, terms, D, BF, BF), "out")
+    assert out.isfinite().all()
+    assert not nv._workspaces[nv._workspace_key(out.device)][:1 << 20].any()  # every ticket is zero again
+
+
 @pytest.mark.parametrize("L", [1, 6, 80])
 def test_c_call_with_key_mass_of_no_length(L, path):
     """A buffer of no entries keeps no score, and the output is written all the same."""
