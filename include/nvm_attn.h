@@ -197,7 +197,8 @@ int nvm_paged_attention_noalloc(const void* q, int q_dtype, const void* k_pages,
  * workspace      at least nvm_paged_attention_window_workspace_size(...) bytes, under the
  *                same rules as nvm_paged_attention's (and it may be the same buffer).  With
  *                key_mass and at most eight query rows per kv head it holds 4 bytes a query
- *                row and key.
+ *                row and key of the block table's width (max_pages * page_size), for as many
+ *                sequences at a time as take 2.25 GiB (at least one).
  */
 int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, const void* v_pages,
                                int kv_dtype, const void* k_scales, const void* v_scales, int scale_dtype,

@@ -151,17 +151,35 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
   return NVM_OK;
 }
 
+// Bytes of the scores that the n8 decode tile keeps (key_mass.cu says why), 0 if it does not
+// serve the plan.
+size_t score_bytes(const PagedArgs& a, const MmaPlan& plan) {
+  if (!plan.eligible || plan.nwm != 0) return 0;
+  const int64_t rows = (a.Hq / a.Hkv * a.L + 1) & ~int64_t(1);
+  return (size_t)(plan.n_units * plan.n_chunks * plan.chunk_tiles * 16 * rows) * sizeof(float);
+}
+// Scores of more than this are kept for a part of the batch at a time.  They are sized by the block
+// tables' width, 4 bytes a query row and key, and stay with the stream's workspace (256 requests of
+// 128K-token tables, 64/8 heads: 8.6 GB in one part).  Parts cost their last waves: 256 requests of
+// 500-8000 tokens in such tables, 32/8 heads, 1041 us in one (4.3 GB) and 1144 us in two; of 100-1000
+// tokens 463 and 470 us.
+constexpr size_t kMaxScoreBytes = size_t(9) << 28;
+
 // Sequences of each launch of the mma.sync kernel (but the last) and its plan: all of them, unless
-// their units outnumber the merge tickets.
-int64_t plan_parts(const PagedArgs& a, MmaPlan* plan) {
+// their units outnumber the merge tickets, or their kept scores (`scored`) the limit above.
+int64_t plan_parts(const PagedArgs& a, bool scored, MmaPlan* plan) {
   PagedArgs x = a;
-  *plan = plan_paged_mma(x);
-  while (!plan->eligible && plan->max_batch > 0 && plan->max_batch < x.B) {
-    const int64_t parts = (a.B + plan->max_batch - 1) / plan->max_batch;
-    x.B = (a.B + parts - 1) / parts;
+  for (;;) {
     *plan = plan_paged_mma(x);
+    int64_t most = x.B;  // sequences of a part
+    if (!plan->eligible && plan->max_batch > 0) most = plan->max_batch;
+    const size_t bytes = scored ? score_bytes(x, *plan) : 0;
+    if (bytes > kMaxScoreBytes) most = (int64_t)(kMaxScoreBytes / (bytes / (size_t)x.B));
+    if (most < 1) most = 1;
+    if (most >= x.B) return x.B;
+    const int64_t parts = (a.B + most - 1) / most;
+    x.B = (a.B + parts - 1) / parts;
   }
-  return x.B;
 }
 // Sequences b0 .. b0 + n - 1 of a call.
 PagedArgs batch_part(const PagedArgs& a, int64_t b0, int64_t n) {
@@ -215,13 +233,6 @@ constexpr int64_t kDeferUnits = 148;
 struct WindowWs {
   size_t lse, scores, total;
 };
-// Bytes of the scores that the n8 decode tile keeps (key_mass.cu says why), 0 if it does not
-// serve the plan.
-size_t score_bytes(const PagedArgs& a, const MmaPlan& plan) {
-  if (!plan.eligible || plan.nwm != 0) return 0;
-  const int64_t rows = (a.Hq / a.Hkv * a.L + 1) & ~int64_t(1);
-  return (size_t)(plan.n_units * plan.n_chunks * plan.chunk_tiles * 16 * rows) * sizeof(float);
-}
 WindowWs window_ws(const PagedArgs& a, size_t attn_bytes, size_t score_bytes, bool with_mass) {
   auto al = [](size_t x) { return (x + 255) & ~size_t(255); };
   WindowWs w{};
@@ -304,7 +315,7 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
   // q's dtype is not known here: cover the tcgen05 plan (taken when q matches the pages)
   // and the mma.sync plan (taken otherwise).
   MmaPlan plan{};
-  const int64_t n = plan_parts(a, &plan);
+  const int64_t n = plan_parts(a, false, &plan);
   size_t need = n > 0 ? parts_ws(a, n, plan) : 0;
   if (!env_flag("NVM_ATTN_NO_SM100")) {
     const Sm100Plan sp = plan_sm100(a, true);
@@ -341,7 +352,7 @@ int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const v
       }
     }
     MmaPlan plan{};
-    const int64_t n = plan_parts(a, &plan);
+    const int64_t n = plan_parts(a, false, &plan);
     if (plan.eligible) {
       const size_t need = parts_ws(a, n, plan);
       if (need > 0 && (workspace == nullptr || workspace_bytes < need))
@@ -417,7 +428,7 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
     }
     if (t > total) total = t;
     MmaPlan plan{};
-    const int64_t n = plan_parts(a, &plan);
+    const int64_t n = plan_parts(a, with_mass != 0, &plan);
     if (n > 0) t = parts_window_ws(a, n, plan, with_mass != 0);
     if (t > total) total = t;
   }
@@ -452,7 +463,7 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
   int64_t n = B;
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
     if (!env_flag("NVM_ATTN_NO_SM100")) sp = plan_sm100(a, false);
-    if (!sp.eligible) n = plan_parts(a, &plan);
+    if (!sp.eligible) n = plan_parts(a, key_mass != nullptr, &plan);
   }
   const size_t need = sp.eligible ? window_ws(a, sp.ws_bytes, 0, key_mass != nullptr).total
                                   : parts_window_ws(a, n, plan, key_mass != nullptr);

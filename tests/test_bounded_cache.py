@@ -112,6 +112,18 @@ def test_more_units_than_merge_tickets_go_in_parts():
     assert L_.nvm_paged_attention_workspace_size(2, 8, 1, 262144 * 9, 64, 16, 545, 2) == 0  # too many in one prompt
 
 
+@pytest.mark.parametrize("L,Hq", [(1, 64), (1, 32), (2, 32), (1, 8)])
+def test_kept_scores_do_not_grow_with_the_batch(L, Hq):
+    """4 bytes a query row (their number made even) and key of the table: kept for 2.25 GiB's worth of requests at a
+    time."""
+    size = lambda B, width: nv.lib().nvm_paged_attention_window_workspace_size(B, Hq, 8, L, 128, 16, width // 16, 2, 0, 0, 1)  # noqa: E731
+    bare = lambda B, width: nv.lib().nvm_paged_attention_workspace_size(B, Hq, 8, L, 128, 16, width // 16, 2)  # noqa: E731
+    for B, width in ((64, 131072), (256, 131072), (300, 70000), (1024, 40000), (77, 1 << 20)):
+        assert size(B, width) <= (9 << 28) + bare(B, width) + (1 << 22), (B, width, size(B, width), bare(B, width))
+    one = 8 * ((L * Hq // 8 + 1) // 2 * 2) * 4 << 23  # one request is never split
+    assert one <= size(1, 1 << 23) <= 1.02 * one + bare(1, 1 << 23) + (1 << 22)
+
+
 def test_evict_c_entry_refusals():
     def call(B=1, D=128, budget=4, sinks=0, recent=0, kv=2, sb=8):
         return nv.lib().nvm_paged_evict(None, None, kv, None, None, 1, None, None, None, None, sb, 8, 8, None, 8, 8, B, 2, D,

@@ -212,6 +212,33 @@ def test_a_query_row_of_nan_shows_in_every_score_it_makes(L, D, kv, path):
         assert_within(gm[0, 1], mref[0, 1], merr[0, 1] + 1e-30, "the other kv head")
 
 
+@pytest.mark.parametrize("L,Hq,kv", [(1, 64, BF), (2, 32, I8)])
+def test_scores_of_wide_tables_are_kept_in_parts(L, Hq, kv):
+    """81 requests of 128K-token tables, 8 rows a kv head: 2.7 GB of scores, taken in two parts of 41 and 40."""
+    B, Hkv, D = 81, 8, 128
+    ctx = [0, 1, 17, 5000] + torch.randint(2, 400, (B - 6,), generator=torch.Generator().manual_seed(8)).tolist() + [2600, 3]
+    prob = make_problem(5, ctx, L, Hq, Hkv, D, 16, kv)
+    prob["bt"] = torch.nn.functional.pad(prob["bt"], (0, 8192 - prob["bt"].shape[1]), value=-1)
+    S = 4000  # shorter than one context
+    store = torch.rand(Hkv, B, S + 2).cuda()
+    gm = store.transpose(0, 1)[:, :, :S]
+    p = to_gpu(prob)
+    prob["bt"] = prob["bt"][:, :320]  # what the reference walks
+    ref, terms, mref, merr = paged_reference(prob, mass=gm.cpu())
+    before = store.clone()
+    got = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], mask="causal", key_mass=gm)
+    bound = out_bound(ref, terms, D, kv, F32)
+    if kv == I8:
+        # The weight times the value's scale is rounded to half: below 2^-14 by up to 2^-25, and then
+        # multiplies the 8-bit value, |v| / scale.  `terms[2]` is the sum of |v| over the denominator.
+        bound = bound + 2.0 ** -25 * terms[2] / float(prob["vs"].min())
+    assert_within(got, ref, bound, "out")
+    assert_within(gm, mref, merr + 1e-30, "mass")
+    assert torch.equal(store[:, :, S:], before[:, :, S:])
+    for b, n in enumerate(ctx):
+        assert torch.equal(gm[b, :, n:], before.transpose(0, 1)[b, :, n:S])
+
+
 @pytest.mark.parametrize("window", [None, 5000])
 def test_more_units_than_merge_tickets(window):
     """257 prompts of 8192 tokens and 8 heads: 263168 blocks of 64 rows, whose chunks merge in two launches."""
