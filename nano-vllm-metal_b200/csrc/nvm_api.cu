@@ -547,6 +547,9 @@ int nvm_paged_evict(void* k_pages, void* v_pages, int kv_dtype, void* k_scales, 
   if (D > 256) return fail(NVM_ERR_UNSUPPORTED, "evict: head dimension must be <= 256 (got %lld)", (long long)D);
   if (budget > INT32_MAX || page_size > INT32_MAX || B * Hkv > INT32_MAX)
     return fail(NVM_ERR_UNSUPPORTED, "evict: budget, page_size and B * Hkv must be below 2^31");
+  // the kernels count a row's positions in 32 bits, up to a sweep of 32 x 1024 past its end
+  if (mass_len > INT32_MAX - 65536 && max_pages > (INT32_MAX - 65536) / page_size)
+    return fail(NVM_ERR_UNSUPPORTED, "evict: requests of more than 2^31 - 65537 tokens are not supported");
   if (B == 0) return NVM_OK;
   if (!k_pages || !v_pages || !block_table || !context_lens || !key_mass || !mass_out || !keep_index || !kept ||
       !dropped || !refused || (kv_dtype == NVM_I8 && (!k_scales || !v_scales)))

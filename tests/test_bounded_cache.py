@@ -135,6 +135,16 @@ def test_evict_c_entry_refusals():
     assert call(B=0, D=300) == -2
 
 
+@pytest.mark.parametrize("ps,pages", [(16, 1 << 27), (1 << 20, 2048), (7, (1 << 31) // 7)])
+def test_evict_refuses_rows_past_its_32_bit_positions(ps, pages):
+    """A sweep looks up to 32 * 1024 positions past a row's end."""
+    def call(S, mp):
+        return nv.lib().nvm_paged_evict(None, None, 2, None, None, 1, None, None, None, None, S, S, S, None, S, S, 0, 2, 128, 4, ps,
+                                        mp, 4, 0, 0, None, None, None, None, None, None)
+    assert call(2 ** 31 - 1, pages) == -2 and call(2 ** 31 - 65536, pages) == -2 and call(1 << 40, pages) == -2
+    assert call(2 ** 31 - 65537, pages) == 0 and call(1 << 40, pages // 2) == 0
+
+
 def test_request_cache_evict_checks_on_the_host():
     pool = TinyKvPagedPool(page_size=4)
     cache = TinyKvPagedCache(pool)
