@@ -103,6 +103,9 @@ def plan_evict(key_pages, value_pages, block_table, context_lens, key_mass, budg
         if mass_out.shape != key_mass.shape or mass_out.dtype is not torch.float32:
             raise RuntimeError(f"{op}: mass_out must be float32 with the shape of key_mass")
         osb, osh = _row_strides(f"{op}: mass_out", mass_out)
+        S = key_mass.shape[2]
+        if 0 < abs(mass_out.data_ptr() - key_mass.data_ptr()) < 4 * B * Hkv * S and msb == osb == Hkv * S and msh == osh == S:
+            raise RuntimeError(f"{op}: mass_out must be key_mass itself or share no memory with it")
     sdt = nv.NVM_F16
     if dtype not in _PAGE_DTYPES:
         raise RuntimeError(f"{op}: pages must be float32, float16, bfloat16 or int8")

@@ -162,6 +162,32 @@ def test_request_cache_evict_checks_on_the_host():
     assert cache.offset == 10 and cache.num_pages == 3
 
 
+def test_evict_refuses_a_mass_out_that_overlaps(monkeypatch):
+    """Rows would be written where other requests' weights have yet to be read."""
+    calls = []
+
+    class Lib:
+        def nvm_paged_evict(self, *args):
+            calls.append(args)
+            return 0
+
+    monkeypatch.setattr(nv, "lib", Lib)
+    monkeypatch.setattr(nv, "require_cuda", lambda op, *t: torch.device("cpu"))
+    monkeypatch.setattr(nv, "stream_ptr", lambda dev: 0)
+    k, v = (torch.zeros(8, 2, 16, 64) for _ in range(2))
+    bt, cl, store = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(1000)
+    mass = store[100:484].view(3, 2, 64)
+    for at in (99, 101, 100 - 383, 483):
+        with pytest.raises(RuntimeError, match="mass_out"):
+            evict_tokens(k, v, bt, cl, mass, 8, mass_out=store[max(at, 0):max(at, 0) + 384].view(3, 2, 64))
+    assert calls == []
+    evict_tokens(k, v, bt, cl, mass, 8, mass_out=mass)
+    evict_tokens(k, v, bt, cl, mass, 8, mass_out=store[484:868].view(3, 2, 64))
+    both = torch.zeros(3, 2, 2, 64)  # side by side, row after row
+    evict_tokens(k, v, bt, cl, both[:, 0], 8, mass_out=both[:, 1])
+    assert len(calls) == 3
+
+
 def _layer(int8=False, P=8, D=64):
     dt = torch.int8 if int8 else torch.bfloat16
     k, v = (torch.zeros(P, 2, 16, D, dtype=dt) for _ in range(2))
