@@ -143,6 +143,14 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
                                           int kv_dtype);
 
 /*
+ * The id of the stream capture that `stream` is part of, different for every capture of the
+ * process, or 0 when it is not capturing.  A graph replays with the workspace whose address it
+ * captured: give every capture one of its own, and zero its tickets inside the graph, ahead of
+ * the first call (memory of the graph may hold something else between its replays).
+ */
+int nvm_stream_capture_id(void* stream, unsigned long long* id);
+
+/*
  * nvm_paged_attention without a workspace argument.  No counterpart in the
  * reference: it exists for callers that cannot allocate device memory on their
  * hot path (an engine that gives all free HBM to its page pools up front, a decode

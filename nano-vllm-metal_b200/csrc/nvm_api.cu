@@ -301,6 +301,17 @@ int nvm_device_error(void* stream, int clear) {
   return v;
 }
 
+int nvm_stream_capture_id(void* stream, unsigned long long* id) {
+  if (id == nullptr) return fail(NVM_ERR_INVALID_ARGUMENT, "nvm_stream_capture_id: null pointer");
+  *id = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long which = 0;
+  const int st = check_cuda(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &which),
+                            "nvm_stream_capture_id");
+  if (st == NVM_OK && status == cudaStreamCaptureStatusActive) *id = which;
+  return st;
+}
+
 size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D,
                                           int64_t page_size, int64_t max_pages, int kv_dtype) {
   PagedArgs a{};

@@ -53,6 +53,7 @@ SIGNATURES = {
                                         _I64, _P]),
     "nvm_paged_evict": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64,
                              _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P]),
+    "nvm_stream_capture_id": (_I, [_P, _P]),
     "nvm_reshape_and_cache": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I, _P, _P, _I, _P, _I64, _I64, _I64, _I64,
                                    _I64, _P]),
     "nvm_paged_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P]),
@@ -145,9 +146,6 @@ def on_device(device: torch.device):
 # the GPU.  A call whose bounded wait expired may leave tickets non-zero, so
 # device_error() re-zeroes every workspace of the device after a non-zero word.
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
-# Buffers that a CUDA graph captured: kept when a larger call replaces them, as the graph replays
-# with their addresses.
-_captured: dict[int, torch.Tensor] = {}
 # A call that uses the workspace may launch several kernels, the later ones on what the first left
 # there, and ctypes drops the interpreter lock meanwhile: host threads that share a stream take turns.
 _workspace_locks: dict[tuple[int, int], threading.Lock] = {}
@@ -170,9 +168,18 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
-    if torch.cuda.is_current_stream_capturing():
-        _captured[ws.data_ptr()] = ws
     return ws
+
+
+# The workspace of the capture that runs (or ran last) on a stream, with that capture's id.
+_captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
+
+
+def capture_id(stream: int) -> int:
+    """The id of the CUDA graph capture on a stream, different for every capture (0: none)."""
+    out = ctypes.c_uint64(0)
+    check(lib().nvm_stream_capture_id(stream, ctypes.byref(out)))
+    return out.value
 
 
 def call_with_workspace(device: torch.device, size, call) -> None:
@@ -180,25 +187,32 @@ def call_with_workspace(device: torch.device, size, call) -> None:
 
     The buffer cached for (device, stream) is offered first, whatever its size: a call that
     needs more says so before any GPU work, and only then is the size asked for and the buffer
-    grown.  Threads on one stream take turns (0.5 us).  While a CUDA graph is being captured the
-    call gets a buffer of its own instead (from the graph's memory pool; the zero fill of its
-    tickets becomes a graph node): a graph replays with the addresses it captured, on any stream
-    and beside any other graph."""
-    stream = stream_ptr(device)
-    if torch.cuda.is_current_stream_capturing():
-        nbytes = size()
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        if ws is not None:
-            ws[:1 << 20].zero_()
-        check(call(ptr(ws), nbytes, stream))
-        return
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+    grown.  Threads on one stream take turns (0.5 us).
+
+    While a CUDA graph is being captured, the calls of one capture and stream share a buffer of
+    their graph's memory pool instead, whose tickets a node of the graph zeroes in front of the
+    first of them (1.3-2 us a replay): a graph replays with the addresses it captured, on any
+    stream, beside any other graph, and after eager calls that needed a larger buffer."""
+    key = _workspace_key(device)
+    stream = key[1]
     with _workspace_locks.get(key) or workspace_lock(device):
-        ws = _workspaces.get(key)
-        status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
-        if status == NVM_ERR_WORKSPACE:
-            nbytes = size()
-            status = call(ptr(workspace(device, nbytes)), nbytes, stream)
+        if torch.cuda.is_current_stream_capturing():
+            graph = capture_id(stream)
+            held, ws = _captured.get(key, (0, None))
+            if held != graph:
+                ws = None
+            status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
+            if status == NVM_ERR_WORKSPACE:
+                ws = torch.empty(size(), dtype=torch.uint8, device=device)
+                ws[:1 << 20].zero_()
+                _captured[key] = graph, ws
+                status = call(ptr(ws), ws.numel(), stream)
+        else:
+            ws = _workspaces.get(key)
+            status = call(ptr(ws), 0 if ws is None else ws.numel(), stream)
+            if status == NVM_ERR_WORKSPACE:
+                nbytes = size()
+                status = call(ptr(workspace(device, nbytes)), nbytes, stream)
     check(status)
 
 

@@ -283,11 +283,11 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
     L_ = nv.lib()
     kvc = nv.dtype_code(kp.dtype)
-    ws_bytes = L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc)
-    with torch.cuda.device(dev), nv.workspace_lock(dev):
-        ws = nv.workspace(dev, ws_bytes)
-        nv.check(L_.nvm_paged_attention(
-            q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
-            bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps,
-            bt.shape[1], float(factor), int(mask == "causal"), nv.ptr(ws), ws_bytes, nv.stream_ptr(dev)))
+    with nv.on_device(dev):
+        nv.call_with_workspace(
+            dev, lambda: L_.nvm_paged_attention_workspace_size(B, Hq, Hkv, L, D, ps, bt.shape[1], kvc),
+            lambda ws, ws_bytes, stream: L_.nvm_paged_attention(
+                q.data_ptr(), nv.dtype_code(q.dtype), kp.data_ptr(), vp.data_ptr(), kvc, nv.ptr(ks), nv.ptr(vs), sdt,
+                bt.data_ptr(), cl.data_ptr(), out.data_ptr(), nv.dtype_code(out.dtype), B, Hq, Hkv, L, D, P, ps,
+                bt.shape[1], float(factor), int(mask == "causal"), ws, ws_bytes, stream))
     return out

@@ -1,11 +1,11 @@
 """The bounded-cache operators' refusals and host bookkeeping (no GPU needed)."""
 
 import contextlib
+import ctypes
 import random
 import re
 import threading
 import time
-import weakref
 
 import pytest
 import torch
@@ -304,24 +304,63 @@ def test_threads_on_one_stream_take_turns_without_a_window(monkeypatch):
     monkeypatch.setattr(nv, "lib", lambda: Lib)
     monkeypatch.setattr(nv, "require_cuda", lambda op, *t: torch.device("cuda", 0))
     monkeypatch.setattr(nv, "stream_ptr", lambda d: 7)
+    monkeypatch.setattr(nv, "on_device", lambda d: contextlib.nullcontext())
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     pages, q = torch.zeros(2, 2, 16, 64), torch.zeros(1, 4, 1, 64)
     bt, cl = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     _in_threads(4, lambda i: [paged_attention(q, pages, pages, bt, cl, 16, out=torch.zeros_like(q)) for _ in range(3)])
     assert call.most == 1
 
 
-def test_a_captured_workspace_outlives_a_larger_call(monkeypatch):
-    """A graph of unwindowed calls replays with the stream's buffer, also after a scored call grew it."""
-    capturing = [True]
-    monkeypatch.setattr(nv, "_workspace_key", lambda d: (0, 123))
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+@pytest.mark.parametrize("window", [None, 8])
+def test_a_capture_has_a_workspace_of_its_own(monkeypatch, window):
+    """A graph replays with the addresses it captured, beside other graphs and whatever eager calls need: its calls
+    share a buffer whose tickets it zeroes itself, and the stream's buffer stays out of it."""
+    seen, capture, need = [], [5], [2 << 20]
+
+    def attend(*args):
+        ws, nbytes = args[-3], args[-2]
+        if nbytes < need[0]:
+            return nv.NVM_ERR_WORKSPACE
+        seen.append((ws, ctypes.string_at(ws, 1 << 20) == bytes(1 << 20)))
+        ctypes.memset(ws + (1 << 20), 7, nbytes - (1 << 20))  # the tickets are zero again
+        return 0
+
+    class Lib:
+        nvm_paged_attention = nvm_paged_attention_window = staticmethod(attend)
+        nvm_paged_attention_workspace_size = nvm_paged_attention_window_workspace_size = staticmethod(lambda *args: need[0])
+
+    monkeypatch.setattr(nv, "lib", lambda: Lib)
+    monkeypatch.setattr(nv, "require_cuda", lambda op, *t: torch.device("cpu"))
+    monkeypatch.setattr(nv, "stream_ptr", lambda d: 9)
+    monkeypatch.setattr(nv, "capture_id", lambda s: capture[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture[0] != 0)
     monkeypatch.setattr(nv, "_workspaces", {})
     monkeypatch.setattr(nv, "_captured", {}, raising=False)
-    cpu = torch.device("cpu")
-    captured = weakref.ref(nv.workspace(cpu, 1 << 21))
-    capturing[0] = False
-    larger = weakref.ref(nv.workspace(cpu, 1 << 22))
-    assert captured() is not None and nv.workspace(cpu, 1 << 21) is larger()
-    nv.workspace(cpu, 1 << 23)
-    assert larger() is None  # one that no graph holds is given back
+    pages, q = torch.zeros(2, 2, 16, 64), torch.zeros(1, 4, 1, 64)
+    bt, cl = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+
+    def run():
+        paged_attention(q, pages, pages, bt, cl, 16, window=window, out=torch.zeros_like(q))
+        at, zero = seen[-1]
+        assert zero
+        return at
+
+    first = run()
+    assert run() == first and nv._workspaces == {}
+    held = nv._captured[(0, 9)][1]  # as the graph's pool would
+    capture[0] = 0
+    eager = run()
+    assert eager != first and [ws.data_ptr() for ws in nv._workspaces.values()] == [eager]
+    capture[0] = 6  # another graph on the same stream
+    other = run()
+    assert other not in (first, eager) and run() == other
+    need[0] = 4 << 20
+    larger = run()
+    assert larger != other and run() == larger
+    capture[0] = 0
+    run()
+    assert held.data_ptr() == first

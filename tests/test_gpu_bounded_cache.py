@@ -593,6 +593,36 @@ def test_two_captured_graphs_replayed_side_by_side(L):
 
 
 @pytest.mark.parametrize("L", [1, 6, 80])
+def test_graphs_without_a_window_have_workspaces_of_their_own(L):
+    """Captured without a warm-up, the second replayed first, then side by side, after an eager call that needs more."""
+    probs = [make_problem(25 + i, [2500, 2900, 9000], L, 64 if L == 1 else 16, 8, 128, 16, BF) for i in range(2)]
+    gpu = [to_gpu(p) for p in probs]
+    refs = [paged_reference(p) for p in probs]
+    graphs, outs = [], []
+    for p in gpu:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal"))
+        graphs.append(graph)
+    p = gpu[0]
+    paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, mask="causal", key_mass=torch.zeros(3, 8, 9000, device="cuda"))
+    for i in (1, 0):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        ref, terms, _, _ = refs[i]
+        assert_within(outs[i], ref, out_bound(ref, terms, 128, BF, F32), f"graph {i}")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    first = [out.clone() for out in outs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, x) for out, x in zip(outs, first))
+
+
+@pytest.mark.parametrize("L", [1, 6, 80])
 def test_two_streams_at_once(L):
     probs = [make_problem(60 + i, [1500, 2900, 700], L, 64 if L == 1 else 16, 8, 128, 16, BF) for i in range(2)]
     masses = [torch.rand(3, 8, 2900) for _ in range(2)]
