@@ -202,6 +202,9 @@ int nvm_paged_attention_noalloc(const void* q, int q_dtype, const void* k_pages,
  * included).  A key that one query token sees but another does not must hold finite values.
  * As in nvm_paged_attention, q enters the tensor-core products in the pages' type (f16 over
  * int8 pages).
+ * A query row that holds NaN or an infinity has no defined output (NaN or zeros, as in
+ * nvm_paged_attention) and changes no other row's; the keys that a row of NaN sees get a NaN
+ * key_mass.
  * workspace      at least nvm_paged_attention_window_workspace_size(...) bytes, under the
  *                same rules as nvm_paged_attention's (and it may be the same buffer).  With
  *                key_mass and at most eight query rows per kv head it holds 4 bytes a query

@@ -2,7 +2,8 @@
 // with a sliding window, sinks and row log-sum-exps, one per default variant of the plan.
 // Measured on a B200: 64 requests of 4K-16K keys under a window of 4096 with 4 sinks, 32/8 heads,
 // bf16: 170-177 us, 6.1-6.3 TB/s of the keys seen (0.93-0.96 of a copy's rate); 48 requests under 2048, 64/8
-// heads, int8 pages: 59 us, 3.5 TB/s, bound by the int8 tile's instructions as without a window.
+// heads, int8 pages: 59 us, 3.5 TB/s, bound by latency: two chunks a unit make 768 CTAs of 1184 slots,
+// 9.5 warps an SM, which the int8 tile's conversions keep waiting (0.45 instructions a cycle).
 #include "paged_mma.cuh"
 
 namespace nvm {

@@ -202,13 +202,16 @@ def test_a_query_row_of_nan_shows_in_every_score_it_makes(L, D, kv, path):
         if row >= L:
             continue
         prob = make_problem(50, [ctx], L, 8, 2, D, 16, kv)
-        _, _, mref, merr = paged_reference(prob, mass=mass)
+        ref, terms, mref, merr = paged_reference(prob, mass=mass)
         prob["q"][0, head, row] = math.nan
         p, gm = to_gpu(prob), mass.cuda()
-        paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], mask="causal", key_mass=gm)
+        out = paged_attention(p["q"], p["k"], p["v"], p["bt"], p["cl"], 16, p["ks"], p["vs"], mask="causal", key_mass=gm)
         seen = ctx - L + row + 1  # by the NaN row
         assert gm[0, 0, :seen].isnan().all(), (head, row, int(gm[0, 0, :seen].isnan().sum()))
         assert_within(gm[0, 0, seen:], mref[0, 0, seen:], merr[0, 0, seen:] + 1e-30, "keys it does not see")
+        others = torch.ones(8, L, dtype=torch.bool)
+        others[head, row] = False
+        assert_within(out[0].cpu()[others], ref[0][others], out_bound(ref, terms, D, kv, F32)[0][others], "other rows")
         assert_within(gm[0, 1], mref[0, 1], merr[0, 1] + 1e-30, "the other kv head")
 
 
