@@ -148,16 +148,17 @@ def on_device(device: torch.device):
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 # A call that uses the workspace may launch several kernels, the later ones on what the first left
 # there, and ctypes drops the interpreter lock meanwhile: host threads that share a stream take turns.
-_workspace_locks: dict[tuple[int, int], threading.Lock] = {}
+# Reentrant, since a signal handler or a finaliser may call from inside a call of its own thread.
+_workspace_locks: dict = {}  # (device, stream) -> threading.RLock
 
 
 def _workspace_key(device: torch.device) -> tuple[int, int]:
     return device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device)
 
 
-def workspace_lock(device: torch.device) -> threading.Lock:
+def workspace_lock(device: torch.device):
     """To be held from ``workspace(device, ...)`` until the call that uses it has returned."""
-    return _workspace_locks.setdefault(_workspace_key(device), threading.Lock())
+    return _workspace_locks.setdefault(_workspace_key(device), threading.RLock())
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:

@@ -294,6 +294,31 @@ def test_threads_on_one_stream_take_turns(monkeypatch):
     assert both.most == 2
 
 
+def test_a_call_inside_a_call_of_the_same_thread(monkeypatch):
+    """As a signal handler makes it, between a refused workspace and the larger one."""
+    dev, calls = torch.device("cuda", 0), []
+    monkeypatch.setattr(nv, "stream_ptr", lambda d: 8)
+    monkeypatch.setattr(nv, "workspace", lambda d, n: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+    def inner(*args):
+        calls.append("inner")
+        return 0
+
+    def outer(*args):
+        calls.append("outer")
+        return nv.NVM_ERR_WORKSPACE if calls == ["outer"] else 0
+
+    def size():
+        nv.call_with_workspace(dev, lambda: 0, inner)
+        return 0
+
+    t = threading.Thread(target=nv.call_with_workspace, args=(dev, size, outer), daemon=True)
+    t.start()
+    t.join(20)
+    assert not t.is_alive() and calls == ["outer", "inner", "outer"]
+
+
 def test_threads_on_one_stream_take_turns_without_a_window(monkeypatch):
     call = _Turns()
 
