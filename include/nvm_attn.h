@@ -52,8 +52,22 @@ typedef enum nvm_dtype {
   NVM_BF16 = 2,
   NVM_I8 = 3,
   NVM_I32 = 4,
-  NVM_I64 = 5
+  NVM_I64 = 5,
+  NVM_U4 = 6 /* pages only: two 4-bit codes a byte, with scales and offsets (below) */
 } nvm_dtype;
+
+/*
+ * 4-bit pages (kv_dtype == NVM_U4; no counterpart in the reference), D = 64 or 128.  A row (one
+ * token of one kv head) is D/2 bytes of codes, byte j = code of element 2j | code of 2j + 1 << 4,
+ * and for each group of 64 elements a scale s and an offset z of scale_dtype (F16/BF16):
+ *   value = s * code + z
+ *   k_pages, v_pages    uint8 [P, Hkv, page_size, D/2], starting on a 16-byte boundary
+ *   k_scales, v_scales  [P, Hkv, page_size, 2 * D/64], (s, z) of every group, on an 8-byte one
+ * Writing: z = the group's least value, rounded toward -inf to scale_dtype; s = (greatest - z) / 15
+ * rounded toward +inf; code = clip(round_half_even((x - z) / s), 0, 15), 0 where s = 0.  No value
+ * is off by more than half a step s.  A group that holds a NaN or an infinity, or whose span
+ * scale_dtype cannot hold, reads back as NaN.
+ */
 
 /* Status codes (0 = success). */
 typedef enum nvm_status {
@@ -111,10 +125,11 @@ int nvm_selftest_wait_expiry(int64_t limit_ns, unsigned long long* waited_ns, vo
  *
  * q            [B*Hq, L, D] of q_dtype (F32/F16/BF16), row n = b*Hq + head.
  * k_pages,
- * v_pages      [P, Hkv, page_size, D] of kv_dtype (F32/F16/BF16/I8).
+ * v_pages      [P, Hkv, page_size, D] of kv_dtype (F32/F16/BF16/I8), or 4-bit rows.
  * k_scales,
  * v_scales     [P, Hkv, page_size, 1] of scale_dtype (F32/F16/BF16); required iff
- *              kv_dtype == NVM_I8, else NULL.  value = int8 * scale.
+ *              kv_dtype == NVM_I8, else NULL.  value = int8 * scale.  4-bit pages: see
+ *              nvm_dtype above.
  * block_table  [B, max_pages] int32 physical page ids; entries < 0 (or >= P) are
  *              holes whose positions are skipped, as in paged_attention.cpp:216-222.
  * context_lens [B] int32; context_len <= 0 gives a zero output row block.
@@ -304,7 +319,8 @@ int nvm_flash_attention(const void* q, const void* k, const void* v, int dtype, 
  *                amax = max|x| (fp32); s = amax > 0 ? amax/127 : 1;
  *                q = clip(round_half_even(x / s), -127, 127);
  *              and stores s rounded to scale_dtype in k_scales / v_scales
- *              [P, Hkv, page_size, 1] (paged.py:153-158).
+ *              [P, Hkv, page_size, 1] (paged.py:153-158); kv_dtype == NVM_U4
+ *              quantises groups of 64 elements (nvm_dtype above).
  * Pages are mutated in place (the reference's buffer-donating slice-assign).
  */
 int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t stride_t,
@@ -312,6 +328,17 @@ int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t st
                           void* k_scales, void* v_scales, int scale_dtype,
                           const int64_t* slot_mapping, int64_t T, int64_t Hkv, int64_t D,
                           int64_t P, int64_t page_size, void* stream);
+
+/*
+ * Reads slots back (no counterpart in the reference, whose read_page returns whole pages):
+ * k, v [T, Hkv, D] of out_dtype (F32/F16/BF16) receive the values that the rows at
+ * slot_mapping[t] stand for, rounded once; tokens whose slot is < 0 or past the pool are zero.
+ * Pages and scales of any type that nvm_reshape_and_cache writes.
+ */
+int nvm_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const void* k_scales,
+                   const void* v_scales, int scale_dtype, const int64_t* slot_mapping, void* k, void* v,
+                   int out_dtype, int64_t T, int64_t Hkv, int64_t D, int64_t P, int64_t page_size,
+                   void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* Fused per-layer preparation: q/k RMSNorm + RoPE + K/V scatter-write        */
@@ -331,7 +358,9 @@ int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t st
  *   q_out_L > 0 (the [B, Hq, L, D] layout paged_attention takes);
  *   K (normalised, rotated) and V (as given) go to the pages at slot_mapping[t]
  *   (page_id * page_size + offset; negative = skip), copied or int8-quantised as
- *   nvm_reshape_and_cache does.  D must be 64 or 128.  Rounding follows the reference:
+ *   nvm_reshape_and_cache does, or quantised to 4 bits (scale_dtype == dtype).  D must be 64
+ *   or 128.  With both norm weights NULL the rows are rotated as they are (models without
+ *   q/k norm).  Rounding follows the reference:
  *   the norm result and the rotation result are each rounded to dtype, the rotation is
  *   computed in fp32 from the rounded norm result.
  */

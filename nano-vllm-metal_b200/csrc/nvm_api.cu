@@ -120,13 +120,33 @@ namespace {
 
 bool is_float_dtype(int d) { return d == NVM_F32 || d == NVM_F16 || d == NVM_BF16; }
 
+// What every call over 4-bit pages needs: whole groups, scales of a 16-bit type, rows numbered in 32
+// bits (a pool of 2^32 rows would be 300 GB), rows that start on 16-byte boundaries.
+int validate_u4(const char* op, int scale_dtype, int64_t D, int64_t P, int64_t Hkv, int64_t page_size) {
+  if (D != 64 && D != 128)
+    return fail(NVM_ERR_UNSUPPORTED, "%s: 4-bit pages need a head dimension of 64 or 128 (got %lld)", op, (long long)D);
+  if (scale_dtype != NVM_F16 && scale_dtype != NVM_BF16)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: scales of 4-bit pages must be float16 or bfloat16", op);
+  if (Hkv > INT32_MAX || page_size > INT32_MAX || P > INT32_MAX || Hkv * page_size > INT32_MAX ||
+      P * (Hkv * page_size) >= (int64_t)UINT32_MAX)
+    return fail(NVM_ERR_UNSUPPORTED, "%s: 4-bit pools of 2^32 rows or more are not supported", op);
+  return NVM_OK;
+}
+int validate_u4_pointers(const char* op, const void* kp, const void* vp, const void* ks, const void* vs) {
+  if (kp == nullptr || vp == nullptr || ks == nullptr || vs == nullptr)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: 4-bit pages need pages and scales of keys and values", op);
+  if (((uintptr_t)kp | (uintptr_t)vp) % 16 != 0 || ((uintptr_t)ks | (uintptr_t)vs) % 8 != 0)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: 4-bit pages must start on 16-byte boundaries, their scales on 8-byte ones", op);
+  return NVM_OK;
+}
+
 // Shared validation of nvm_paged_attention / nvm_paged_attention_workspace_size.
 int validate_paged(const PagedArgs& a, bool check_ptrs) {
   const char* op = a.kv_dtype == NVM_I8 ? "paged_attention_int8_decode" : "paged_attention";
   if (!is_float_dtype(a.q_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "%s: q must be float32, float16 or bfloat16", op);
-  if (!is_float_dtype(a.kv_dtype) && a.kv_dtype != NVM_I8)
+  if (!is_float_dtype(a.kv_dtype) && a.kv_dtype != NVM_I8 && a.kv_dtype != NVM_U4)
     return fail(NVM_ERR_INVALID_ARGUMENT,
-                "paged_attention: key_pages and value_pages must be float32, float16, bfloat16 or int8");
+                "paged_attention: key_pages and value_pages must be float32, float16, bfloat16, int8 or 4-bit");
   if (!is_float_dtype(a.out_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "%s: output dtype must be floating point", op);
   if (a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.L <= 0 || a.D <= 0 || a.P < 0 || a.page_size <= 0 ||
       a.max_pages < 0)
@@ -139,6 +159,14 @@ int validate_paged(const PagedArgs& a, bool check_ptrs) {
       return fail(NVM_ERR_INVALID_ARGUMENT, "%s: key_scales and value_scales must be floating point", op);
     if (check_ptrs && (a.k_scales == nullptr || a.v_scales == nullptr))
       return fail(NVM_ERR_INVALID_ARGUMENT, "%s: int8 pages need key_scales and value_scales", op);
+  }
+  if (a.kv_dtype == NVM_U4) {
+    const int st = validate_u4(op, a.scale_dtype, a.D, a.P, a.Hkv, a.page_size);
+    if (st != NVM_OK) return st;
+    if (check_ptrs && a.max_pages > 0 && a.P > 0) {
+      const int aligned = validate_u4_pointers(op, a.k_pages, a.v_pages, a.k_scales, a.v_scales);
+      if (aligned != NVM_OK) return aligned;
+    }
   }
   if (check_ptrs && a.B > 0) {
     if (a.q == nullptr || a.out == nullptr || a.context_lens == nullptr || a.block_table == nullptr)
@@ -322,6 +350,7 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
   a.is_causal = 1;
   if (validate_paged(a, false) != NVM_OK) return 0;
+  if (kv_dtype == NVM_U4) return 0;
   if (env_flag("NVM_ATTN_FORCE_GENERIC")) return 0;
   // q's dtype is not known here: cover the tcgen05 plan (taken when q matches the pages)
   // and the mma.sync plan (taken otherwise).
@@ -351,6 +380,7 @@ int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const v
   if (st != NVM_OK) return st;
   if (B == 0) return NVM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (kv_dtype == NVM_U4) return launch_paged_u4(a, s);
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
     if (!env_flag("NVM_ATTN_NO_SM100") && flash2q_eligible(a)) return launch_flash2q(a, s);
     if (!env_flag("NVM_ATTN_NO_SM100")) {
@@ -425,7 +455,9 @@ size_t nvm_paged_attention_window_workspace_size(int64_t B, int64_t Hq, int64_t 
   a.out_dtype = NVM_F32;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
   a.window = window; a.sinks = sinks;
-  if (validate_paged(a, false) != NVM_OK || validate_window(window, sinks, "paged_attention") != NVM_OK) return 0;
+  if (kv_dtype == NVM_U4 || validate_paged(a, false) != NVM_OK ||
+      validate_window(window, sinks, "paged_attention") != NVM_OK)
+    return 0;
   if (with_mass) a.lse = &kLseLater;
   // q's dtype and the mask are not known here: cover both kernels' plans, and both masks (without
   // the causal limit the rows of a block see on to the last key, so windows take more chunks)
@@ -460,6 +492,8 @@ int nvm_paged_attention_window(const void* q, int q_dtype, const void* k_pages, 
   a.block_table = block_table; a.context_lens = context_lens; a.out = out; a.out_dtype = out_dtype;
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = P; a.page_size = page_size; a.max_pages = max_pages;
   a.scale = scale; a.is_causal = is_causal ? 1 : 0; a.window = window; a.sinks = sinks;
+  if (kv_dtype == NVM_U4)
+    return fail(NVM_ERR_UNSUPPORTED, "paged_attention: window, sinks and key_mass do not go with 4-bit pages");
   int st = validate_paged(a, true);
   if (st != NVM_OK) return st;
   st = validate_window(window, sinks, "paged_attention");
@@ -582,8 +616,8 @@ int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t st
                           int scale_dtype, const int64_t* slot_mapping, int64_t T, int64_t Hkv, int64_t D,
                           int64_t P, int64_t page_size, void* stream) {
   if (!is_float_dtype(in_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "write_page_slice: key/value must be floating point");
-  if (kv_dtype != in_dtype && kv_dtype != NVM_I8)
-    return fail(NVM_ERR_INVALID_ARGUMENT, "write_page_slice: page dtype must equal the input dtype or be int8");
+  if (kv_dtype != in_dtype && kv_dtype != NVM_I8 && kv_dtype != NVM_U4)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "write_page_slice: page dtype must equal the input dtype or be int8 or 4-bit");
   if (kv_dtype == NVM_I8 && (k_scales == nullptr || v_scales == nullptr || !is_float_dtype(scale_dtype)))
     return fail(NVM_ERR_INVALID_ARGUMENT, "write_page_slice: int8 pages need floating-point key/value scales");
   if (T < 0 || Hkv <= 0 || D <= 0 || P < 0 || page_size <= 0)
@@ -591,8 +625,40 @@ int nvm_reshape_and_cache(const void* k, const void* v, int in_dtype, int64_t st
   if (T == 0) return NVM_OK;
   if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr || slot_mapping == nullptr)
     return fail(NVM_ERR_INVALID_ARGUMENT, "write_page_slice: null tensor pointer");
+  if (kv_dtype == NVM_U4) {
+    int st = validate_u4("write_page_slice", scale_dtype, D, P, Hkv, page_size);
+    if (st == NVM_OK) st = validate_u4_pointers("write_page_slice", k_pages, v_pages, k_scales, v_scales);
+    if (st != NVM_OK) return st;
+    if (T > INT32_MAX / Hkv) return fail(NVM_ERR_UNSUPPORTED, "write_page_slice: too many rows");
+    return launch_u4_write(k, v, in_dtype, stride_t, stride_h, k_pages, v_pages, k_scales, v_scales, scale_dtype, slot_mapping, T,
+                           Hkv, D, P, page_size, static_cast<cudaStream_t>(stream));
+  }
   return launch_kv_write(k, v, in_dtype, stride_t, stride_h, k_pages, v_pages, kv_dtype, k_scales, v_scales,
                          scale_dtype, slot_mapping, T, Hkv, D, P, page_size, static_cast<cudaStream_t>(stream));
+}
+
+int nvm_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const void* k_scales, const void* v_scales,
+                   int scale_dtype, const int64_t* slot_mapping, void* k, void* v, int out_dtype, int64_t T, int64_t Hkv,
+                   int64_t D, int64_t P, int64_t page_size, void* stream) {
+  const char* op = "read_slots";
+  if (!is_float_dtype(out_dtype)) return fail(NVM_ERR_INVALID_ARGUMENT, "%s: key/value must be floating point", op);
+  if (!is_float_dtype(kv_dtype) && kv_dtype != NVM_I8 && kv_dtype != NVM_U4)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: pages must be float32, float16, bfloat16, int8 or 4-bit", op);
+  if (T < 0 || Hkv <= 0 || D <= 0 || P < 0 || page_size <= 0)
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", op);
+  if (T > INT32_MAX / Hkv) return fail(NVM_ERR_UNSUPPORTED, "%s: too many rows", op);
+  if (kv_dtype == NVM_I8 && (k_scales == nullptr || v_scales == nullptr || !is_float_dtype(scale_dtype)))
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: int8 pages need floating-point key/value scales", op);
+  if (kv_dtype == NVM_U4) {
+    int st = validate_u4(op, scale_dtype, D, P, Hkv, page_size);
+    if (st == NVM_OK && T > 0 && P > 0) st = validate_u4_pointers(op, k_pages, v_pages, k_scales, v_scales);
+    if (st != NVM_OK) return st;
+  }
+  if (T == 0) return NVM_OK;
+  if (k == nullptr || v == nullptr || slot_mapping == nullptr || (P > 0 && (k_pages == nullptr || v_pages == nullptr)))
+    return fail(NVM_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
+  return launch_read_slots(k_pages, v_pages, kv_dtype, k_scales, v_scales, scale_dtype, slot_mapping, k, v, out_dtype, T, Hkv, D,
+                           P, page_size, static_cast<cudaStream_t>(stream));
 }
 
 int nvm_paged_append(int32_t* block_table, int32_t* context_lens, const int32_t* new_tokens, int32_t* free_stack,

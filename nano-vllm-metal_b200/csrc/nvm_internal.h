@@ -176,6 +176,15 @@ int launch_kv_write(const void* k, const void* v, int in_dtype, int64_t stride_t
                     int scale_dtype, const int64_t* slot_mapping, int64_t T, int64_t Hkv, int64_t D,
                     int64_t P, int64_t page_size, cudaStream_t s);
 
+// 4-bit cache (u4.cuh): scatter-write, reading slots back (any page type), attention.
+int launch_u4_write(const void* k, const void* v, int in_dtype, int64_t stride_t, int64_t stride_h, void* k_pages, void* v_pages,
+                    void* k_scales, void* v_scales, int scale_dtype, const int64_t* slots, int64_t T, int64_t Hkv, int64_t D,
+                    int64_t P, int64_t page_size, cudaStream_t s);
+int launch_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const void* k_scales, const void* v_scales,
+                      int scale_dtype, const int64_t* slots, void* k, void* v, int out_dtype, int64_t T, int64_t Hkv, int64_t D,
+                      int64_t P, int64_t page_size, cudaStream_t s);
+int launch_paged_u4(const PagedArgs& a, cudaStream_t s);
+
 int launch_paged_append(int32_t* block_table, int32_t* context_lens, const int32_t* new_tokens,
                         int32_t* free_stack, int32_t* free_top, int32_t* num_pages,
                         int32_t* page_refcount, int64_t* slot_mapping, int64_t slot_capacity, int32_t* status, int64_t B,

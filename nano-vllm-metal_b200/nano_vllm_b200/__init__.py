@@ -5,7 +5,8 @@ page pools: ``paged_attention``, ``flash_attention``, ``TinyKvPagedPool``,
 ``TinyKvPagedCache``, ``BatchingKvCache`` keep the reference's names and
 signatures (the reference's ``PrefixCache`` runs unchanged over these pools); the
 kernels live in ``libnvm_attn.so`` (C ABI in ``include/nvm_attn.h``).  A cache is kept bounded
-by ``window`` / ``sinks`` and ``key_mass`` of the attention calls and by ``evict_tokens``.
+by ``window`` / ``sinks`` and ``key_mass`` of the attention calls and by ``evict_tokens``, and small
+by 8- or 4-bit pages (``kv_bits`` of the pool).
 """
 
 from .layers.attention import (  # noqa: F401
@@ -14,6 +15,8 @@ from .layers.attention import (  # noqa: F401
     paged_attention,
     scaled_dot_product_attention_grouped,
 )
+from .layers.qk_prep import qk_norm_rope_write  # noqa: F401
+from .layers.rotary_embedding import RoPE  # noqa: F401
 from .cache.evict import EvictResult, evict_tokens  # noqa: F401
 from .cache.kv_cache import BatchingKvCache, TinyKvCache  # noqa: F401
 from .cache.paged import (  # noqa: F401
@@ -21,6 +24,7 @@ from .cache.paged import (  # noqa: F401
     PagedKvMetadata,
     TinyKvPagedCache,
     TinyKvPagedPool,
+    read_slots,
     write_slots,
 )
 from .spec_verify import VerifyResult, verify_accept  # noqa: F401

@@ -17,7 +17,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnvm_attn.so")
 
-NVM_F32, NVM_F16, NVM_BF16, NVM_I8, NVM_I32, NVM_I64 = 0, 1, 2, 3, 4, 5
+NVM_F32, NVM_F16, NVM_BF16, NVM_I8, NVM_I32, NVM_I64, NVM_U4 = 0, 1, 2, 3, 4, 5, 6
 NVM_OK = 0
 NVM_ERR_WORKSPACE = -3
 
@@ -28,7 +28,9 @@ _DTYPE_CODE = {
     torch.int8: NVM_I8,
     torch.int32: NVM_I32,
     torch.int64: NVM_I64,
+    torch.uint8: NVM_U4,  # pages of packed 4-bit codes
 }
+U4_GROUP = 64  # elements of a 4-bit row that share a scale and an offset
 
 # Every exported symbol of include/nvm_attn.h with (restype, argtypes).
 _P, _I, _I64, _F, _SZ, _CP = (ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float,
@@ -56,6 +58,7 @@ SIGNATURES = {
     "nvm_stream_capture_id": (_I, [_P, _P]),
     "nvm_reshape_and_cache": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I, _P, _P, _I, _P, _I64, _I64, _I64, _I64,
                                    _I64, _P]),
+    "nvm_read_slots": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _P]),
     "nvm_paged_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P]),
     "nvm_paged_rewind": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "nvm_paged_attach": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
@@ -119,6 +122,28 @@ def require_cuda(op: str, *tensors: torch.Tensor) -> torch.device:
     if dev is None:
         raise RuntimeError(f"{op}: no tensor given")
     return dev
+
+
+def require_u4(op: str, D: int, key_pages: torch.Tensor, value_pages: torch.Tensor, key_scales: torch.Tensor | None,
+               value_scales: torch.Tensor | None) -> None:
+    """The pools of a 4-bit cache of head dim D: uint8 [P, Hkv, page_size, D/2] with scales and offsets
+    [P, Hkv, page_size, D/32], all contiguous."""
+    if D not in (64, 128):
+        raise RuntimeError(f"{op}: 4-bit pages need a head dimension of 64 or 128 (got {D})")
+    shape = key_pages.shape
+    if value_pages.dtype is not torch.uint8 or len(shape) != 4 or value_pages.shape != shape or shape[3] * 2 != D:
+        raise RuntimeError(f"{op}: 4-bit key_pages and value_pages must be uint8 [P, Hkv, page_size, D / 2]")
+    if key_scales is None or value_scales is None:
+        raise RuntimeError(f"{op}: 4-bit pages need key_scales and value_scales")
+    want = (*shape[:3], 2 * D // U4_GROUP)
+    if tuple(key_scales.shape) != want or tuple(value_scales.shape) != want:
+        raise RuntimeError(f"{op}: scales of 4-bit pages must be [P, Hkv, page_size, {want[3]}] (a scale and an offset for every "
+                           f"{U4_GROUP} elements)")
+    if key_scales.dtype is not value_scales.dtype or key_scales.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"{op}: scales of 4-bit pages must both be float16 or both bfloat16")
+    if not (key_pages.is_contiguous() and value_pages.is_contiguous() and key_scales.is_contiguous()
+            and value_scales.is_contiguous()):
+        raise RuntimeError(f"{op}: 4-bit pages and their scales must be contiguous")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -2,7 +2,9 @@
 
 * ``TinyKvPagedPool`` (reference ``paged.py:21-210``): page storage is a device
   tensor ``[capacity, H, page_size, D]`` (int8 + scales ``[capacity, H, page_size, 1]``
-  for ``kv_bits=8``).  The free list, reference counts, page-id order and capacity
+  for ``kv_bits=8``; packed 4-bit codes ``[capacity, H, page_size, D/2]`` + scales and
+  offsets ``[capacity, H, page_size, D/32]`` for ``kv_bits=4, kv_group_size=64``).  The free
+  list, reference counts, page-id order and capacity
   growth policy are the reference's, so page ids and pool shapes match it exactly.
   ``reserve_pages`` optionally pre-allocates HBM for that many pages so growth
   becomes a view change instead of a reallocate + copy.
@@ -31,7 +33,7 @@ from .. import _native as nv
 from .kv_cache import TinyKvCache
 
 __all__ = ["PagedKvMetadata", "TinyKvPagedPool", "TinyKvPagedCache", "DevicePageTable",
-           "write_slots"]
+           "write_slots", "read_slots"]
 
 
 @dataclass
@@ -53,11 +55,19 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, key
 
     ``key``/``value`` are ``[T, H, D]`` views (any token/head strides, D contiguous),
     e.g. ``k[0].transpose(0, 1)`` of a ``[1, H, S, D]`` chunk.  ``slots[t]`` is
-    ``page_id * page_size + offset`` (< 0 skips the token).
+    ``page_id * page_size + offset`` (< 0 skips the token).  Pages hold the rows' own type,
+    int8 (scales ``[P, H, page_size, 1]``) or packed 4-bit codes (uint8 ``[P, H, page_size,
+    D/2]``, D 64 or 128, scales ``[P, H, page_size, D/32]``: scale and offset of every 64
+    elements, float16 or bfloat16).
     """
     T, H, D = key.shape
     P, Hp, ps, Dp = key_pages.shape
-    assert Hp == H and Dp == D and value.shape == key.shape
+    u4 = key_pages.dtype is torch.uint8
+    assert Hp == H and (u4 or Dp == D) and value.shape == key.shape
+    if u4:
+        nv.require_u4("write_page_slice", D, key_pages, value_pages, key_scales, value_scales)
+        if key.dtype is not value.dtype or slots.numel() != T:
+            raise RuntimeError("write_page_slice: key and value must share one dtype and have one slot a token")
     dev = nv.require_cuda("write_page_slice", key, value, slots, key_pages, value_pages, key_scales, value_scales)
     if key.stride(2) != 1:
         key = key.contiguous()
@@ -74,14 +84,62 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, key
             nv.ptr(value_scales), sdt, slots.data_ptr(), T, H, D, P, ps, nv.stream_ptr(dev)))
 
 
+def read_slots(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+               key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
+               dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The inverse of ``write_slots``: the values of the rows at ``slots`` ``[T]``, as contiguous
+    ``[T, H, D]`` keys and values.
+
+    Pages and scales as ``write_slots`` takes them; int8 and 4-bit rows are dequantised (in fp32,
+    rounded once).  ``dtype`` (float32, float16 or bfloat16) defaults to the pages' own, or to
+    that of the scales.  A slot below 0 or past the pool reads as zeros.
+    """
+    op = "read_slots"
+    dev = nv.require_cuda(op, slots, key_pages, value_pages, key_scales, value_scales)
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype is not value_pages.dtype:
+        raise RuntimeError(f"{op}: key_pages and value_pages must be [P, H, page_size, D] of one dtype")
+    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{op}: slots must be one row of int32 or int64")
+    P, H, ps, D = key_pages.shape
+    ks, vs = key_scales, value_scales
+    if key_pages.dtype is torch.uint8:
+        D = 2 * D
+        nv.require_u4(op, D, key_pages, value_pages, ks, vs)
+    elif key_pages.dtype is torch.int8:
+        if ks is None or vs is None or tuple(ks.shape) != (P, H, ps, 1) or vs.shape != ks.shape or ks.dtype is not vs.dtype:
+            raise RuntimeError(f"{op}: int8 pages need key_scales and value_scales [P, H, page_size, 1] of one dtype")
+        if not (ks.is_contiguous() and vs.is_contiguous()):
+            raise RuntimeError(f"{op}: pages and scales must be contiguous")
+    else:
+        ks = vs = None
+    if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
+        raise RuntimeError(f"{op}: pages and scales must be contiguous")
+    if dtype is None:
+        dtype = key_pages.dtype if ks is None else ks.dtype
+    T = slots.shape[0]
+    key, value = (torch.empty((T, H, D), dtype=dtype, device=dev) for _ in range(2))
+    rows = slots.to(torch.int64).contiguous()
+    with nv.on_device(dev):
+        nv.check(nv.lib().nvm_read_slots(
+            key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(ks), nv.ptr(vs),
+            nv.NVM_F16 if ks is None else nv.dtype_code(ks.dtype), rows.data_ptr(), key.data_ptr(), value.data_ptr(),
+            nv.dtype_code(dtype), T, H, D, P, ps, nv.stream_ptr(dev)))
+    return key, value
+
+
 class TinyKvPagedPool:
     """Model-local physical storage for paged KV (one pool per layer in the model)."""
 
     def __init__(self, page_size: int = 128, kv_bits: int | None = None, device: torch.device | str | None = None,
-                 reserve_pages: int | None = None):
+                 reserve_pages: int | None = None, kv_group_size: int | None = None):
         assert page_size > 0
-        if kv_bits is not None and kv_bits != 8:
-            raise ValueError("TinyKvPagedPool currently supports only int8 KV")
+        if kv_bits == 4:
+            if kv_group_size != nv.U4_GROUP:
+                raise ValueError(f"4-bit KV needs kv_group_size={nv.U4_GROUP} (elements that share a scale and an offset)")
+        elif kv_bits is not None and kv_bits != 8:
+            raise ValueError("TinyKvPagedPool currently supports only int8 and 4-bit KV")
+        elif kv_group_size is not None:
+            raise ValueError("kv_group_size goes with kv_bits=4 only")
         self.page_size = page_size
         self.kv_bits = kv_bits
         self.device = torch.device(device) if device is not None else None
@@ -145,6 +203,10 @@ class TinyKvPagedPool:
             raise ValueError(f"Page {page_id} has no storage")
         if page_id >= self.num_pages:
             raise ValueError(f"Page {page_id} is out of range")
+        if self.kv_bits == 4:
+            slots = torch.arange(page_id * self.page_size, (page_id + 1) * self.page_size, device=self.key_pages.device)
+            k, v = read_slots(slots, self.key_pages, self.value_pages, self.key_scales, self.value_scales, torch.float32)
+            return k.transpose(0, 1)[None], v.transpose(0, 1)[None]
         if self.kv_bits == 8:
             return (self.key_pages[page_id:page_id + 1].float() * self.key_scales[page_id:page_id + 1].float(),
                     self.value_pages[page_id:page_id + 1].float() * self.value_scales[page_id:page_id + 1].float())
@@ -160,10 +222,17 @@ class TinyKvPagedPool:
         return max(self.num_pages, self._capacity * 2)
 
     def _ensure_page_storage(self, key: torch.Tensor) -> None:
-        """Grow device storage to the logical capacity (zero pages, unit scales)."""
+        """Grow device storage to the logical capacity (zero pages; unit scales, zero ones for 4 bits)."""
         B, H, _, D = key.shape
         assert B == 1
-        storage_dtype = torch.int8 if self.kv_bits == 8 else key.dtype
+        storage_dtype = {8: torch.int8, 4: torch.uint8}.get(self.kv_bits, key.dtype)
+        scale_dtype, scale_width, new_scales = key.dtype, 1, torch.ones
+        if self.kv_bits == 4:
+            if D not in (64, 128):
+                raise ValueError(f"4-bit KV needs a head dimension of 64 or 128 (got {D})")
+            # a 16-bit scale and offset for every 64 elements; float32 keys take the type with their range
+            scale_dtype = torch.bfloat16 if key.dtype == torch.float32 else key.dtype
+            D, scale_width, new_scales = D // 2, 2 * D // nv.U4_GROUP, torch.zeros
         if self.device is None:
             self.device = key.device
         cap = self._capacity
@@ -172,16 +241,15 @@ class TinyKvPagedPool:
             assert self.key_pages.dtype == storage_dtype
             if self.key_pages.shape[0] == cap:
                 return
-        scale_dtype = key.dtype
         if self.reserve_pages is not None and cap <= self.reserve_pages:
             if self._store is None:
                 R = self.reserve_pages
                 k = torch.zeros((R, H, self.page_size, D), dtype=storage_dtype, device=self.device)
                 v = torch.zeros_like(k)
                 ks = vs = None
-                if self.kv_bits == 8:
-                    ks = torch.ones((R, H, self.page_size, 1), dtype=scale_dtype, device=self.device)
-                    vs = torch.ones_like(ks)
+                if self.kv_bits is not None:
+                    ks, vs = (new_scales((R, H, self.page_size, scale_width), dtype=scale_dtype, device=self.device)
+                              for _ in range(2))
                 self._store = (k, v, ks, vs)
             k, v, ks, vs = self._store
             self.key_pages, self.value_pages = k[:cap], v[:cap]
@@ -195,9 +263,9 @@ class TinyKvPagedPool:
             new_k[:old] = self.key_pages
             new_v[:old] = self.value_pages
         self.key_pages, self.value_pages = new_k, new_v
-        if self.kv_bits == 8:
-            new_ks = torch.ones((cap, H, self.page_size, 1), dtype=scale_dtype, device=self.device)
-            new_vs = torch.ones_like(new_ks)
+        if self.kv_bits is not None:
+            new_ks, new_vs = (new_scales((cap, H, self.page_size, scale_width), dtype=scale_dtype, device=self.device)
+                              for _ in range(2))
             if self.key_scales is not None:
                 old = self.key_scales.shape[0]
                 new_ks[:old] = self.key_scales

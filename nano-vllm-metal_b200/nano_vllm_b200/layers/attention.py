@@ -158,6 +158,8 @@ def _paged_attention_window(query, key_pages, value_pages, block_table, context_
     """paged_attention with a window or key scores."""
     op = "paged_attention"
     _check_window(op, window, sinks)
+    if key_pages.dtype is torch.uint8:
+        raise NotImplementedError("paged_attention: window, sinks and key_mass do not go with 4-bit pages")
     if isinstance(mask, torch.Tensor):
         raise NotImplementedError("Paged attention only supports mask=None or causal")
     if mask is not None and mask != "causal":
@@ -228,7 +230,9 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     """Paged attention over block-paged K/V pools (reference attention.py:154-230).
 
     query ``[B, Hq, L, D]``; key_pages/value_pages ``[P, Hkv, page_size, D]`` (fp32,
-    fp16, bf16, or int8 with ``key_scales``/``value_scales`` ``[P, Hkv, page_size, 1]``);
+    fp16, bf16, or int8 with ``key_scales``/``value_scales`` ``[P, Hkv, page_size, 1]``), or
+    packed 4-bit codes, uint8 ``[P, Hkv, page_size, D/2]`` (D 64 or 128) with ``key_scales``/
+    ``value_scales`` ``[P, Hkv, page_size, D/32]`` (a scale and an offset for every 64 elements);
     block_table ``[B, max_pages]`` (-1 padded); context_lens ``[B]`` (tokens of each
     sequence, the new L included).  Returns ``[B, Hq, L, D]`` (fp32 by default).
 
@@ -258,7 +262,13 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         raise RuntimeError("paged_attention: key_pages and value_pages must have the same dtype")
     if key_pages.shape != value_pages.shape:
         raise RuntimeError("paged_attention: key_pages and value_pages must have the same shape")
-    if key_pages.shape[3] != D:
+    if key_pages.dtype is torch.uint8:
+        nv.require_u4("paged_attention", D, key_pages, value_pages, key_scales, value_scales)
+        if ps != page_size:
+            raise RuntimeError("paged_attention: pages must be [P, Hkv, page_size, D / 2]")
+        if out is not None and (tuple(out.shape) != (B, Hq, L, D) or not out.is_contiguous() or out.device != query.device):
+            raise RuntimeError("paged_attention: out must be a contiguous [B, Hq, L, D] tensor on the query's device")
+    elif key_pages.shape[3] != D:
         raise RuntimeError("paged_attention: q and page tensors must have the same head dimension")
     q = query.contiguous()
     kp = key_pages.contiguous()
@@ -279,6 +289,8 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         if ks.dtype != vs.dtype:
             vs = vs.to(ks.dtype)
         sdt = nv.dtype_code(ks.dtype)
+    elif kp.dtype is torch.uint8:
+        ks, vs, sdt = key_scales, value_scales, nv.dtype_code(key_scales.dtype)
     if out is None:
         out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
     L_ = nv.lib()

@@ -26,15 +26,18 @@ def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x.contiguous(), H * D
 
 
-def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_weight: torch.Tensor,
-                       k_norm_weight: torch.Tensor, rope: RoPE, positions: torch.Tensor, key_pages: torch.Tensor,
+def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_weight: torch.Tensor | None,
+                       k_norm_weight: torch.Tensor | None, rope: RoPE, positions: torch.Tensor, key_pages: torch.Tensor,
                        value_pages: torch.Tensor, slot_mapping: torch.Tensor, *, eps: float = 1e-5,
                        key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """q [B, L, Hq, D], k/v [B, L, Hkv, D] (the projections, f16/bf16); positions [B, L]
     (request offset + index); slot_mapping [B * L] int64 (page_id * page_size + offset,
     negative = skip).  Returns q normalised and rotated, [B, Hq, L, D]; K (normalised,
-    rotated) and V are written into key_pages / value_pages [P, Hkv, page_size, D]."""
+    rotated) and V are written into key_pages / value_pages [P, Hkv, page_size, D], of q's
+    dtype, int8 or packed 4-bit codes (uint8 [P, Hkv, page_size, D / 2] with scales of q's
+    dtype, see ``cache.paged.write_slots``).  Without norm weights (both None: models that
+    have no q/k norm) the rows are rotated as they are."""
     nv.require_cuda("qk_norm_rope_write", q, k, v, q_norm_weight, k_norm_weight, positions, key_pages, value_pages,
                     slot_mapping)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
@@ -54,21 +57,28 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
     if k_st != v_st:
         kc, vc = k.contiguous(), v.contiguous()
         k_st = v_st = Hkv * D
-    wq = q_norm_weight.to(q.dtype).contiguous()
-    wk = k_norm_weight.to(q.dtype).contiguous()
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise RuntimeError("qk_norm_rope_write: q and k are normalised both or not at all")
+    wq = wk = None
+    if q_norm_weight is not None:
+        wq, wk = q_norm_weight.to(q.dtype).contiguous(), k_norm_weight.to(q.dtype).contiguous()
     pos = positions.reshape(T).to(torch.int32).contiguous()
     slots = slot_mapping.reshape(T).to(torch.int64).contiguous()
     cos = rope.cos_freqs.to(q.device).contiguous()
     sin = rope.sin_freqs.to(q.device).contiguous()
     kp, vp = key_pages, value_pages
     P, Hkv_p, ps, D_p = kp.shape
-    if Hkv_p != Hkv or D_p != D or vp.shape != kp.shape:
+    int8, u4 = kp.dtype == torch.int8, kp.dtype == torch.uint8
+    if Hkv_p != Hkv or (D_p != D and not u4) or vp.shape != kp.shape:
         raise RuntimeError("qk_norm_rope_write: page pools must be [P, Hkv, page_size, D] matching k")
     if not (kp.is_contiguous() and vp.is_contiguous()):
         raise RuntimeError("qk_norm_rope_write: page pools must be contiguous (written in place)")
     if positions.numel() != T or slot_mapping.numel() != T:
         raise RuntimeError("qk_norm_rope_write: positions and slot_mapping need one entry per token")
-    int8 = kp.dtype == torch.int8
+    if u4:
+        nv.require_u4("qk_norm_rope_write", D, kp, vp, key_scales, value_scales)
+        if key_scales.dtype != q.dtype:
+            raise RuntimeError("qk_norm_rope_write: scales of 4-bit pages must be of q's dtype")
     if int8:
         if key_scales is None or value_scales is None:
             raise RuntimeError("qk_norm_rope_write: int8 pages need key_scales and value_scales")
@@ -81,11 +91,11 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
         out = torch.empty((B, Hq, L, D), dtype=q.dtype, device=q.device)
     elif tuple(out.shape) != (B, Hq, L, D) or out.dtype != q.dtype or not out.is_contiguous():
         raise RuntimeError("qk_norm_rope_write: out must be a contiguous [B, Hq, L, D] tensor of q's dtype")
-    ks = key_scales if int8 else None
-    vs = value_scales if int8 else None
+    ks = key_scales if int8 or u4 else None
+    vs = value_scales if int8 or u4 else None
     nv.check(nv.lib().nvm_qk_norm_rope_write(
-        qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, wq.data_ptr(),
-        wk.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0,
+        qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, nv.ptr(wq),
+        nv.ptr(wk), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0,
         pos.data_ptr(), out.data_ptr(), L, kp.data_ptr(), vp.data_ptr(), nv.dtype_code(kp.dtype),
         ks.data_ptr() if ks is not None else None, vs.data_ptr() if vs is not None else None,
         nv.dtype_code(ks.dtype) if ks is not None else nv.NVM_F16, slots.data_ptr(), T, Hq, Hkv, D, P, ps,
