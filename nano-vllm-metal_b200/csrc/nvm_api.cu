@@ -350,7 +350,7 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
   a.is_causal = 1;
   if (validate_paged(a, false) != NVM_OK) return 0;
-  if (kv_dtype == NVM_U4) return 0;
+  if (kv_dtype == NVM_U4) return plan_paged_u4(a).ws_bytes;
   if (env_flag("NVM_ATTN_FORCE_GENERIC")) return 0;
   // q's dtype is not known here: cover the tcgen05 plan (taken when q matches the pages)
   // and the mma.sync plan (taken otherwise).
@@ -380,7 +380,13 @@ int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const v
   if (st != NVM_OK) return st;
   if (B == 0) return NVM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv_dtype == NVM_U4) return launch_paged_u4(a, s);
+  if (kv_dtype == NVM_U4) {
+    const U4Plan plan = plan_paged_u4(a);
+    if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes))
+      return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", plan.ws_bytes,
+                  workspace_bytes);
+    return launch_paged_u4(a, plan, workspace, s);
+  }
   if (!env_flag("NVM_ATTN_FORCE_GENERIC")) {
     if (!env_flag("NVM_ATTN_NO_SM100") && flash2q_eligible(a)) return launch_flash2q(a, s);
     if (!env_flag("NVM_ATTN_NO_SM100")) {

@@ -183,7 +183,13 @@ int launch_u4_write(const void* k, const void* v, int in_dtype, int64_t stride_t
 int launch_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const void* k_scales, const void* v_scales,
                       int scale_dtype, const int64_t* slots, void* k, void* v, int out_dtype, int64_t T, int64_t Hkv, int64_t D,
                       int64_t P, int64_t page_size, cudaStream_t s);
-int launch_paged_u4(const PagedArgs& a, cudaStream_t s);
+struct U4Plan {
+  int tiles;                                    // of 8 query rows a block
+  int64_t row_blocks, units, chunk, n_chunks;   // a unit is a row block of one (request, kv head)
+  size_t ws_bytes;
+};
+U4Plan plan_paged_u4(const PagedArgs& a);
+int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s);
 
 int launch_paged_append(int32_t* block_table, int32_t* context_lens, const int32_t* new_tokens,
                         int32_t* free_stack, int32_t* free_top, int32_t* num_pages,
