@@ -184,8 +184,8 @@ int launch_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, co
                       int scale_dtype, const int64_t* slots, void* k, void* v, int out_dtype, int64_t T, int64_t Hkv, int64_t D,
                       int64_t P, int64_t page_size, cudaStream_t s);
 struct U4Plan {
-  int tiles;                                    // of 8 query rows a block
-  int64_t row_blocks, units, chunk, n_chunks;   // a unit is a row block of one (request, kv head)
+  int tiles;                   // of 8 query rows a unit
+  int64_t row_blocks, blocks;  // row blocks of one (request, kv head), thread blocks
   size_t ws_bytes;
 };
 U4Plan plan_paged_u4(const PagedArgs& a);

@@ -13,10 +13,12 @@
 // Queries are held in f16, each row scaled by a power of two (exact for 16-bit queries).
 //
 // Weights are 2^(t - M), t the base-2 score and M a running reference per row, held in f16 once they
-// are multiplied by s'.  M is kept within 2^10 of the largest t + log2 |v| so far, the largest
-// contribution rather than the largest weight: f16 then holds what matters to 11 bits however small
-// the values of the keys that are attended to.  Sums of weights and of p z' are fp32.
+// are multiplied by s'.  M follows the largest t + log2 s' so far, the largest contribution rather than
+// the largest weight: f16 then holds what matters to 11 bits however small the values of the keys
+// that are attended to.  M moves only where a contribution passes it by kSlack, which one vote over the
+// largest weight and the largest scale of a tile finds.  Sums of weights and of p z' are fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "nvm_internal.h"
 #include "u4.cuh"
@@ -27,8 +29,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
 constexpr int kStages = 3;   // of each warp's own ring
-constexpr float kSlack = 10.0f;    // log2 of how far a contribution may pass M
-constexpr float kLeast = -40.0f;   // log2 of the least size that a key's values count as
+constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
+constexpr int kFan = 16;     // partial results that are joined at a time
+constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
+constexpr float kLeast = 0x1p-44f;  // least scale that a key's values count as
 constexpr float kNoKeys = -1e30f;  // M of a row that has seen no key
 
 template <int D>
@@ -49,17 +53,17 @@ struct U4Params {
   const int32_t* block_table;
   const int32_t* context_lens;
   void* out;
-  float2* part_ml;  // [units][n_chunks][rows of a block]: (M, sum of weights)
-  float* part_o;    // [units][n_chunks][rows of a block][D]
-  int* tickets;     // [units], zero between calls
+  float2* part_ml;  // [2 * blocks][rows of a unit]: (M, sum of weights)
+  float* part_o;    // [2 * blocks][rows of a unit][D]
+  int* tickets;     // [3 * blocks], zero between calls: of groups by their leader's place, of units by their first block
   int q_dtype, out_dtype, causal;
-  int Hkv, L, rows, row_blocks, P, ps, mp, n_units, n_chunks, chunk;
+  int B, Hkv, L, rows, row_blocks, P, ps, mp;
   uint32_t ps_mul, ps_shift;  // key / ps = key * ps_mul >> ps_shift
   float scale_log2;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int kBytes>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool there) {
@@ -96,10 +100,24 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 // bits 4-7 of both halves as 64 + code
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
   uint32_t d;
   asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(d) : "r"(w));
+  return d;
+}
+
+// w << 4 on the multiply-add unit: logic operations, byte moves and shifts share the busiest one
+__device__ __forceinline__ uint32_t times16(uint32_t w) {
+  uint32_t d;
+  asm("mad.lo.u32 %0, %1, 16, 0;" : "=r"(d) : "r"(w));
   return d;
 }
 
@@ -132,55 +150,128 @@ struct Pairs {
       z[g] = p.y;
     }
   }
-  // log2 of the largest number that the key's values may have
-  __device__ __forceinline__ float size_log2() const {
-    float m = fmaxf(fabsf(z[0]), 16.0f * s[0]);
-    if constexpr (kGroups == 2) m = fmaxf(m, fmaxf(fabsf(z[1]), 16.0f * s[1]));
-    return fmaxf(lg2(m), kLeast);
-  }
+  __device__ __forceinline__ float size() const { return kGroups == 2 ? fmaxf(s[0], s[kGroups - 1]) : s[0]; }
 };
 
-// One block: kTiles x 8 query rows of one (request, kv head) against one chunk of keys, every warp
-// on tiles of 32 keys of its own, joined in shared memory; chunks are joined by the unit's last block.
+// Keys of a request that some query row may see, in steps of kStep; one at least, so that every row
+// is written.
+__device__ __forceinline__ int steps_of(const U4Params& p, int b) {
+  const int keys = min(__ldg(p.context_lens + b), p.mp * p.ps);
+  return max(1, (keys + kStep - 1) / kStep);
+}
+
+// Joins `count` partial results (M, sum, output in units of 2^M) of a unit, the k-th in place of(k), into
+// the output or, with `to` >= 0, into that place.  All threads of the block; `scratch` holds count x kRows.
+template <int D, int kRows, typename Of>
+__device__ __forceinline__ void join(const U4Params& p, float2* scratch, int count, Of&& of, int rows, size_t out_row0, int to) {
+  for (int i = threadIdx.x; i < count * kRows; i += kWarps * 32)
+    scratch[i] = __ldcg(p.part_ml + (size_t)of(i / kRows) * kRows + i % kRows);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kWarps * 32) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float top = kNoKeys, sum = 0.0f;
+    for (int k = 0; k < count; ++k) top = fmaxf(top, scratch[k * kRows + row].x);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < count; ++k) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((size_t)of(k) * kRows + row) * D + d));
+      const float2 ml = scratch[k * kRows + row];
+      const float f = ex2(ml.x - top);
+      sum = fmaf(f, ml.y, sum);
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
+    }
+    if (to >= 0) {
+      *reinterpret_cast<float4*>(p.part_o + ((size_t)to * kRows + row) * D + d) = o;
+      if (d == 0) p.part_ml[(size_t)to * kRows + row] = make_float2(top, sum);
+    } else {
+      const int64_t at = (int64_t)(out_row0 + row) * D + d;
+      const float inv = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+      store_dyn(p.out, at, p.out_dtype, o.x * inv);
+      store_dyn(p.out, at + 1, p.out_dtype, o.y * inv);
+      store_dyn(p.out, at + 2, p.out_dtype, o.z * inv);
+      store_dyn(p.out, at + 3, p.out_dtype, o.w * inv);
+    }
+  }
+}
+
+// A unit is kTiles x 8 query rows of one (request, kv head).  The units' keys, in steps of kStep, form
+// one line that is dealt to the blocks in equal parts, so that requests of any lengths load every SM
+// alike; a block takes the units on its part one after another.  Its warps walk tiles of 32 keys, each
+// through a ring of its own, and are joined in shared memory.  A unit that several blocks share is
+// joined by the last of them (in groups of kFan, then the groups).
 template <typename T, int D, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_kernel(const U4Params p) {
   using R = Ring<D>;
   constexpr int G = R::kGroups, kRows = 8 * kTiles;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 s_ml[kWarps][kRows];
-  __shared__ uint32_t s_there[kWarps][kStages];
   __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 
-  const int chunk = blockIdx.x / p.n_units, unit = blockIdx.x - chunk * p.n_units;
-  const int rb = unit % p.row_blocks, bh = unit / p.row_blocks, b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  // the line's length, this block's part of it and the request that the part begins in
+  const int heads = p.Hkv * p.row_blocks;  // units of a request
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int mine = b0 + lane < p.B ? steps_of(p, b0 + lane) : 0;
+    total += __reduce_add_sync(0xffffffffu, mine);
+  }
+  total *= heads;
+  const int64_t blocks = min((int64_t)gridDim.x, total);
+  if (blockIdx.x >= blocks) return;
+  // block i has steps [total * i / blocks, total * (i + 1) / blocks); step x is in block_of(x)
+  auto block_of = [&](int64_t x) -> int { return (int)(((x + 1) * blocks - 1) / total); };
+  int64_t pos = total * blockIdx.x / blocks;
+  const int64_t pos_end = total * (blockIdx.x + 1) / blocks;
+  int b = 0, steps = 1;
+  int64_t request_at = 0;  // where request b begins
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int mine = b0 + lane < p.B ? steps_of(p, b0 + lane) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, request_at + (int64_t)upto * heads > pos);
+    if (past != 0) {
+      const int l0 = __ffs(past) - 1;
+      b = b0 + l0;
+      steps = __shfl_sync(0xffffffffu, mine, l0);
+      request_at += (int64_t)(__shfl_sync(0xffffffffu, upto, l0) - steps) * heads;
+      break;
+    }
+    request_at += (int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads;
+  }
+
+  while (pos < pos_end) {
+  if (pos >= request_at + (int64_t)steps * heads) {
+    request_at += (int64_t)steps * heads;
+    ++b;
+    steps = steps_of(p, b);
+  }
+  const int in_request = (int)((pos - request_at) / steps);
+  const int64_t unit_at = request_at + (int64_t)in_request * steps;
+  const int kvh = in_request / p.row_blocks, rb = in_request - kvh * p.row_blocks, bh = b * p.Hkv + kvh;
+  const int step0 = (int)(pos - unit_at), step1 = (int)min((int64_t)steps, pos_end - unit_at);
+  pos = unit_at + step1;
   const int row0 = rb * kRows, rows = min(kRows, p.rows - row0);
-  const int ctx = p.context_lens[b];
-  const int cap = p.mp * p.ps, limit = min(ctx, cap);
-  // keys that the block's rows see: [0, most) by some row, [0, least) by every row
+  const int ctx = __ldg(p.context_lens + b), limit = min(ctx, p.mp * p.ps);
+  // keys that the unit's rows see: [0, most) by some row, [0, least) by every row
   int most = limit, least = limit;
   if (p.causal) {
-    int lo = p.L, hi = 0;
-    if (rows >= p.L) {
+    int lo = row0 % p.L, hi = (row0 + rows - 1) % p.L;
+    if (rows >= p.L || lo > hi) {
       lo = 0;
       hi = p.L - 1;
-    } else {
-      lo = row0 % p.L;
-      hi = (row0 + rows - 1) % p.L;
-      if (lo > hi) {
-        lo = 0;
-        hi = p.L - 1;
-      }
     }
     most = min(limit, hi + ctx - p.L + 1);
     least = min(limit, lo + ctx - p.L + 1);
   }
   most = max(most, 0);
-  // this unit's chunks: as many of p.chunk keys as it needs, evened out
-  const int chunks = max(1, (most + p.chunk - 1) / p.chunk);
-  if (chunk >= chunks) return;
-  const int share = ((most + chunks - 1) / chunks + kWarps * kTile - 1) / (kWarps * kTile) * (kWarps * kTile);
-  const int begin = min(chunk * share, most), end = min(begin + share, most);
+  const int begin = min(step0 * kStep, most), end = min(step1 * kStep, most);
 
   const size_t out_row0 = (size_t)bh * p.rows + row0;
   uint8_t* ring = smem + warp * R::kWarp;
@@ -192,45 +283,46 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     const int pid = __ldg(bt + (uint32_t)((uint64_t)(uint32_t)key * p.ps_mul >> p.ps_shift));
     return pid < p.P ? pid : -1;
   };
-  // copies the tile whose first key is k0 (a lane's key lies in page pid) into a stage
-  auto issue = [&](int k0, int pid, int stage) {
+  // Copies the tile whose first key is k0 (a lane's key lies in page pid) into a stage and says which of
+  // its keys are there.  The others read codes of the pool's first row, which are numbers in any case,
+  // with scales and offsets of zero.
+  constexpr int kParts = R::kRow / 16, kKeysAStep = 32 / kParts;
+  const uint8_t* k_lane = p.kp + lane % kParts * 16;
+  const uint8_t* v_lane = p.vp + lane % kParts * 16;
+  const uint32_t dst_lane = ring_at + lane / kParts * R::kRow +
+                            ((D == 128 ? lane % kParts ^ swizzle(lane / kParts) : lane % kParts) << 4);
+  auto issue = [&](int k0, int pid, int stage) -> uint32_t {
     const uint32_t page = (uint32_t)((uint64_t)(uint32_t)(k0 + lane) * p.ps_mul >> p.ps_shift);
     const uint32_t off = (uint32_t)(k0 + lane) - page * (uint32_t)p.ps;
-    const uint32_t row = pid < 0 ? 0xffffffffu : ((uint32_t)pid * p.Hkv + kvh) * p.ps + off;
-    const uint32_t there = __ballot_sync(0xffffffffu, pid >= 0);
-    if (lane == 0) s_there[warp][stage] = there;
-    const uint32_t at = ring_at + stage * R::kStage;
-    constexpr int kParts = R::kRow / 16, kKeysAStep = 32 / kParts;
+    const uint32_t row = pid < 0 ? 0u : ((uint32_t)pid * p.Hkv + kvh) * p.ps + off;
+    const uint32_t dst = dst_lane + stage * R::kStage;
 #pragma unroll
     for (int i = 0; i < kTile / kKeysAStep; ++i) {
-      const int key = i * kKeysAStep + lane / kParts, part = lane % kParts;
-      const uint32_t krow = __shfl_sync(0xffffffffu, row, key);
-      const bool ok = krow != 0xffffffffu;
-      const size_t src = ok ? (size_t)krow * R::kRow + part * 16 : 0;
-      const uint32_t dst = at + key * R::kRow + ((D == 128 ? part ^ swizzle(key) : part) << 4);
-      cp_async16(dst, p.kp + src, ok);
-      cp_async16(dst + R::kV, p.vp + src, ok);
+      const uint32_t krow = __shfl_sync(0xffffffffu, row, i * kKeysAStep + lane / kParts);
+      cp_async16(dst + i * kKeysAStep * R::kRow, k_lane + (uint64_t)krow * R::kRow);
+      cp_async16(dst + R::kV + i * kKeysAStep * R::kRow, v_lane + (uint64_t)krow * R::kRow);
     }
-    const size_t src = pid >= 0 ? (size_t)row * (4 * G) : 0;
-    cp_async_small<4 * G>(at + R::kKs + lane * 4 * G, p.ks + src, pid >= 0);
-    cp_async_small<4 * G>(at + R::kVs + lane * 4 * G, p.vs + src, pid >= 0);
+    const uint32_t at = ring_at + stage * R::kStage + lane * 4 * G;
+    cp_async_small<4 * G>(at + R::kKs, p.ks + (uint64_t)row * (4 * G), pid >= 0);
+    cp_async_small<4 * G>(at + R::kVs, p.vs + (uint64_t)row * (4 * G), pid >= 0);
+    return __ballot_sync(0xffffffffu, pid >= 0);
   };
 
-  const int step = kWarps * kTile;
   int k_next = begin + warp * kTile;  // first key of the tile to copy next
   int pid = page_of_key(k_next + lane);
+  uint32_t there_next[kStages - 1];  // of the tiles on their way
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (k_next < end) issue(k_next, pid, s);
+    there_next[s] = k_next < end ? issue(k_next, pid, s) : 0;
     cp_async_commit();
-    k_next += step;
+    k_next += kStep;
     pid = page_of_key(k_next + lane);
   }
 
   // Queries as B fragments (lane: row r of each tile of 8, 16 elements a group), scaled per row so that
   // the largest is in [2^8, 2^9); kap undoes it and turns scores to base 2.
   uint32_t qf[kTiles][G][4][2];
-  float kap[kTiles][2], qsum[kTiles][2][G];
+  float kap[kTiles][2], qsum[kTiles][2][G], start[kTiles][G][4];  // start: -64 times the row's sum
   int seen[kTiles][2];  // keys [0, seen) are seen by the lane's rows 2c, 2c + 1
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
@@ -282,7 +374,10 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     for (int i = 0; i < 2; ++i) {
       kap[j][i] = __shfl_sync(0xffffffffu, down, (2 * c + i) * 4);
 #pragma unroll
-      for (int g = 0; g < G; ++g) qsum[j][i][g] = __shfl_sync(0xffffffffu, sum[g], (2 * c + i) * 4);
+      for (int g = 0; g < G; ++g) {
+        qsum[j][i][g] = __shfl_sync(0xffffffffu, sum[g], (2 * c + i) * 4);
+        start[j][g][i] = start[j][g][2 + i] = -64.0f * qsum[j][i][g];
+      }
       const int rr = row0 + 8 * j + 2 * c + i;
       seen[j][i] = rr - row0 >= rows ? INT32_MAX : p.causal ? min(limit, rr % p.L + ctx - p.L + 1) : limit;
     }
@@ -322,15 +417,17 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
   }
 
   int stage = 0, stage_in = kStages - 1;
-  for (int k0 = begin + warp * kTile; k0 < end; k0 += step) {
+  for (int k0 = begin + warp * kTile; k0 < end; k0 += kStep) {
     cp_async_wait<kStages - 2>();
     __syncwarp();
-    if (k_next < end) issue(k_next, pid, stage_in);
+    const uint32_t there = there_next[0];
+#pragma unroll
+    for (int s = 0; s + 2 < kStages; ++s) there_next[s] = there_next[s + 1];
+    if (k_next < end) there_next[kStages - 2] = issue(k_next, pid, stage_in);
     cp_async_commit();
-    k_next += step;
+    k_next += kStep;
     pid = page_of_key(k_next + lane);
     const uint32_t at = ring_at + stage * R::kStage;
-    const uint32_t there = s_there[warp][stage];
     stage_in = stage;
     stage = stage + 1 == kStages ? 0 : stage + 1;
 
@@ -344,26 +441,24 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint2 lo = lds64(at + k_off[g] + 16 * mt * R::kRow), hi = lds64(at + k_off[g] + (16 * mt + 8) * R::kRow);
-        float dot[kTiles][4];
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) dot[j][0] = dot[j][1] = dot[j][2] = dot[j][3] = 0.0f;
+        float dot[kTiles][4];  // of the codes
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t u = w == 0 ? lo.x : lo.y, v = w == 0 ? hi.x : hi.y;
-          const uint32_t a0[4] = {codes_f16(u << 4), codes_f16(v << 4), codes_f16(u), codes_f16(v)};
-          const uint32_t a1[4] = {codes_f16(u >> 4), codes_f16(v >> 4), codes_f16(u >> 8), codes_f16(v >> 8)};
+          const uint32_t u8 = u >> 8, v8 = v >> 8;
+          const uint32_t a0[4] = {codes_f16(times16(u)), codes_f16(times16(v)), codes_f16(u), codes_f16(v)};
+          const uint32_t a1[4] = {codes_f16(times16(u8)), codes_f16(times16(v8)), codes_f16(u8), codes_f16(v8)};
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
-            mma16816<__half>(dot[j], a0, qf[j][g][2 * w][0], qf[j][g][2 * w][1]);
+            mma_from(dot[j], a0, qf[j][g][2 * w][0], qf[j][g][2 * w][1], w == 0 ? start[j][g] : dot[j]);
             mma16816<__half>(dot[j], a1, qf[j][g][2 * w + 1][0], qf[j][g][2 * w + 1][1]);
           }
         }
-        const float za = fmaf(-64.0f, a.s[g], a.z[g]), zd = fmaf(-64.0f, d.s[g], d.z[g]);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float s = e < 2 ? a.s[g] : d.s[g], z = e < 2 ? za : zd;
+            const float s = e < 2 ? a.s[g] : d.s[g], z = e < 2 ? a.z[g] : d.z[g];
             const float off = g == 0 ? z * qsum[j][e & 1][g] : fmaf(z, qsum[j][e & 1][g], x[mt][j][e]);
             x[mt][j][e] = fmaf(s, dot[j][e], off);
           }
@@ -371,13 +466,13 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     }
 
     Pairs<T, G> vz[2][2];
-    float size[2][2];
+    float size = kLeast;  // the largest scale
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         vz[mt][h].load(at + R::kVs + (kr + 16 * mt + 8 * h) * 4 * G);
-        size[mt][h] = vz[mt][h].size_log2();
+        size = fmaxf(size, vz[mt][h].size());
       }
 
     const bool masked = there != 0xffffffffu || k0 + kTile > least;
@@ -394,19 +489,18 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
           }
     }
 
-    // references that some contribution passes by 2^kSlack move to the largest one
-    float u[2][kTiles][4];
-    bool over = false;
+    // weights 2^(t - M); references that some contribution passes by kSlack move to the largest one
+    float w[2][kTiles][4], heavy = 0.0f;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          u[mt][j][e] = fmaf(kap[j][e & 1], x[mt][j][e], -M[j][e & 1]);
-          over |= u[mt][j][e] + size[mt][e >> 1] > kSlack;
+          w[mt][j][e] = ex2(fmaf(kap[j][e & 1], x[mt][j][e], -M[j][e & 1]));
+          heavy = fmaxf(heavy, w[mt][j][e]);
         }
-    if (__any_sync(0xffffffffu, over)) {
+    if (__any_sync(0xffffffffu, heavy * size > kSlack)) {
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
@@ -415,7 +509,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) top = fmaxf(top, fmaf(kap[j][i], x[mt][j][2 * h + i], size[mt][h]));
+            for (int h = 0; h < 2; ++h)
+              top = fmaxf(top, fmaf(kap[j][i], x[mt][j][2 * h + i], lg2(fmaxf(vz[mt][h].size(), kLeast))));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -436,34 +531,44 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) u[mt][j][2 * h + i] = fmaf(kap[j][i], x[mt][j][2 * h + i], -top);
+            for (int h = 0; h < 2; ++h) w[mt][j][2 * h + i] = ex2(fmaf(kap[j][i], x[mt][j][2 * h + i], -top));
         }
     }
 
-    // weights, their sums, and the weights times the values' scales as B fragments
+    // their sums, and the weights times the values' scales as B fragments; in a masked tile a key that the
+    // row does not see counts nothing whatever its values
     uint32_t pf[2][kTiles][G][2];
+    auto weigh = [&](auto hidden) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
+        for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Pairs<T, G>& v = vz[mt][h];
-          const float w0 = ex2(u[mt][j][2 * h]), w1 = ex2(u[mt][j][2 * h + 1]);
-          l[j][0] += w0;
-          l[j][1] += w1;
+          for (int h = 0; h < 2; ++h) {
+            const Pairs<T, G>& v = vz[mt][h];
+            const float w0 = w[mt][j][2 * h], w1 = w[mt][j][2 * h + 1];
+            l[j][0] += w0;
+            l[j][1] += w1;
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            float s0 = w0 * v.s[g], s1 = w1 * v.s[g], z0 = w0 * v.z[g], z1 = w1 * v.z[g];
-            if (masked) {  // a key that the row does not see counts nothing, whatever its values
-              if (w0 == 0.0f) s0 = z0 = 0.0f;
-              if (w1 == 0.0f) s1 = z1 = 0.0f;
+            for (int g = 0; g < G; ++g) {
+              float s0 = w0 * v.s[g], s1 = w1 * v.s[g];
+              if constexpr (decltype(hidden)::value) {
+                if (w0 == 0.0f) s0 = 0.0f;
+                if (w1 == 0.0f) s1 = 0.0f;
+                zsum[j][0][g] += w0 == 0.0f ? 0.0f : w0 * v.z[g];
+                zsum[j][1][g] += w1 == 0.0f ? 0.0f : w1 * v.z[g];
+              } else {
+                zsum[j][0][g] = fmaf(w0, v.z[g], zsum[j][0][g]);
+                zsum[j][1][g] = fmaf(w1, v.z[g], zsum[j][1][g]);
+              }
+              pf[mt][j][g][h] = transpose8x8(pack2<__half>(s0, s1));
             }
-            zsum[j][0][g] += z0;
-            zsum[j][1][g] += z1;
-            pf[mt][j][g][h] = transpose8x8(pack2<__half>(s0, s1));
           }
-        }
+    };
+    if (masked)
+      weigh(std::true_type{});
+    else
+      weigh(std::false_type{});
 
     const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
@@ -474,10 +579,12 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
         const uint32_t k80 = lds32(at + v_off0[g] + (16 * mt + 8) * R::kRow), k81 = lds32(at + v_off1[g] + (16 * mt + 8) * R::kRow);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7632u : 0x5410u;
+          // bytes 2 half and 2 half + 1 of the keys of a fragment column pair, in the low bytes of the halves
+          const uint32_t sel = half ? 0x7632u : 0x5410u, sel1 = half ? 0x7733u : 0x5511u;
           const uint32_t y = prmt(k00, k01, sel), y8 = prmt(k80, k81, sel);
-          const uint32_t a0[4] = {codes_f16(y << 4), codes_f16(y), codes_f16(y8 << 4), codes_f16(y8)};
-          const uint32_t a1[4] = {codes_f16(y >> 4), codes_f16(y >> 8), codes_f16(y8 >> 4), codes_f16(y8 >> 8)};
+          const uint32_t w = prmt(k00, k01, sel1), w8 = prmt(k80, k81, sel1);
+          const uint32_t a0[4] = {codes_f16(times16(y)), codes_f16(y), codes_f16(times16(y8)), codes_f16(y8)};
+          const uint32_t a1[4] = {codes_f16(times16(w)), codes_f16(w), codes_f16(times16(w8)), codes_f16(w8)};
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
             mma16816<__half>(acc[g][2 * half][j], a0, pf[mt][j][g][0], pf[mt][j][g][1]);
@@ -524,7 +631,10 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     }
   __syncthreads();
 
-  const size_t slot = ((size_t)unit * p.n_chunks + chunk) * kRows;
+  // Blocks first .. last share the unit.  A block's partial results: 2 i + 1 of a unit that it begins,
+  // 2 i of one that it continues.
+  const bool whole = step0 == 0 && step1 == steps;
+  const int place = 2 * blockIdx.x + (step0 == 0);
   for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
     const int row = i / D, d = i - row * D;
     float top = s_ml[0][row].x, sum = 0.0f, o = 0.0f;
@@ -537,33 +647,41 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
       sum = fmaf(f, ml.y, sum);
       o = fmaf(f, reinterpret_cast<const float*>(smem)[(w * kRows + row) * kPitch + d], o);
     }
-    if (chunks == 1) {
-      store_dyn(p.out, (int64_t)(out_row0 + row) * D + d, p.out_dtype, sum == 0.0f ? 0.0f : o / sum);
+    if (whole) {
+      store_dyn(p.out, (int64_t)(out_row0 + row) * D + d, p.out_dtype, sum == 0.0f ? 0.0f : o * __frcp_rn(sum));
     } else {
-      p.part_o[(slot + row) * D + d] = o;
-      if (d == 0) p.part_ml[slot + row] = make_float2(top, sum);
+      p.part_o[((size_t)place * kRows + row) * D + d] = o;
+      if (d == 0) p.part_ml[(size_t)place * kRows + row] = make_float2(top, sum);
     }
   }
-  if (chunks == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(p.tickets + unit, 1) == chunks - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  if (threadIdx.x == 0) p.tickets[unit] = 0;
-  const size_t base = (size_t)unit * p.n_chunks * kRows;
-  for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
-    const int row = i / D, d = i - row * D;
-    float top = kNoKeys, sum = 0.0f, o = 0.0f;
-    for (int k = 0; k < chunks; ++k) top = fmaxf(top, __ldcg(&p.part_ml[base + (size_t)k * kRows + row].x));
-    for (int k = 0; k < chunks; ++k) {
-      const float2 ml = __ldcg(&p.part_ml[base + (size_t)k * kRows + row]);
-      const float f = ex2(ml.x - top);
-      sum = fmaf(f, ml.y, sum);
-      o = fmaf(f, __ldcg(&p.part_o[(base + (size_t)k * kRows + row) * D + d]), o);
+  if (!whole) {
+    const int first = block_of(unit_at), last = block_of(unit_at + steps - 1);
+    const int share = last - first + 1, mine = (int)blockIdx.x - first, group = mine / kFan;
+    const int groups = (share + kFan - 1) / kFan, count = min(kFan, share - group * kFan);
+    const int leader = first + group * kFan;
+    auto place_of = [&](int block) { return 2 * block + (block == first); };
+    float2* scratch = reinterpret_cast<float2*>(smem);
+    // the last of `n` blocks to come, which finds what the others left
+    auto last_of = [&](int* ticket, int n) -> bool {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        s_last = atomicAdd(ticket, 1) == n - 1;
+        if (s_last) *ticket = 0;
+      }
+      __syncthreads();
+      const bool yes = s_last != 0;
+      if (yes) __threadfence();
+      return yes;
+    };
+    if (last_of(p.tickets + place_of(leader), count)) {
+      join<D, kRows>(p, scratch, count, [&](int k) { return place_of(leader + k); }, rows, out_row0,
+                     groups > 1 ? place_of(leader) : -1);
+      if (groups > 1 && last_of(p.tickets + 2 * gridDim.x + first, groups))
+        join<D, kRows>(p, scratch, groups, [&](int k) { return place_of(first + k * kFan); }, rows, out_row0, -1);
     }
-    store_dyn(p.out, (int64_t)(out_row0 + row) * D + d, p.out_dtype, sum == 0.0f ? 0.0f : o / sum);
+  }
+  __syncthreads();  // the rings are free for the next unit
   }
 }
 
@@ -586,24 +704,22 @@ int launch_d(const U4Params& p, int64_t D, int tiles, int64_t blocks, cudaStream
 
 U4Plan plan_paged_u4(const PagedArgs& a) {
   U4Plan plan{};
-  const int64_t rows = a.Hq / a.Hkv * a.L, keys = a.max_pages * a.page_size;
+  const int64_t rows = a.Hq / a.Hkv * a.L;
   plan.tiles = rows <= 8 ? 1 : 2;
   plan.row_blocks = (rows + 8 * plan.tiles - 1) / (8 * plan.tiles);
-  plan.units = a.B * a.Hkv * plan.row_blocks;
-  const int64_t slots = 148 * 4, least = kWarps * kTile;
-  int64_t chunk = (keys * plan.units + 3 * slots - 1) / (3 * slots);
-  chunk = std::max<int64_t>((chunk + least - 1) / least * least, least);
-  if (plan.units > (int64_t)(kTicketRegionBytes / sizeof(int))) chunk = std::max<int64_t>(keys, 1);
-  plan.chunk = chunk;
-  plan.n_chunks = std::max<int64_t>((keys + chunk - 1) / chunk, 1);
-  if (plan.n_chunks > 1)
-    plan.ws_bytes = kTicketRegionBytes + (size_t)(plan.units * plan.n_chunks * 8 * plan.tiles) * (a.D + 2) * sizeof(float);
+  const int64_t steps = std::max<int64_t>((a.max_pages * a.page_size + kStep - 1) / kStep, 1);
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t most = (int64_t)sms * (plan.tiles == 1 ? 4 : 3), units = a.B * a.Hkv * plan.row_blocks;
+  plan.blocks = units > most / steps ? most : units * steps;
+  plan.ws_bytes = kTicketRegionBytes + (size_t)(plan.blocks * 2 * 8 * plan.tiles) * (a.D + 2) * sizeof(float);
   return plan;
 }
 
 int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s) {
-  const int64_t blocks = plan.units * plan.n_chunks;
-  if (blocks > INT32_MAX || a.max_pages * a.page_size > INT32_MAX - 4096 || a.Hq / a.Hkv * a.L > INT32_MAX / 2)
+  const int64_t blocks = plan.blocks;
+  if (a.max_pages * a.page_size > INT32_MAX - 4096 || a.Hq / a.Hkv * a.L > INT32_MAX / 2 || a.B > INT32_MAX / 2 ||
+      a.Hkv * plan.row_blocks > INT32_MAX)
     return fail(NVM_ERR_UNSUPPORTED, "paged_attention: 4-bit pages: too many rows or keys");
   U4Params p{};
   p.q = a.q;
@@ -617,16 +733,14 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
   p.q_dtype = a.q_dtype;
   p.out_dtype = a.out_dtype;
   p.causal = a.is_causal;
+  p.B = (int)a.B;
   p.Hkv = (int)a.Hkv;
   p.L = (int)a.L;
   p.rows = (int)(a.Hq / a.Hkv * a.L);
   p.row_blocks = (int)plan.row_blocks;
   p.P = (int)a.P;
   p.ps = (int)a.page_size;
-  p.mp = (int)a.max_pages;
-  p.n_units = (int)plan.units;
-  p.n_chunks = (int)plan.n_chunks;
-  p.chunk = (int)std::min<int64_t>(plan.chunk, INT32_MAX / 2);
+  p.mp = a.P > 0 ? (int)a.max_pages : 0;  // a pool without pages: no key, and nothing to read
   p.scale_log2 = a.scale * 1.4426950408889634f;
   // key / ps for keys below 2^31: with 2^(n - 1) < ps <= 2^n and m = floor(2^(31 + n) / ps) + 1 the error
   // m ps - 2^(31 + n) is at most 2^n, so key * m >> 31 + n is exact
@@ -634,11 +748,9 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
   while ((int64_t(1) << n) < a.page_size) ++n;
   p.ps_mul = (uint32_t)((uint64_t(1) << (31 + n)) / (uint64_t)a.page_size + 1);
   p.ps_shift = (uint32_t)(31 + n);
-  if (plan.ws_bytes > 0) {
-    p.tickets = static_cast<int*>(ws);
-    p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kTicketRegionBytes);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.units * plan.n_chunks * 8 * plan.tiles * a.D);
-  }
+  p.tickets = static_cast<int*>(ws);
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kTicketRegionBytes);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + blocks * 2 * 8 * plan.tiles * a.D);
   return a.scale_dtype == NVM_BF16 ? launch_d<__nv_bfloat16>(p, a.D, plan.tiles, blocks, s)
                                    : launch_d<__half>(p, a.D, plan.tiles, blocks, s);
 }
