@@ -7,9 +7,10 @@
 // Mathematics.  With K = s c + z and V = s' c' + z' (one pair a group of 64 elements) a score is
 //   q.k = sum over groups of s (q . c) + z (sum of q),
 // and an output element of group g is (sum p s'_g c' + sum p z'_g) / sum p: codes enter the matrix
-// instructions as they are, scales and offsets act on scores and weights.  A code becomes the f16 number
-// 64 + code by one shift and one logic operation for two (bits 4-7 of 64.0h); the 64 is taken out again
-// with sum q, and with the sum of the weights as the matrix unit saw them (a product with ones).
+// instructions as they are, scales and offsets act on scores and weights.  A code needs no conversion:
+// bits 0-3 of a 16-bit word are the f16 subnormal code * 2^-24 and bits 4-7 code * 2^-20, so one logic
+// operation makes two operands (and one shift serves the upper bytes), exactly and without a bias that
+// sums would have to lose again; the powers of two go into the queries and into the output.
 // Queries are held in f16, each row scaled by a power of two (exact for 16-bit queries).
 //
 // Weights are 2^(t - M), t the base-2 score and M a running reference per row, held in f16 once they
@@ -100,35 +101,23 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %11, %12, %13};"
+      "{%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// bits 4-7 of both halves as 64 + code
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(d) : "r"(w));
-  return d;
-}
+// the codes in bits 0-3 and 4-7 of both halves, as f16 subnormals
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00f000f0u; }
+constexpr float kLowUnit = 0x1p24f, kHighUnit = 0x1p20f;  // what undoes their size
 
-// w << 4 on the multiply-add unit: logic operations, byte moves and shifts share the busiest one
-__device__ __forceinline__ uint32_t times16(uint32_t w) {
-  uint32_t d;
-  asm("mad.lo.u32 %0, %1, 16, 0;" : "=r"(d) : "r"(w));
-  return d;
+// The 16-byte parts of rows are swapped so that the eight rows of a matrix load touch every bank once.
+template <int D>
+__device__ __forceinline__ int swizzle(int key) {
+  return D == 128 ? key >> 1 & 3 : key >> 2 & 1;
 }
-
-// A tile's key in row m of a matrix fragment (and + 8 in row m + 8).  With the 16-byte parts of a
-// row's 64 swapped by swizzle(), both the 8-byte reads of K (rows 2i, 2i + 1 and four lanes a row)
-// and the 4-byte reads of V (rows 2c over the lanes c) touch every bank once.
-__device__ __forceinline__ int key_of(int m) {
-  const int base = (m >> 1 & 1) << 1 | m >> 2;
-  return m & 1 ? (base ^ 1) + 4 : base;
-}
-__device__ __forceinline__ int swizzle(int key) { return (key >> 1 & 1) << 1; }
 
 // (scale, offset) of a key's groups.
 template <typename T, int kGroups>
@@ -290,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
   const uint8_t* k_lane = p.kp + lane % kParts * 16;
   const uint8_t* v_lane = p.vp + lane % kParts * 16;
   const uint32_t dst_lane = ring_at + lane / kParts * R::kRow +
-                            ((D == 128 ? lane % kParts ^ swizzle(lane / kParts) : lane % kParts) << 4);
+                            ((lane % kParts ^ swizzle<D>(lane / kParts)) << 4);
   auto issue = [&](int k0, int pid, int stage) -> uint32_t {
     const uint32_t page = (uint32_t)((uint64_t)(uint32_t)(k0 + lane) * p.ps_mul >> p.ps_shift);
     const uint32_t off = (uint32_t)(k0 + lane) - page * (uint32_t)p.ps;
@@ -319,10 +308,11 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     pid = page_of_key(k_next + lane);
   }
 
-  // Queries as B fragments (lane: row r of each tile of 8, 16 elements a group), scaled per row so that
-  // the largest is in [2^8, 2^9); kap undoes it and turns scores to base 2.
+  // Queries as B fragments (lane: row r of each tile of 8; of a group, elements 8c to 8c + 7 of each half),
+  // scaled per row so that the largest is in [2^10, 2^11), and 16 times that where they meet low codes;
+  // kap undoes it and turns scores to base 2.
   uint32_t qf[kTiles][G][4][2];
-  float kap[kTiles][2], qsum[kTiles][2][G], start[kTiles][G][4];  // start: -64 times the row's sum
+  float kap[kTiles][2], qsum[kTiles][2][G];  // qsum in units of the scores before kap
   int seen[kTiles][2];  // keys [0, seen) are seen by the lane's rows 2c, 2c + 1
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
@@ -334,7 +324,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
       for (int e = 0; e < 16; e += 2) {
         float2 v = make_float2(0.0f, 0.0f);
         if (row < rows) {
-          const int64_t at = (int64_t)(out_row0 + row) * D + g * kU4Group + c * 16 + e;
+          const int64_t at = (int64_t)(out_row0 + row) * D + g * kU4Group + (e >> 3) * 32 + c * 8 + (e & 7);
           v = p.q_dtype == NVM_BF16  ? load_pair<__nv_bfloat16>(p.q, at)
               : p.q_dtype == NVM_F16 ? load_pair<__half>(p.q, at)
                                      : load_pair<float>(p.q, at);
@@ -346,8 +336,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e2 = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
-    float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
-    float down = p.scale_log2 * __uint_as_float((uint32_t)(127 - 8 + e2) << 23);
+    float up = __uint_as_float((uint32_t)(127 + 10 - e2) << 23);
+    float down = p.scale_log2 * __uint_as_float((uint32_t)(127 - 10 + e2) << 23) * kHighUnit;
     if (down == 0.0f) {  // every score is 0; masks need a factor that is not
       up = 0.0f;
       down = 1.0f;
@@ -362,10 +352,11 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {  // elements (2h + i, 2h + i + 4) of word w
-            const __half2 v = __floats2half2_rn(x[g][8 * w + 2 * h + i] * up, x[g][8 * w + 2 * h + i + 4] * up);
+            const float unit = i == 0 ? up * (kLowUnit / kHighUnit) : up;
+            const __half2 v = __floats2half2_rn(x[g][8 * w + 2 * h + i] * unit, x[g][8 * w + 2 * h + i + 4] * unit);
             qf[j][g][2 * w + h][i] = *reinterpret_cast<const uint32_t*>(&v);
             const float2 f = __half22float2(v);
-            sum[g] += f.x + f.y;
+            sum[g] += (f.x + f.y) * (i == 0 ? 1.0f / kLowUnit : 1.0f / kHighUnit);
           }
       sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
       sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
@@ -374,45 +365,36 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     for (int i = 0; i < 2; ++i) {
       kap[j][i] = __shfl_sync(0xffffffffu, down, (2 * c + i) * 4);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        qsum[j][i][g] = __shfl_sync(0xffffffffu, sum[g], (2 * c + i) * 4);
-        start[j][g][i] = start[j][g][2 + i] = -64.0f * qsum[j][i][g];
-      }
+      for (int g = 0; g < G; ++g) qsum[j][i][g] = __shfl_sync(0xffffffffu, sum[g], (2 * c + i) * 4);
       const int rr = row0 + 8 * j + 2 * c + i;
       seen[j][i] = rr - row0 >= rows ? INT32_MAX : p.causal ? min(limit, rr % p.L + ctx - p.L + 1) : limit;
     }
   }
 
-  float acc[G][4][kTiles][4], wsum[G][kTiles][4], M[kTiles][2], l[kTiles][2], zsum[kTiles][2][G];
+  float acc[G][4][kTiles][4], M[kTiles][2], l[kTiles][2], zsum[kTiles][2][G];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        wsum[g][j][e] = 0.0f;
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[g][i][j][e] = 0.0f;
-      }
       zsum[j][0][g] = zsum[j][1][g] = 0.0f;
     }
     M[j][0] = M[j][1] = kNoKeys;
     l[j][0] = l[j][1] = 0.0f;
   }
 
-  const int kr = key_of(r), kc0 = key_of(2 * c), kc1 = key_of(2 * c + 1);
-  // byte offsets inside a stage: K rows of fragment row r, V rows of fragment columns 2c and 2c + 1
-  uint32_t k_off[G], v_off0[G], v_off1[G];
+  // what a lane addresses in a matrix load of 16 keys: K rows 0-7 in matrices 0 and 1 (the group's halves),
+  // 8-15 in 2 and 3; V (transposed) rows 0-7 in matrices 0 and 2, 8-15 in 1 and 3
+  uint32_t k_off[G], v_off[G];
+  {
+    const int m = lane >> 3, k_key = (lane & 7) + 8 * (m >> 1), v_key = (lane & 7) + 8 * (m & 1);
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    if constexpr (D == 128) {
-      k_off[g] = kr * R::kRow + (((2 * g + (c >> 1)) ^ swizzle(kr)) << 4) + (c & 1) * 8;
-      v_off0[g] = R::kV + kc0 * R::kRow + (((2 * g + (r >> 2)) ^ swizzle(kc0)) << 4) + (r & 3) * 4;
-      v_off1[g] = R::kV + kc1 * R::kRow + (((2 * g + (r >> 2)) ^ swizzle(kc1)) << 4) + (r & 3) * 4;
-    } else {
-      k_off[g] = kr * R::kRow + c * 8;
-      v_off0[g] = R::kV + kc0 * R::kRow + r * 4;
-      v_off1[g] = R::kV + kc1 * R::kRow + r * 4;
+    for (int g = 0; g < G; ++g) {
+      k_off[g] = k_key * R::kRow + (((2 * g + (m & 1)) ^ swizzle<D>(k_key)) << 4);
+      v_off[g] = R::kV + v_key * R::kRow + (((2 * g + (m >> 1)) ^ swizzle<D>(v_key)) << 4);
     }
   }
 
@@ -431,26 +413,29 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     stage_in = stage;
     stage = stage + 1 == kStages ? 0 : stage + 1;
 
-    // x[mt][j][e]: score / kap of key key_of(r) + 16 mt + 8 (e / 2), row 2c + e % 2 of tile j
+    // x[mt][j][e]: score / kap of key r + 16 mt + 8 (e / 2), row 2c + e % 2 of tile j
     float x[2][kTiles][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       Pairs<T, G> a, d;
-      a.load(at + R::kKs + (kr + 16 * mt) * 4 * G);
-      d.load(at + R::kKs + (kr + 16 * mt + 8) * 4 * G);
+      a.load(at + R::kKs + (r + 16 * mt) * 4 * G);
+      d.load(at + R::kKs + (r + 16 * mt + 8) * 4 * G);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint2 lo = lds64(at + k_off[g] + 16 * mt * R::kRow), hi = lds64(at + k_off[g] + (16 * mt + 8) * R::kRow);
-        float dot[kTiles][4];  // of the codes
+        uint32_t k[4];  // words of rows r and r + 8 in the group's halves
+        ldsm_x4(at + k_off[g] + 16 * mt * R::kRow, k[0], k[1], k[2], k[3]);
+        float dot[kTiles][4];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const uint32_t u = w == 0 ? lo.x : lo.y, v = w == 0 ? hi.x : hi.y;
-          const uint32_t u8 = u >> 8, v8 = v >> 8;
-          const uint32_t a0[4] = {codes_f16(times16(u)), codes_f16(times16(v)), codes_f16(u), codes_f16(v)};
-          const uint32_t a1[4] = {codes_f16(times16(u8)), codes_f16(times16(v8)), codes_f16(u8), codes_f16(v8)};
+          const uint32_t u = k[w], v = k[2 + w], u8 = u >> 8, v8 = v >> 8;
+          const uint32_t a0[4] = {low_codes(u), low_codes(v), high_codes(u), high_codes(v)};
+          const uint32_t a1[4] = {low_codes(u8), low_codes(v8), high_codes(u8), high_codes(v8)};
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
-            mma_from(dot[j], a0, qf[j][g][2 * w][0], qf[j][g][2 * w][1], w == 0 ? start[j][g] : dot[j]);
+            if (w == 0)
+              mma_first(dot[j], a0, qf[j][g][0][0], qf[j][g][0][1]);
+            else
+              mma16816<__half>(dot[j], a0, qf[j][g][2][0], qf[j][g][2][1]);
             mma16816<__half>(dot[j], a1, qf[j][g][2 * w + 1][0], qf[j][g][2 * w + 1][1]);
           }
         }
@@ -471,7 +456,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        vz[mt][h].load(at + R::kVs + (kr + 16 * mt + 8 * h) * 4 * G);
+        vz[mt][h].load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
         size = fmaxf(size, vz[mt][h].size());
       }
 
@@ -483,7 +468,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = kr + 16 * mt + 8 * (e >> 1);
+            const int key = r + 16 * mt + 8 * (e >> 1);
             const bool ok = (there >> key & 1) && k0 + key < seen[j][e & 1];
             if (!ok) x[mt][j][e] = kap[j][e & 1] < 0.0f ? INFINITY : -INFINITY;  // kap * x = -inf
           }
@@ -520,8 +505,6 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
 #pragma unroll
           for (int g = 0; g < G; ++g) {
             zsum[j][i][g] *= fade;
-            wsum[g][j][i] *= fade;
-            wsum[g][j][2 + i] *= fade;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               acc[g][t][j][i] *= fade;
@@ -570,29 +553,23 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
     else
       weigh(std::false_type{});
 
-    const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint32_t k00 = lds32(at + v_off0[g] + 16 * mt * R::kRow), k01 = lds32(at + v_off1[g] + 16 * mt * R::kRow);
-        const uint32_t k80 = lds32(at + v_off0[g] + (16 * mt + 8) * R::kRow), k81 = lds32(at + v_off1[g] + (16 * mt + 8) * R::kRow);
+        uint32_t v[4];  // keys (2c, 2c + 1) and (2c, 2c + 1) + 8: elements 4r to 4r + 3 of the group's halves
+        ldsm_x4_t(at + v_off[g] + 16 * mt * R::kRow, v[0], v[1], v[2], v[3]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          // bytes 2 half and 2 half + 1 of the keys of a fragment column pair, in the low bytes of the halves
-          const uint32_t sel = half ? 0x7632u : 0x5410u, sel1 = half ? 0x7733u : 0x5511u;
-          const uint32_t y = prmt(k00, k01, sel), y8 = prmt(k80, k81, sel);
-          const uint32_t w = prmt(k00, k01, sel1), w8 = prmt(k80, k81, sel1);
-          const uint32_t a0[4] = {codes_f16(times16(y)), codes_f16(y), codes_f16(times16(y8)), codes_f16(y8)};
-          const uint32_t a1[4] = {codes_f16(times16(w)), codes_f16(w), codes_f16(times16(w8)), codes_f16(w8)};
+          const uint32_t y = v[2 * half], z = v[2 * half + 1], y8 = y >> 8, z8 = z >> 8;
+          const uint32_t a0[4] = {low_codes(y), high_codes(y), low_codes(z), high_codes(z)};
+          const uint32_t a1[4] = {low_codes(y8), high_codes(y8), low_codes(z8), high_codes(z8)};
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
             mma16816<__half>(acc[g][2 * half][j], a0, pf[mt][j][g][0], pf[mt][j][g][1]);
             mma16816<__half>(acc[g][2 * half + 1][j], a1, pf[mt][j][g][0], pf[mt][j][g][1]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) mma16816<__half>(wsum[g][j], one, pf[mt][j][g][0], pf[mt][j][g][1]);
       }
   }
   cp_async_wait<0>();
@@ -621,12 +598,13 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_ker
       if (r == 0) s_ml[warp][row] = make_float2(M[j][i], l[j][i]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float more = fmaf(-64.0f, wsum[g][j][i], zsum[j][i][g]);
-        float* dst = part + row * kPitch + g * kU4Group + r * 8;
+        const float more = zsum[j][i][g];
+        float* dst = part + row * kPitch + g * kU4Group + r * 4;
 #pragma unroll
-        for (int t = 0; t < 4; t += 2)
-          *reinterpret_cast<float4*>(dst + 2 * t) = make_float4(acc[g][t][j][i] + more, acc[g][t][j][2 + i] + more,
-                                                                acc[g][t + 1][j][i] + more, acc[g][t + 1][j][2 + i] + more);
+        for (int half = 0; half < 2; ++half)
+          *reinterpret_cast<float4*>(dst + 32 * half) =
+              make_float4(fmaf(kLowUnit, acc[g][2 * half][j][i], more), fmaf(kHighUnit, acc[g][2 * half][j][2 + i], more),
+                          fmaf(kLowUnit, acc[g][2 * half + 1][j][i], more), fmaf(kHighUnit, acc[g][2 * half + 1][j][2 + i], more));
       }
     }
   __syncthreads();
