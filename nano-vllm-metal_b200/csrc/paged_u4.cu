@@ -29,7 +29,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
-constexpr int kStages = 3;   // of each warp's own ring
+constexpr int kStages = 2;   // of each warp's own ring
+constexpr int kBlocks1 = 4, kBlocks2 = 3;  // blocks an SM holds, of one or two tiles of rows
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
 constexpr int kFan = 16;     // partial results that are joined at a time
 constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
@@ -192,7 +193,7 @@ __device__ __forceinline__ void join(const U4Params& p, float2* scratch, int cou
 // through a ring of its own, and are joined in shared memory.  A unit that several blocks share is
 // joined by the last of them (in groups of kFan, then the groups).
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 4 : 3) paged_u4_kernel(const U4Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2) paged_u4_kernel(const U4Params p) {
   using R = Ring<D>;
   constexpr int G = R::kGroups, kRows = 8 * kTiles;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -688,7 +689,7 @@ U4Plan plan_paged_u4(const PagedArgs& a) {
   const int64_t steps = std::max<int64_t>((a.max_pages * a.page_size + kStep - 1) / kStep, 1);
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t most = (int64_t)sms * (plan.tiles == 1 ? 4 : 3), units = a.B * a.Hkv * plan.row_blocks;
+  const int64_t most = (int64_t)sms * (plan.tiles == 1 ? kBlocks1 : kBlocks2), units = a.B * a.Hkv * plan.row_blocks;
   plan.blocks = units > most / steps ? most : units * steps;
   plan.ws_bytes = kTicketRegionBytes + (size_t)(plan.blocks * 2 * 8 * plan.tiles) * (a.D + 2) * sizeof(float);
   return plan;
