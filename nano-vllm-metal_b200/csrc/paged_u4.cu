@@ -29,9 +29,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
-constexpr int kStages = 2;   // of each warp's own ring
+constexpr int kStages = 2;   // of each warp's own ring: one tile is copied while one is worked on
 constexpr int kBlocks1 = 4, kBlocks2 = 3;  // blocks an SM holds, of one or two tiles of rows
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
+constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of
 constexpr int kFan = 16;     // partial results that are joined at a time
 constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
 constexpr float kLeast = 0x1p-44f;  // least scale that a key's values count as
@@ -59,6 +60,7 @@ struct U4Params {
   float* part_o;    // [2 * blocks][rows of a unit][D]
   int* tickets;     // [3 * blocks], zero between calls: of groups by their leader's place, of units by their first block
   int q_dtype, out_dtype, causal;
+  int q_fast;  // rows of 16-bit numbers on 16-byte boundaries
   int B, Hkv, L, rows, row_blocks, P, ps, mp;
   uint32_t ps_mul, ps_shift;  // key / ps = key * ps_mul >> ps_shift
   float scale_log2;
@@ -73,10 +75,7 @@ __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bo
                : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int n>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
-}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
@@ -201,57 +200,51 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
   __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 
-  // the line's length, this block's part of it and the request that the part begins in
+  // The line's length, this block's part of it and the request that the part begins in.  Every unit
+  // counts kUnitCost steps more than it has (where there is more than a step a block): that long a block
+  // is busy with beginning and ending one.  Lane i adds up the requests [i * per, (i + 1) * per).
   const int heads = p.Hkv * p.row_blocks;  // units of a request
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int mine = b0 + lane < p.B ? steps_of(p, b0 + lane) : 0;
-    total += __reduce_add_sync(0xffffffffu, mine);
-  }
-  total *= heads;
-  const int64_t blocks = min((int64_t)gridDim.x, total);
-  if (blockIdx.x >= blocks) return;
-  // block i has steps [total * i / blocks, total * (i + 1) / blocks); step x is in block_of(x)
-  auto block_of = [&](int64_t x) -> int { return (int)(((x + 1) * blocks - 1) / total); };
-  int64_t pos = total * blockIdx.x / blocks;
-  const int64_t pos_end = total * (blockIdx.x + 1) / blocks;
-  int b = 0, steps = 1;
-  int64_t request_at = 0;  // where request b begins
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int mine = b0 + lane < p.B ? steps_of(p, b0 + lane) : 0;
-    int upto = mine;
+  const int per = (p.B + 31) / 32;
+  int upto = 0;
+  for (int i = lane * per; i < min((lane + 1) * per, p.B); ++i) upto += steps_of(p, i);
+  const int real = __reduce_add_sync(0xffffffffu, upto) * heads;
+  const int cost = real > (int)gridDim.x ? kUnitCost : 0;
+  upto += cost * max(min(per, p.B - lane * per), 0);
+  const int mine = upto;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, request_at + (int64_t)upto * heads > pos);
-    if (past != 0) {
-      const int l0 = __ffs(past) - 1;
-      b = b0 + l0;
-      steps = __shfl_sync(0xffffffffu, mine, l0);
-      request_at += (int64_t)(__shfl_sync(0xffffffffu, upto, l0) - steps) * heads;
-      break;
-    }
-    request_at += (int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
+  const int total = __shfl_sync(0xffffffffu, upto, 31) * heads, blocks = min((int)gridDim.x, total);
+  if ((int)blockIdx.x >= blocks) return;
+  // the first `more` blocks take share + 1 steps, the others share; step x is in block_of(x)
+  const int share = total / blocks, more = total - share * blocks;
+  auto block_of = [&](int x) -> int {
+    return x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share;
+  };
+  int pos = (int)blockIdx.x * share + min((int)blockIdx.x, more);
+  const int pos_end = pos + share + ((int)blockIdx.x < more);
+  const int in_lane = __ffs(__ballot_sync(0xffffffffu, upto * heads > pos)) - 1;
+  int b = in_lane * per, request_at = __shfl_sync(0xffffffffu, upto - mine, in_lane) * heads;  // where request b begins
+  int steps = steps_of(p, b);
 
   while (pos < pos_end) {
-  if (pos >= request_at + (int64_t)steps * heads) {
-    request_at += (int64_t)steps * heads;
-    ++b;
-    steps = steps_of(p, b);
+  while (pos >= request_at + (steps + cost) * heads) {
+    request_at += (steps + cost) * heads;
+    steps = steps_of(p, ++b);
   }
-  const int in_request = (int)((pos - request_at) / steps);
-  const int64_t unit_at = request_at + (int64_t)in_request * steps;
-  const int kvh = in_request / p.row_blocks, rb = in_request - kvh * p.row_blocks, bh = b * p.Hkv + kvh;
-  const int step0 = (int)(pos - unit_at), step1 = (int)min((int64_t)steps, pos_end - unit_at);
+  const int in_request = (pos - request_at) / (steps + cost);
+  const int unit_at = request_at + in_request * (steps + cost) + cost;  // its first step
+  if (unit_at >= pos_end) break;
+  const int step0 = max(pos - unit_at, 0), step1 = min(steps, pos_end - unit_at);
   pos = unit_at + step1;
+  const int kvh = in_request / p.row_blocks, rb = in_request - kvh * p.row_blocks, bh = b * p.Hkv + kvh;
   const int row0 = rb * kRows, rows = min(kRows, p.rows - row0);
   const int ctx = __ldg(p.context_lens + b), limit = min(ctx, p.mp * p.ps);
   // keys that the unit's rows see: [0, most) by some row, [0, least) by every row
   int most = limit, least = limit;
-  if (p.causal) {
+  if (p.causal && p.L > 1) {
     int lo = row0 % p.L, hi = (row0 + rows - 1) % p.L;
     if (rows >= p.L || lo > hi) {
       lo = 0;
@@ -300,14 +293,26 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 
   int k_next = begin + warp * kTile;  // first key of the tile to copy next
   int pid = page_of_key(k_next + lane);
-  uint32_t there_next[kStages - 1];  // of the tiles on their way
+  const int pid1 = page_of_key(k_next + kStep + lane);
+  // 16-bit rows on 16-byte boundaries: a lane's elements are on their way before the tile's pages are known
+  uint4 raw[kTiles][G][2];
+  if (p.q_fast) {
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    there_next[s] = k_next < end ? issue(k_next, pid, s) : 0;
-    cp_async_commit();
-    k_next += kStep;
-    pid = page_of_key(k_next + lane);
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          raw[j][g][h] = make_uint4(0, 0, 0, 0);
+          if (8 * j + r < rows)
+            raw[j][g][h] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (out_row0 + 8 * j + r) * D) +
+                                 (g * kU4Group + h * 32 + c * 8) / 8);
+        }
   }
+  uint32_t there_next = k_next < end ? issue(k_next, pid, 0) : 0;  // the keys of the tile on its way
+  cp_async_commit();
+  k_next += kStep;
+  pid = pid1;
 
   // Queries as B fragments (lane: row r of each tile of 8; of a group, elements 8c to 8c + 7 of each half),
   // scaled per row so that the largest is in [2^10, 2^11), and 16 times that where they meet low codes;
@@ -322,17 +327,23 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        float2 v = make_float2(0.0f, 0.0f);
-        if (row < rows) {
-          const int64_t at = (int64_t)(out_row0 + row) * D + g * kU4Group + (e >> 3) * 32 + c * 8 + (e & 7);
-          v = p.q_dtype == NVM_BF16  ? load_pair<__nv_bfloat16>(p.q, at)
-              : p.q_dtype == NVM_F16 ? load_pair<__half>(p.q, at)
-                                     : load_pair<float>(p.q, at);
+      for (int h = 0; h < 2; ++h) {
+        if (p.q_fast) {
+          const uint4 v = raw[j][g][h];
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = p.q_dtype == NVM_BF16 ? u4_pair<__nv_bfloat16>(u[i]) : u4_pair<__half>(u[i]);
+            x[g][8 * h + 2 * i] = f.x;
+            x[g][8 * h + 2 * i + 1] = f.y;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            x[g][8 * h + i] = row < rows ? load_dyn(p.q, (int64_t)(out_row0 + row) * D + g * kU4Group + h * 32 + c * 8 + i, p.q_dtype) : 0.0f;
         }
-        x[g][e] = v.x;
-        x[g][e + 1] = v.y;
-        top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[g][8 * h + i]));
       }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -367,8 +378,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       kap[j][i] = __shfl_sync(0xffffffffu, down, (2 * c + i) * 4);
 #pragma unroll
       for (int g = 0; g < G; ++g) qsum[j][i][g] = __shfl_sync(0xffffffffu, sum[g], (2 * c + i) * 4);
-      const int rr = row0 + 8 * j + 2 * c + i;
-      seen[j][i] = rr - row0 >= rows ? INT32_MAX : p.causal ? min(limit, rr % p.L + ctx - p.L + 1) : limit;
+      const int rr = 8 * j + 2 * c + i;
+      seen[j][i] = rr >= rows || !p.causal ? limit : min(limit, (p.L == 1 ? 0 : (row0 + rr) % p.L) + ctx - p.L + 1);
     }
   }
 
@@ -399,20 +410,17 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
     }
   }
 
-  int stage = 0, stage_in = kStages - 1;
+  int stage = 0;
   for (int k0 = begin + warp * kTile; k0 < end; k0 += kStep) {
-    cp_async_wait<kStages - 2>();
+    cp_async_wait_all();
     __syncwarp();
-    const uint32_t there = there_next[0];
-#pragma unroll
-    for (int s = 0; s + 2 < kStages; ++s) there_next[s] = there_next[s + 1];
-    if (k_next < end) there_next[kStages - 2] = issue(k_next, pid, stage_in);
+    const uint32_t there = there_next;
+    if (k_next < end) there_next = issue(k_next, pid, stage ^ 1);
     cp_async_commit();
     k_next += kStep;
     pid = page_of_key(k_next + lane);
     const uint32_t at = ring_at + stage * R::kStage;
-    stage_in = stage;
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    stage ^= 1;
 
     // x[mt][j][e]: score / kap of key r + 16 mt + 8 (e / 2), row 2c + e % 2 of tile j
     float x[2][kTiles][4];
@@ -573,7 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
         }
       }
   }
-  cp_async_wait<0>();
+  cp_async_wait_all();
 
   // the warp's rows: (M, sum of weights) and sum of weight * value, in units of 2^M
 #pragma unroll
@@ -696,26 +704,23 @@ U4Plan plan_paged_u4(const PagedArgs& a) {
 }
 
 int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s) {
-  const int64_t blocks = plan.blocks;
-  if (a.max_pages * a.page_size > INT32_MAX - 4096 || a.Hq / a.Hkv * a.L > INT32_MAX / 2 || a.B > INT32_MAX / 2 ||
-      a.Hkv * plan.row_blocks > INT32_MAX)
+  const int64_t rows = a.Hq / a.Hkv * a.L, keys = a.max_pages * a.page_size, heads = a.Hkv * plan.row_blocks;
+  // steps are counted in 32 bits, requests by the part
+  const int64_t line = heads * ((keys + kStep - 1) / kStep + 1 + kUnitCost);
+  if (keys > INT32_MAX - 4096 || rows > INT32_MAX / 2 || line > INT32_MAX / 2)
     return fail(NVM_ERR_UNSUPPORTED, "paged_attention: 4-bit pages: too many rows or keys");
   U4Params p{};
-  p.q = a.q;
   p.kp = static_cast<const uint8_t*>(a.k_pages);
   p.vp = static_cast<const uint8_t*>(a.v_pages);
   p.ks = static_cast<const uint8_t*>(a.k_scales);
   p.vs = static_cast<const uint8_t*>(a.v_scales);
-  p.block_table = a.block_table;
-  p.context_lens = a.context_lens;
-  p.out = a.out;
   p.q_dtype = a.q_dtype;
   p.out_dtype = a.out_dtype;
   p.causal = a.is_causal;
-  p.B = (int)a.B;
+  p.q_fast = a.q_dtype != NVM_F32 && (uintptr_t)a.q % 16 == 0;
   p.Hkv = (int)a.Hkv;
   p.L = (int)a.L;
-  p.rows = (int)(a.Hq / a.Hkv * a.L);
+  p.rows = (int)rows;
   p.row_blocks = (int)plan.row_blocks;
   p.P = (int)a.P;
   p.ps = (int)a.page_size;
@@ -729,9 +734,20 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
   p.ps_shift = (uint32_t)(31 + n);
   p.tickets = static_cast<int*>(ws);
   p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kTicketRegionBytes);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + blocks * 2 * 8 * plan.tiles * a.D);
-  return a.scale_dtype == NVM_BF16 ? launch_d<__nv_bfloat16>(p, a.D, plan.tiles, blocks, s)
-                                   : launch_d<__half>(p, a.D, plan.tiles, blocks, s);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.blocks * 2 * 8 * plan.tiles * a.D);
+  const int64_t part = std::min<int64_t>(INT32_MAX / line, INT32_MAX / 64);
+  for (int64_t b0 = 0; b0 < a.B; b0 += part) {
+    const int64_t first_row = b0 * a.Hq * a.L * a.D;
+    p.B = (int)std::min(part, a.B - b0);
+    p.q = static_cast<const uint8_t*>(a.q) + first_row * (int64_t)dtype_size(a.q_dtype);
+    p.out = static_cast<uint8_t*>(a.out) + first_row * (int64_t)dtype_size(a.out_dtype);
+    p.block_table = a.block_table + b0 * a.max_pages;
+    p.context_lens = a.context_lens + b0;
+    const int st = a.scale_dtype == NVM_BF16 ? launch_d<__nv_bfloat16>(p, a.D, plan.tiles, plan.blocks, s)
+                                             : launch_d<__half>(p, a.D, plan.tiles, plan.blocks, s);
+    if (st != NVM_OK) return st;
+  }
+  return NVM_OK;
 }
 
 }  // namespace nvm
