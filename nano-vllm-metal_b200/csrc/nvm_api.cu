@@ -659,6 +659,8 @@ int nvm_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const
     int st = validate_u4(op, scale_dtype, D, P, Hkv, page_size);
     if (st == NVM_OK && T > 0 && P > 0) st = validate_u4_pointers(op, k_pages, v_pages, k_scales, v_scales);
     if (st != NVM_OK) return st;
+    if (((uintptr_t)k | (uintptr_t)v) % 16 != 0)
+      return fail(NVM_ERR_INVALID_ARGUMENT, "%s: keys and values of 4-bit pages must start on 16-byte boundaries", op);
   }
   if (T == 0) return NVM_OK;
   if (k == nullptr || v == nullptr || slot_mapping == nullptr || (P > 0 && (k_pages == nullptr || v_pages == nullptr)))

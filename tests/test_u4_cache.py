@@ -191,9 +191,11 @@ def test_c_entry_points_refuse():
     assert write(sdt=0) == -1 and write(ks=None) == -1 and write(kp=8) == -1
     assert write(T=2 ** 31) == -2 and "too many rows" in message()
     read = lambda **k: L.nvm_read_slots(*[k.get("kp", 16)] * 2, k.get("kv", nv.NVM_U4), *[k.get("ks", 16)] * 2,  # noqa: E731
-                                        k.get("sdt", 2), 16, 16, 16, k.get("out", 2), k.get("T", 1), 2, k.get("D", 128), 4, 16, None)
+                                        k.get("sdt", 2), 16, k.get("k", 16), 16, k.get("out", 2), k.get("T", 1), 2, k.get("D", 128), 4, 16,
+                                        None)
     assert read(out=3) == -1 and read(kv=4) == -1 and read(D=32) == -2 and read(ks=None) == -1 and read(kp=8) == -1
     assert read(kv=nv.NVM_I8, ks=None) == -1 and read(T=2 ** 31) == -2 and read(T=0) == 0 and read(D=0) == -1
+    assert read(k=8) == -1 and "16-byte" in message()
     prep = lambda **k: L.nvm_qk_norm_rope_write(16, 16, 16, 2, 512, 256, k.get("wq", None), k.get("wk", None), 1e-6, 16,  # noqa: E731
                                                 16, 8, 0, 16, 16, 1, 16, 16, nv.NVM_U4, k.get("ks", 16), 16, k.get("sdt", 2), 16,
                                                 k.get("T", 0), 4, 2, 128, 4, 16, None)
