@@ -652,7 +652,7 @@ int nvm_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: pages must be float32, float16, bfloat16, int8 or 4-bit", op);
   if (T < 0 || Hkv <= 0 || D <= 0 || P < 0 || page_size <= 0)
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", op);
-  if (T > INT32_MAX / Hkv) return fail(NVM_ERR_UNSUPPORTED, "%s: too many rows", op);
+  if (T > INT32_MAX / Hkv || page_size > INT32_MAX) return fail(NVM_ERR_UNSUPPORTED, "%s: too many rows", op);
   if (kv_dtype == NVM_I8 && (k_scales == nullptr || v_scales == nullptr || !is_float_dtype(scale_dtype)))
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: int8 pages need floating-point key/value scales", op);
   if (kv_dtype == NVM_U4) {

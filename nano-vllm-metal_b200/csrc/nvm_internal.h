@@ -183,6 +183,30 @@ int launch_u4_write(const void* k, const void* v, int in_dtype, int64_t stride_t
 int launch_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, const void* k_scales, const void* v_scales,
                       int scale_dtype, const int64_t* slots, void* k, void* v, int out_dtype, int64_t T, int64_t Hkv, int64_t D,
                       int64_t P, int64_t page_size, cudaStream_t s);
+struct U4AppendArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  int dtype;
+  int64_t q_stride_t, kv_stride_t;
+  const void* wq;
+  const void* wk;
+  float eps;
+  const float* cos_table;
+  const float* sin_table;
+  int64_t table_rows;
+  bool traditional;
+  const int32_t* positions;
+  void* q_out;
+  int64_t q_out_L;
+  void* k_pages;
+  void* v_pages;
+  void* k_scales;
+  void* v_scales;
+  const int64_t* slots;
+  int64_t T, Hq, Hkv, D, P, page_size;
+};
+int launch_u4_append(const U4AppendArgs& a, cudaStream_t s);
 struct U4Plan {
   int tiles;                   // of 8 query rows a unit
   int64_t row_blocks, blocks;  // row blocks of one (request, kv head), thread blocks

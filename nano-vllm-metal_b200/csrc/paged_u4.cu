@@ -62,7 +62,7 @@ struct U4Params {
   int q_dtype, out_dtype, causal;
   int q_fast;  // rows of 16-bit numbers on 16-byte boundaries
   int B, Hkv, L, rows, row_blocks, P, ps, mp;
-  uint32_t ps_mul, ps_shift;  // key / ps = key * ps_mul >> ps_shift
+  FastDiv by_ps;
   float scale_log2;
 };
 
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 
   auto page_of_key = [&](int key) -> int {
     if (key >= end) return -1;
-    const int pid = __ldg(bt + (uint32_t)((uint64_t)(uint32_t)key * p.ps_mul >> p.ps_shift));
+    const int pid = __ldg(bt + p.by_ps((uint32_t)key));
     return pid < p.P ? pid : -1;
   };
   // Copies the tile whose first key is k0 (a lane's key lies in page pid) into a stage and says which of
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
   const uint32_t dst_lane = ring_at + lane / kParts * R::kRow +
                             ((lane % kParts ^ swizzle<D>(lane / kParts)) << 4);
   auto issue = [&](int k0, int pid, int stage) -> uint32_t {
-    const uint32_t page = (uint32_t)((uint64_t)(uint32_t)(k0 + lane) * p.ps_mul >> p.ps_shift);
+    const uint32_t page = p.by_ps((uint32_t)(k0 + lane));
     const uint32_t off = (uint32_t)(k0 + lane) - page * (uint32_t)p.ps;
     const uint32_t row = pid < 0 ? 0u : ((uint32_t)pid * p.Hkv + kvh) * p.ps + off;
     const uint32_t dst = dst_lane + stage * R::kStage;
@@ -726,12 +726,7 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
   p.ps = (int)a.page_size;
   p.mp = a.P > 0 ? (int)a.max_pages : 0;  // a pool without pages: no key, and nothing to read
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  // key / ps for keys below 2^31: with 2^(n - 1) < ps <= 2^n and m = floor(2^(31 + n) / ps) + 1 the error
-  // m ps - 2^(31 + n) is at most 2^n, so key * m >> 31 + n is exact
-  int n = 0;
-  while ((int64_t(1) << n) < a.page_size) ++n;
-  p.ps_mul = (uint32_t)((uint64_t(1) << (31 + n)) / (uint64_t)a.page_size + 1);
-  p.ps_shift = (uint32_t)(31 + n);
+  p.by_ps = FastDiv(a.page_size);
   p.tickets = static_cast<int*>(ws);
   p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kTicketRegionBytes);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.blocks * 2 * 8 * plan.tiles * a.D);

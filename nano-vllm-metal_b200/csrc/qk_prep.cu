@@ -26,7 +26,6 @@
 
 #include "nvm_common.cuh"
 #include "nvm_internal.h"
-#include "u4.cuh"
 
 namespace nvm {
 namespace {
@@ -38,7 +37,6 @@ int64_t env_int(const char* name, int64_t dflt) {
   if (v == nullptr || v[0] == '\0') return dflt;
   return std::atoll(v);
 }
-enum Pages { kSame, kInt8, kU4 };  // the pool holds the input type, int8 or 4-bit rows
 constexpr int kBatch = 8;       // head rows whose loads are issued together
 constexpr int kBlocksPerSm = 3;  // resident blocks per SM at <= 80 registers
 
@@ -120,12 +118,9 @@ __device__ __forceinline__ V pack(const float* x) {
 // two butterfly steps (2, 1) finish; lane l ends with row (l >> 2) & 7.  Every addition
 // pairs the same two partial sums as the one-row butterfly v += shfl_xor(v, o) for
 // o = 16, 8, 4, 2, 1, so each row's sum is bitwise the one-row result.
-enum Reduce { kSumOf, kMaxOf, kMaxOfNumbers };  // the last ignores NaN
-template <Reduce kHow>
+template <bool kMax>
 __device__ __forceinline__ float reduce8(const float (&v)[8], int lane) {
-  auto op = [](float a, float b) {
-    return kHow == kSumOf ? __fadd_rn(a, b) : kHow == kMaxOf ? max_nan(a, b) : fmaxf(a, b);
-  };
+  auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : __fadd_rn(a, b); };
   const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
   float a[4], c[2];
 #pragma unroll
@@ -230,7 +225,7 @@ __device__ __forceinline__ void norm_rope_batch(const T* src_tok, int h0, int co
     }
     // mean = ss / D computed as ss * (1 / D): D is a power of two, so both are the same
     // correctly rounded value; 1 / sqrt as the correctly rounded reciprocal of the root
-    inv_mine = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(reduce8<kSumOf>(red, lane), 1.0f / (float)D), eps)));
+    inv_mine = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(reduce8<false>(red, lane), 1.0f / (float)D), eps)));
   }
   float w[2 * EH];
   unpack<T, EH>(w_lo, w);
@@ -301,7 +296,7 @@ __device__ __forceinline__ void quantize_batch(const typename Lane<T, D>::V (&rl
     for (int e = 0; e < 2 * EH; ++e) m = fmaxf(m, fabsf(x[e]));
     red[i] = m;
   }
-  const float amax_mine = reduce8<kMaxOfNumbers>(red, lane);
+  const float amax_mine = reduce8<true>(red, lane);
   const float s_mine = amax_mine > 0.0f ? __fdiv_rn(amax_mine, 127.0f) : 1.0f;
   const float r_mine = __frcp_rn(s_mine);
 #pragma unroll
@@ -317,83 +312,12 @@ __device__ __forceinline__ void quantize_batch(const typename Lane<T, D>::V (&rl
   }
 }
 
-// 4-bit write of up to eight rows already rounded to T (u4.cuh has the format): the extremes of the
-// rows' groups are reduced for the eight rows together, then lane l writes the byte of its two codes
-// in each group (D = 64: even lanes, with their neighbour's).  Pool row of head h: row0 + h * row_step.
-template <typename T, int D>
-__device__ __forceinline__ void quantize_batch_u4(const typename Lane<T, D>::V (&rlo)[kBatch],
-                                                  const typename Lane<T, D>::V (&rhi)[kBatch], int h0, int count,
-                                                  uint8_t* codes, void* scales, int64_t row0, int64_t row_step, int lane) {
-  constexpr int EH = Lane<T, D>::EH, kGroups = D / kU4Group;
-  float top[kGroups][kBatch], low[kGroups][kBatch];  // of x and of -x
-#pragma unroll
-  for (int i = 0; i < kBatch; ++i) {
-    float x[2 * EH];
-    unpack<T, EH>(rlo[i], x);
-    unpack<T, EH>(rhi[i], x + EH);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      top[g][i] = max_nan(x[2 * g], x[2 * g + 1]);
-      low[g][i] = max_nan(-x[2 * g], -x[2 * g + 1]);
-    }
-  }
-  float2 sz_mine[kGroups];  // of row (lane >> 2) & 7
-  float r_mine[kGroups];
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    sz_mine[g] = u4_scale<T>(-reduce8<kMaxOf>(low[g], lane), reduce8<kMaxOf>(top[g], lane));
-    r_mine[g] = u4_inverse(sz_mine[g].x);
-  }
-#pragma unroll
-  for (int i = 0; i < kBatch; ++i) {
-    float x[2 * EH], s[kGroups], z[kGroups], r[kGroups];
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      s[g] = __shfl_sync(0xffffffffu, sz_mine[g].x, i * 4);
-      z[g] = __shfl_sync(0xffffffffu, sz_mine[g].y, i * 4);
-      r[g] = __shfl_sync(0xffffffffu, r_mine[g], i * 4);
-    }
-    if (h0 + i >= count) break;  // warp-uniform
-    unpack<T, EH>(rlo[i], x);
-    unpack<T, EH>(rhi[i], x + EH);
-    int c[2 * EH];
-    bool amb[2 * EH], any = false;
-#pragma unroll
-    for (int e = 0; e < 2 * EH; ++e) {
-      const int g = e * kGroups / (2 * EH);
-      c[e] = u4_code_fast(x[e], z[g], r[g], amb[e]);
-      any |= amb[e];
-    }
-    if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-      for (int e = 0; e < 2 * EH; ++e)
-        if (amb[e]) c[e] = u4_code_div(x[e], z[e * kGroups / (2 * EH)], s[e * kGroups / (2 * EH)]);
-    }
-    const int64_t row = row0 + (int64_t)(h0 + i) * row_step;
-    uint8_t* dst = codes + row * (D / 2);
-    if constexpr (EH == 2) {
-      dst[lane] = (uint8_t)(c[0] | c[1] << 4);
-      dst[32 + lane] = (uint8_t)(c[2] | c[3] << 4);
-      if (lane == 0)
-        reinterpret_cast<uint2*>(scales)[row] = make_uint2(u4_pack_pair<T>(make_float2(s[0], z[0])),
-                                                           u4_pack_pair<T>(make_float2(s[1], z[1])));
-    } else {
-      const int n0 = __shfl_down_sync(0xffffffffu, c[0], 1), n1 = __shfl_down_sync(0xffffffffu, c[1], 1);
-      if ((lane & 1) == 0) {
-        dst[lane / 2] = (uint8_t)(c[0] | n0 << 4);
-        dst[16 + lane / 2] = (uint8_t)(c[1] | n1 << 4);
-      }
-      if (lane == 0) reinterpret_cast<uint32_t*>(scales)[row] = u4_pack_pair<T>(make_float2(s[0], z[0]));
-    }
-  }
-}
-
 // Persistent grid over work units of one token's rows (all of them, or one segment of
 // consecutive eight-row batches when tokens are few), grid-stride in token-major order.
 // A unit reads the token's position and slot and its lanes' cos/sin entries once, then
 // runs its batches of eight rows of one kind.  Rows whose result is not needed (q/k
 // rows at a bad position, k/v rows of a skipped or bad slot) are not read.
-template <typename T, int D, bool kTrad, Pages kPages>
+template <typename T, int D, bool kTrad, bool kInt8>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(const QkPrepParams p) {
   using L = Lane<T, D>;
   using V = typename L::V;
@@ -502,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
       const int e_end = min(b_end, nbq + nbk);
       for (int bt = max(b_begin, nbq); bt < e_end; ++bt) {
         const int h0 = (bt - nbq) * kBatch;
-        if constexpr (kPages != kSame) {
+        if constexpr (kInt8) {
           V qlo[kBatch], qhi[kBatch];
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) qlo[i] = qhi[i] = 0;
@@ -514,11 +438,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
                 qhi[j] = yhi;
               }
           });
-          if constexpr (kPages == kInt8)
-            quantize_batch<T, D>(qlo, qhi, h0, Hkv, static_cast<int8_t*>(p.kp) + prow0 * D, pool_head, p.ks, prow0, p.ps,
-                                 p.scale_dtype, lane);
-          else
-            quantize_batch_u4<T, D>(qlo, qhi, h0, Hkv, static_cast<uint8_t*>(p.kp), p.ks, prow0, p.ps, lane);
+          quantize_batch<T, D>(qlo, qhi, h0, Hkv, static_cast<int8_t*>(p.kp) + prow0 * D, pool_head, p.ks, prow0, p.ps,
+                               p.scale_dtype, lane);
         } else {
           T* k_row0 = static_cast<T*>(p.kp) + prow0 * D;
           norm_rope_batch<T, D, kTrad>(k_tok, h0, Hkv, wk_lo, wk_hi, rot, p.eps, norm, lane, [&](int, int h, V ylo, V yhi) {
@@ -545,9 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
             rhi[i] = __ldg(reinterpret_cast<const V*>(src + hi));
           }
         }
-        if constexpr (kPages == kU4) {
-          quantize_batch_u4<T, D>(rlo, rhi, h0, Hkv, static_cast<uint8_t*>(p.vp), p.vs, prow0, p.ps, lane);
-        } else if constexpr (kPages == kInt8) {
+        if constexpr (kInt8) {
           quantize_batch<T, D>(rlo, rhi, h0, Hkv, static_cast<int8_t*>(p.vp) + prow0 * D, pool_head, p.vs, prow0,
                                p.ps, p.scale_dtype, lane);
         } else {
@@ -565,14 +484,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
   }
 }
 
-template <typename T, int D, bool kTrad>
+template <typename T, int D, bool kTrad, bool kInt8>
 void launch_one(const QkPrepParams& p, unsigned grid, cudaStream_t s) {
-  if (p.kv_dtype == NVM_U4)
-    qk_prep_kernel<T, D, kTrad, kU4><<<grid, kWarps * 32, 0, s>>>(p);
-  else if (p.kv_dtype == NVM_I8)
-    qk_prep_kernel<T, D, kTrad, kInt8><<<grid, kWarps * 32, 0, s>>>(p);
-  else
-    qk_prep_kernel<T, D, kTrad, kSame><<<grid, kWarps * 32, 0, s>>>(p);
+  qk_prep_kernel<T, D, kTrad, kInt8><<<grid, kWarps * 32, 0, s>>>(p);
 }
 
 template <typename T>
@@ -598,10 +512,18 @@ int launch_t(const QkPrepParams& p, int64_t D, cudaStream_t s) {
   const int64_t blocks_needed = (p.T * q.segs + kWarps - 1) / kWarps;
   const int64_t grid = std::min<int64_t>(blocks_needed, (int64_t)sms * kBlocksPerSm);
   const unsigned g = (unsigned)grid;
-  if (D == 128)
-    p.traditional ? launch_one<T, 128, true>(q, g, s) : launch_one<T, 128, false>(q, g, s);
-  else
-    p.traditional ? launch_one<T, 64, true>(q, g, s) : launch_one<T, 64, false>(q, g, s);
+  const bool i8 = q.kv_dtype == NVM_I8;
+  if (D == 128) {
+    if (p.traditional)
+      i8 ? launch_one<T, 128, true, true>(q, g, s) : launch_one<T, 128, true, false>(q, g, s);
+    else
+      i8 ? launch_one<T, 128, false, true>(q, g, s) : launch_one<T, 128, false, false>(q, g, s);
+  } else {
+    if (p.traditional)
+      i8 ? launch_one<T, 64, true, true>(q, g, s) : launch_one<T, 64, true, false>(q, g, s);
+    else
+      i8 ? launch_one<T, 64, false, true>(q, g, s) : launch_one<T, 64, false, false>(q, g, s);
+  }
   return check_cuda(cudaGetLastError(), "qk_norm_rope_write: kernel launch");
 }
 
@@ -622,6 +544,8 @@ extern "C" int nvm_qk_norm_rope_write(const void* q, const void* k, const void* 
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: q/k/v must be float16 or bfloat16", op);
   if (kv_dtype != dtype && kv_dtype != NVM_I8 && kv_dtype != NVM_U4)
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: page dtype must equal the input dtype or be int8 or 4-bit", op);
+  if (kv_dtype == NVM_U4 && page_size > INT32_MAX)
+    return fail(NVM_ERR_UNSUPPORTED, "%s: 4-bit pages of 2^31 rows or more are not supported", op);
   if (kv_dtype == NVM_U4 && (scale_dtype != dtype || k_scales == nullptr || v_scales == nullptr))
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: 4-bit pages need key/value scales of the input dtype", op);
   if ((q_norm_weight == nullptr) != (k_norm_weight == nullptr))
@@ -636,7 +560,8 @@ extern "C" int nvm_qk_norm_rope_write(const void* q, const void* k, const void* 
   if (q_stride_t < Hq * D || kv_stride_t < Hkv * D)
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: token strides must cover every head row", op);
   // lanes move D/32 elements (8 bytes for D = 128, 4 for 64) as one vector
-  const int64_t vec_elems = D / 32;
+  // (4-bit pages: 8 bytes for both)
+  const int64_t vec_elems = kv_dtype == NVM_U4 ? 4 : D / 32;
   if (q_stride_t % vec_elems != 0 || kv_stride_t % vec_elems != 0 ||
       reinterpret_cast<uintptr_t>(q) % (vec_elems * 2) != 0 || reinterpret_cast<uintptr_t>(k) % (vec_elems * 2) != 0 ||
       reinterpret_cast<uintptr_t>(v) % (vec_elems * 2) != 0 ||
@@ -647,8 +572,7 @@ extern "C" int nvm_qk_norm_rope_write(const void* q, const void* k, const void* 
       reinterpret_cast<uintptr_t>(sin_table) % (vec_elems * 4) != 0 ||
       reinterpret_cast<uintptr_t>(k_pages) % (vec_elems * 2) != 0 ||
       reinterpret_cast<uintptr_t>(v_pages) % (vec_elems * 2) != 0 ||
-      (kv_dtype == NVM_U4 && (reinterpret_cast<uintptr_t>(k_scales) % (vec_elems * 2) != 0 ||
-                              reinterpret_cast<uintptr_t>(v_scales) % (vec_elems * 2) != 0)))
+      (kv_dtype == NVM_U4 && (reinterpret_cast<uintptr_t>(k_scales) % 8 != 0 || reinterpret_cast<uintptr_t>(v_scales) % 8 != 0)))
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: rows must start on %lld-byte boundaries (strides in whole vectors)", op,
                 (long long)(vec_elems * 2));
   if (q_out_L < 0 || (q_out_L > 0 && T % q_out_L != 0))
@@ -657,6 +581,13 @@ extern "C" int nvm_qk_norm_rope_write(const void* q, const void* k, const void* 
   if (q == nullptr || k == nullptr || v == nullptr || cos_table == nullptr || sin_table == nullptr || positions == nullptr || q_out == nullptr ||
       slot_mapping == nullptr || (P > 0 && (k_pages == nullptr || v_pages == nullptr)))
     return fail(NVM_ERR_INVALID_ARGUMENT, "%s: null pointer", op);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (kv_dtype == NVM_U4) {
+    const U4AppendArgs u{q, k, v, dtype, q_stride_t, kv_stride_t, q_norm_weight, k_norm_weight, eps, cos_table, sin_table,
+                         table_rows, traditional != 0, positions, q_out, q_out_L, k_pages, v_pages, k_scales, v_scales,
+                         slot_mapping, T, Hq, Hkv, D, P, page_size};
+    return launch_u4_append(u, s);
+  }
   QkPrepParams p{};
   p.q = q; p.k = k; p.v = v; p.wq = q_norm_weight; p.wk = k_norm_weight;
   p.cos_t = cos_table; p.sin_t = sin_table; p.pos = positions; p.q_out = q_out;
@@ -665,6 +596,5 @@ extern "C" int nvm_qk_norm_rope_write(const void* q, const void* k, const void* 
   p.q_st = q_stride_t; p.kv_st = kv_stride_t; p.table_rows = table_rows; p.q_out_L = q_out_L;
   p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.P = P; p.ps = page_size; p.eps = eps;
   p.dtype = dtype; p.kv_dtype = kv_dtype; p.scale_dtype = scale_dtype; p.traditional = traditional ? 1 : 0;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == NVM_BF16 ? launch_t<__nv_bfloat16>(p, D, s) : launch_t<__half>(p, D, s);
 }

@@ -13,7 +13,7 @@
 namespace nvm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kRead = 4;  // rows a thread reads at a time
 
 struct RowsParams {
@@ -27,20 +27,21 @@ struct RowsParams {
   const int64_t* slots;
   int64_t P, ps;
   uint32_t items, Hkv, parts;  // items: threads with work, tokens * Hkv * parts; parts: D / 8
+  FastDiv by_parts, by_heads, by_ps;
   int dtype, kv_dtype, scale_dtype, fast;  // fast: 16-byte vectors of the values, whole ones of the pages
 };
 
 // Where an item's row lies in the pool (false: it is skipped).
 __device__ __forceinline__ bool find_row(const RowsParams& p, uint32_t item, uint32_t& t, uint32_t& h, uint32_t& part, int64_t& row) {
-  const uint32_t w = item / p.parts;
+  const uint32_t w = p.by_parts(item);
   part = item - w * p.parts;
-  t = w / p.Hkv;
+  t = p.by_heads(w);
   h = w - t * p.Hkv;
   const int64_t slot = __ldg(p.slots + t);
   if (slot < 0) return false;
   int64_t pid, off;
-  if ((slot | p.ps) <= 0x7fffffffLL) {  // a 64-bit division costs as much as the rest
-    pid = (uint32_t)slot / (uint32_t)p.ps;
+  if (slot <= 0x7fffffffLL) {  // a 64-bit division costs as much as the rest
+    pid = p.by_ps((uint32_t)slot);
     off = (uint32_t)slot - (uint32_t)pid * (uint32_t)p.ps;
   } else {
     pid = slot / p.ps;
@@ -132,10 +133,15 @@ struct Raw<NVM_U4> {
   }
   __device__ __forceinline__ void values(int scale_dtype, float (&x)[8]) const {
     const float2 sz = scale_dtype == NVM_BF16 ? u4_pair<__nv_bfloat16>(pair) : u4_pair<__half>(pair);
+    // the codes at 4 i and 4 i + 16 are the f16 subnormals code * 2^-24 once shifted: exact, two an operation;
+    // the factor goes into s in two steps, so that it overflows no s
+    const float s = sz.x * 0x1p12f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // code + 2^23 is an exact fp32 number, without the conversion unit
-      const float c = __fsub_rn(__uint_as_float(0x4B000000u | (codes >> (4 * i) & 15)), 8388608.0f);
-      x[i] = fmaf(sz.x, c, sz.y);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = codes >> (4 * i) & 0x000f000fu;
+      const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      x[i] = fmaf(s, c.x * 0x1p12f, sz.y);
+      x[i + 4] = fmaf(s, c.y * 0x1p12f, sz.y);
     }
   }
 };
@@ -249,6 +255,9 @@ int launch_u4_write(const void* k, const void* v, int in_dtype, int64_t stride_t
   const int64_t e = (int64_t)dtype_size(in_dtype);
   p.st = stride_t; p.sh = stride_h; p.kp = k_pages; p.vp = v_pages; p.ks = k_scales; p.vs = v_scales;
   p.P = P; p.ps = page_size; p.Hkv = (uint32_t)Hkv; p.parts = (uint32_t)(D / 8);
+  p.by_parts = FastDiv(p.parts);
+  p.by_heads = FastDiv(Hkv);
+  p.by_ps = FastDiv(page_size);
   p.dtype = in_dtype;
   p.fast = aligned16(k, v) && stride_t * e % 16 == 0 && stride_h * e % 16 == 0;
   const int64_t row_items = Hkv * (D / 8), most = INT32_MAX / row_items;  // tokens of a launch: items are counted in 32 bits
@@ -279,6 +288,9 @@ int launch_read_slots(const void* k_pages, const void* v_pages, int kv_dtype, co
   p.P = P; p.ps = page_size; p.Hkv = (uint32_t)Hkv; p.dtype = out_dtype; p.kv_dtype = kv_dtype; p.scale_dtype = scale_dtype;
   const bool fast = D % 8 == 0 && aligned16(k, v) && aligned16(k_pages, v_pages);
   p.parts = (uint32_t)(fast ? D / 8 : D);
+  p.by_parts = FastDiv(p.parts);
+  p.by_heads = FastDiv(Hkv);
+  p.by_ps = FastDiv(page_size);
   const int64_t row_items = Hkv * p.parts, most = INT32_MAX / row_items;
   if (most < 1) return fail(NVM_ERR_UNSUPPORTED, "read_slots: rows of more than 2^31 elements a token");
   for (int64_t t0 = 0; t0 < T; t0 += most) {
