@@ -112,6 +112,7 @@ struct Sm100Params {
   int64_t window, sinks;  // kExt: window == 0 for none
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
   int cluster;            // kExt: the n_chunks CTAs of a unit are one cluster and merge over DSMEM
+  const float* out_scale;  // [B * Hkv] factors of the output, or null
 };
 
 // Pairs q (keys 2q, 2q+1 of a 64-key tile) whose exponentials run on the FMA pipe.
@@ -665,6 +666,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     int gt = 0;  // tiles processed by this CTA so far
     int kq = 0, iw = 0;
     bool ok = true;
+    // 1 / (sum of a row's weights) times the item's factor
+    auto inverse = [&](const Item& it, float sum) {
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      return p.out_scale != nullptr ? inv * __ldg(p.out_scale + it.b * p.Hkv + it.kvh) : inv;
+    };
     // With one item per CTA (stage_out) the K/V ring is free once the item's MMAs are done:
     // O rows go to shared memory in the TMA store's 128B-swizzled box layout (boxes of 128
     // bytes of columns x 128 rows, 16 KB each; row r's 16-byte chunk c of a box at
@@ -997,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         merged = true;
       } else if (it.n_chunks_unit == 1) {
         put_lse(it, m, lsum);
-        const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+        const float inv = inverse(it, lsum);
 #pragma unroll 1
         for (int c1 = 0; c1 < kD; c1 += 64) {
           float ov2[64];
@@ -1075,7 +1081,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (ml.x != -INFINITY) lt += ml.y * exp2f(ml.x - mxc);
               }
             }
-            const float inv = lt > 0.f ? 1.f / lt : 0.f;
+            const float inv = inverse(it, lt);
             put_lse(it, mxc, lt);
 #pragma unroll 1
             for (int c0 = 0; c0 < kD; c0 += 32) {
@@ -1457,6 +1463,7 @@ int launch_sm100(const PagedArgs& a, const Sm100Plan& plan, void* ws, cudaStream
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.causal = a.is_causal; p.dense = a.dense; p.box_rows = box_rows;
   p.window = a.window; p.sinks = a.sinks; p.lse = a.lse;
+  p.out_scale = a.out_scale;
   p.split_below = env_int("NVM_SM100_SPLIT_BELOW", kSplitBelowKeys);  // tuning: 0 = never, huge = always
   p.grouped = plan.grouped;
   p.g = a.Hq / a.Hkv;

@@ -350,7 +350,12 @@ size_t nvm_paged_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.L = L; a.D = D; a.P = 1; a.page_size = page_size; a.max_pages = max_pages;
   a.is_causal = 1;
   if (validate_paged(a, false) != NVM_OK) return 0;
-  if (kv_dtype == NVM_U4) return plan_paged_u4(a).ws_bytes;
+  if (kv_dtype == NVM_U4) {  // the scale and the output's address are not known here: cover both kernels
+    a.scale = 1.0f;
+    const U4PromptPlan prompt = plan_u4_prompt(a);
+    const size_t rows = plan_paged_u4(a).ws_bytes;
+    return prompt.eligible && prompt.ws_bytes > rows ? prompt.ws_bytes : rows;
+  }
   if (env_flag("NVM_ATTN_FORCE_GENERIC")) return 0;
   // q's dtype is not known here: cover the tcgen05 plan (taken when q matches the pages)
   // and the mma.sync plan (taken otherwise).
@@ -381,6 +386,15 @@ int nvm_paged_attention(const void* q, int q_dtype, const void* k_pages, const v
   if (B == 0) return NVM_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (kv_dtype == NVM_U4) {
+    if ((uintptr_t)workspace % 16 != 0)
+      return fail(NVM_ERR_INVALID_ARGUMENT, "paged_attention: the workspace must start on a 16-byte boundary");
+    const U4PromptPlan prompt = plan_u4_prompt(a);
+    if (prompt.eligible) {
+      if (workspace == nullptr || workspace_bytes < prompt.ws_bytes)
+        return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", prompt.ws_bytes,
+                    workspace_bytes);
+      return launch_u4_prompt(a, prompt, workspace, s);
+    }
     const U4Plan plan = plan_paged_u4(a);
     if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes))
       return fail(NVM_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes required, %zu given", plan.ws_bytes,

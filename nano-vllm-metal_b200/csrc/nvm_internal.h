@@ -66,6 +66,7 @@ struct PagedArgs {
   int defer;          // with scores: leave the merge through the workspace to the kernel over the scores
   float* mass;        // with scores, and no merge through the workspace: add the weights, or NULL
   int64_t mass_sb, mass_sh, mass_len;
+  const float* out_scale;  // tcgen05 kernel only: [B * Hkv] factors of the output, or NULL
 };
 inline bool paged_is_ext(const PagedArgs& a) { return a.window > 0 || a.lse != nullptr; }
 
@@ -207,6 +208,15 @@ struct U4AppendArgs {
   int64_t T, Hq, Hkv, D, P, page_size;
 };
 int launch_u4_append(const U4AppendArgs& a, cudaStream_t s);
+// Many query rows: pages unpacked into the workspace for the tcgen05 kernel (u4_prompt.cu).
+constexpr int64_t kU4PromptRows = 96;
+struct U4PromptPlan {
+  bool eligible;
+  int64_t batch;  // requests taken at a time
+  size_t ws_bytes, attention_bytes;
+};
+U4PromptPlan plan_u4_prompt(const PagedArgs& a);
+int launch_u4_prompt(const PagedArgs& a, const U4PromptPlan& plan, void* ws, cudaStream_t s);
 struct U4Plan {
   int tiles;                   // of 8 query rows a unit
   int64_t row_blocks, blocks;  // row blocks of one (request, kv head), thread blocks

@@ -59,16 +59,26 @@ def parts64(packed, scales):
     return (codes * sz[..., :1]).flatten(-2), (one * sz[..., :1]).flatten(-2), (one * sz[..., 1:].abs()).flatten(-2)
 
 
+def unpacked(rows, D, ps, scale):
+    """Whether a call of so many query rows a kv head goes through unpacked pages."""
+    return rows >= 96 and D == 128 and ps % 16 == 0 and scale > 0
+
+
 def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
     """(out, bound): attention in 64 bits, request by request, and how far an fp32 result may be off.
 
     The bound counts, per output element: the weight times the value's scale held in 16 bits with 11
     (2^-11 of it, over s * code), the score held in fp32 (the matrix unit adds codes raised by 64, so
     2^-22 of sum |q| (64 + code) s and of |q| |z|, 2^-22 for the exponential) which moves weight and
-    normaliser, and q held in 11 bits where it is fp32.  Rounding to the output type is the caller's."""
+    normaliser, and q held in 11 bits where it is fp32.  Rounding to the output type is the caller's.
+
+    Calls of many rows (``unpacked``) hold K and V in f16, brought below 32 by a power of two: 2^-12 of a
+    value, or 2^-25 of a unit below the normals, that is 2^-29 of the largest value; q likewise where it
+    was not f16 (2^-25 of a unit against values below 32); weights are rounded to 11 bits against V itself."""
     B, Hq, L, D = q.shape
     Hkv = kp.shape[1]
     scale = D ** -0.5 if scale is None else scale
+    many = unpacked(Hq // Hkv * L, D, ps, scale)
     out = torch.zeros(B, Hq, L, D, dtype=torch.float64, device=q.device)
     bound = torch.zeros_like(out)
     for b in range(B):
@@ -101,8 +111,14 @@ def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
                 d = 2.0 ** -22 * abs(scale) * (x.abs() @ (64 * s_k + sc_k + z_k).T) + 2.0 ** -22 * (1 + t.abs())
                 if q.dtype == torch.float32:
                     d = d + 2.0 ** -11 * abs(scale) * (x.abs() @ k.abs().T)
+                if many:
+                    d = d + abs(scale) * (2.0 ** -12 * (x.abs() @ k.abs().T) + 2.0 ** -29 * k.abs().max() * x.abs().sum(-1, keepdim=True))
+                    if not (q.dtype == ks.dtype == torch.float16):
+                        d = d + 2.0 ** -25 * 32 * D
                 d = d.masked_fill(~seen, 0).amax(-1, keepdim=True)
-                bound[b, hq] = 2.0 ** -11 * (p @ sc_v) + (2 * d + 2.0 ** -20) * (p @ (64 * s_v + sc_v + z_v))
+                if many:
+                    bound[b, hq] = (2.0 ** -11 + 2.0 ** -12) * (p @ v.abs()) + 2.0 ** -29 * v.abs().max()
+                bound[b, hq] += 2.0 ** -11 * (p @ sc_v) + (2 * d + 2.0 ** -20) * (p @ (64 * s_v + sc_v + z_v))
     return out, bound
 
 
