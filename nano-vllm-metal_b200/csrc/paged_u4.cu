@@ -35,7 +35,7 @@ constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the
 constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of
 constexpr int kFan = 16;     // partial results that are joined at a time
 constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
-constexpr float kLeast = 0x1p-44f;  // least scale that a key's values count as
+constexpr float kLeast = 0x1p-80f;  // least scale that a key's values count as
 constexpr float kNoKeys = -1e30f;  // M of a row that has seen no key
 
 template <int D>
@@ -383,15 +383,17 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
     }
   }
 
-  float acc[G][4][kTiles][4], M[kTiles][2], l[kTiles][2], zsum[kTiles][2][G];
+  float acc[G][4][kTiles][4], wsum[G][kTiles][4], M[kTiles][2], l[kTiles][2], zsum[kTiles][2][G];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        wsum[g][j][e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[g][i][j][e] = 0.0f;
+      }
       zsum[j][0][g] = zsum[j][1][g] = 0.0f;
     }
     M[j][0] = M[j][1] = kNoKeys;
@@ -459,16 +461,6 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       }
     }
 
-    Pairs<T, G> vz[2][2];
-    float size = kLeast;  // the largest scale
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        vz[mt][h].load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
-        size = fmaxf(size, vz[mt][h].size());
-      }
-
     const bool masked = there != 0xffffffffu || k0 + kTile > least;
     if (masked) {
 #pragma unroll
@@ -484,7 +476,12 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
     }
 
     // weights 2^(t - M); references that some contribution passes by kSlack move to the largest one
-    float w[2][kTiles][4], heavy = 0.0f;
+    float w[2][kTiles][4], heavy = 0.0f, size;
+    {  // the largest scale of the tile's values, of the lane's key first (positive numbers compare as integers)
+      Pairs<T, G> v;
+      v.load(at + R::kVs + lane * 4 * G);
+      size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.size(), kLeast))));
+    }
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -503,8 +500,11 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              top = fmaxf(top, fmaf(kap[j][i], x[mt][j][2 * h + i], lg2(fmaxf(vz[mt][h].size(), kLeast))));
+            for (int h = 0; h < 2; ++h) {
+              Pairs<T, G> v;
+              v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
+              top = fmaxf(top, fmaf(kap[j][i], x[mt][j][2 * h + i], lg2(fmaxf(v.size(), kLeast))));
+            }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -514,6 +514,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
           for (int g = 0; g < G; ++g) {
             zsum[j][i][g] *= fade;
+            wsum[g][j][i] *= fade;
+            wsum[g][j][2 + i] *= fade;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               acc[g][t][j][i] *= fade;
@@ -527,59 +529,65 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
         }
     }
 
-    // their sums, and the weights times the values' scales as B fragments; in a masked tile a key that the
-    // row does not see counts nothing whatever its values
-    uint32_t pf[2][kTiles][G][2];
-    auto weigh = [&](auto hidden) {
+    // The weights' sums, the weights times the values' scales as B fragments, and those times the codes.  What
+    // f16 rounds off a weight counts times the code less 8 (the sum of weight * (offset + 8 scale) is exact, and
+    // 8 times the sum of the rounded weights, a product with ones, is taken out at the end): half of what it would
+    // times the code.  In a masked tile a key that the row does not see counts nothing whatever its values.
+    auto values = [&](auto hidden) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t pf[kTiles][G][2];
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
+        for (int h = 0; h < 2; ++h) {
+          Pairs<T, G> v;
+          v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const Pairs<T, G>& v = vz[mt][h];
+          for (int j = 0; j < kTiles; ++j) {
             const float w0 = w[mt][j][2 * h], w1 = w[mt][j][2 * h + 1];
             l[j][0] += w0;
             l[j][1] += w1;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
+              const float middle = fmaf(8.0f, v.s[g], v.z[g]);
               float s0 = w0 * v.s[g], s1 = w1 * v.s[g];
               if constexpr (decltype(hidden)::value) {
                 if (w0 == 0.0f) s0 = 0.0f;
                 if (w1 == 0.0f) s1 = 0.0f;
-                zsum[j][0][g] += w0 == 0.0f ? 0.0f : w0 * v.z[g];
-                zsum[j][1][g] += w1 == 0.0f ? 0.0f : w1 * v.z[g];
+                zsum[j][0][g] += w0 == 0.0f ? 0.0f : w0 * middle;
+                zsum[j][1][g] += w1 == 0.0f ? 0.0f : w1 * middle;
               } else {
-                zsum[j][0][g] = fmaf(w0, v.z[g], zsum[j][0][g]);
-                zsum[j][1][g] = fmaf(w1, v.z[g], zsum[j][1][g]);
+                zsum[j][0][g] = fmaf(w0, middle, zsum[j][0][g]);
+                zsum[j][1][g] = fmaf(w1, middle, zsum[j][1][g]);
               }
-              pf[mt][j][g][h] = transpose8x8(pack2<__half>(s0, s1));
+              pf[j][g][h] = transpose8x8(pack2<__half>(s0, s1));
             }
           }
-    };
-    if (masked)
-      weigh(std::true_type{});
-    else
-      weigh(std::false_type{});
-
+        }
+        const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+        for (int g = 0; g < G; ++g) {
+          uint32_t v[4];  // keys (2c, 2c + 1) and (2c, 2c + 1) + 8: elements 4r to 4r + 3 of the group's halves
+          ldsm_x4_t(at + v_off[g] + 16 * mt * R::kRow, v[0], v[1], v[2], v[3]);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        uint32_t v[4];  // keys (2c, 2c + 1) and (2c, 2c + 1) + 8: elements 4r to 4r + 3 of the group's halves
-        ldsm_x4_t(at + v_off[g] + 16 * mt * R::kRow, v[0], v[1], v[2], v[3]);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t y = v[2 * half], z = v[2 * half + 1], y8 = y >> 8, z8 = z >> 8;
+            const uint32_t a0[4] = {low_codes(y), high_codes(y), low_codes(z), high_codes(z)};
+            const uint32_t a1[4] = {low_codes(y8), high_codes(y8), low_codes(z8), high_codes(z8)};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t y = v[2 * half], z = v[2 * half + 1], y8 = y >> 8, z8 = z >> 8;
-          const uint32_t a0[4] = {low_codes(y), high_codes(y), low_codes(z), high_codes(z)};
-          const uint32_t a1[4] = {low_codes(y8), high_codes(y8), low_codes(z8), high_codes(z8)};
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            mma16816<__half>(acc[g][2 * half][j], a0, pf[mt][j][g][0], pf[mt][j][g][1]);
-            mma16816<__half>(acc[g][2 * half + 1][j], a1, pf[mt][j][g][0], pf[mt][j][g][1]);
+            for (int j = 0; j < kTiles; ++j) {
+              mma16816<__half>(acc[g][2 * half][j], a0, pf[j][g][0], pf[j][g][1]);
+              mma16816<__half>(acc[g][2 * half + 1][j], a1, pf[j][g][0], pf[j][g][1]);
+            }
           }
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) mma16816<__half>(wsum[g][j], one, pf[j][g][0], pf[j][g][1]);
         }
       }
+    };
+    if (masked)
+      values(std::true_type{});
+    else
+      values(std::false_type{});
   }
   cp_async_wait_all();
 
@@ -607,7 +615,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       if (r == 0) s_ml[warp][row] = make_float2(M[j][i], l[j][i]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float more = zsum[j][i][g];
+        const float more = fmaf(-8.0f, wsum[g][j][i], zsum[j][i][g]);
         float* dst = part + row * kPitch + g * kU4Group + r * 4;
 #pragma unroll
         for (int half = 0; half < 2; ++half)

@@ -52,11 +52,12 @@ def values64(packed: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 def parts64(packed, scales):
-    """(s * code, s, |z|) of every element, for the error bound."""
+    """(s * code, s, |z|, s * |code - 8|) of every element, for the error bound."""
     codes = torch.stack([packed & 15, packed >> 4], -1).flatten(-2).double().unflatten(-1, (-1, GROUP))
     sz = scales.double().unflatten(-1, (-1, 2))
     one = torch.ones_like(codes)
-    return (codes * sz[..., :1]).flatten(-2), (one * sz[..., :1]).flatten(-2), (one * sz[..., 1:].abs()).flatten(-2)
+    return (codes * sz[..., :1]).flatten(-2), (one * sz[..., :1]).flatten(-2), (one * sz[..., 1:].abs()).flatten(-2), \
+        ((codes - 8).abs() * sz[..., :1]).flatten(-2)
 
 
 def unpacked(rows, D, ps, scale):
@@ -67,8 +68,9 @@ def unpacked(rows, D, ps, scale):
 def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
     """(out, bound): attention in 64 bits, request by request, and how far an fp32 result may be off.
 
-    The bound counts, per output element: the weight times the value's scale held in 16 bits with 11
-    (2^-11 of it, over s * code), the score held in fp32 (the matrix unit adds codes raised by 64, so
+    The bound counts, per output element: the weight times the value's scale held in 16 bits with 11,
+    which multiplies the code less 8 (weight * (offset + 8 scale) is summed in fp32, and the sum of the
+    rounded weights taken out 8 times): 2^-11 of weight * s * |code - 8|; the score held in fp32 (the matrix unit adds codes raised by 64, so
     2^-22 of sum |q| (64 + code) s and of |q| |z|, 2^-22 for the exponential) which moves weight and
     normaliser, and q held in 11 bits where it is fp32.  Rounding to the output type is the caller's.
 
@@ -97,8 +99,8 @@ def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
             for r in rows:
                 r[~any_row] = 0
             k, v = values64(*rows[:2]), values64(*rows[2:])
-            sc_k, s_k, z_k = parts64(*rows[:2])
-            sc_v, s_v, z_v = parts64(*rows[2:])
+            sc_k, s_k, z_k, _ = parts64(*rows[:2])
+            sc_v, s_v, z_v, off_v = parts64(*rows[2:])
             for hq in range(h * (Hq // Hkv), (h + 1) * (Hq // Hkv)):
                 x = q[b, hq].double()
                 t = (x @ k.T) * scale
@@ -118,7 +120,7 @@ def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
                 d = d.masked_fill(~seen, 0).amax(-1, keepdim=True)
                 if many:
                     bound[b, hq] = (2.0 ** -11 + 2.0 ** -12) * (p @ v.abs()) + 2.0 ** -29 * v.abs().max()
-                bound[b, hq] += 2.0 ** -11 * (p @ sc_v) + (2 * d + 2.0 ** -20) * (p @ (64 * s_v + sc_v + z_v))
+                bound[b, hq] += 2.0 ** -11 * (p @ off_v) + (2 * d + 2.0 ** -20) * (p @ (64 * s_v + sc_v + z_v))
     return out, bound
 
 
