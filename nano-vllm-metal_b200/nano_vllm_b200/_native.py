@@ -128,22 +128,28 @@ def require_u4(op: str, D: int, key_pages: torch.Tensor, value_pages: torch.Tens
                value_scales: torch.Tensor | None) -> None:
     """The pools of a 4-bit cache of head dim D: uint8 [P, Hkv, page_size, D/2] with scales and offsets
     [P, Hkv, page_size, D/32], all contiguous."""
-    if D not in (64, 128):
+    if D != 128 and D != 64:
         raise RuntimeError(f"{op}: 4-bit pages need a head dimension of 64 or 128 (got {D})")
     shape = key_pages.shape
     if value_pages.dtype is not torch.uint8 or len(shape) != 4 or value_pages.shape != shape or shape[3] * 2 != D:
         raise RuntimeError(f"{op}: 4-bit key_pages and value_pages must be uint8 [P, Hkv, page_size, D / 2]")
     if key_scales is None or value_scales is None:
         raise RuntimeError(f"{op}: 4-bit pages need key_scales and value_scales")
-    want = (*shape[:3], 2 * D // U4_GROUP)
-    if tuple(key_scales.shape) != want or tuple(value_scales.shape) != want:
-        raise RuntimeError(f"{op}: scales of 4-bit pages must be [P, Hkv, page_size, {want[3]}] (a scale and an offset for every "
-                           f"{U4_GROUP} elements)")
-    if key_scales.dtype is not value_scales.dtype or key_scales.dtype not in (torch.float16, torch.bfloat16):
+    scales = key_scales.shape
+    if scales != (*shape[:3], 2 * D // U4_GROUP) or value_scales.shape != scales:
+        raise RuntimeError(f"{op}: scales of 4-bit pages must be [P, Hkv, page_size, {2 * D // U4_GROUP}] (a scale and an offset "
+                           f"for every {U4_GROUP} elements)")
+    dtype = key_scales.dtype
+    if dtype is not value_scales.dtype or (dtype is not torch.bfloat16 and dtype is not torch.float16):
         raise RuntimeError(f"{op}: scales of 4-bit pages must both be float16 or both bfloat16")
     if not (key_pages.is_contiguous() and value_pages.is_contiguous() and key_scales.is_contiguous()
             and value_scales.is_contiguous()):
         raise RuntimeError(f"{op}: 4-bit pages and their scales must be contiguous")
+
+
+def packed(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """x as contiguous numbers of a type; x itself where it is that already (two calls fewer, 1 us)."""
+    return x if x.dtype is dtype and x.is_contiguous() else x.to(dtype).contiguous()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

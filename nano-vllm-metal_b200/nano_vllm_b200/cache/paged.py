@@ -98,7 +98,7 @@ def read_slots(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.
     dev = nv.require_cuda(op, slots, key_pages, value_pages, key_scales, value_scales)
     if key_pages.dim() != 4 or key_pages.shape != value_pages.shape or key_pages.dtype is not value_pages.dtype:
         raise RuntimeError(f"{op}: key_pages and value_pages must be [P, H, page_size, D] of one dtype")
-    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+    if slots.dim() != 1 or (slots.dtype is not torch.int64 and slots.dtype is not torch.int32):
         raise RuntimeError(f"{op}: slots must be one row of int32 or int64")
     P, H, ps, D = key_pages.shape
     ks, vs = key_scales, value_scales
@@ -117,8 +117,8 @@ def read_slots(slots: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.
     if dtype is None:
         dtype = key_pages.dtype if ks is None else ks.dtype
     T = slots.shape[0]
-    key, value = (torch.empty((T, H, D), dtype=dtype, device=dev) for _ in range(2))
-    rows = slots.to(torch.int64).contiguous()
+    key, value = key_pages.new_empty((T, H, D), dtype=dtype), key_pages.new_empty((T, H, D), dtype=dtype)
+    rows = nv.packed(slots, torch.int64)
     with nv.on_device(dev):
         nv.check(nv.lib().nvm_read_slots(
             key_pages.data_ptr(), value_pages.data_ptr(), nv.dtype_code(key_pages.dtype), nv.ptr(ks), nv.ptr(vs),

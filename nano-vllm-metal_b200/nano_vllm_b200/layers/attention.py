@@ -150,7 +150,7 @@ def flash_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
 
 def _int32_rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+    return nv.packed(x, torch.int32)
 
 
 def _paged_attention_window(query, key_pages, value_pages, block_table, context_lens, page_size, key_scales, value_scales,
@@ -273,8 +273,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     q = query.contiguous()
     kp = key_pages.contiguous()
     vp = value_pages.contiguous()
-    bt = block_table.to(torch.int32).contiguous()
-    cl = context_lens.to(torch.int32).contiguous()
+    bt, cl = _int32_rows(block_table), _int32_rows(context_lens)
     if bt.dim() != 2 or cl.dim() != 1:
         raise RuntimeError("paged_attention: block_table must be 2D and context_lens must be 1D")
     if bt.shape[0] != cl.shape[0] or bt.shape[0] != B:
@@ -292,7 +291,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     elif kp.dtype is torch.uint8:
         ks, vs, sdt = key_scales, value_scales, nv.dtype_code(key_scales.dtype)
     if out is None:
-        out = torch.empty((B, Hq, L, D), dtype=out_dtype, device=dev)
+        out = q.new_empty((B, Hq, L, D), dtype=out_dtype)
     L_ = nv.lib()
     kvc = nv.dtype_code(kp.dtype)
     with nv.on_device(dev):

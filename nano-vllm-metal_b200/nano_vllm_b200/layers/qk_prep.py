@@ -21,8 +21,9 @@ def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     Views of a fused QKV projection ([B, L, (Hq + 2 Hkv) * D] split along the last
     axis) keep their token stride and are read without a copy."""
     B, L, H, D = x.shape
-    if x.stride(3) == 1 and x.stride(2) == D and (B == 1 or x.stride(0) == L * x.stride(1)) and x.stride(1) >= H * D:
-        return x, x.stride(1)
+    sb, st, sh, sd = x.stride()
+    if sd == 1 and sh == D and (B == 1 or sb == L * st) and st >= H * D:
+        return x, st
     return x.contiguous(), H * D
 
 
@@ -38,8 +39,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
     dtype, int8 or packed 4-bit codes (uint8 [P, Hkv, page_size, D / 2] with scales of q's
     dtype, see ``cache.paged.write_slots``).  Without norm weights (both None: models that
     have no q/k norm) the rows are rotated as they are."""
-    nv.require_cuda("qk_norm_rope_write", q, k, v, q_norm_weight, k_norm_weight, positions, key_pages, value_pages,
-                    slot_mapping)
+    dev = nv.require_cuda("qk_norm_rope_write", q, k, v, q_norm_weight, k_norm_weight, positions, key_pages, value_pages,
+                          slot_mapping, key_scales, value_scales, out)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise RuntimeError("qk_norm_rope_write: q must be [B, L, Hq, D], k and v [B, L, Hkv, D]")
     B, L, Hq, D = q.shape
@@ -61,11 +62,14 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
         raise RuntimeError("qk_norm_rope_write: q and k are normalised both or not at all")
     wq = wk = None
     if q_norm_weight is not None:
-        wq, wk = q_norm_weight.to(q.dtype).contiguous(), k_norm_weight.to(q.dtype).contiguous()
-    pos = positions.reshape(T).to(torch.int32).contiguous()
-    slots = slot_mapping.reshape(T).to(torch.int64).contiguous()
-    cos = rope.cos_freqs.to(q.device).contiguous()
-    sin = rope.sin_freqs.to(q.device).contiguous()
+        wq, wk = nv.packed(q_norm_weight, q.dtype), nv.packed(k_norm_weight, q.dtype)
+    if positions.numel() != T or slot_mapping.numel() != T:
+        raise RuntimeError("qk_norm_rope_write: positions and slot_mapping need one entry per token")
+    pos, slots = nv.packed(positions, torch.int32), nv.packed(slot_mapping, torch.int64)
+    cos, sin = rope.cos_freqs, rope.sin_freqs
+    if cos.device != dev or sin.device != dev:
+        cos, sin = cos.to(dev), sin.to(dev)
+    cos, sin = cos.contiguous(), sin.contiguous()
     kp, vp = key_pages, value_pages
     P, Hkv_p, ps, D_p = kp.shape
     int8, u4 = kp.dtype == torch.int8, kp.dtype == torch.uint8
@@ -73,8 +77,6 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
         raise RuntimeError("qk_norm_rope_write: page pools must be [P, Hkv, page_size, D] matching k")
     if not (kp.is_contiguous() and vp.is_contiguous()):
         raise RuntimeError("qk_norm_rope_write: page pools must be contiguous (written in place)")
-    if positions.numel() != T or slot_mapping.numel() != T:
-        raise RuntimeError("qk_norm_rope_write: positions and slot_mapping need one entry per token")
     if u4:
         nv.require_u4("qk_norm_rope_write", D, kp, vp, key_scales, value_scales)
         if key_scales.dtype != q.dtype:
@@ -88,16 +90,16 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
         if key_scales.dtype != value_scales.dtype:
             raise RuntimeError("qk_norm_rope_write: key and value scales must share one dtype")
     if out is None:
-        out = torch.empty((B, Hq, L, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, Hq, L, D))
     elif tuple(out.shape) != (B, Hq, L, D) or out.dtype != q.dtype or not out.is_contiguous():
         raise RuntimeError("qk_norm_rope_write: out must be a contiguous [B, Hq, L, D] tensor of q's dtype")
     ks = key_scales if int8 or u4 else None
     vs = value_scales if int8 or u4 else None
-    nv.check(nv.lib().nvm_qk_norm_rope_write(
-        qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, nv.ptr(wq),
-        nv.ptr(wk), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0,
-        pos.data_ptr(), out.data_ptr(), L, kp.data_ptr(), vp.data_ptr(), nv.dtype_code(kp.dtype),
-        ks.data_ptr() if ks is not None else None, vs.data_ptr() if vs is not None else None,
-        nv.dtype_code(ks.dtype) if ks is not None else nv.NVM_F16, slots.data_ptr(), T, Hq, Hkv, D, P, ps,
-        nv.stream_ptr(q.device)))
+    with nv.on_device(dev):
+        nv.check(nv.lib().nvm_qk_norm_rope_write(
+            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, nv.ptr(wq), nv.ptr(wk), eps,
+            cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0, pos.data_ptr(), out.data_ptr(), L,
+            kp.data_ptr(), vp.data_ptr(), nv.dtype_code(kp.dtype), nv.ptr(ks), nv.ptr(vs),
+            nv.dtype_code(ks.dtype) if ks is not None else nv.NVM_F16, slots.data_ptr(), T, Hq, Hkv, D, P, ps,
+            nv.stream_ptr(dev)))
     return out
