@@ -209,7 +209,7 @@ struct U4AppendArgs {
 };
 int launch_u4_append(const U4AppendArgs& a, cudaStream_t s);
 // Many query rows: pages unpacked into the workspace for the tcgen05 kernel (u4_prompt.cu).
-constexpr int64_t kU4PromptRows = 96;
+constexpr int64_t kU4PromptRows = 256;
 struct U4PromptPlan {
   bool eligible;
   int64_t batch;  // requests taken at a time

@@ -30,7 +30,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
 constexpr int kStages = 2;   // of each warp's own ring: one tile is copied while one is worked on
-constexpr int kBlocks1 = 4, kBlocks2 = 3;  // blocks an SM holds, of one or two tiles of rows
+constexpr int kBlocks1 = 4, kBlocks2 = 2;  // blocks an SM holds, of one or two tiles of rows
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
 constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of
 constexpr int kFan = 16;     // partial results that are joined at a time
@@ -95,6 +95,25 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two fp32 operations as one: d = a * b + c, d = a * b, d = a + b
+__device__ __forceinline__ void fma2(float a0, float a1, float b0, float b1, float c0, float c1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float a0, float a1, float b0, float b1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float a0, float a1, float b0, float b1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
 __device__ __forceinline__ float lg2(float x) {
   float y;
@@ -453,10 +472,14 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 4; e += 2) {
             const float s = e < 2 ? a.s[g] : d.s[g], z = e < 2 ? a.z[g] : d.z[g];
-            const float off = g == 0 ? z * qsum[j][e & 1][g] : fmaf(z, qsum[j][e & 1][g], x[mt][j][e]);
-            x[mt][j][e] = fmaf(s, dot[j][e], off);
+            float o0, o1;
+            if (g == 0)
+              mul2(z, z, qsum[j][0][g], qsum[j][1][g], o0, o1);
+            else
+              fma2(z, z, qsum[j][0][g], qsum[j][1][g], x[mt][j][e], x[mt][j][e + 1], o0, o1);
+            fma2(s, s, dot[j][e], dot[j][e + 1], o0, o1, x[mt][j][e], x[mt][j][e + 1]);
           }
       }
     }
@@ -487,9 +510,12 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[mt][j][e] = ex2(fmaf(kap[j][e & 1], x[mt][j][e], -M[j][e & 1]));
-          heavy = fmaxf(heavy, w[mt][j][e]);
+        for (int e = 0; e < 4; e += 2) {
+          float u0, u1;
+          fma2(kap[j][0], kap[j][1], x[mt][j][e], x[mt][j][e + 1], -M[j][0], -M[j][1], u0, u1);
+          w[mt][j][e] = ex2(u0);
+          w[mt][j][e + 1] = ex2(u1);
+          heavy = fmaxf(heavy, fmaxf(w[mt][j][e], w[mt][j][e + 1]));
         }
     if (__any_sync(0xffffffffu, heavy * size > kSlack)) {
 #pragma unroll
@@ -544,20 +570,19 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
             const float w0 = w[mt][j][2 * h], w1 = w[mt][j][2 * h + 1];
-            l[j][0] += w0;
-            l[j][1] += w1;
+            add2(l[j][0], l[j][1], w0, w1, l[j][0], l[j][1]);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               const float middle = fmaf(8.0f, v.s[g], v.z[g]);
-              float s0 = w0 * v.s[g], s1 = w1 * v.s[g];
+              float s0, s1;
+              mul2(w0, w1, v.s[g], v.s[g], s0, s1);
               if constexpr (decltype(hidden)::value) {
                 if (w0 == 0.0f) s0 = 0.0f;
                 if (w1 == 0.0f) s1 = 0.0f;
                 zsum[j][0][g] += w0 == 0.0f ? 0.0f : w0 * middle;
                 zsum[j][1][g] += w1 == 0.0f ? 0.0f : w1 * middle;
               } else {
-                zsum[j][0][g] = fmaf(w0, middle, zsum[j][0][g]);
-                zsum[j][1][g] = fmaf(w1, middle, zsum[j][1][g]);
+                fma2(w0, w1, middle, middle, zsum[j][0][g], zsum[j][1][g], zsum[j][0][g], zsum[j][1][g]);
               }
               pf[j][g][h] = transpose8x8(pack2<__half>(s0, s1));
             }

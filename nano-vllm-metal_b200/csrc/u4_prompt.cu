@@ -21,7 +21,8 @@ constexpr int kD = 128;
 constexpr int kThreads = 128;
 constexpr int kUnroll = 4;                            // keys of a thread
 constexpr int kKeys = kThreads / (kD / 8) * kUnroll;  // of a block
-constexpr int kSizeKeys = 2048;                       // keys of a block that looks at sizes
+constexpr int kSizeUnroll = 4;
+constexpr int kSizeKeys = 256 * kSizeUnroll;          // keys of a block that looks at sizes
 constexpr int kTarget = 4;  // values are brought below 2^(kTarget + 1)
 // Bytes that unpacked pages may take; larger batches are taken in parts.
 constexpr size_t kMostBytes = size_t(1) << 30;
@@ -43,7 +44,7 @@ struct PromptParams {
   FastDiv by_ps, by_heads, by_blocks;
   int B, Hq, Hkv, P, ps, mp, groups, blocks;  // blocks: of a (request, kv head)
   int64_t q_vectors, vectors_of_head;         // of eight elements, all of q's and those of a q head
-  int q_dtype;
+  int q_dtype, q_fast, q_blocks;              // q_fast: 16-bit vectors
   float q_scale;
 };
 
@@ -70,11 +71,21 @@ __global__ void __launch_bounds__(256) u4_sizes_kernel(const PromptParams p) {
   const int b = (int)p.by_heads((uint32_t)bh), h = bh - b * p.Hkv;
   const int keys = min(min(__ldg(p.context_lens + b), p.mp * p.ps), k0 + kSizeKeys);
   float mk = 0.0f, mv = 0.0f;
-  for (int key = k0 + threadIdx.x; key < keys; key += 256) {
-    const int64_t row = pool_row(p, b, h, key);
-    if (row < 0) continue;
-    mk = fmaxf(mk, size_of<T>(__ldg(reinterpret_cast<const uint2*>(p.ks) + row)));
-    mv = fmaxf(mv, size_of<T>(__ldg(reinterpret_cast<const uint2*>(p.vs) + row)));
+  uint2 pk[kSizeUnroll], pv[kSizeUnroll];
+#pragma unroll
+  for (int i = 0; i < kSizeUnroll; ++i) {
+    const int key = k0 + i * 256 + threadIdx.x;
+    const int64_t row = key < keys ? pool_row(p, b, h, key) : -1;
+    pk[i] = pv[i] = make_uint2(0, 0);
+    if (row >= 0) {
+      pk[i] = __ldg(reinterpret_cast<const uint2*>(p.ks) + row);
+      pv[i] = __ldg(reinterpret_cast<const uint2*>(p.vs) + row);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSizeUnroll; ++i) {
+    mk = fmaxf(mk, size_of<T>(pk[i]));
+    mv = fmaxf(mv, size_of<T>(pv[i]));
   }
   mk = warp_max(mk);
   mv = warp_max(mv);
@@ -103,11 +114,61 @@ __device__ __forceinline__ uint4 unpack8(uint32_t codes, uint32_t pair, float fa
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ __forceinline__ float into_half(float x) {  // NaN stays
+  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+}
+
+// q in f16, times the scale's power of two and what K was divided by: kUnroll vectors a thread
+__device__ __forceinline__ void take_queries(const PromptParams& p, int64_t block) {
+  const int64_t first = block * (kThreads * kUnroll) + threadIdx.x;
+  if (p.sizes != nullptr)
+    for (int64_t i = block * kThreads + threadIdx.x; i < (int64_t)p.B * p.Hkv; i += (int64_t)p.q_blocks * kThreads)
+      p.out_scale[i] = power_of_two(exponent_of(__ldcg(p.sizes + (int64_t)p.B * p.Hkv + i)) - kTarget);
+  uint4 raw[kUnroll];
+  if (p.q_fast) {
+#pragma unroll
+    for (int e = 0; e < kUnroll; ++e)
+      if (first + e * kThreads < p.q_vectors) raw[e] = __ldg(static_cast<const uint4*>(p.q) + first + e * kThreads);
+  }
+#pragma unroll
+  for (int e = 0; e < kUnroll; ++e) {
+    const int64_t i = first + e * kThreads;
+    if (i >= p.q_vectors) return;
+    float f = p.q_scale;
+    if (p.sizes != nullptr) {
+      const uint32_t head = (uint32_t)(i / p.vectors_of_head);  // b * Hq + q head: a kv head's are neighbours
+      f = fminf(f * power_of_two(exponent_of(__ldcg(p.sizes + head / (uint32_t)(p.Hq / p.Hkv))) - kTarget), 3.0e38f);
+    }
+    float x[8];
+    const uint32_t u[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (p.q_fast) {
+        const float2 v = p.q_dtype == NVM_BF16 ? u4_pair<__nv_bfloat16>(u[k]) : u4_pair<__half>(u[k]);
+        x[2 * k] = v.x;
+        x[2 * k + 1] = v.y;
+      } else {
+        x[2 * k] = load_dyn(p.q, i * 8 + 2 * k, p.q_dtype);
+        x[2 * k + 1] = load_dyn(p.q, i * 8 + 2 * k + 1, p.q_dtype);
+      }
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = pack2<__half>(into_half(x[2 * k] * f), into_half(x[2 * k + 1] * f));
+    reinterpret_cast<uint4*>(p.q16)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // Block (request, kv head, kKeys keys); rows from the context's end to that of its group of 16 are zero
-// (a weight of zero times what lies there).  The blocks of kv head 0 write the table of the groups.
+// (a weight of zero times what lies there).  The blocks of kv head 0 write the table of the groups, the
+// first q_blocks take the queries.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) u4_unpack_kernel(const PromptParams p) {
-  const int bh = (int)p.by_blocks(blockIdx.x), k0 = (blockIdx.x - bh * p.blocks) * kKeys;
+  if ((int)blockIdx.x < p.q_blocks) {
+    take_queries(p, blockIdx.x);
+    return;
+  }
+  const int block = blockIdx.x - p.q_blocks, bh = (int)p.by_blocks((uint32_t)block), k0 = (block - bh * p.blocks) * kKeys;
   const int b = (int)p.by_heads((uint32_t)bh), h = bh - b * p.Hkv;
   const int keys = max(min(__ldg(p.context_lens + b), p.mp * p.ps), 0);
   if (h == 0 && threadIdx.x < kKeys / 16) {
@@ -142,26 +203,6 @@ __global__ void __launch_bounds__(kThreads) u4_unpack_kernel(const PromptParams 
     reinterpret_cast<uint4*>(p.k16)[to] = unpack8<T>(codes[0][i], pairs[0][i], fk);
     reinterpret_cast<uint4*>(p.v16)[to] = unpack8<T>(codes[1][i], pairs[1][i], fv);
   }
-}
-
-__device__ __forceinline__ float into_half(float x) {  // NaN stays
-  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
-}
-
-// q in f16, times the scale's power of two and what K was divided by
-__global__ void __launch_bounds__(256) u4_queries_kernel(const PromptParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (p.sizes != nullptr && i < (int64_t)p.B * p.Hkv)
-    p.out_scale[i] = power_of_two(exponent_of(__ldcg(p.sizes + (int64_t)p.B * p.Hkv + i)) - kTarget);
-  if (i >= p.q_vectors) return;
-  const uint32_t head = (uint32_t)(i / p.vectors_of_head);  // b * Hq + q head: a kv head's are neighbours
-  float f = p.q_scale;
-  if (p.sizes != nullptr) f = fminf(f * power_of_two(exponent_of(__ldcg(p.sizes + head / (uint32_t)(p.Hq / p.Hkv))) - kTarget), 3.0e38f);
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    w[e] = pack2<__half>(into_half(load_dyn(p.q, i * 8 + 2 * e, p.q_dtype) * f), into_half(load_dyn(p.q, i * 8 + 2 * e + 1, p.q_dtype) * f));
-  reinterpret_cast<uint4*>(p.q16)[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -213,11 +254,11 @@ U4PromptPlan plan_u4_prompt(const PagedArgs& a) {
   const int64_t one = std::max<int64_t>(a.max_pages * a.page_size * a.Hkv * kD * 4, 1);
   const int64_t parts = (a.B * one + (int64_t)kMostBytes - 1) / (int64_t)kMostBytes;
   x.B = std::max<int64_t>((a.B + parts - 1) / parts, 1);
-  for (; x.B > 1 && (x.B * x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX || x.B * x.Hq * x.L > INT32_MAX);)
+  for (; x.B > 1 && (x.B * x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX / 2 || x.B * x.Hq * x.L > INT32_MAX / 2);)
     x.B = (x.B + 1) / 2;
   const Layout none = layout_of(x, 0);
   const PagedArgs inner = unpacked(x, none, nullptr);
-  if (x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX) return plan;
+  if (x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX / 2) return plan;
   const Sm100Plan attention = plan_sm100(inner, true);
   if (!attention.eligible) return plan;
   plan.attention_bytes = attention.ws_bytes;
@@ -282,19 +323,17 @@ int launch_u4_prompt(const PagedArgs& a, const U4PromptPlan& plan, void* workspa
     }
     p.blocks = (int)((keys + kKeys - 1) / kKeys);
     p.by_blocks = FastDiv(p.blocks);
-    const unsigned grid = (unsigned)(x.B * a.Hkv * p.blocks);
-    bf ? u4_unpack_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p) : u4_unpack_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-    int st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit unpack kernel launch");
-    if (st != NVM_OK) return st;
     if (copied) {
-      const int64_t n = std::max(p.q_vectors, sized ? x.B * a.Hkv : (int64_t)0);
-      u4_queries_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
-      st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit queries kernel launch");
-      if (st != NVM_OK) return st;
+      p.q_fast = a.q_dtype != NVM_F32 && (uintptr_t)x.q % 16 == 0;
+      p.q_blocks = (int)((p.q_vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll));
       y.q = p.q16;
       y.scale = mantissa;
       y.out_scale = sized ? p.out_scale : nullptr;
     }
+    const unsigned grid = (unsigned)(x.B * a.Hkv * p.blocks + p.q_blocks);
+    bf ? u4_unpack_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p) : u4_unpack_kernel<__half><<<grid, kThreads, 0, s>>>(p);
+    int st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit unpack kernel launch");
+    if (st != NVM_OK) return st;
     const Sm100Plan sp = plan_sm100(y, false);
     if (!sp.eligible || sp.ws_bytes > w.k) return fail(NVM_ERR_UNSUPPORTED, "paged_attention: 4-bit prompt plan");
     st = launch_sm100(y, sp, workspace, s);

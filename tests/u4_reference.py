@@ -62,7 +62,7 @@ def parts64(packed, scales):
 
 def unpacked(rows, D, ps, scale):
     """Whether a call of so many query rows a kv head goes through unpacked pages."""
-    return rows >= 96 and D == 128 and ps % 16 == 0 and scale > 0
+    return rows >= 256 and D == 128 and ps % 16 == 0 and scale > 0
 
 
 def attend64(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
