@@ -187,14 +187,14 @@ struct Rot {
   float c[kAngles], s[kAngles];
 };
 
-// RMSNorm (with `norm`) then RoPE of up to eight head rows (rows [h0, min(h0 + 8, count)) of one kind
+// RMSNorm (kNorm) then RoPE of up to eight head rows (rows [h0, min(h0 + 8, count)) of one kind
 // for one token), written by `emit(i, h, lo_bits, hi_bits)` (int8 pools: by quantising).
 // Loads of the eight rows are issued first; the eight sums of squares are reduced
 // together and 1 / sqrt(mean + eps) is evaluated once per row by the lanes that hold it.
-template <typename T, int D, bool kTrad, typename Emit>
+template <typename T, int D, bool kTrad, bool kNorm, typename Emit>
 __device__ __forceinline__ void norm_rope_batch(const T* src_tok, int h0, int count, typename Lane<T, D>::V w_lo,
                                                 typename Lane<T, D>::V w_hi, const Rot<D, kTrad>& rot, float eps,
-                                                bool norm, int lane, Emit&& emit) {
+                                                int lane, Emit&& emit) {
   using L = Lane<T, D>;
   using V = typename L::V;
   constexpr int EH = L::EH;
@@ -211,7 +211,7 @@ __device__ __forceinline__ void norm_rope_batch(const T* src_tok, int h0, int co
     }
   }
   float inv_mine = 1.0f;
-  if (norm) {
+  if constexpr (kNorm) {
     float red[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -238,7 +238,7 @@ __device__ __forceinline__ void norm_rope_batch(const T* src_tok, int h0, int co
     unpack<T, EH>(rlo[i], x);
     unpack<T, EH>(rhi[i], x + EH);
     // normalised value rounded to T (pairs converted together)
-    if (norm) {
+    if constexpr (kNorm) {
 #pragma unroll
       for (int e = 0; e < 2 * EH; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], inv), w[e]);
       unpack<T, EH>(pack<T, EH, V>(x), x);
@@ -317,7 +317,7 @@ __device__ __forceinline__ void quantize_batch(const typename Lane<T, D>::V (&rl
 // A unit reads the token's position and slot and its lanes' cos/sin entries once, then
 // runs its batches of eight rows of one kind.  Rows whose result is not needed (q/k
 // rows at a bad position, k/v rows of a skipped or bad slot) are not read.
-template <typename T, int D, bool kTrad, bool kInt8>
+template <typename T, int D, bool kTrad, bool kInt8, bool kNorm>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(const QkPrepParams p) {
   using L = Lane<T, D>;
   using V = typename L::V;
@@ -330,9 +330,8 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
   const int lo = lane * EH, hi = kHalf + lane * EH;  // first element of each half
   const int64_t pool_head = p.ps * D;                 // elements between kv heads of a page
   // norm weights of the lane's elements, kept packed; none: rows are rotated as they are
-  const bool norm = p.wq != nullptr;
   V wq_lo = 0, wq_hi = 0, wk_lo = 0, wk_hi = 0;
-  if (norm) {
+  if constexpr (kNorm) {
     wq_lo = __ldg(reinterpret_cast<const V*>(static_cast<const T*>(p.wq) + lo));
     wq_hi = __ldg(reinterpret_cast<const V*>(static_cast<const T*>(p.wq) + hi));
     wk_lo = __ldg(reinterpret_cast<const V*>(static_cast<const T*>(p.wk) + lo));
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
       const T* q_tok = static_cast<const T*>(p.q) + t * p.q_st;
       const int e_end = min(b_end, nbq);
       for (int bt = b_begin; bt < e_end; ++bt) {
-        norm_rope_batch<T, D, kTrad>(q_tok, bt * kBatch, Hq, wq_lo, wq_hi, rot, p.eps, norm, lane,
+        norm_rope_batch<T, D, kTrad, kNorm>(q_tok, bt * kBatch, Hq, wq_lo, wq_hi, rot, p.eps, lane,
                                      [&](int, int h, V ylo, V yhi) {
                                        T* dst = q_out + (int64_t)h * q_mul * D;
                                        *reinterpret_cast<V*>(dst + lo) = ylo;
@@ -430,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
           V qlo[kBatch], qhi[kBatch];
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) qlo[i] = qhi[i] = 0;
-          norm_rope_batch<T, D, kTrad>(k_tok, h0, Hkv, wk_lo, wk_hi, rot, p.eps, norm, lane, [&](int i, int, V ylo, V yhi) {
+          norm_rope_batch<T, D, kTrad, kNorm>(k_tok, h0, Hkv, wk_lo, wk_hi, rot, p.eps, lane, [&](int i, int, V ylo, V yhi) {
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
               if (j == i) {
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
                                p.scale_dtype, lane);
         } else {
           T* k_row0 = static_cast<T*>(p.kp) + prow0 * D;
-          norm_rope_batch<T, D, kTrad>(k_tok, h0, Hkv, wk_lo, wk_hi, rot, p.eps, norm, lane, [&](int, int h, V ylo, V yhi) {
+          norm_rope_batch<T, D, kTrad, kNorm>(k_tok, h0, Hkv, wk_lo, wk_hi, rot, p.eps, lane, [&](int, int h, V ylo, V yhi) {
             T* dst = k_row0 + (int64_t)h * pool_head;
             *reinterpret_cast<V*>(dst + lo) = ylo;
             *reinterpret_cast<V*>(dst + hi) = yhi;
@@ -486,7 +485,10 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_prep_kernel(cons
 
 template <typename T, int D, bool kTrad, bool kInt8>
 void launch_one(const QkPrepParams& p, unsigned grid, cudaStream_t s) {
-  qk_prep_kernel<T, D, kTrad, kInt8><<<grid, kWarps * 32, 0, s>>>(p);
+  if (p.wq != nullptr)
+    qk_prep_kernel<T, D, kTrad, kInt8, true><<<grid, kWarps * 32, 0, s>>>(p);
+  else
+    qk_prep_kernel<T, D, kTrad, kInt8, false><<<grid, kWarps * 32, 0, s>>>(p);
 }
 
 template <typename T>
