@@ -58,9 +58,9 @@ __device__ __forceinline__ uint2 pack4(const float* x) {
 }
 
 // Steps [0, n) of a warp's rows of one kind (a step is kRows heads, the lane's at `head` and up): rotated
-// (with `w`, normalised first), then stored at dst + step * dst_step or quantised into the rows at
+// (kNorm: normalised first, with weights w), then stored at dst + step * dst_step or quantised into the rows at
 // pool_row + step * pool_step of codes / scales.
-template <typename T, int D, bool kTrad, bool kRope, bool kQuant>
+template <typename T, int D, bool kTrad, bool kRope, bool kQuant, bool kNorm>
 __device__ __forceinline__ void walk(const T* src, int head, int heads, int n, const uint2* w, float eps, const float (&c)[4],
                                      const float (&sn)[4], T* dst, int64_t dst_step, uint8_t* codes, uint32_t* scales,
                                      int64_t pool_row, int64_t pool_step, int j) {
@@ -77,7 +77,7 @@ __device__ __forceinline__ void walk(const T* src, int head, int heads, int n, c
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) load(i, lo[i], hi[i]);
   uint2 w_lo = make_uint2(0, 0), w_hi = w_lo;
-  if (kRope && w != nullptr) {
+  if (kNorm) {
     w_lo = __ldg(w + j);
     w_hi = __ldg(w + kHalf / 4 + j);
   }
@@ -94,7 +94,7 @@ __device__ __forceinline__ void walk(const T* src, int head, int heads, int n, c
     load(i + kAhead, lo[kAhead - 1], hi[kAhead - 1]);
     const bool mine = head + i * kRows < heads;
     if constexpr (kRope) {
-      if (w != nullptr) {
+      if constexpr (kNorm) {
         // the order of qk_prep.cu: its lane l holds elements l * D/64 and up of both halves, and sums over
         // lanes l ^ 16, 8, 4, 2, 1; two (D = 128) or four of its lanes are one here
         float part[4];
@@ -200,7 +200,7 @@ __device__ __forceinline__ void walk(const T* src, int head, int heads, int n, c
   }
 }
 
-template <typename T, int D, bool kTrad>
+template <typename T, int D, bool kTrad, bool kNorm>
 __global__ void __launch_bounds__(kWarps * 32, kBlocks) u4_append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes, kHalf = D / 2;  // lanes of a row, rows of a step
   const int lane = threadIdx.x & 31, j = lane % kLanes, sub = lane / kLanes;
@@ -262,25 +262,26 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocks) u4_append_kernel(const A
       row = ((int64_t)bb * p.Hq + head) * p.q_out_L + (t - bb * (int)p.q_out_L);
       mul = p.q_out_L;
     }
-    walk<T, D, kTrad, true, false>(static_cast<const T*>(p.q) + first, head, heads, n, static_cast<const uint2*>(p.wq), p.eps, c, sn,
+    walk<T, D, kTrad, true, false, kNorm>(static_cast<const T*>(p.q) + first, head, heads, n, static_cast<const uint2*>(p.wq), p.eps, c, sn,
                                    static_cast<T*>(p.q_out) + row * D, mul * (kRows * D), nullptr, nullptr, 0, 0, j);
     return;
   }
   const int64_t row = (pid * p.Hkv + head) * p.ps + off, step = kRows * p.ps;
   if (kind == 1)
-    walk<T, D, kTrad, true, true>(static_cast<const T*>(p.k) + first, head, heads, n, static_cast<const uint2*>(p.wk), p.eps, c, sn,
+    walk<T, D, kTrad, true, true, kNorm>(static_cast<const T*>(p.k) + first, head, heads, n, static_cast<const uint2*>(p.wk), p.eps, c, sn,
                                   nullptr, 0, p.kp, static_cast<uint32_t*>(p.ks), row, step, j);
   else
-    walk<T, D, kTrad, false, true>(static_cast<const T*>(p.v) + first, head, heads, n, nullptr, p.eps, c, sn, nullptr, 0, p.vp,
+    walk<T, D, kTrad, false, true, false>(static_cast<const T*>(p.v) + first, head, heads, n, nullptr, p.eps, c, sn, nullptr, 0, p.vp,
                                    static_cast<uint32_t*>(p.vs), row, step, j);
 }
 
 template <typename T, int D>
 void launch(const AppendParams& p, bool traditional, unsigned grid, cudaStream_t s) {
+  const bool norm = p.wq != nullptr;
   if (traditional)
-    u4_append_kernel<T, D, true><<<grid, kWarps * 32, 0, s>>>(p);
+    norm ? u4_append_kernel<T, D, true, true><<<grid, kWarps * 32, 0, s>>>(p) : u4_append_kernel<T, D, true, false><<<grid, kWarps * 32, 0, s>>>(p);
   else
-    u4_append_kernel<T, D, false><<<grid, kWarps * 32, 0, s>>>(p);
+    norm ? u4_append_kernel<T, D, false, true><<<grid, kWarps * 32, 0, s>>>(p) : u4_append_kernel<T, D, false, false><<<grid, kWarps * 32, 0, s>>>(p);
 }
 
 }  // namespace
