@@ -523,3 +523,187 @@ def test_a_generation_over_the_device_table(cuda):
         at += L - back
     table.check_status()
     assert nv.device_error(torch.device("cuda:0")) == 0
+
+
+# ---------------------------------------------------------------------------
+# calls in company, odd addresses, large pools
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("L", [1, 5, 70])
+@pytest.mark.parametrize("qdt", [BF, HF, FF])
+def test_odd_addresses(cuda, L, qdt):
+    """Queries and outputs that start on no vector's boundary."""
+    gen = torch.Generator().manual_seed(21)
+    P, bt, cl = random_table(gen, [L, 100 + L], 16)
+    kp, vp, ks, vs = random_pools(gen, P, 2, 16, 128, HF if qdt == HF else BF)
+    n = 2 * 8 * L * 128
+    q = torch.randn(n + 3, generator=gen).to(qdt).cuda()[3:].view(2, 8, L, 128)
+    out = torch.zeros(n + 5, dtype=qdt, device="cuda")[5:].view(2, 8, L, 128)
+    want = attend64(q, kp, vp, ks, vs, bt, cl, 16)
+    _close(lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal", out_dtype=qdt), *want)
+    lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal", out=out)
+    _close(out, *want)
+
+
+@pytest.mark.parametrize("sdt", [BF, HF])
+def test_captured_prompts(cuda, sdt):
+    """Prompts captured into graphs, replayed on new queries, pages and lengths beside one another."""
+    gen = torch.Generator().manual_seed(22)
+
+    def problem(lens, L):
+        P, bt, cl = random_table(gen, lens, 16, width=40)
+        return [torch.randn(len(lens), 8, L, 128, generator=gen).to(sdt).cuda(), *random_pools(gen, P, 2, 16, 128, sdt), bt, cl]
+
+    def call(x):
+        q, kp, vp, ks, vs, bt, cl = x
+        return lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal", out_dtype=sdt)
+
+    problems = [problem([200, 90], 70), problem([600], 300)]
+    [call(x) for x in problems]
+    graphs, outs = [], []
+    for x in problems:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(x))
+        graphs.append(g)
+    call(problem([630, 600, 500, 400], 128))
+    for x, n in zip(problems, (150, 333)):
+        x[0].copy_(torch.randn(x[0].shape, generator=gen).to(sdt))
+        x[3].mul_(1.5)
+        x[6][-1] = n
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for x, o in zip(problems, outs):
+        q, kp, vp, ks, vs, bt, cl = x
+        _close(o, *attend64(q, kp, vp, ks, vs, bt, cl, 16))
+
+
+def test_one_workspace_for_every_kind_of_call(cuda):
+    """4-bit, 16-bit and scored calls take turns over a stream's workspace: what each leaves, the next finds."""
+    gen = torch.Generator().manual_seed(23)
+    P, bt, cl = random_table(gen, [2500, 700], 16)
+    kp, vp, ks, vs = random_pools(gen, P, 2, 16, 128, BF)
+    k16, v16 = (torch.randn(P, 2, 16, 128, generator=gen).to(BF).cuda() for _ in range(2))
+    mass = torch.zeros(2, 2, bt.shape[1] * 16, device="cuda")
+    calls = []
+    for L in (1, 5, 70):
+        q = torch.randn(2, 8, L, 128, generator=gen).to(BF).cuda()
+        calls += [lambda q=q: lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal"),
+                  lambda q=q: lib.paged_attention(q, k16, v16, bt, cl, 16, mask="causal")]
+    calls.append(lambda: lib.paged_attention(q[:, :, :1].contiguous(), k16, v16, bt, cl, 16, mask="causal", key_mass=mass))
+    alone = [c() for c in calls]
+    for order in range(3):
+        for i in torch.randperm(len(calls), generator=gen).tolist():
+            assert torch.equal(calls[i](), alone[i]), (order, i)
+
+
+def test_threads_on_one_stream(cuda):
+    import threading
+
+    gen = torch.Generator().manual_seed(24)
+    P, bt, cl = random_table(gen, [3000, 2000], 16)
+    kp, vp, ks, vs = random_pools(gen, P, 2, 16, 128, BF)
+    qs = [torch.randn(2, 8, L, 128, generator=gen).to(BF).cuda() for L in (1, 1, 3, 70)]
+    call = lambda q: lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal")  # noqa: E731
+    want, bad = [call(q) for q in qs], []
+
+    def work(i):
+        for _ in range(20):
+            if not torch.equal(call(qs[i]), want[i]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_wide_tables_taken_in_parts(cuda):
+    """Tables a million pages wide: the batch is taken in parts, whose requests are found by their own rows."""
+    gen = torch.Generator().manual_seed(25)
+    B, L, ps, D = 9, 64, 1024, 64
+    lens = [64, 100, 65, 1030, 70, 2000, 64, 90, 1500]
+    P, bt, cl = random_table(gen, lens, ps, width=1 << 20)
+    kp, vp, ks, vs = random_pools(gen, P, 2, ps, D, HF)
+    q = torch.randn(B, 8, L, D, generator=gen).to(HF).cuda()
+    got = lib.paged_attention(q, kp, vp, bt, cl, ps, ks, vs, mask="causal", out_dtype=HF)
+    _close(got, *attend64(q, kp, vp, ks, vs, bt, cl, ps))
+
+
+def test_pools_past_four_gigabytes(cuda):
+    """Rows behind 2^32 bytes and 2^31 elements: append, read back, attention of one token and of many."""
+    gen = torch.Generator().manual_seed(26)
+    P, Hkv, ps, D, n = 40000, 8, 256, 128, 700
+    kp, vp = (torch.empty(P, Hkv, ps, D // 2, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(P, Hkv, ps, 4, dtype=BF, device="cuda") for _ in range(2))
+    bt = torch.tensor([[P - 1, P - 5, P - 2]], dtype=torch.int32, device="cuda")
+    cl = torch.tensor([n], dtype=torch.int32, device="cuda")
+    key = torch.arange(n, device="cuda")
+    slots = bt[0].long()[key // ps] * ps + key % ps
+    q, k, v = (torch.randn(1, n, h, D, generator=gen).to(BF).cuda() for h in (32, Hkv, Hkv))
+    rope = RoPE(D, n, device="cuda")
+    rq = qk_norm_rope_write(q, k, v, None, None, rope, key.int()[None], kp, vp, slots, key_scales=ks, value_scales=vs)
+    at = bt[0].long()
+    small = [x[at].contiguous() for x in (kp, vp, ks, vs)]
+    near = torch.arange(3, dtype=torch.int32, device="cuda")[None]
+    gk, gv = lib.read_slots(slots, kp, vp, ks, vs)
+    wk, wv = lib.read_slots(key, *small)
+    assert torch.equal(gk, wk) and torch.equal(gv, wv) and (gv.float() - v[0].float()).abs().max() < 0.5
+    for L in (1, 3, n):
+        x = rq[:, :, n - L:].contiguous()
+        far = lib.paged_attention(x, kp, vp, bt, cl, ps, ks, vs, mask="causal", out_dtype=BF)
+        assert torch.equal(far, lib.paged_attention(x, *small[:2], near, cl, ps, *small[2:], mask="causal", out_dtype=BF))
+    lib.write_slots(v[0], k[0], slots, kp, vp, ks, vs)
+    assert torch.equal(lib.read_slots(slots, kp, vp, ks, vs)[0], gv)
+
+
+def test_positions_and_slots_out_of_range(cuda):
+    """Bad positions and slots are skipped and show in the device error word; nothing else is touched."""
+    dev = torch.device("cuda:0")
+    nv.device_error(dev)
+    B, L, Hq, Hkv, D, ps, P = 1, 5, 4, 2, 128, 8, 2
+    q, k, v = (torch.randn(B, L, h, D, device="cuda").to(BF) for h in (Hq, Hkv, Hkv))
+    rope = RoPE(D, 16, device="cuda")
+    pos = torch.tensor([[0, 16, -1, 3, 4]], dtype=torch.int32, device="cuda")
+    slots = torch.tensor([3, 4, 5, P * ps, -7], device="cuda")
+    pools = _empty_pools(P, Hkv, ps, D, BF)
+    out = torch.full((B, Hq, L, D), 9.0, dtype=BF, device="cuda")
+    qk_norm_rope_write(q, k, v, None, None, rope, pos, *pools[:2], slots, key_scales=pools[2], value_scales=pools[3], out=out)
+    assert nv.device_error(dev) == 7 and nv.device_error(dev) == 0
+    good = [0, 3, 4]
+    assert torch.equal(out[0, :, good], rope.apply(q, pos.clamp(0, 15))[0, good].transpose(0, 1)) and (out[0, :, 1:3] == 9).all()
+    before = [t.cpu() for t in _empty_pools(P, Hkv, ps, D, BF)]
+    keys, _ = _expect_rows(rope.apply(k, pos.clamp(0, 15))[0, :1], slots[:1], before[0], before[2], ps)
+    values, _ = _expect_rows(v[0, :3], slots[:3], before[1], before[3], ps)
+    assert torch.equal(pools[0].cpu(), keys) and torch.equal(pools[1].cpu(), values)
+
+
+def test_entry_point_without_a_workspace(cuda):
+    gen = torch.Generator().manual_seed(27)
+    P, bt, cl = random_table(gen, [900, 60], 16)
+    kp, vp, ks, vs = random_pools(gen, P, 2, 16, 128, BF)
+    for L in (1, 5):
+        q = torch.randn(2, 8, L, 128, generator=gen).to(BF).cuda()
+        out = torch.empty_like(q)
+        nv.check(nv.lib().nvm_paged_attention_noalloc(
+            q.data_ptr(), 2, kp.data_ptr(), vp.data_ptr(), nv.NVM_U4, ks.data_ptr(), vs.data_ptr(), 2, bt.data_ptr(),
+            cl.data_ptr(), out.data_ptr(), 2, 2, 8, 2, L, 128, P, 16, bt.shape[1], 128 ** -0.5, 1, nv.stream_ptr(cuda)))
+        assert torch.equal(out, lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal", out_dtype=BF))
+
+
+def test_nan_queries_stay_in_their_rows(cuda):
+    gen = torch.Generator().manual_seed(28)
+    P, bt, cl = random_table(gen, [300], 16)
+    kp, vp, ks, vs = random_pools(gen, P, 2, 16, 128, BF)
+    for L in (1, 4):
+        q = torch.randn(1, 8, L, 128, generator=gen).to(BF).cuda()
+        clean = lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal")
+        q[0, 2, 0, 5], q[0, 5, L - 1, 7] = float("nan"), float("inf")
+        got = lib.paged_attention(q, kp, vp, bt, cl, 16, ks, vs, mask="causal")
+        bad = torch.zeros(1, 8, L, dtype=torch.bool, device="cuda")
+        bad[0, 2, 0], bad[0, 5, L - 1] = True, True
+        assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])

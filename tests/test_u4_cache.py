@@ -204,3 +204,17 @@ def test_c_entry_points_refuse():
     assert prep(sdt=1) == -1 and prep(ks=None) == -1 and prep(ks=4) == -1
 
 
+
+
+def test_quotient_by_fifteen_is_rounded_as_the_division():
+    """The kernels' over15 restated, for every fp32 mantissa (the exponent only shifts both): with y = fl(1/15)
+    and q = fl(x y), fl(fl(x - 15 q) y + q) is fl(x / 15).  x - 15 q is exact in 64 bits; the last step is an
+    addition of numbers 2^20 apart, whose 64-bit sum is rounded to fp32 unless it is a tie of that rounding,
+    and those are none (an exact tie of x / 15 would need 15 to divide a power of two)."""
+    y = np.float32(1) / np.float32(15)
+    m = np.arange(1 << 23, 1 << 24, dtype=np.int64)
+    x = m.astype(np.float32)
+    q = x * y
+    r = (x.astype(np.float64) - 15.0 * q.astype(np.float64)).astype(np.float32)
+    got = (r.astype(np.float64) * np.float64(y) + q.astype(np.float64)).astype(np.float32)
+    assert np.array_equal(got, x / np.float32(15))
