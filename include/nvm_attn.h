@@ -2,7 +2,7 @@
  * nvm_attn.h -- C ABI of libnvm_attn.so, the B200 (sm_100a) attention hot path of
  * nano-vllm-metal: paged-attention decode / multi-query, dense flash attention,
  * the paged KV scatter-write (with int8 quantise-on-write), device-side page
- * allocation for a batch of appends, and the fused per-layer q/k RMSNorm + RoPE +
+ * allocation for a batch of appends, a cache in 4 bits, and the fused per-layer q/k RMSNorm + RoPE +
  * K/V write that precedes every attention call, the 4-bit (W4A16) matmul of the
  * projections around it, and what keeps a long generation's cache bounded: a sliding
  * window with sinks, accumulated attention weights, eviction by them.
@@ -141,6 +141,8 @@ int nvm_selftest_wait_expiry(int64_t limit_ns, unsigned long long* waited_ns, vo
  *              filled before the first use and every successful call leaves it
  *              zero again, so one workspace serves calls of any shape; the rest
  *              is overwritten by every call.  May be NULL if the size is 0.
+ *              4-bit pages need one for every call, on a 16-byte boundary; from 256 query
+ *              rows a kv head it holds the unpacked pages, up to 1 GiB (or one request's).
  *              Calls that share one workspace must not overlap on the GPU, nor on the
  *              host: a call may launch several kernels, so two host threads on one
  *              stream have to take turns.
@@ -312,7 +314,8 @@ int nvm_flash_attention(const void* q, const void* k, const void* v, int dtype, 
  *
  * k, v         token t, head h element d at k[t*stride_t + h*stride_h + d]
  *              (element strides; d is contiguous), of in_dtype (F32/F16/BF16).
- * slot_mapping [T] int64: slot = page_id*page_size + offset, or < 0 to skip.
+ * slot_mapping [T] int64: slot = page_id*page_size + offset, or < 0 to skip; no two
+ *              tokens of a call may have the same.
  * k_pages,
  * v_pages      [P, Hkv, page_size, D] of kv_dtype.  kv_dtype == in_dtype copies the
  *              bits; kv_dtype == NVM_I8 quantises each (token, head) row:

@@ -18,6 +18,13 @@
 // the largest weight: f16 then holds what matters to 11 bits however small the values of the keys
 // that are attended to.  M moves only where a contribution passes it by kSlack, which one vote over the
 // largest weight and the largest scale of a tile finds.  Sums of weights and of p z' are fp32.
+//
+// The floor of a decode step is HBM: 144 bytes a key and kv head (D = 128).  64 requests of 2K-16K keys, 32/8
+// heads, take 128 us, 0.80 of a copy's rate (48 of 4K-12K, 64/8 heads, f16: 96 us, 0.71).  What bounds it is
+// the latency of the instructions: about 450 a tile of 32 keys and warp (unpacking 160, weights and sums
+// 180, matrix instructions 36, copies 60), 16 warps an SM at 127 registers, issue slots 54 % busy.  Twelve
+// warps took 145 us; twenty spill.  Tiles come by 16-byte asynchronous copies, a ring to each warp, so that no
+// warp waits for another inside a unit; a third or fourth stage gained nothing (137, 145 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -27,13 +34,13 @@
 namespace nvm {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;    // 2 or 8: one request 13.6 or 11.3 us for 11.3, 64 requests 132 or 146 for 136
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
 constexpr int kStages = 2;   // of each warp's own ring: one tile is copied while one is worked on
-constexpr int kBlocks1 = 4, kBlocks2 = 2;  // blocks an SM holds, of one or two tiles of rows
+constexpr int kBlocks1 = 4, kBlocks2 = 2;  // blocks an SM holds, of one or two tiles of rows (3 of two: spills, 93 us for 90)
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
-constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of
-constexpr int kFan = 16;     // partial results that are joined at a time
+constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of (0: 64 requests 136 us for 126; 6: 129)
+constexpr int kFan = 16;     // partial results that are joined at a time (one request of 90K-130K keys: 8 31, 16 29.5, 40 33 us)
 constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
 constexpr float kLeast = 0x1p-80f;  // least scale that a key's values count as
 constexpr float kNoKeys = -1e30f;  // M of a row that has seen no key

@@ -4,11 +4,12 @@
 // The same operator as qk_prep.cu over another kind of pages, with its rounding points and, for the
 // norm, its order of summation, so that q and the rows handed to the quantiser are bit for bit those
 // that 16-bit pages would get.  A lane holds four neighbouring elements of each half of a row (8-byte
-// vectors), so a warp works on 256 / D rows at once, all q, all k or all v: a group's extremes are
-// three or four shuffles away, a lane's codes of a half are 16 bits, and half the instructions an
-// element of the 32-lane rows that qk_prep.cu's other kinds use are left (8192 tokens, 32/8 heads, bf16:
-// 68 us with those).  A warp walks such steps of one token with the loads of the next kAhead in flight; few
-// tokens are spread over more warps, down to one step each.
+// vectors), so a warp works on 256 / D rows at once: a group's extremes are three or four shuffles away and
+// a lane's codes of a half are 16 bits.  A warp walks rows of one kind of one token, all q, all k or all v,
+// with the loads of the next kAhead steps in flight; few tokens are spread over more warps, down to one
+// step each.  Bound by HBM (22 KB a token, 32/8 heads) as far as issue allows: 8192 tokens, bf16, 47.5 us
+// without a norm (3.8 TB/s, issue slots 71 % busy) and 57 with one; one token 3.1 us.  In qk_prep.cu's
+// layout (a row over 32 lanes, eight rows unrolled) the same took 68, 86 and 6.1 us.
 #include <algorithm>
 
 #include "nvm_internal.h"
@@ -18,8 +19,8 @@ namespace nvm {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kBlocks = 4;  // of an SM
-constexpr int kMost = 8;   // steps of a warp
+constexpr int kBlocks = 4;  // of an SM (3: 56 us, 5: 52, which spills)
+constexpr int kMost = 8;   // steps of a warp (4: 55 us, 16: 60)
 constexpr int kAhead = 4;  // steps whose loads are in flight
 
 struct AppendParams {

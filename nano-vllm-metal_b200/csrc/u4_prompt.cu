@@ -3,7 +3,9 @@
 //
 // A row block of paged_u4.cu unpacks the keys that it sees for itself, which costs it more than the
 // matrix instructions do once a kv head has many blocks; here a key is unpacked once for all of them and
-// the tensor cores run from TMA tiles (4 x 512 tokens against 2K-8K keys, 32/8 heads: 885 us in row blocks).
+// the tensor cores run from TMA tiles: 4 x 512 tokens against 2K-8K keys, 32/8 heads, take 247 us, 200 of
+// them the tcgen05 kernel's (885 us in row blocks).  Calls of fewer rows a kv head stay with the row blocks
+// (kU4PromptRows has both sides).
 // Values of bfloat16 range are brought into f16 by a power of two for every (request, kv head): K's goes
 // into the queries together with the softmax scale's power of two, V's into the output; f16 then rounds
 // them to 11 bits, eight times finer than bfloat16 would.  The unpacking is bound by HBM (144 bytes in,

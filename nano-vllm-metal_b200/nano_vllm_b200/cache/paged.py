@@ -9,7 +9,8 @@
   ``reserve_pages`` optionally pre-allocates HBM for that many pages so growth
   becomes a view change instead of a reallocate + copy.
 * Writes go through one ``nvm_reshape_and_cache`` launch per append (all pages of
-  the chunk at once), in place; int8 quantisation happens in that kernel.
+  the chunk at once), in place; int8 and 4-bit quantisation happen in that kernel.
+  ``read_slots`` takes rows out again.
 * The reference's ``PrefixCache`` (``paged.py:213-397``) is host bookkeeping that
   touches a pool only through ``page_size``, ``incref``, ``free_page`` and
   ``ref_counts`` and a request cache only through ``offset``, ``num_pages``,
@@ -55,7 +56,8 @@ def write_slots(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, key
 
     ``key``/``value`` are ``[T, H, D]`` views (any token/head strides, D contiguous),
     e.g. ``k[0].transpose(0, 1)`` of a ``[1, H, S, D]`` chunk.  ``slots[t]`` is
-    ``page_id * page_size + offset`` (< 0 skips the token).  Pages hold the rows' own type,
+    ``page_id * page_size + offset`` (< 0 skips the token); no two tokens of a call may have
+    the same.  Pages hold the rows' own type,
     int8 (scales ``[P, H, page_size, 1]``) or packed 4-bit codes (uint8 ``[P, H, page_size,
     D/2]``, D 64 or 128, scales ``[P, H, page_size, D/32]``: scale and offset of every 64
     elements, float16 or bfloat16).
