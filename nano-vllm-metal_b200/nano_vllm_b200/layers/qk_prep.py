@@ -22,6 +22,8 @@ def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     axis) keep their token stride and are read without a copy."""
     B, L, H, D = x.shape
     sb, st, sh, sd = x.stride()
+    if L == 1:  # the stride of one token says nothing (a view of a decode step's projection gives H * D)
+        st = sb if B > 1 else H * D
     if sd == 1 and sh == D and (B == 1 or sb == L * st) and st >= H * D:
         return x, st
     return x.contiguous(), H * D

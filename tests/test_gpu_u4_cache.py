@@ -707,3 +707,37 @@ def test_nan_queries_stay_in_their_rows(cuda):
         bad = torch.zeros(1, 8, L, dtype=torch.bool, device="cuda")
         bad[0, 2, 0], bad[0, 5, L - 1] = True, True
         assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("B,L", [(1, 1), (5, 1), (1, 6), (3, 4)])
+@pytest.mark.parametrize("kv", ["u4", BF])
+def test_fused_projections_are_read_in_place(cuda, B, L, kv, monkeypatch):
+    """Views of one projection, of a decode step and of a prompt, are not copied, and give what copies give."""
+    gen = torch.Generator().manual_seed(B + L)
+    Hq, Hkv, D, ps, P = 8, 2, 128, 16, 4
+    views = [x.view(B, L, -1, D) for x in torch.randn(B, L, (Hq + 2 * Hkv) * D, generator=gen).to(BF).cuda()
+             .split([Hq * D, Hkv * D, Hkv * D], -1)]
+    rope = RoPE(D, 64, device="cuda")
+    pos = torch.randint(0, 64, (B, L), generator=gen).int().cuda()
+    slots = torch.randperm(P * ps, generator=gen)[:B * L].cuda()
+
+    def call(q, k, v):
+        pools = _empty_pools(P, Hkv, ps, D, BF)
+        if kv == "u4":
+            q = qk_norm_rope_write(q, k, v, None, None, rope, pos, *pools[:2], slots, key_scales=pools[2], value_scales=pools[3])
+            return [q, *pools]
+        pages = [torch.zeros(P, Hkv, ps, D, dtype=BF, device="cuda") for _ in range(2)]
+        return [qk_norm_rope_write(q, k, v, None, None, rope, pos, *pages, slots), *pages]
+
+    want = call(*(x.clone() for x in views))
+    from nano_vllm_b200.layers import qk_prep
+
+    whole = qk_prep._token_rows
+
+    def rows(x):
+        got = whole(x)
+        assert got[0].data_ptr() == x.data_ptr()
+        return got
+
+    monkeypatch.setattr(qk_prep, "_token_rows", rows)
+    assert all(torch.equal(a, b) for a, b in zip(call(*views), want))
