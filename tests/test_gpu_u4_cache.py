@@ -741,3 +741,17 @@ def test_fused_projections_are_read_in_place(cuda, B, L, kv, monkeypatch):
 
     monkeypatch.setattr(qk_prep, "_token_rows", rows)
     assert all(torch.equal(a, b) for a, b in zip(call(*views), want))
+
+
+@pytest.mark.parametrize("sdt,qdt", [(BF, BF), (HF, BF), (HF, HF)])
+def test_prompts_taken_in_parts(cuda, sdt, qdt):
+    """Tables so wide that the unpacked pages of a batch pass the workspace's limit: parts of it, each with its
+    own lengths, empty requests and holes among them."""
+    gen = torch.Generator().manual_seed(30)
+    lens = [128, 700, 0, 129, 400, 2000, 128]
+    P, bt, cl = random_table(gen, lens, 32, holes=True, width=2048)
+    kp, vp, ks, vs = random_pools(gen, P, 8, 32, 128, sdt)
+    q = torch.randn(7, 16, 128, 128, generator=gen).to(qdt).cuda()
+    got = lib.paged_attention(q, kp, vp, bt, cl, 32, ks, vs, mask="causal", out_dtype=qdt)
+    _close(got, *attend64(q, kp, vp, ks, vs, bt, cl, 32))
+    assert (got[2] == 0).all()
