@@ -248,7 +248,7 @@ PagedArgs unpacked(const PagedArgs& a, const Layout& w, uint8_t* ws) {
 U4PromptPlan plan_u4_prompt(const PagedArgs& a) {
   U4PromptPlan plan{};
   const int64_t rows = a.Hq / a.Hkv * a.L;
-  if (a.D != kD || a.page_size % 16 != 0 || rows < kU4PromptRows || !(a.scale > 0.0f) || !std::isfinite(a.scale) ||
+  if (a.B <= 0 || a.D != kD || a.page_size % 16 != 0 || rows < kU4PromptRows || !(a.scale > 0.0f) || !std::isfinite(a.scale) ||
       (uintptr_t)a.out % 16 != 0 || a.P <= 0 || a.max_pages <= 0 || a.max_pages * a.page_size > INT32_MAX - 4096 ||
       a.Hq * a.L > INT32_MAX / 16)
     return plan;
