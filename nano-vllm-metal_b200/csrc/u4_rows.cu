@@ -135,14 +135,13 @@ struct Raw<NVM_U4> {
   __device__ __forceinline__ void values(int scale_dtype, float (&x)[8]) const {
     const float2 sz = scale_dtype == NVM_BF16 ? u4_pair<__nv_bfloat16>(pair) : u4_pair<__half>(pair);
     // the codes at 4 i and 4 i + 16 are the f16 subnormals code * 2^-24 once shifted: exact, two an operation;
-    // the factor goes into s in two steps, so that it overflows no s
-    const float s = sz.x * 0x1p12f;
+    // the factor goes to the code, since bf16 scales go up to 2^124
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w = codes >> (4 * i) & 0x000f000fu;
       const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&w));
-      x[i] = fmaf(s, c.x * 0x1p12f, sz.y);
-      x[i + 4] = fmaf(s, c.y * 0x1p12f, sz.y);
+      x[i] = fmaf(sz.x, c.x * 0x1p24f, sz.y);
+      x[i + 4] = fmaf(sz.x, c.y * 0x1p24f, sz.y);
     }
   }
 };
