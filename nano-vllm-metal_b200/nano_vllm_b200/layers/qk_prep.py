@@ -29,6 +29,13 @@ def _token_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x.contiguous(), H * D
 
 
+def _on_vectors(x: torch.Tensor, stride: int, elements: int) -> tuple[torch.Tensor, int]:
+    """Rows as ``_token_rows`` gives them, copied where they do not start on the vectors that the kernels move."""
+    if stride % elements == 0 and x.data_ptr() % (2 * elements) == 0:
+        return x, stride
+    return x.clone(memory_format=torch.contiguous_format), x.shape[2] * x.shape[3]
+
+
 def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_weight: torch.Tensor | None,
                        k_norm_weight: torch.Tensor | None, rope: RoPE, positions: torch.Tensor, key_pages: torch.Tensor,
                        value_pages: torch.Tensor, slot_mapping: torch.Tensor, *, eps: float = 1e-5,
@@ -54,11 +61,12 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
     if rope.dims != D:
         raise RuntimeError("qk_norm_rope_write: the RoPE tables are for a different head dim")
     T = B * L
-    qc, q_st = _token_rows(q)
-    kc, k_st = _token_rows(k)
-    vc, v_st = _token_rows(v)
+    vec = 4 if key_pages.dtype is torch.uint8 else max(D // 32, 1)  # elements a lane moves at a time
+    qc, q_st = _on_vectors(*_token_rows(q), vec)
+    kc, k_st = _on_vectors(*_token_rows(k), vec)
+    vc, v_st = _on_vectors(*_token_rows(v), vec)
     if k_st != v_st:
-        kc, vc = k.contiguous(), v.contiguous()
+        kc, vc = (x if st == Hkv * D else x.contiguous() for x, st in ((kc, k_st), (vc, v_st)))
         k_st = v_st = Hkv * D
     if (q_norm_weight is None) != (k_norm_weight is None):
         raise RuntimeError("qk_norm_rope_write: q and k are normalised both or not at all")

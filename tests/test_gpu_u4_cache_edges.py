@@ -5,6 +5,8 @@ import torch
 
 import nano_vllm_b200 as lib
 from nano_vllm_b200 import _native as nv
+from nano_vllm_b200.layers.qk_prep import qk_norm_rope_write
+from nano_vllm_b200.layers.rotary_embedding import RoPE
 from u4_reference import random_pools, values64
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +60,54 @@ def test_read_back_over_every_exponent(cuda):
         sc = torch.stack([s, -7 * s, s, torch.zeros_like(s)], -1).view(T, 1, 1, 4).cuda()
         got = lib.read_slots(torch.arange(T, device="cuda"), kp, kp, sc, sc, FF)[0]
         assert torch.equal(got, values64(kp, sc).float()[:, :, 0])
+
+
+@pytest.mark.parametrize("kv", ["u4", BF, torch.int8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,L,width,first", [(5, 1, 1, 0), (5, 1, 2, 0), (5, 1, 4, 1), (3, 4, 1, 0), (3, 4, 2, 2), (1, 1, 4, 3), (1, 7, 4, 1)])
+def test_append_of_rows_off_the_vectors(cuda, kv, D, B, L, width, first):
+    """Rows of a projection with a few more columns than the heads take, or that starts on no vector's boundary,
+    give what their copies give."""
+    gen = torch.Generator().manual_seed(B * L + D)
+    Hq, Hkv, ps, P = 8, 2, 16, 4
+    n = (Hq + 2 * Hkv) * D
+    wide = torch.randn(B * L * (n + width) + first, generator=gen).to(BF).cuda()[first:].view(B, L, n + width)
+    q, k, v = (x.view(B, L, -1, D) for x in wide[..., :n].split([Hq * D, Hkv * D, Hkv * D], -1))
+    w = [torch.randn(D, generator=gen).to(BF).cuda() for _ in range(2)]
+    rope = RoPE(D, 64, device="cuda")
+    pos = torch.randint(0, 64, (B, L), generator=gen).int().cuda()
+    slots = torch.randperm(P * ps, generator=gen)[:B * L].cuda()
+
+    def call(q, k, v):
+        E = D // 2 if kv == "u4" else D
+        pages = [torch.zeros(P, Hkv, ps, E, dtype=torch.uint8 if kv == "u4" else kv, device="cuda") for _ in range(2)]
+        sc = [None, None]
+        if kv != BF:
+            sc = [torch.ones(P, Hkv, ps, D // 32 if kv == "u4" else 1, dtype=BF, device="cuda") for _ in range(2)]
+        got = qk_norm_rope_write(q, k, v, *w, rope, pos, *pages, slots, key_scales=sc[0], value_scales=sc[1])
+        return [got, *pages, *(x for x in sc if x is not None)]
+
+    for a, b in zip(call(q, k, v), call(q.clone(), k.clone(), v.clone())):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kv", ["u4", BF])
+def test_append_of_keys_and_values_laid_out_apart(cuda, kv):
+    """Contiguous keys that start on no vector's boundary next to values that are a view of something wider."""
+    gen = torch.Generator().manual_seed(6)
+    B, L, Hq, Hkv, D, ps = 3, 4, 4, 2, 128, 16
+    q = torch.randn(B, L, Hq, D, generator=gen).to(BF).cuda()
+    k = torch.randn(B * L * Hkv * D + 1, generator=gen).to(BF).cuda()[1:].view(B, L, Hkv, D)
+    v = torch.randn(B, L, 3 * Hkv * D, generator=gen).to(BF).cuda()[..., Hkv * D:2 * Hkv * D].view(B, L, Hkv, D)
+    rope, pos = RoPE(D, 16, device="cuda"), torch.arange(L, device="cuda").expand(B, L)
+
+    def call(q, k, v):
+        E, dt = (D // 2, torch.uint8) if kv == "u4" else (D, BF)
+        pages = [torch.zeros(1, Hkv, ps, E, dtype=dt, device="cuda") for _ in range(2)]
+        sc = [torch.ones(1, Hkv, ps, 4, dtype=BF, device="cuda") for _ in range(2)] if kv == "u4" else [None, None]
+        return [qk_norm_rope_write(q, k, v, None, None, rope, pos, *pages, torch.arange(B * L, device="cuda"), key_scales=sc[0],
+                                   value_scales=sc[1]), *pages]
+
+    for x, y in ((k, v), (v, k)):
+        for a, b in zip(call(q, x, y), call(q, x.clone(), y.clone())):
+            assert torch.equal(a, b)
