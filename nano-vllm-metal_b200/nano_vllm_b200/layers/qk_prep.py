@@ -107,8 +107,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm
     vs = value_scales if int8 or u4 else None
     with nv.on_device(dev):
         nv.check(nv.lib().nvm_qk_norm_rope_write(
-            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, nv.ptr(wq), nv.ptr(wk), eps,
-            cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0, pos.data_ptr(), out.data_ptr(), L,
+            qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), nv.dtype_code(q.dtype), q_st, k_st, nv.ptr(wq), nv.ptr(wk),
+            float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], 1 if rope.traditional else 0, pos.data_ptr(), out.data_ptr(), L,
             kp.data_ptr(), vp.data_ptr(), nv.dtype_code(kp.dtype), nv.ptr(ks), nv.ptr(vs),
             nv.dtype_code(ks.dtype) if ks is not None else nv.NVM_F16, slots.data_ptr(), T, Hq, Hkv, D, P, ps,
             nv.stream_ptr(dev)))

@@ -111,3 +111,19 @@ def test_append_of_keys_and_values_laid_out_apart(cuda, kv):
     for x, y in ((k, v), (v, k)):
         for a, b in zip(call(q, x, y), call(q, x.clone(), y.clone())):
             assert torch.equal(a, b)
+
+
+def test_append_takes_any_kind_of_number_as_eps(cuda):
+    import numpy as np
+
+    x = torch.randn(1, 3, 2, 128, device="cuda").to(BF)
+    w = torch.ones(128, dtype=BF, device="cuda")
+    rope, pos = RoPE(128, 4, device="cuda"), torch.arange(3, device="cuda")[None]
+
+    def call(eps):
+        kp, vp = (torch.zeros(1, 2, 4, 128, dtype=BF, device="cuda") for _ in range(2))
+        return qk_norm_rope_write(x, x, x, w, w, rope, pos, kp, vp, torch.arange(3, device="cuda"), eps=eps), kp
+
+    want = call(0.5)
+    for eps in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5), np.asarray(0.5)):
+        assert all(torch.equal(a, b) for a, b in zip(call(eps), want))
