@@ -234,6 +234,8 @@ class TinyKvPagedPool:
                 raise ValueError(f"4-bit KV needs a head dimension of 64 or 128 (got {D})")
             # a 16-bit scale and offset for every 64 elements; float32 keys take the type with their range
             scale_dtype = torch.bfloat16 if key.dtype == torch.float32 else key.dtype
+            if self.key_scales is not None:  # rounded to another type, rows would stand for other values
+                scale_dtype = self.key_scales.dtype
             D, scale_width, new_scales = D // 2, 2 * D // nv.U4_GROUP, torch.zeros
         if self.device is None:
             self.device = key.device

@@ -1,7 +1,9 @@
 """The 4-bit cache's corners without a GPU."""
 
 import pytest
+import torch
 
+import nano_vllm_b200 as lib
 from nano_vllm_b200 import _native as nv
 
 
@@ -12,3 +14,23 @@ def test_workspace_of_an_empty_batch(L, D):
     size = nv.lib().nvm_paged_attention_workspace_size
     empty, one = (size(B, 32, 8, L, D, 16, 500, nv.NVM_U4) for B in (0, 1))
     assert 0 <= empty <= one
+
+
+@pytest.mark.parametrize("first,then", [(torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("reserve", [None, 2])
+def test_growth_keeps_scales_as_they_are(first, then, reserve):
+    """Rows of another type do not change the type of the scales that are there: rounded to it they would stand
+    for other values."""
+    pool = lib.TinyKvPagedPool(page_size=4, kv_bits=4, kv_group_size=64, device="cpu", reserve_pages=reserve)
+    pool.allocate_page()
+    pool.grow()
+    pool._ensure_page_storage(torch.zeros(1, 2, 1, 128, dtype=first))
+    one = 1 + torch.finfo(first).eps
+    pool.key_scales.fill_(one)
+    pool.value_scales.fill_(-one)
+    for _ in range(3):
+        pool.allocate_page()
+        pool.grow()
+        pool._ensure_page_storage(torch.zeros(1, 2, 1, 128, dtype=then))
+        assert pool.key_scales.dtype == pool.value_scales.dtype == first
+        assert (pool.key_scales[0] == one).all() and (pool.value_scales[0] == -one).all()
