@@ -13,11 +13,13 @@
 // sums would have to lose again; the powers of two go into the queries and into the output.
 // Queries are held in f16, each row scaled by a power of two (exact for 16-bit queries).
 //
-// Weights are 2^(t - M), t the base-2 score and M a running reference per row, held in f16 once they
-// are multiplied by s'.  M follows the largest t + log2 s' so far, the largest contribution rather than
-// the largest weight: f16 then holds what matters to 11 bits however small the values of the keys
-// that are attended to.  M moves only where a contribution passes it by kSlack, which one vote over the
-// largest weight and the largest scale of a tile finds.  Sums of weights and of p z' are fp32.
+// Weights are 2^(t - M), t the base-2 score and M a reference of the row's near the largest t so far; their sum and
+// that of p z' are fp32.  Multiplied by s' they are held in f16, in a unit of the row's and the group's own: F, a
+// power of two, brings the largest product so far to about 1, and f16 holds what matters to 11 bits however the
+// values of the keys that are attended to, or the two groups of a key, differ in size.  M and F move only where a
+// weight or a product passes them by kSlack, which one vote over a tile's largest weights and scales finds, and
+// only by keys that the row sees.  (One reference for weights and both groups took 3 to 5 % less time, and lost
+// the smaller group's bits from a ratio of 2^14, all of them at 2^26.)
 //
 // The floor of a decode step is HBM: 144 bytes a key and kv head (D = 128).  64 requests of 2K-16K keys, 32/8
 // heads, take 128 us, 0.80 of a copy's rate (48 of 4K-12K, 64/8 heads, f16: 96 us, 0.71).  What bounds it is
@@ -41,8 +43,8 @@ constexpr int kBlocks1 = 4, kBlocks2 = 2;  // blocks an SM holds, of one or two 
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
 constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of (0: 64 requests 136 us for 126; 6: 129)
 constexpr int kFan = 16;     // partial results that are joined at a time (one request of 90K-130K keys: 8 31, 16 29.5, 40 33 us)
-constexpr float kSlack = 1024.0f;   // how far a weight times a scale may pass 2^M
-constexpr float kLeast = 0x1p-80f;  // least scale that a key's values count as
+constexpr float kSlack = 1024.0f;   // how far a weight may pass 2^M, and a weight times a scale its unit
+constexpr float kLeast = 0x1p-100f;  // least scale that a key's values count as
 constexpr float kNoKeys = -1e30f;  // M of a row that has seen no key
 
 template <int D>
@@ -165,7 +167,6 @@ struct Pairs {
       z[g] = p.y;
     }
   }
-  __device__ __forceinline__ float size() const { return kGroups == 2 ? fmaxf(s[0], s[kGroups - 1]) : s[0]; }
 };
 
 // Keys of a request that some query row may see, in steps of kStep; one at least, so that every row
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
     }
   }
 
-  float acc[G][4][kTiles][4], wsum[G][kTiles][4], M[kTiles][2], l[kTiles][2], zsum[kTiles][2][G];
+  // l and zsum in units of 2^M, acc and wsum of 2^M / F
+  float acc[G][4][kTiles][4], wsum[G][kTiles][4], M[kTiles][2], F[kTiles][2][G], l[kTiles][2], zsum[kTiles][2][G];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
@@ -421,6 +423,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
         for (int i = 0; i < 4; ++i) acc[g][i][j][e] = 0.0f;
       }
       zsum[j][0][g] = zsum[j][1][g] = 0.0f;
+      F[j][0][g] = F[j][1][g] = 1.0f;
     }
     M[j][0] = M[j][1] = kNoKeys;
     l[j][0] = l[j][1] = 0.0f;
@@ -505,56 +508,86 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
           }
     }
 
-    // weights 2^(t - M); references that some contribution passes by kSlack move to the largest one
-    float w[2][kTiles][4], heavy = 0.0f, size;
-    {  // the largest scale of the tile's values, of the lane's key first (positive numbers compare as integers)
+    // weights 2^(t - M); a row whose weight, or whose weight times a scale, passes its unit by kSlack moves to the
+    // largest so far (only what the row itself sees moves it, so keys that it does not see leave no trace)
+    float w[2][kTiles][4], heavy = 0.0f, size[G];
+    {  // the largest scales of the tile's values, of the lane's key first (positive numbers compare as integers)
       Pairs<T, G> v;
       v.load(at + R::kVs + lane * 4 * G);
-      size = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.size(), kLeast))));
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        size[g] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v.s[g], 0.0f))));
     }
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           float u0, u1;
           fma2(kap[j][0], kap[j][1], x[mt][j][e], x[mt][j][e + 1], -M[j][0], -M[j][1], u0, u1);
           w[mt][j][e] = ex2(u0);
           w[mt][j][e + 1] = ex2(u1);
-          heavy = fmaxf(heavy, fmaxf(w[mt][j][e], w[mt][j][e + 1]));
         }
-    if (__any_sync(0xffffffffu, heavy * size > kSlack)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float unit = 1.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) unit = fmaxf(unit, F[j][i][g] * size[g]);
+        heavy = fmaxf(heavy, unit * fmaxf(fmaxf(w[0][j][i], w[0][j][2 + i]), fmaxf(w[1][j][i], w[1][j][2 + i])));
+      }
+    }
+    if (__any_sync(0xffffffffu, heavy > kSlack)) {
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = M[j][i];
+          float own = 0.0f, top = M[j][i], most_of[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) most_of[g] = kNoKeys;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               Pairs<T, G> v;
               v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
-              top = fmaxf(top, fmaf(kap[j][i], x[mt][j][2 * h + i], lg2(fmaxf(v.size(), kLeast))));
+              const float t = kap[j][i] * x[mt][j][2 * h + i];
+              top = fmaxf(top, t);
+              float unit = 1.0f;
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                unit = fmaxf(unit, F[j][i][g] * v.s[g]);
+                most_of[g] = fmaxf(most_of[g], t + lg2(fmaxf(v.s[g], kLeast)));
+              }
+              own = fmaxf(own, unit * w[mt][j][2 * h + i]);
             }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float fade = ex2(M[j][i] - top);
-          M[j][i] = top;
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1) {
+            own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+            for (int g = 0; g < G; ++g) most_of[g] = fmaxf(most_of[g], __shfl_xor_sync(0xffffffffu, most_of[g], o));
+          }
+          if (!(own > kSlack)) continue;
+          const float step = M[j][i] - top, fade = ex2(step);
           l[j][i] *= fade;
 #pragma unroll
           for (int g = 0; g < G; ++g) {
+            // the unit's logarithm is M - log2 F; F stays a power of two
+            const int was = (int)(__float_as_uint(F[j][i][g]) >> 23) - 127;
+            const int now = min(max(__float2int_rd(top - fmaxf(M[j][i] - (float)was, most_of[g])), -126), 126);
+            F[j][i][g] = __uint_as_float((uint32_t)(127 + now) << 23);
+            const float fade_g = ex2(step + (float)(now - was));
             zsum[j][i][g] *= fade;
-            wsum[g][j][i] *= fade;
-            wsum[g][j][2 + i] *= fade;
+            wsum[g][j][i] *= fade_g;
+            wsum[g][j][2 + i] *= fade_g;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              acc[g][t][j][i] *= fade;
-              acc[g][t][j][2 + i] *= fade;
+              acc[g][t][j][i] *= fade_g;
+              acc[g][t][j][2 + i] *= fade_g;
             }
           }
+          M[j][i] = top;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -582,7 +615,8 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
             for (int g = 0; g < G; ++g) {
               const float middle = fmaf(8.0f, v.s[g], v.z[g]);
               float s0, s1;
-              mul2(w0, w1, v.s[g], v.s[g], s0, s1);
+              mul2(w0, w1, F[j][0][g], F[j][1][g], s0, s1);
+              mul2(s0, s1, v.s[g], v.s[g], s0, s1);
               if constexpr (decltype(hidden)::value) {
                 if (w0 == 0.0f) s0 = 0.0f;
                 if (w1 == 0.0f) s1 = 0.0f;
@@ -647,13 +681,16 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       if (r == 0) s_ml[warp][row] = make_float2(M[j][i], l[j][i]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float more = fmaf(-8.0f, wsum[g][j][i], zsum[j][i][g]);
+        const float less = -8.0f * wsum[g][j][i], more = zsum[j][i][g];
+        const float unit = __uint_as_float((254u << 23) - __float_as_uint(F[j][i][g]));  // 1 / F
         float* dst = part + row * kPitch + g * kU4Group + r * 4;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-          *reinterpret_cast<float4*>(dst + 32 * half) =
-              make_float4(fmaf(kLowUnit, acc[g][2 * half][j][i], more), fmaf(kHighUnit, acc[g][2 * half][j][2 + i], more),
-                          fmaf(kLowUnit, acc[g][2 * half + 1][j][i], more), fmaf(kHighUnit, acc[g][2 * half + 1][j][2 + i], more));
+          *reinterpret_cast<float4*>(dst + 32 * half) = make_float4(
+              fmaf(fmaf(kLowUnit, acc[g][2 * half][j][i], less), unit, more),
+              fmaf(fmaf(kHighUnit, acc[g][2 * half][j][2 + i], less), unit, more),
+              fmaf(fmaf(kLowUnit, acc[g][2 * half + 1][j][i], less), unit, more),
+              fmaf(fmaf(kHighUnit, acc[g][2 * half + 1][j][2 + i], less), unit, more));
       }
     }
   __syncthreads();

@@ -7,7 +7,8 @@ import nano_vllm_b200 as lib
 from nano_vllm_b200 import _native as nv
 from nano_vllm_b200.layers.qk_prep import qk_norm_rope_write
 from nano_vllm_b200.layers.rotary_embedding import RoPE
-from u4_reference import random_pools, values64
+from u4_bounds import attention, close
+from u4_reference import random_pools, random_table, values64
 
 pytestmark = pytest.mark.gpu
 BF, HF, FF = torch.bfloat16, torch.float16, torch.float32
@@ -127,3 +128,104 @@ def test_append_takes_any_kind_of_number_as_eps(cuda):
     want = call(0.5)
     for eps in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5), np.asarray(0.5)):
         assert all(torch.equal(a, b) for a, b in zip(call(eps), want))
+
+
+# ---------------------------------------------------------------------------
+# keys that a row does not see, and values of any size
+# ---------------------------------------------------------------------------
+def _call(x, ps=16, causal=True, **kw):
+    q, kp, vp, ks, vs, bt, cl = x
+    return lib.paged_attention(q, kp, vp, bt, cl, ps, ks, vs, mask="causal" if causal else None, **kw)
+
+
+def _problem(gen, lens, L, sdt=BF, qdt=None, Hq=8, Hkv=2, D=128, ps=16):
+    P, bt, cl = random_table(gen, lens, ps)
+    q = torch.randn(len(lens), Hq, L, D, generator=gen).to(qdt or sdt).cuda()
+    return [q, *random_pools(gen, P, Hkv, ps, D, sdt), bt, cl]
+
+
+@pytest.mark.parametrize("L", [1, 5])
+@pytest.mark.parametrize("sdt", [BF, HF])
+@pytest.mark.parametrize("what", ["nan", "huge"])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("back", [1, 3])
+def test_hidden_keys_have_no_influence_on_a_row(cuda, L, sdt, what, which, back):
+    """A late token of a chunk holds NaN, or numbers 2^13 to 2^100 times the others: the rows before it are bit for
+    bit what they are without it, those behind it what the definition says."""
+    gen = torch.Generator().manual_seed(L + back)
+    x = _problem(gen, [L, L + 130, 300], L, sdt)
+    clean = _call(x, out_dtype=FF)
+    n = L + 130
+    page, off = x[5][1, (n - back) // 16].item(), (n - back) % 16
+    scales = x[3 if which == "k" else 4]
+    if what == "nan":
+        scales[page, 0, off, 2:] = float("nan")
+    elif which == "k":  # met with small numbers of the queries, so that scores stay ordinary
+        scales[page, 0, off, 2:] *= 2.0 ** (20 if sdt == BF else 13)
+        x[0][1, :4, :, 64:] *= 2.0 ** (-20 if sdt == BF else -13)
+        y = [t.clone() for t in x]
+        y[3][page, 0, off, 2:] = 0
+        clean[1, :4] = _call(y, out_dtype=FF)[1, :4]
+    else:
+        scales[page, 0, off, 2:] *= 2.0 ** (100 if sdt == BF else 13)
+    got = _call(x, out_dtype=FF)
+    hidden = torch.ones(3, 8, L, dtype=torch.bool, device="cuda")
+    hidden[1, :4, L - back:] = False
+    assert torch.equal(got[hidden], clean[hidden])
+    if what == "nan":
+        rows = got[1, :4, L - back:]
+        assert rows[..., 64:].isnan().all() and (rows.isnan().all() if which == "k" else not rows[..., :64].isnan().any())
+    else:
+        want, rows, prompts = attention(*x, 16)
+        bound = rows if L < 64 or sdt == BF else torch.maximum(rows, prompts)
+        close(got[~hidden], want[~hidden], bound[~hidden], "rows that see it")
+
+
+@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 64)])
+@pytest.mark.parametrize("sdt,size", [(BF, 2.0 ** -90), (BF, 2.0 ** -30), (BF, 2.0 ** 40), (BF, 2.0 ** 100), (HF, 2.0 ** -10), (HF, 2.0 ** 11)])
+def test_values_of_any_size_at_any_length(cuda, sdt, size, L, D):
+    """Values 2^-20 (float16: 2^-6) of the others' size, and as often attended to."""
+    gen = torch.Generator().manual_seed(9)
+    x = _problem(gen, [L, 70 + L, 400], L, sdt, BF, D=D)
+    small = torch.rand(x[4].shape[0], 1, 16, 1, generator=gen).cuda() < 0.5
+    x[4].copy_((x[4].double() * torch.where(small, 2.0 ** (-20 if sdt == BF else -6), 1.0) * size).to(sdt))
+    want, rows, prompts = attention(*x, 16)
+    close(_call(x, out_dtype=FF), want, rows if L < 70 or sdt == BF else torch.maximum(rows, prompts))
+
+
+# ---------------------------------------------------------------------------
+# groups and keys of unlike size
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("L", [1, 5])
+@pytest.mark.parametrize("sdt,ratio", [(BF, 2.0 ** -12), (BF, 2.0 ** -17), (BF, 2.0 ** -24), (BF, 2.0 ** -60), (BF, 2.0 ** 40), (HF, 2.0 ** -9)])
+def test_groups_of_unlike_size(cuda, L, sdt, ratio):
+    """A value's second group far below or above its first: each keeps its own precision."""
+    gen = torch.Generator().manual_seed(31)
+    x = _problem(gen, [L, 70, 700], L, sdt)
+    x[4][..., 2:] *= ratio
+    want, rows, _ = attention(*x, 16)
+    close(_call(x, out_dtype=FF), want, rows, ratio)
+
+
+@pytest.mark.parametrize("L", [1, 5])
+def test_groups_whose_ratio_turns(cuda, L):
+    """Keys whose first group is 2^30 times the second next to keys of the opposite kind, attended to by turns."""
+    gen = torch.Generator().manual_seed(32)
+    x = _problem(gen, [900, 300], L, BF)
+    turn = torch.rand(x[4].shape[0], 1, 16, 1, generator=gen).cuda() < 0.5
+    up = torch.tensor([1.0, 1.0, 2.0 ** -30, 2.0 ** -30], device="cuda")
+    x[4].copy_((x[4].float() * torch.where(turn, up, up.flip(0))).to(BF))
+    want, rows, _ = attention(*x, 16)
+    close(_call(x, out_dtype=FF), want, rows)
+
+
+@pytest.mark.parametrize("L", [1, 5])
+@pytest.mark.parametrize("sdt,value", [(BF, 2.0 ** 40), (BF, 2.0 ** 120), (HF, 30000.0), (BF, -2.0 ** -100)])
+@pytest.mark.parametrize("groups", [slice(0, 4), slice(2, 4)])
+def test_values_without_a_span(cuda, L, sdt, value, groups):
+    """Groups whose elements are all alike have no scale, only an offset, of any size."""
+    gen = torch.Generator().manual_seed(33)
+    x = _problem(gen, [1000], L, sdt)
+    x[4][..., groups] = torch.tensor([0.0, value] * 2, device="cuda")[groups].to(sdt)
+    want, rows, prompts = attention(*x, 16)
+    close(_call(x, out_dtype=FF), want, torch.maximum(rows, prompts) if L == 70 else rows)
