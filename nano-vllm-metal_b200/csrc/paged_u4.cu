@@ -45,7 +45,11 @@ constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes th
 constexpr int kFan = 16;     // partial results that are joined at a time (one request of 90K-130K keys: 8 31, 16 29.5, 40 33 us)
 constexpr float kSlack = 1024.0f;   // how far a weight may pass 2^M, and a weight times a scale its unit
 constexpr float kLeast = 0x1p-100f;  // least scale that a key's values count as
-constexpr float kNoKeys = -1e30f;  // M of a row that has seen no key
+constexpr float kNoKeys = -0x1p127f;  // M of a row that has seen no key
+// From scores of this size on the exact product of score and factor is further from M, the rounded one, than a
+// weight may pass it by (4 here, 128 at 2^31, which is infinity): such a row's factor becomes a power of two, whose
+// product is exact.  Scores of this size are 8 apart, and ordered as before.
+constexpr float kFar = 0x1p27f;
 
 template <int D>
 struct Ring {
@@ -542,40 +546,58 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float own = 0.0f, top = M[j][i], most_of[G];
-#pragma unroll
-          for (int g = 0; g < G; ++g) most_of[g] = kNoKeys;
+          float own = 0.0f, most = -INFINITY, product[G];
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               Pairs<T, G> v;
               v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
-              const float t = kap[j][i] * x[mt][j][2 * h + i];
-              top = fmaxf(top, t);
               float unit = 1.0f;
 #pragma unroll
-              for (int g = 0; g < G; ++g) {
-                unit = fmaxf(unit, F[j][i][g] * v.s[g]);
-                most_of[g] = fmaxf(most_of[g], t + lg2(fmaxf(v.s[g], kLeast)));
-              }
+              for (int g = 0; g < G; ++g) unit = fmaxf(unit, F[j][i][g] * v.s[g]);
               own = fmaxf(own, unit * w[mt][j][2 * h + i]);
+              most = fmaxf(most, kap[j][i] < 0.0f ? -x[mt][j][2 * h + i] : x[mt][j][2 * h + i]);
             }
 #pragma unroll
           for (int o = 4; o <= 16; o <<= 1) {
             own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-            for (int g = 0; g < G; ++g) most_of[g] = fmaxf(most_of[g], __shfl_xor_sync(0xffffffffu, most_of[g], o));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
           }
-          if (!(own > kSlack)) continue;
+          const bool move = own > kSlack;
+          float top = fmaxf(M[j][i], fabsf(kap[j][i]) * most);
+          if (move && fabsf(top) >= kFar) {  // the row goes on with the power of two below its factor
+            const float was = kap[j][i];
+            kap[j][i] = __uint_as_float(__float_as_uint(was) & 0xff800000u);
+            M[j][i] *= __fdiv_rn(kap[j][i], was);
+            top = fabsf(kap[j][i]) * most;
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g) product[g] = kNoKeys;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              Pairs<T, G> v;
+              v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
+              const float u = fmaf(kap[j][i], x[mt][j][2 * h + i], -top);
+              if (move) w[mt][j][2 * h + i] = ex2(u);
+#pragma unroll
+              for (int g = 0; g < G; ++g) product[g] = fmaxf(product[g], u + lg2(fmaxf(v.s[g], kLeast)));
+            }
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1)
+#pragma unroll
+            for (int g = 0; g < G; ++g) product[g] = fmaxf(product[g], __shfl_xor_sync(0xffffffffu, product[g], o));
+          if (!move) continue;
           const float step = M[j][i] - top, fade = ex2(step);
+          M[j][i] = top;
           l[j][i] *= fade;
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            // the unit's logarithm is M - log2 F; F stays a power of two
+            // the old unit's logarithm was M - log2 F, in terms of the new M: step - log2 F
             const int was = (int)(__float_as_uint(F[j][i][g]) >> 23) - 127;
-            const int now = min(max(__float2int_rd(top - fmaxf(M[j][i] - (float)was, most_of[g])), -126), 126);
+            const int now = min(max(__float2int_rd(-fmaxf(step - (float)was, product[g])), -126), 126);
             F[j][i][g] = __uint_as_float((uint32_t)(127 + now) << 23);
             const float fade_g = ex2(step + (float)(now - was));
             zsum[j][i][g] *= fade;
@@ -587,11 +609,6 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
               acc[g][t][j][2 + i] *= fade_g;
             }
           }
-          M[j][i] = top;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[mt][j][2 * h + i] = ex2(fmaf(kap[j][i], x[mt][j][2 * h + i], -top));
         }
     }
 
@@ -678,7 +695,9 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 8 * j + 2 * c + i;
-      if (r == 0) s_ml[warp][row] = make_float2(M[j][i], l[j][i]);
+      // M in terms of the scores' own factor, also where the warp took a power of two
+      const float factor = (__float_as_uint(kap[j][i]) & 0x7fffffu) == 0 ? __uint_as_float((__float_as_uint(p.scale_log2) & 0x7fffffu) | 0x3f800000u) : 1.0f;
+      if (r == 0) s_ml[warp][row] = make_float2(M[j][i] * factor, l[j][i]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float less = -8.0f * wsum[g][j][i], more = zsum[j][i][g];

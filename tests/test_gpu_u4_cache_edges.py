@@ -131,7 +131,7 @@ def test_append_takes_any_kind_of_number_as_eps(cuda):
 
 
 # ---------------------------------------------------------------------------
-# keys that a row does not see, and values of any size
+# attention
 # ---------------------------------------------------------------------------
 def _call(x, ps=16, causal=True, **kw):
     q, kp, vp, ks, vs, bt, cl = x
@@ -144,6 +144,41 @@ def _problem(gen, lens, L, sdt=BF, qdt=None, Hq=8, Hkv=2, D=128, ps=16):
     return [q, *random_pools(gen, P, Hkv, ps, D, sdt), bt, cl]
 
 
+@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 64)])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 26, 2.0 ** 30, 2.0 ** 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_apart(cuda, L, D, size, sign):
+    """Scores beyond 2^31, where fp32 has no fractions left: a row is the value of the key with the largest."""
+    gen = torch.Generator().manual_seed(41)
+    x = _problem(gen, [L, 70 + L, 900], L, BF, FF, D=D)
+    x[0] *= size
+    got = _call(x, out_dtype=FF, scale=sign * 0.1)
+    want, rows, prompts = attention(*x, 16, sign * 0.1)
+    # how far a score may be off (2^-20 of its terms, and of a float32 query's 11 bits; from 256 rows a kv head of the
+    # keys' too) moves weights between keys that are that close: the output then lies between their values
+    t = torch.full_like(want[..., 0], float("inf"))
+    for b, n in enumerate([L, 70 + L, 900]):
+        key = torch.arange(n, device="cuda")
+        page = x[5][b].long()[key // 16]
+        for h in range(8):
+            k = values64(x[1][page, h // 4, key % 16], x[3][page, h // 4, key % 16])
+            s = x[0][b, h].double() @ k.T * (sign * 0.1)
+            err = 0.1 * (x[0][b, h].double().abs() @ k.abs().T).amax(-1) * 2.0 ** -9 + 2.0 ** -18 * s.abs().amax(-1)
+            s = s.masked_fill(key > torch.arange(L, device="cuda")[:, None] + n - L, float("-inf"))
+            two = s.topk(min(2, n), -1).values
+            gap = two[:, 0] - two[:, -1] if n > 1 else torch.full_like(err, float("inf"))
+            gap[two[:, -1] == float("-inf")] = float("inf")
+            t[b, h] = gap - 2 * err - 40
+    clear = t > 0  # the largest is alone by more than that: its value, to what a value is held to
+    assert clear.float().mean() > 0.1
+    # (a scale of at most 0.33 times a code less 8, to 11 bits; or a value and a weight, each to 11 bits)
+    close(got[clear], want[clear], 2.0 ** -10 * (want[clear].abs() + 1.4))
+    assert got.isfinite().all() and got.abs().max() < 16
+
+
+# ---------------------------------------------------------------------------
+# keys that a row does not see, and values of any size
+# ---------------------------------------------------------------------------
 @pytest.mark.parametrize("L", [1, 5])
 @pytest.mark.parametrize("sdt", [BF, HF])
 @pytest.mark.parametrize("what", ["nan", "huge"])
