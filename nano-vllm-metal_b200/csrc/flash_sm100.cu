@@ -112,7 +112,7 @@ struct Sm100Params {
   int64_t window, sinks;  // kExt: window == 0 for none
   float* lse;             // kExt: log2 of every row's sum of 2^z ([B*Hq*L], +inf: no key), or null
   int cluster;            // kExt: the n_chunks CTAs of a unit are one cluster and merge over DSMEM
-  const float* out_scale;  // [B * Hkv] factors of the output, or null
+  float out_scale;        // factor of the output
 };
 
 // Pairs q (keys 2q, 2q+1 of a 64-key tile) whose exponentials run on the FMA pipe.
@@ -666,11 +666,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     int gt = 0;  // tiles processed by this CTA so far
     int kq = 0, iw = 0;
     bool ok = true;
-    // 1 / (sum of a row's weights) times the item's factor
-    auto inverse = [&](const Item& it, float sum) {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      return p.out_scale != nullptr ? inv * __ldg(p.out_scale + it.b * p.Hkv + it.kvh) : inv;
-    };
+    // 1 / (sum of a row's weights) times the output's factor
+    auto inverse = [&](float sum) { return sum > 0.f ? p.out_scale / sum : 0.f; };
     // With one item per CTA (stage_out) the K/V ring is free once the item's MMAs are done:
     // O rows go to shared memory in the TMA store's 128B-swizzled box layout (boxes of 128
     // bytes of columns x 128 rows, 16 KB each; row r's 16-byte chunk c of a box at
@@ -1003,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         merged = true;
       } else if (it.n_chunks_unit == 1) {
         put_lse(it, m, lsum);
-        const float inv = inverse(it, lsum);
+        const float inv = inverse(lsum);
 #pragma unroll 1
         for (int c1 = 0; c1 < kD; c1 += 64) {
           float ov2[64];
@@ -1081,7 +1078,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (ml.x != -INFINITY) lt += ml.y * exp2f(ml.x - mxc);
               }
             }
-            const float inv = inverse(it, lt);
+            const float inv = inverse(lt);
             put_lse(it, mxc, lt);
 #pragma unroll 1
             for (int c0 = 0; c0 < kD; c0 += 32) {

@@ -66,7 +66,7 @@ struct PagedArgs {
   int defer;          // with scores: leave the merge through the workspace to the kernel over the scores
   float* mass;        // with scores, and no merge through the workspace: add the weights, or NULL
   int64_t mass_sb, mass_sh, mass_len;
-  const float* out_scale;  // tcgen05 kernel only: [B * Hkv] factors of the output, or NULL
+  float out_scale = 1.0f;  // factor of the output, of the tcgen05 kernel only
 };
 inline bool paged_is_ext(const PagedArgs& a) { return a.window > 0 || a.lse != nullptr; }
 
@@ -225,7 +225,15 @@ struct U4Plan {
   size_t ws_bytes;
 };
 U4Plan plan_paged_u4(const PagedArgs& a);
-int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s);
+// The query rows that a call over unpacked pages could not hold: those that see a key from `first` on (of each
+// (request, kv head): 2^31 - 1 less the key, 0 for none) and those marked in `rows`; a request
+// without any has a zero in `some`.
+struct U4Some {
+  const uint32_t* first;
+  const uint8_t* rows;
+  const int* some;
+};
+int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s, const U4Some* some = nullptr);
 
 int launch_paged_append(int32_t* block_table, int32_t* context_lens, const int32_t* new_tokens,
                         int32_t* free_stack, int32_t* free_top, int32_t* num_pages,

@@ -74,7 +74,8 @@ struct U4Params {
   int* tickets;     // [3 * blocks], zero between calls: of groups by their leader's place, of units by their first block
   int q_dtype, out_dtype, causal;
   int q_fast;  // rows of 16-bit numbers on 16-byte boundaries
-  int B, Hkv, L, rows, row_blocks, P, ps, mp;
+  int B, Hkv, L, rows, row_block0, row_blocks, P, ps, mp;  // the launch's row blocks of a (request, kv head)
+  U4Some some;
   FastDiv by_ps;
   float scale_log2;
 };
@@ -174,16 +175,20 @@ struct Pairs {
 };
 
 // Keys of a request that some query row may see, in steps of kStep; one at least, so that every row
-// is written.
+// is written (kSome: none where no row is to be).
+template <bool kSome>
 __device__ __forceinline__ int steps_of(const U4Params& p, int b) {
+  if (kSome && __ldg(p.some.some + b) == 0) return 0;
   const int keys = min(__ldg(p.context_lens + b), p.mp * p.ps);
   return max(1, (keys + kStep - 1) / kStep);
 }
 
 // Joins `count` partial results (M, sum, output in units of 2^M) of a unit, the k-th in place of(k), into
-// the output or, with `to` >= 0, into that place.  All threads of the block; `scratch` holds count x kRows.
+// the output's rows in `chosen` or, with `to` >= 0, into that place.  All threads of the block; `scratch` holds
+// count x kRows.
 template <int D, int kRows, typename Of>
-__device__ __forceinline__ void join(const U4Params& p, float2* scratch, int count, Of&& of, int rows, size_t out_row0, int to) {
+__device__ __forceinline__ void join(const U4Params& p, float2* scratch, int count, Of&& of, int rows, size_t out_row0, int to,
+                                     uint32_t chosen) {
   for (int i = threadIdx.x; i < count * kRows; i += kWarps * 32)
     scratch[i] = __ldcg(p.part_ml + (size_t)of(i / kRows) * kRows + i % kRows);
   __syncthreads();
@@ -206,7 +211,7 @@ __device__ __forceinline__ void join(const U4Params& p, float2* scratch, int cou
     if (to >= 0) {
       *reinterpret_cast<float4*>(p.part_o + ((size_t)to * kRows + row) * D + d) = o;
       if (d == 0) p.part_ml[(size_t)to * kRows + row] = make_float2(top, sum);
-    } else {
+    } else if (chosen >> row & 1) {
       const int64_t at = (int64_t)(out_row0 + row) * D + d;
       const float inv = sum == 0.0f ? 0.0f : __frcp_rn(sum);
       store_dyn(p.out, at, p.out_dtype, o.x * inv);
@@ -221,8 +226,9 @@ __device__ __forceinline__ void join(const U4Params& p, float2* scratch, int cou
 // one line that is dealt to the blocks in equal parts, so that requests of any lengths load every SM
 // alike; a block takes the units on its part one after another.  Its warps walk tiles of 32 keys, each
 // through a ring of its own, and are joined in shared memory.  A unit that several blocks share is
-// joined by the last of them (in groups of kFan, then the groups).
-template <typename T, int D, int kTiles>
+// joined by the last of them (in groups of kFan, then the groups).  kSome: only the rows that U4Some names
+// are computed and written.
+template <typename T, int D, int kTiles, bool kSome>
 __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2) paged_u4_kernel(const U4Params p) {
   using R = Ring<D>;
   constexpr int G = R::kGroups, kRows = 8 * kTiles;
@@ -236,11 +242,15 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
   // is busy with beginning and ending one.  Lane i adds up the requests [i * per, (i + 1) * per).
   const int heads = p.Hkv * p.row_blocks;  // units of a request
   const int per = (p.B + 31) / 32;
-  int upto = 0;
-  for (int i = lane * per; i < min((lane + 1) * per, p.B); ++i) upto += steps_of(p, i);
+  int upto = 0, requests = max(min(per, p.B - lane * per), 0);
+  for (int i = lane * per; i < min((lane + 1) * per, p.B); ++i) {
+    const int n = steps_of<kSome>(p, i);
+    upto += n;
+    if (kSome && n == 0) --requests;
+  }
   const int real = __reduce_add_sync(0xffffffffu, upto) * heads;
   const int cost = real > (int)gridDim.x ? kUnitCost : 0;
-  upto += cost * max(min(per, p.B - lane * per), 0);
+  upto += cost * requests;
   const int mine = upto;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -258,19 +268,19 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
   const int pos_end = pos + share + ((int)blockIdx.x < more);
   const int in_lane = __ffs(__ballot_sync(0xffffffffu, upto * heads > pos)) - 1;
   int b = in_lane * per, request_at = __shfl_sync(0xffffffffu, upto - mine, in_lane) * heads;  // where request b begins
-  int steps = steps_of(p, b);
+  int steps = steps_of<kSome>(p, b);
 
   while (pos < pos_end) {
-  while (pos >= request_at + (steps + cost) * heads) {
-    request_at += (steps + cost) * heads;
-    steps = steps_of(p, ++b);
+  while ((kSome && steps == 0) || pos >= request_at + (steps + cost) * heads) {
+    if (!kSome || steps > 0) request_at += (steps + cost) * heads;
+    steps = steps_of<kSome>(p, ++b);
   }
   const int in_request = (pos - request_at) / (steps + cost);
   const int unit_at = request_at + in_request * (steps + cost) + cost;  // its first step
   if (unit_at >= pos_end) break;
   const int step0 = max(pos - unit_at, 0), step1 = min(steps, pos_end - unit_at);
   pos = unit_at + step1;
-  const int kvh = in_request / p.row_blocks, rb = in_request - kvh * p.row_blocks, bh = b * p.Hkv + kvh;
+  const int kvh = in_request / p.row_blocks, rb = p.row_block0 + in_request - kvh * p.row_blocks, bh = b * p.Hkv + kvh;
   const int row0 = rb * kRows, rows = min(kRows, p.rows - row0);
   const int ctx = __ldg(p.context_lens + b), limit = min(ctx, p.mp * p.ps);
   // keys that the unit's rows see: [0, most) by some row, [0, least) by every row
@@ -288,6 +298,17 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
   const int begin = min(step0 * kStep, most), end = min(step1 * kStep, most);
 
   const size_t out_row0 = (size_t)bh * p.rows + row0;
+  uint32_t chosen = 0xffffffffu;
+  if constexpr (kSome) {
+    const uint32_t first = __ldg(p.some.first + bh);
+    bool mine = false;
+    if (lane < rows) {
+      const int see = p.causal ? min(limit, (row0 + lane) % p.L + ctx - p.L + 1) : limit;
+      mine = (first != 0 && INT32_MAX - (int)first < see) || __ldg(p.some.rows + out_row0 + lane) != 0;
+    }
+    chosen = __ballot_sync(0xffffffffu, mine);
+    if (chosen == 0) continue;
+  }
   uint8_t* ring = smem + warp * R::kWarp;
   const uint32_t ring_at = smem_u32(ring);
   const int32_t* bt = p.block_table + (size_t)b * p.mp;
@@ -731,7 +752,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
       o = fmaf(f, reinterpret_cast<const float*>(smem)[(w * kRows + row) * kPitch + d], o);
     }
     if (whole) {
-      store_dyn(p.out, (int64_t)(out_row0 + row) * D + d, p.out_dtype, sum == 0.0f ? 0.0f : o * __frcp_rn(sum));
+      if (chosen >> row & 1) store_dyn(p.out, (int64_t)(out_row0 + row) * D + d, p.out_dtype, sum == 0.0f ? 0.0f : o * __frcp_rn(sum));
     } else {
       p.part_o[((size_t)place * kRows + row) * D + d] = o;
       if (d == 0) p.part_ml[(size_t)place * kRows + row] = make_float2(top, sum);
@@ -759,26 +780,27 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2
     };
     if (last_of(p.tickets + place_of(leader), count)) {
       join<D, kRows>(p, scratch, count, [&](int k) { return place_of(leader + k); }, rows, out_row0,
-                     groups > 1 ? place_of(leader) : -1);
+                     groups > 1 ? place_of(leader) : -1, chosen);
       if (groups > 1 && last_of(p.tickets + 2 * gridDim.x + first, groups))
-        join<D, kRows>(p, scratch, groups, [&](int k) { return place_of(first + k * kFan); }, rows, out_row0, -1);
+        join<D, kRows>(p, scratch, groups, [&](int k) { return place_of(first + k * kFan); }, rows, out_row0, -1, chosen);
     }
   }
   __syncthreads();  // the rings are free for the next unit
   }
 }
 
-template <typename T, int D, int kTiles>
+template <typename T, int D, int kTiles, bool kSome = false>
 int launch(const U4Params& p, int64_t blocks, cudaStream_t s) {
   constexpr int bytes = kWarps * Ring<D>::kWarp;
-  const cudaError_t e = cudaFuncSetAttribute(paged_u4_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = cudaFuncSetAttribute(paged_u4_kernel<T, D, kTiles, kSome>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return check_cuda(e, "paged_attention: cudaFuncSetAttribute");
-  paged_u4_kernel<T, D, kTiles><<<(unsigned)blocks, kWarps * 32, bytes, s>>>(p);
+  paged_u4_kernel<T, D, kTiles, kSome><<<(unsigned)blocks, kWarps * 32, bytes, s>>>(p);
   return check_cuda(cudaGetLastError(), "paged_attention: 4-bit kernel launch");
 }
 
 template <typename T>
 int launch_d(const U4Params& p, int64_t D, int tiles, int64_t blocks, cudaStream_t s) {
+  if (p.some.some != nullptr) return launch<T, 128, 2, true>(p, blocks, s);  // (pages are unpacked for no other shape)
   if (D == 128) return tiles == 1 ? launch<T, 128, 1>(p, blocks, s) : launch<T, 128, 2>(p, blocks, s);
   return tiles == 1 ? launch<T, 64, 1>(p, blocks, s) : launch<T, 64, 2>(p, blocks, s);
 }
@@ -799,12 +821,14 @@ U4Plan plan_paged_u4(const PagedArgs& a) {
   return plan;
 }
 
-int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s) {
-  const int64_t rows = a.Hq / a.Hkv * a.L, keys = a.max_pages * a.page_size, heads = a.Hkv * plan.row_blocks;
-  // steps are counted in 32 bits, requests by the part
-  const int64_t line = heads * ((keys + kStep - 1) / kStep + 1 + kUnitCost);
-  if (keys > INT32_MAX - 4096 || rows > INT32_MAX / 2 || line > INT32_MAX / 2)
+int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream_t s, const U4Some* some) {
+  const int64_t rows = a.Hq / a.Hkv * a.L, keys = a.max_pages * a.page_size;
+  // steps are counted in 32 bits: a launch takes as many row blocks and then requests as fit
+  const int64_t unit = (keys + kStep - 1) / kStep + 1 + kUnitCost;
+  const int64_t slice = std::min(plan.row_blocks, INT32_MAX / 2 / (a.Hkv * unit));
+  if (keys > INT32_MAX - 4096 || rows > INT32_MAX / 2 || slice < 1)
     return fail(NVM_ERR_UNSUPPORTED, "paged_attention: 4-bit pages: too many rows or keys");
+  const int64_t line = a.Hkv * slice * unit;
   U4Params p{};
   p.kp = static_cast<const uint8_t*>(a.k_pages);
   p.vp = static_cast<const uint8_t*>(a.v_pages);
@@ -817,7 +841,6 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
   p.Hkv = (int)a.Hkv;
   p.L = (int)a.L;
   p.rows = (int)rows;
-  p.row_blocks = (int)plan.row_blocks;
   p.P = (int)a.P;
   p.ps = (int)a.page_size;
   p.mp = a.P > 0 ? (int)a.max_pages : 0;  // a pool without pages: no key, and nothing to read
@@ -834,9 +857,15 @@ int launch_paged_u4(const PagedArgs& a, const U4Plan& plan, void* ws, cudaStream
     p.out = static_cast<uint8_t*>(a.out) + first_row * (int64_t)dtype_size(a.out_dtype);
     p.block_table = a.block_table + b0 * a.max_pages;
     p.context_lens = a.context_lens + b0;
-    const int st = a.scale_dtype == NVM_BF16 ? launch_d<__nv_bfloat16>(p, a.D, plan.tiles, plan.blocks, s)
-                                             : launch_d<__half>(p, a.D, plan.tiles, plan.blocks, s);
-    if (st != NVM_OK) return st;
+    if (some != nullptr)
+      p.some = U4Some{some->first + b0 * a.Hkv, some->rows + b0 * a.Hq * a.L, some->some + b0};
+    for (int64_t r0 = 0; r0 < plan.row_blocks; r0 += slice) {
+      p.row_block0 = (int)r0;
+      p.row_blocks = (int)std::min(slice, plan.row_blocks - r0);
+      const int st = a.scale_dtype == NVM_BF16 ? launch_d<__nv_bfloat16>(p, a.D, plan.tiles, plan.blocks, s)
+                                               : launch_d<__half>(p, a.D, plan.tiles, plan.blocks, s);
+      if (st != NVM_OK) return st;
+    }
   }
   return NVM_OK;
 }

@@ -6,10 +6,15 @@
 // the tensor cores run from TMA tiles: 4 x 512 tokens against 2K-8K keys, 32/8 heads, take 247 us, 200 of
 // them the tcgen05 kernel's (885 us in row blocks).  Calls of fewer rows a kv head stay with the row blocks
 // (kU4PromptRows has both sides).
-// Values of bfloat16 range are brought into f16 by a power of two for every (request, kv head): K's goes
-// into the queries together with the softmax scale's power of two, V's into the output; f16 then rounds
-// them to 11 bits, eight times finer than bfloat16 would.  The unpacking is bound by HBM (144 bytes in,
-// 512 out a key) and its result mostly stays in L2 for the attention.
+// f16 rounds values and queries of bfloat16 range to 11 bits, eight times finer than bfloat16 would, as long
+// as they lie in its range.  Fixed powers of two bring ordinary ones into its middle (Held; the queries' makes
+// the softmax scale's power up), and are undone in the scores' scale and in the output.  They do not follow
+// the data: a power of two from all keys of a request lets a key change rows that do not see it.  What f16
+// cannot hold (larger, far smaller, NaN) is left out of the unpacked pages and noted: the rows that see such a
+// key, or are themselves too large, are computed by the row blocks in a second step, which ends at once
+// where there are none (3 us).  So a row depends on what it sees only, bit for bit.
+// The unpacking is bound by HBM (144 bytes in, 512 out a key) and its result mostly stays in L2 for the
+// attention.
 #include <algorithm>
 #include <cmath>
 
@@ -23,11 +28,27 @@ constexpr int kD = 128;
 constexpr int kThreads = 128;
 constexpr int kUnroll = 4;                            // keys of a thread
 constexpr int kKeys = kThreads / (kD / 8) * kUnroll;  // of a block
-constexpr int kSizeUnroll = 4;
-constexpr int kSizeKeys = 256 * kSizeUnroll;          // keys of a block that looks at sizes
-constexpr int kTarget = 4;  // values are brought below 2^(kTarget + 1)
+constexpr float kHalfMax = 65504.0f;
 // Bytes that unpacked pages may take; larger batches are taken in parts.
 constexpr size_t kMostBytes = size_t(1) << 30;
+
+// What K and V are multiplied by in f16, the most that they may be there, and the least size of a value group whose
+// elements keep 12 bits of it there (below 2^-14 f16 has steps of 2^-24, here of 2^-30).  Numbers of float16
+// pages are whole steps of f16 however small, and go as they are.
+template <typename T>
+struct Held;
+template <>
+struct Held<__nv_bfloat16> {
+  static constexpr float kKeys = 0x1p4f, kMostKey = kHalfMax, kValues = 0x1p6f, kLeastValue = 0x1p-18f;
+};
+template <>
+struct Held<__half> {
+  static constexpr float kKeys = 1.0f, kMostKey = kHalfMax / 16, kValues = 1.0f, kLeastValue = 0.0f;
+};
+// Queries are multiplied by 2^8 and the softmax scale's power of two, and may be 2^15 then.  Scores (base 2) then stay
+// below 128 * 2^7 * 4094 * 1.45 < 2^27, where the tcgen05 kernel's weights pass their reference by less than 2^12.
+constexpr int kQueryShift = 8;
+constexpr float kMostQuery = 0x1p15f;
 
 struct PromptParams {
   const uint8_t* kp;
@@ -39,68 +60,29 @@ struct PromptParams {
   const void* q;
   __half* k16;        // [B * groups][Hkv][16][D]
   __half* v16;
-  __half* q16;        // [B * Hq * L][D], or NULL: q goes as it is
+  __half* q16;        // [B * Hq * L][D], or NULL: q goes as it is, and is only looked at
   int32_t* table;     // [B][groups]
-  uint32_t* sizes;    // bits of the largest |K| and |V|: [2][B * Hkv], or NULL: nothing is scaled
-  float* out_scale;   // [B * Hkv]
+  uint32_t* first;    // U4Some, zero to begin with but for the rows
+  int* some;
+  uint8_t* far_rows;
   FastDiv by_ps, by_heads, by_blocks;
   int B, Hq, Hkv, P, ps, mp, groups, blocks;  // blocks: of a (request, kv head)
   int64_t q_vectors, vectors_of_head;         // of eight elements, all of q's and those of a q head
   int q_dtype, q_fast, q_blocks;              // q_fast: 16-bit vectors
-  float q_scale;
+  float q_scale, q_size;                      // of the copy, and of what may be kMostQuery
 };
-
-// 2^e that brings numbers of this size below 2^(kTarget + 1), and back
-__device__ __forceinline__ int exponent_of(uint32_t size) { return size == 0 ? kTarget : min(max((int)(size >> 23) - 127, -100), 127); }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + min(max(e, -126), 127)) << 23); }
 
 __device__ __forceinline__ int64_t pool_row(const PromptParams& p, int b, int h, int key) {
   const int page = (int)p.by_ps((uint32_t)key), pid = __ldg(p.block_table + (int64_t)b * p.mp + page);
   return pid < 0 || pid >= p.P ? -1 : ((int64_t)pid * p.Hkv + h) * p.ps + (key - page * p.ps);
 }
 
+// Whether a group's values, which lie between z and z + 15 s, are in range.
 template <typename T>
-__device__ __forceinline__ float size_of(uint2 pairs) {
-  const float2 a = u4_pair<T>(pairs.x), b = u4_pair<T>(pairs.y);
-  const float m = fmaxf(fmaxf(fabsf(a.y), fabsf(fmaf(15.0f, a.x, a.y))), fmaxf(fabsf(b.y), fabsf(fmaf(15.0f, b.x, b.y))));
-  return fminf(m, 3.0e38f);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) u4_sizes_kernel(const PromptParams p) {
-  __shared__ float most[2][8];
-  const int bh = (int)p.by_blocks(blockIdx.x), k0 = (blockIdx.x - bh * p.blocks) * kSizeKeys;
-  const int b = (int)p.by_heads((uint32_t)bh), h = bh - b * p.Hkv;
-  const int keys = min(min(__ldg(p.context_lens + b), p.mp * p.ps), k0 + kSizeKeys);
-  float mk = 0.0f, mv = 0.0f;
-  uint2 pk[kSizeUnroll], pv[kSizeUnroll];
-#pragma unroll
-  for (int i = 0; i < kSizeUnroll; ++i) {
-    const int key = k0 + i * 256 + threadIdx.x;
-    const int64_t row = key < keys ? pool_row(p, b, h, key) : -1;
-    pk[i] = pv[i] = make_uint2(0, 0);
-    if (row >= 0) {
-      pk[i] = __ldg(reinterpret_cast<const uint2*>(p.ks) + row);
-      pv[i] = __ldg(reinterpret_cast<const uint2*>(p.vs) + row);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kSizeUnroll; ++i) {
-    mk = fmaxf(mk, size_of<T>(pk[i]));
-    mv = fmaxf(mv, size_of<T>(pv[i]));
-  }
-  mk = warp_max(mk);
-  mv = warp_max(mv);
-  if ((threadIdx.x & 31) == 0) {
-    most[0][threadIdx.x >> 5] = mk;
-    most[1][threadIdx.x >> 5] = mv;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {  // a maximum does not depend on the order of the blocks
-    float m = 0.0f;
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, most[threadIdx.x][w]);
-    if (m > 0.0f) atomicMax(p.sizes + threadIdx.x * (p.B * p.Hkv) + bh, __float_as_uint(m));
-  }
+__device__ __forceinline__ bool fits(uint32_t pair, float factor, float most, float least) {
+  const float2 sz = u4_pair<T>(pair);
+  const float size = max_nan(fabsf(sz.y), fabsf(fmaf(15.0f, sz.x, sz.y)));
+  return size * factor <= most && (size >= least || size == 0.0f);  // false for NaN
 }
 
 template <typename T>
@@ -117,15 +99,13 @@ __device__ __forceinline__ uint4 unpack8(uint32_t codes, uint32_t pair, float fa
 }
 
 __device__ __forceinline__ float into_half(float x) {  // NaN stays
-  return x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x;
+  return x > kHalfMax ? kHalfMax : x < -kHalfMax ? -kHalfMax : x;
 }
 
-// q in f16, times the scale's power of two and what K was divided by: kUnroll vectors a thread
+// q in f16, times q_scale, and the rows that are too large for it: kUnroll vectors a thread, a row in half a warp.
 __device__ __forceinline__ void take_queries(const PromptParams& p, int64_t block) {
   const int64_t first = block * (kThreads * kUnroll) + threadIdx.x;
-  if (p.sizes != nullptr)
-    for (int64_t i = block * kThreads + threadIdx.x; i < (int64_t)p.B * p.Hkv; i += (int64_t)p.q_blocks * kThreads)
-      p.out_scale[i] = power_of_two(exponent_of(__ldcg(p.sizes + (int64_t)p.B * p.Hkv + i)) - kTarget);
+  const uint32_t half = 0xffffu << (threadIdx.x & 16);
   uint4 raw[kUnroll];
   if (p.q_fast) {
 #pragma unroll
@@ -135,12 +115,7 @@ __device__ __forceinline__ void take_queries(const PromptParams& p, int64_t bloc
 #pragma unroll
   for (int e = 0; e < kUnroll; ++e) {
     const int64_t i = first + e * kThreads;
-    if (i >= p.q_vectors) return;
-    float f = p.q_scale;
-    if (p.sizes != nullptr) {
-      const uint32_t head = (uint32_t)(i / p.vectors_of_head);  // b * Hq + q head: a kv head's are neighbours
-      f = fminf(f * power_of_two(exponent_of(__ldcg(p.sizes + head / (uint32_t)(p.Hq / p.Hkv))) - kTarget), 3.0e38f);
-    }
+    if (i >= p.q_vectors) return;  // (whole rows)
     float x[8];
     const uint32_t u[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
 #pragma unroll
@@ -154,10 +129,20 @@ __device__ __forceinline__ void take_queries(const PromptParams& p, int64_t bloc
         x[2 * k + 1] = load_dyn(p.q, i * 8 + 2 * k + 1, p.q_dtype);
       }
     }
-    uint32_t w[4];
+    float top = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = pack2<__half>(into_half(x[2 * k] * f), into_half(x[2 * k + 1] * f));
-    reinterpret_cast<uint4*>(p.q16)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k]));
+    if (p.q16 != nullptr) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = pack2<__half>(into_half(x[2 * k] * p.q_scale), into_half(x[2 * k + 1] * p.q_scale));
+      reinterpret_cast<uint4*>(p.q16)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const bool far = __any_sync(half, top * p.q_size > kMostQuery);
+    if ((threadIdx.x & 15) == 0) {
+      p.far_rows[i / (kD / 8)] = far;
+      if (far) p.some[i / (p.vectors_of_head * p.Hq)] = 1;
+    }
   }
 }
 
@@ -178,11 +163,6 @@ __global__ void __launch_bounds__(kThreads) u4_unpack_kernel(const PromptParams 
     if (g < p.groups) p.table[(int64_t)b * p.groups + g] = 16 * g < keys && pool_row(p, b, 0, 16 * g) >= 0 ? b * p.groups + g : -1;
   }
   if (k0 >= keys) return;
-  float fk = 1.0f, fv = 1.0f;
-  if (p.sizes != nullptr) {
-    fk = power_of_two(kTarget - exponent_of(__ldcg(p.sizes + bh)));
-    fv = power_of_two(kTarget - exponent_of(__ldcg(p.sizes + p.B * p.Hkv + bh)));
-  }
   const int part = threadIdx.x % (kD / 8);
   uint32_t codes[2][kUnroll], pairs[2][kUnroll];
 #pragma unroll
@@ -197,20 +177,31 @@ __global__ void __launch_bounds__(kThreads) u4_unpack_kernel(const PromptParams 
       pairs[1][i] = __ldg(p.vs + row * 2 + part / 8);
     }
   }
+  uint32_t first = 0;  // the thread's first key that f16 does not hold: zeros there, and the rows that see it come later
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
     const int key = k0 + threadIdx.x / (kD / 8) + i * (kKeys / kUnroll);
     if (key >= (keys + 15) / 16 * 16) break;
+    if (!fits<T>(pairs[0][i], Held<T>::kKeys, Held<T>::kMostKey, 0.0f) ||
+        !fits<T>(pairs[1][i], Held<T>::kValues, kHalfMax, Held<T>::kLeastValue)) {
+      codes[0][i] = codes[1][i] = pairs[0][i] = pairs[1][i] = 0;
+      first = max(first, (uint32_t)(INT32_MAX - key));
+    }
     const int64_t to = ((((int64_t)b * p.groups + key / 16) * p.Hkv + h) * 16 + key % 16) * (kD / 8) + part;
-    reinterpret_cast<uint4*>(p.k16)[to] = unpack8<T>(codes[0][i], pairs[0][i], fk);
-    reinterpret_cast<uint4*>(p.v16)[to] = unpack8<T>(codes[1][i], pairs[1][i], fv);
+    reinterpret_cast<uint4*>(p.k16)[to] = unpack8<T>(codes[0][i], pairs[0][i], Held<T>::kKeys);
+    reinterpret_cast<uint4*>(p.v16)[to] = unpack8<T>(codes[1][i], pairs[1][i], Held<T>::kValues);
+  }
+  first = __reduce_max_sync(0xffffffffu, first);
+  if (first != 0 && threadIdx.x % 32 == 0) {
+    atomicMax(p.first + bh, first);
+    p.some[b] = 1;
   }
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Layout {
-  size_t k, v, q, table, sizes, out_scale, total;
+  size_t k, v, q, table, first, some, far_rows, total;  // `first` and `some` are neighbours
   int64_t groups;
 };
 Layout layout_of(const PagedArgs& a, size_t attention) {
@@ -221,9 +212,11 @@ Layout layout_of(const PagedArgs& a, size_t attention) {
   w.v = w.k + rows * kD * 2;
   w.q = w.v + rows * kD * 2;
   w.table = w.q + align256((size_t)(a.B * a.Hq * a.L) * kD * 2);
-  w.sizes = w.table + align256((size_t)(a.B * w.groups) * 4);
-  w.out_scale = w.sizes + align256((size_t)(a.B * a.Hkv) * 8);
-  w.total = w.out_scale + align256((size_t)(a.B * a.Hkv) * 4);
+  // the row blocks' workspace lies over all of the above, which they need no more
+  w.first = align256(std::max(w.table + (size_t)(a.B * w.groups) * 4, plan_paged_u4(a).ws_bytes));
+  w.some = w.first + (size_t)(a.B * a.Hkv) * 4;
+  w.far_rows = w.some + (size_t)a.B * 4;
+  w.total = w.far_rows + align256((size_t)(a.B * a.Hq * a.L));
   return w;
 }
 
@@ -279,6 +272,7 @@ int launch_u4_prompt(const PagedArgs& a, const U4PromptPlan& plan, void* workspa
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int e = 0;
   const float mantissa = std::frexp(a.scale, &e);  // scale = mantissa * 2^e: the power goes into the queries
+  const int shift = std::min(std::max(e + kQueryShift, -126), 127);
   for (int64_t b0 = 0; b0 < a.B; b0 += plan.batch) {
     PagedArgs x = a;
     x.B = std::min(plan.batch, a.B - b0);
@@ -289,7 +283,9 @@ int launch_u4_prompt(const PagedArgs& a, const U4PromptPlan& plan, void* workspa
     x.context_lens = a.context_lens + b0;
     const Layout w = layout_of(x, plan.attention_bytes);
     PagedArgs y = unpacked(x, w, ws);
-    const bool sized = a.scale_dtype == NVM_BF16, copied = sized || a.q_dtype != NVM_F16 || (uintptr_t)x.q % 16 != 0;
+    const bool bf = a.scale_dtype == NVM_BF16;
+    const bool scaled = bf || a.q_dtype != NVM_F16;  // queries
+    const bool copied = scaled || (uintptr_t)x.q % 16 != 0;
     PromptParams p{};
     p.kp = static_cast<const uint8_t*>(a.k_pages);
     p.vp = static_cast<const uint8_t*>(a.v_pages);
@@ -300,45 +296,43 @@ int launch_u4_prompt(const PagedArgs& a, const U4PromptPlan& plan, void* workspa
     p.q = x.q;
     p.k16 = reinterpret_cast<__half*>(ws + w.k);
     p.v16 = reinterpret_cast<__half*>(ws + w.v);
-    p.q16 = reinterpret_cast<__half*>(ws + w.q);
+    p.q16 = copied ? reinterpret_cast<__half*>(ws + w.q) : nullptr;
     p.table = reinterpret_cast<int32_t*>(ws + w.table);
-    p.sizes = sized ? reinterpret_cast<uint32_t*>(ws + w.sizes) : nullptr;
-    p.out_scale = reinterpret_cast<float*>(ws + w.out_scale);
+    p.first = reinterpret_cast<uint32_t*>(ws + w.first);
+    p.some = reinterpret_cast<int*>(ws + w.some);
+    p.far_rows = ws + w.far_rows;
     p.by_ps = FastDiv(a.page_size);
     p.by_heads = FastDiv(a.Hkv);
     p.B = (int)x.B; p.Hq = (int)a.Hq; p.Hkv = (int)a.Hkv; p.P = (int)a.P; p.ps = (int)a.page_size; p.mp = (int)a.max_pages;
     p.groups = (int)w.groups;
     p.vectors_of_head = a.L * (kD / 8);
-    p.q_vectors = copied ? x.B * a.Hq * p.vectors_of_head : 0;
+    p.q_vectors = x.B * a.Hq * p.vectors_of_head;
     p.q_dtype = a.q_dtype;
-    p.q_scale = std::ldexp(1.0f, std::min(std::max(e, -126), 127));
+    p.q_size = std::ldexp(1.0f, shift);
+    p.q_scale = scaled ? p.q_size : 1.0f;
     const int64_t keys = a.max_pages * a.page_size;
-    const bool bf = a.scale_dtype == NVM_BF16;
-    if (sized) {
-      int st = check_cuda(cudaMemsetAsync(p.sizes, 0, (size_t)(x.B * a.Hkv) * 8, s), "paged_attention: cudaMemsetAsync");
-      if (st != NVM_OK) return st;
-      p.blocks = (int)((keys + kSizeKeys - 1) / kSizeKeys);
-      p.by_blocks = FastDiv(p.blocks);
-      u4_sizes_kernel<__nv_bfloat16><<<(unsigned)(x.B * a.Hkv * p.blocks), 256, 0, s>>>(p);
-      st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit sizes kernel launch");
-      if (st != NVM_OK) return st;
-    }
+    int st = check_cuda(cudaMemsetAsync(p.first, 0, (size_t)(x.B * (a.Hkv + 1)) * 4, s), "paged_attention: cudaMemsetAsync");
+    if (st != NVM_OK) return st;
     p.blocks = (int)((keys + kKeys - 1) / kKeys);
     p.by_blocks = FastDiv(p.blocks);
-    if (copied) {
-      p.q_fast = a.q_dtype != NVM_F32 && (uintptr_t)x.q % 16 == 0;
-      p.q_blocks = (int)((p.q_vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll));
-      y.q = p.q16;
-      y.scale = mantissa;
-      y.out_scale = sized ? p.out_scale : nullptr;
+    p.q_fast = a.q_dtype != NVM_F32 && (uintptr_t)x.q % 16 == 0;
+    p.q_blocks = (int)((p.q_vectors + kThreads * kUnroll - 1) / (kThreads * kUnroll));
+    if (copied) y.q = p.q16;
+    if (scaled) y.scale = std::ldexp(mantissa, e - shift);
+    if (bf) {
+      y.scale /= Held<__nv_bfloat16>::kKeys;
+      y.out_scale = 1.0f / Held<__nv_bfloat16>::kValues;
     }
     const unsigned grid = (unsigned)(x.B * a.Hkv * p.blocks + p.q_blocks);
     bf ? u4_unpack_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p) : u4_unpack_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-    int st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit unpack kernel launch");
+    st = check_cuda(cudaGetLastError(), "paged_attention: 4-bit unpack kernel launch");
     if (st != NVM_OK) return st;
     const Sm100Plan sp = plan_sm100(y, false);
     if (!sp.eligible || sp.ws_bytes > w.k) return fail(NVM_ERR_UNSUPPORTED, "paged_attention: 4-bit prompt plan");
     st = launch_sm100(y, sp, workspace, s);
+    if (st != NVM_OK) return st;
+    const U4Some rest{p.first, p.far_rows, p.some};
+    st = launch_paged_u4(x, plan_paged_u4(x), workspace, s, &rest);
     if (st != NVM_OK) return st;
   }
   return NVM_OK;

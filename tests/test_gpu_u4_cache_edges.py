@@ -144,7 +144,7 @@ def _problem(gen, lens, L, sdt=BF, qdt=None, Hq=8, Hkv=2, D=128, ps=16):
     return [q, *random_pools(gen, P, Hkv, ps, D, sdt), bt, cl]
 
 
-@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 64)])
+@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 64), (70, 128)])
 @pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 26, 2.0 ** 30, 2.0 ** 60])
 @pytest.mark.parametrize("sign", [1, -1])
 def test_scores_far_apart(cuda, L, D, size, sign):
@@ -177,9 +177,9 @@ def test_scores_far_apart(cuda, L, D, size, sign):
 
 
 # ---------------------------------------------------------------------------
-# keys that a row does not see, and values of any size
+# many query rows (from 256 a kv head the pages are unpacked first)
 # ---------------------------------------------------------------------------
-@pytest.mark.parametrize("L", [1, 5])
+@pytest.mark.parametrize("L", [5, 70, 200])
 @pytest.mark.parametrize("sdt", [BF, HF])
 @pytest.mark.parametrize("what", ["nan", "huge"])
 @pytest.mark.parametrize("which", ["k", "v"])
@@ -216,7 +216,26 @@ def test_hidden_keys_have_no_influence_on_a_row(cuda, L, sdt, what, which, back)
         close(got[~hidden], want[~hidden], bound[~hidden], "rows that see it")
 
 
-@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 64)])
+@pytest.mark.parametrize("L", [5, 70])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_largest_float16_groups(cuda, L, which):
+    """A group from 0 to 65504 has a scale of 4368 and a top of 65520, past float16's numbers."""
+    gen = torch.Generator().manual_seed(3)
+    x = _problem(gen, [L, L + 90], L, HF)
+    page, off = x[5][1, 2].item(), 5
+    i = 1 if which == "k" else 2
+    x[i][page, 1, off, :32] = 0xF0
+    x[i + 2][page, 1, off, 0], x[i + 2][page, 1, off, 1] = 4368, 0
+    if which == "k":
+        x[0][1, 4:, :, :64] *= 2.0 ** -14
+    got = _call(x, out_dtype=FF)
+    want, rows, prompts = attention(*x, 16)
+    close(got, want, torch.maximum(rows, prompts))
+    sees = torch.arange(L, device="cuda") + 90 >= 37
+    close(got[1, 4:, sees], want[1, 4:, sees], rows[1, 4:, sees], "rows that see it")
+
+
+@pytest.mark.parametrize("L,D", [(1, 128), (5, 128), (5, 64), (70, 128)])
 @pytest.mark.parametrize("sdt,size", [(BF, 2.0 ** -90), (BF, 2.0 ** -30), (BF, 2.0 ** 40), (BF, 2.0 ** 100), (HF, 2.0 ** -10), (HF, 2.0 ** 11)])
 def test_values_of_any_size_at_any_length(cuda, sdt, size, L, D):
     """Values 2^-20 (float16: 2^-6) of the others' size, and as often attended to."""
@@ -226,6 +245,106 @@ def test_values_of_any_size_at_any_length(cuda, sdt, size, L, D):
     x[4].copy_((x[4].double() * torch.where(small, 2.0 ** (-20 if sdt == BF else -6), 1.0) * size).to(sdt))
     want, rows, prompts = attention(*x, 16)
     close(_call(x, out_dtype=FF), want, rows if L < 70 or sdt == BF else torch.maximum(rows, prompts))
+
+
+@pytest.mark.parametrize("qdt,qsize", [(BF, 2.0 ** -60), (BF, 2.0 ** 60), (FF, 2.0 ** 60), (HF, 2.0 ** -10), (HF, 2.0 ** 12)])
+@pytest.mark.parametrize("sdt", [BF, HF])
+def test_some_query_rows_of_another_size(cuda, qdt, qsize, sdt):
+    """Rows beyond float16's range, on either side, among ordinary ones leave those alone."""
+    gen = torch.Generator().manual_seed(12)
+    L = 70
+    x = _problem(gen, [L, 150], L, sdt, qdt)
+    clean = _call(x, out_dtype=FF)
+    x[0][1, 2, 3], x[0][0, 5, 60] = x[0][1, 2, 3] * qsize, x[0][0, 5, 60] * qsize
+    got = _call(x, out_dtype=FF)
+    other = torch.zeros(2, 8, L, dtype=torch.bool, device="cuda")
+    other[1, 2, 3], other[0, 5, 60] = True, True
+    assert torch.equal(got[~other], clean[~other])
+    want, rows, prompts = attention(*x, 16)
+    # scores of 2^60: a row is its largest key's value, whatever the bound on a score's error (which passes 0.05)
+    top = torch.maximum(rows, prompts).clamp(max=2.0 ** -8) if qsize > 2.0 ** 20 else torch.maximum(rows, prompts)
+    close(got[other], want[other], top[other])
+
+
+def _far_keys(x, gen, ps, n_keys, requests):
+    """Makes some keys' values huge or tiny, some keys huge where the queries are small; returns [B, Hkv] of the first."""
+    first = torch.full((x[0].shape[0], x[1].shape[1]), 1 << 30, device="cuda")
+    for b in requests:
+        n = int(x[6][b])
+        for _ in range(n_keys):
+            key, h = int(torch.randint(n, (1,), generator=gen)), int(torch.randint(x[1].shape[1], (1,), generator=gen))
+            page = int(x[5][b, key // ps])
+            if page < 0:
+                continue
+            x[4][page, h, key % ps] *= [2.0 ** 30, 2.0 ** -40][int(torch.randint(2, (1,), generator=gen))]
+            first[b, h] = min(int(first[b, h]), key)
+    return first
+
+
+@pytest.mark.parametrize("L,Hq,Hkv,top", [(33, 16, 2, 3000), (64, 8, 2, 700), (200, 8, 2, 900), (300, 4, 4, 500), (5, 128, 2, 2000)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_of_either_kernel(cuda, L, Hq, Hkv, top, causal):
+    """Some requests have keys that the unpacked pages leave out; calls of few and of many tokens, missing pages,
+    eager and replayed from a graph on other keys."""
+    gen = torch.Generator().manual_seed(L)
+    lens = [top, L, top // 2 + L, 0, top - 77, L + 1]
+    P, bt, cl = random_table(gen, lens, 16, holes=True)
+    q = torch.randn(len(lens), Hq, L, 128, generator=gen).to(BF).cuda()
+    x = [q, *random_pools(gen, P, Hkv, 16, 128, BF), bt, cl]
+    plain = [t.clone() for t in x]
+
+    def check(got, first):
+        want, rows, prompts = attention(*x, 16, causal=causal)
+        last = (torch.arange(L, device="cuda")[None] + cl[:, None] - L) if causal else cl[:, None].expand(-1, L) - 1
+        sees = (last[:, None] >= first[:, :, None]).repeat_interleave(Hq // Hkv, 1)  # [B, Hq, L]
+        close(got, want, torch.where(sees[..., None], rows, prompts))
+
+    call = lambda: _call(x, out_dtype=FF, causal=causal)  # noqa: E731
+    clean = call()
+    check(clean, torch.full((len(lens), Hkv), 1 << 30, device="cuda"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for requests in ((0,), (4, 2), range(len(lens)), ()):
+        x[4].copy_(plain[4])
+        first = _far_keys(x, gen, 16, 3, requests) if max(requests, default=0) < 3 or len(requests) == 2 else \
+            _far_keys(x, gen, 16, 1, [b for b in requests if lens[b]])
+        got = call()
+        check(got, first)
+        graph.replay()
+        assert torch.equal(out, got)
+    assert torch.equal(call(), clean)
+
+
+def test_parts_of_a_batch_with_keys_left_out(cuda):
+    """The tables are so wide that the batch is unpacked in parts."""
+    gen = torch.Generator().manual_seed(43)
+    lens = [128, 700, 150, 129, 400, 1000, 128]
+    P, bt, cl = random_table(gen, lens, 32, width=2048)
+    x = [torch.randn(7, 16, 128, 128, generator=gen).to(BF).cuda(), *random_pools(gen, P, 8, 32, 128, BF), bt, cl]
+    first = _far_keys(x, gen, 32, 6, [1, 5, 6])
+    x[0][4, 3, 17] *= 2.0 ** 20
+    got = _call(x, 32, out_dtype=FF, scale=0.01)
+    want, rows, prompts = attention(*x, 32, 0.01)
+    last = torch.arange(128, device="cuda")[None] + cl[:, None] - 128
+    sees = (last[:, None] >= first[:, :, None]).repeat_interleave(2, 1)
+    sees[4, 3, 17] = True
+    bound = torch.where(sees[..., None], rows, prompts)
+    assert sees.any() and not sees.all()
+    far = torch.zeros_like(sees)
+    far[4, 3, 17] = True  # scores of 2^17: its own bound passes 0.05, and says nothing
+    close(got[~far], want[~far], bound[~far])
+    assert got[far].isfinite().all()
+
+
+def test_more_row_blocks_than_a_launch_counts(cuda):
+    """Many tokens under tables a million pages wide: the row blocks are taken in slices."""
+    gen = torch.Generator().manual_seed(44)
+    L, ps, D, lens = 512, 1024, 64, [512, 1500]
+    P, bt, cl = random_table(gen, lens, ps, width=1 << 20)
+    x = [torch.randn(2, 8, L, D, generator=gen).to(HF).cuda(), *random_pools(gen, P, 2, ps, D, HF), bt, cl]
+    want, rows, _ = attention(*x, ps)
+    close(_call(x, ps, out_dtype=HF), want, rows)
 
 
 # ---------------------------------------------------------------------------
@@ -254,7 +373,7 @@ def test_groups_whose_ratio_turns(cuda, L):
     close(_call(x, out_dtype=FF), want, rows)
 
 
-@pytest.mark.parametrize("L", [1, 5])
+@pytest.mark.parametrize("L", [1, 5, 70])
 @pytest.mark.parametrize("sdt,value", [(BF, 2.0 ** 40), (BF, 2.0 ** 120), (HF, 30000.0), (BF, -2.0 ** -100)])
 @pytest.mark.parametrize("groups", [slice(0, 4), slice(2, 4)])
 def test_values_without_a_span(cuda, L, sdt, value, groups):

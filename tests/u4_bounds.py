@@ -13,7 +13,7 @@ its row and group (the reference may lag 2^10 behind it, never pass it) it is of
 keys.  Everything else is fp32: a sum of n / 16 terms and 64 more takes (n / 16 + 64) 2^-24 of its terms.
 
 Prompts: K times 16 and V times 64 are held in 16 bits (where the scales are float16, as they are), the queries
-times 2^7 and the scale's power of two; K and V are off by 2^-11 and 2^-29 or 2^-31, queries by 2^-32 of a score
+times 2^8 and the scale's power of two; K and V are off by 2^-11 and 2^-29 or 2^-31, queries by 2^-32 of a score
 per unit of K (and 2^-11 where they have 32 bits), weights by 2^-11, or 2^-25 of the row's largest.
 """
 
