@@ -29,8 +29,10 @@ constexpr int kThreads = 128;
 constexpr int kUnroll = 4;                            // keys of a thread
 constexpr int kKeys = kThreads / (kD / 8) * kUnroll;  // of a block
 constexpr float kHalfMax = 65504.0f;
-// Bytes that unpacked pages may take; larger batches are taken in parts.
-constexpr size_t kMostBytes = size_t(1) << 30;
+// Bytes that unpacked pages may take; larger batches are taken in parts.  They are sized by the table's width, since
+// the lengths are on the device: one request may take kMostOfOne (2M keys of 8 heads), and is left to the row
+// blocks, which need no copy, beyond that (a table a million pages wide asked for 4 TB).
+constexpr int64_t kMostBytes = int64_t(1) << 30, kMostOfOne = int64_t(1) << 33;
 
 // What K and V are multiplied by in f16, the most that they may be there, and the least size of a value group whose
 // elements keep 12 bits of it there (below 2^-14 f16 has steps of 2^-24, here of 2^-30).  Numbers of float16
@@ -245,15 +247,16 @@ U4PromptPlan plan_u4_prompt(const PagedArgs& a) {
       (uintptr_t)a.out % 16 != 0 || a.P <= 0 || a.max_pages <= 0 || a.max_pages * a.page_size > INT32_MAX - 4096 ||
       a.Hq * a.L > INT32_MAX / 16)
     return plan;
+  const int64_t keys = a.max_pages * a.page_size, blocks = a.Hkv * ((keys + kKeys - 1) / kKeys);  // of a request
+  const int64_t one = blocks * (kKeys * kD * 4);
+  if (one > kMostOfOne) return plan;
   PagedArgs x = a;
-  const int64_t one = std::max<int64_t>(a.max_pages * a.page_size * a.Hkv * kD * 4, 1);
-  const int64_t parts = (a.B * one + (int64_t)kMostBytes - 1) / (int64_t)kMostBytes;
-  x.B = std::max<int64_t>((a.B + parts - 1) / parts, 1);
-  for (; x.B > 1 && (x.B * x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX / 2 || x.B * x.Hq * x.L > INT32_MAX / 2);)
-    x.B = (x.B + 1) / 2;
+  x.B = std::min(a.B, std::max<int64_t>(kMostBytes / one, 1));
+  while (x.B > 1 && (x.B * blocks > INT32_MAX / 2 || x.B * x.Hq * x.L > INT32_MAX / 2)) x.B = (x.B + 1) / 2;
+  const int64_t parts = (a.B + x.B - 1) / x.B;
+  x.B = (a.B + parts - 1) / parts;  // parts of one size
   const Layout none = layout_of(x, 0);
   const PagedArgs inner = unpacked(x, none, nullptr);
-  if (x.Hkv * ((a.max_pages * a.page_size + kKeys - 1) / kKeys) > INT32_MAX / 2) return plan;
   const Sm100Plan attention = plan_sm100(inner, true);
   if (!attention.eligible) return plan;
   plan.attention_bytes = attention.ws_bytes;

@@ -347,6 +347,15 @@ def test_more_row_blocks_than_a_launch_counts(cuda):
     close(_call(x, ps, out_dtype=HF), want, rows)
 
 
+def test_prompts_under_tables_too_wide_to_unpack(cuda):
+    gen = torch.Generator().manual_seed(45)
+    L, ps, lens = 128, 1024, [128, 1500]
+    P, bt, cl = random_table(gen, lens, ps, width=1 << 18)
+    x = [torch.randn(2, 8, L, 128, generator=gen).to(BF).cuda(), *random_pools(gen, P, 8, ps, 128, BF), bt, cl]
+    want, rows, _ = attention(*x, ps)
+    close(_call(x, ps, out_dtype=BF), want, rows)
+
+
 # ---------------------------------------------------------------------------
 # groups and keys of unlike size
 # ---------------------------------------------------------------------------

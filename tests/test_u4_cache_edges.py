@@ -34,3 +34,12 @@ def test_growth_keeps_scales_as_they_are(first, then, reserve):
         pool._ensure_page_storage(torch.zeros(1, 2, 1, 128, dtype=then))
         assert pool.key_scales.dtype == pool.value_scales.dtype == first
         assert (pool.key_scales[0] == one).all() and (pool.value_scales[0] == -one).all()
+
+
+@pytest.mark.parametrize("width", [1, 1000, 1 << 16, 1 << 20, (1 << 21) - 64])
+@pytest.mark.parametrize("B", [1, 3, 64, 1 << 20])
+def test_workspace_of_wide_tables(width, B):
+    """Unpacked pages take at most 1 GiB of a batch and 8 GiB of one request, whatever the tables have room for."""
+    rows = 16 * 128 * 128 * 2 + 16 * 128  # a request's queries, and a mark for each
+    most = max(8 << 30, (1 << 30) + B * rows) + (16 << 20) + B * 64 + B * width * 256
+    assert nv.lib().nvm_paged_attention_workspace_size(B, 16, 8, 128, 128, 1024, width, nv.NVM_U4) <= most
