@@ -39,7 +39,9 @@ namespace {
 constexpr int kWarps = 4;    // 2 or 8: one request 13.6 or 11.3 us for 11.3, 64 requests 132 or 146 for 136
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
 constexpr int kStages = 2;   // of each warp's own ring: one tile is copied while one is worked on
-constexpr int kBlocks1 = 4, kBlocks2 = 2;  // blocks an SM holds, of one or two tiles of rows (3 of two: spills, 93 us for 90)
+// Blocks an SM holds.  One tile of rows: of 64 elements four at 124 registers (three: 30.7 us for 28.7); of 128
+// three, whose 168 registers hold what four spill (64 requests 140 us for 147).  Two tiles: two.
+constexpr int blocks_of(int64_t D, int tiles) { return tiles == 2 ? 2 : D == 128 ? 3 : 4; }
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
 constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of (0: 64 requests 136 us for 126; 6: 129)
 constexpr int kFan = 16;     // partial results that are joined at a time (one request of 90K-130K keys: 8 31, 16 29.5, 40 33 us)
@@ -229,7 +231,7 @@ __device__ __forceinline__ void join(const U4Params& p, float2* scratch, int cou
 // joined by the last of them (in groups of kFan, then the groups).  kSome: only the rows that U4Some names
 // are computed and written.
 template <typename T, int D, int kTiles, bool kSome>
-__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? kBlocks1 : kBlocks2) paged_u4_kernel(const U4Params p) {
+__global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_kernel(const U4Params p) {
   using R = Ring<D>;
   constexpr int G = R::kGroups, kRows = 8 * kTiles;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -815,7 +817,7 @@ U4Plan plan_paged_u4(const PagedArgs& a) {
   const int64_t steps = std::max<int64_t>((a.max_pages * a.page_size + kStep - 1) / kStep, 1);
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t most = (int64_t)sms * (plan.tiles == 1 ? kBlocks1 : kBlocks2), units = a.B * a.Hkv * plan.row_blocks;
+  const int64_t most = (int64_t)sms * blocks_of(a.D, plan.tiles), units = a.B * a.Hkv * plan.row_blocks;
   plan.blocks = units > most / steps ? most : units * steps;
   plan.ws_bytes = kTicketRegionBytes + (size_t)(plan.blocks * 2 * 8 * plan.tiles) * (a.D + 2) * sizeof(float);
   return plan;
