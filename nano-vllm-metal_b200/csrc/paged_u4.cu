@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_ke
     }
 
     const bool masked = there != 0xffffffffu || k0 + kTile > least;
+    // key of the tile, and where the keys of a row end
+    auto sees = [&](int key, int end_of_row) { return (there >> key & 1) != 0 && k0 + key < end_of_row; };
     if (masked) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
@@ -530,8 +532,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_ke
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = r + 16 * mt + 8 * (e >> 1);
-            const bool ok = (there >> key & 1) && k0 + key < seen[j][e & 1];
-            if (!ok) x[mt][j][e] = kap[j][e & 1] < 0.0f ? INFINITY : -INFINITY;  // kap * x = -inf
+            if (!sees(key, seen[j][e & 1])) x[mt][j][e] = kap[j][e & 1] < 0.0f ? INFINITY : -INFINITY;  // kap * x = -inf
           }
     }
 
@@ -645,8 +646,9 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_ke
         uint32_t pf[kTiles][G][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          const int key = r + 16 * mt + 8 * h;
           Pairs<T, G> v;
-          v.load(at + R::kVs + (r + 16 * mt + 8 * h) * 4 * G);
+          v.load(at + R::kVs + key * 4 * G);
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
             const float w0 = w[mt][j][2 * h], w1 = w[mt][j][2 * h + 1];
@@ -658,10 +660,10 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_ke
               mul2(w0, w1, F[j][0][g], F[j][1][g], s0, s1);
               mul2(s0, s1, v.s[g], v.s[g], s0, s1);
               if constexpr (decltype(hidden)::value) {
-                if (w0 == 0.0f) s0 = 0.0f;
-                if (w1 == 0.0f) s1 = 0.0f;
-                zsum[j][0][g] += w0 == 0.0f ? 0.0f : w0 * middle;
-                zsum[j][1][g] += w1 == 0.0f ? 0.0f : w1 * middle;
+                if (!sees(key, seen[j][0])) s0 = 0.0f;
+                if (!sees(key, seen[j][1])) s1 = 0.0f;
+                zsum[j][0][g] += sees(key, seen[j][0]) ? w0 * middle : 0.0f;
+                zsum[j][1][g] += sees(key, seen[j][1]) ? w1 * middle : 0.0f;
               } else {
                 fma2(w0, w1, middle, middle, zsum[j][0][g], zsum[j][1][g], zsum[j][0][g], zsum[j][1][g]);
               }

@@ -356,6 +356,22 @@ def test_prompts_under_tables_too_wide_to_unpack(cuda):
     close(_call(x, ps, out_dtype=BF), want, rows)
 
 
+@pytest.mark.parametrize("L", [1, 5, 70])
+@pytest.mark.parametrize("key", [3, 130, 394, 398])
+def test_nan_of_a_key_with_no_weight_left(cuda, L, key):
+    """A value that cannot be held is NaN for every row that sees it, also where its weight is below fp32's numbers."""
+    gen = torch.Generator().manual_seed(46)
+    x = _problem(gen, [400], L, BF)
+    page = x[5][0, key // 16].item()
+    x[4][page, 1, key % 16, 0] = float("nan")
+    x[1][page, 1, key % 16], x[3][page, 1, key % 16] = 0, torch.tensor([0.0, -1.0] * 2, device="cuda").to(BF)  # K = -1
+    x[0][0, 4:] = x[0][0, 4:].abs() + 1  # scores of -128 times the scale and less
+    got = _call(x, out_dtype=FF, scale=4.0)
+    sees = torch.arange(L, device="cuda") + 400 - L >= key
+    assert got[0, 4:, sees, :64].isnan().all() and not got[0, 4:, sees, 64:].isnan().any()
+    assert not got[0, 4:, ~sees].isnan().any() and not got[0, :4].isnan().any()
+
+
 # ---------------------------------------------------------------------------
 # groups and keys of unlike size
 # ---------------------------------------------------------------------------
