@@ -142,7 +142,8 @@ int nvm_selftest_wait_expiry(int64_t limit_ns, unsigned long long* waited_ns, vo
  *              zero again, so one workspace serves calls of any shape; the rest
  *              is overwritten by every call.  May be NULL if the size is 0.
  *              4-bit pages need one for every call, on a 16-byte boundary; from 256 query
- *              rows a kv head it holds the unpacked pages, up to 1 GiB (or one request's).
+ *              rows a kv head it holds the unpacked pages, up to 1 GiB (or one request's,
+ *              up to 8 GiB).
  *              Calls that share one workspace must not overlap on the GPU, nor on the
  *              host: a call may launch several kernels, so two host threads on one
  *              stream have to take turns.

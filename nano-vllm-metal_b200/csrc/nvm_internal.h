@@ -209,8 +209,9 @@ struct U4AppendArgs {
 };
 int launch_u4_append(const U4AppendArgs& a, cudaStream_t s);
 // Many query rows: pages unpacked into the workspace for the tcgen05 kernel (u4_prompt.cu), from so many a
-// kv head.  Row blocks / unpacked, us: 32 requests of 4850 keys, 4 heads, 128 rows 259 / 323, 192 380 / 350,
-// 256 500 / 376; 8 requests of 4000, 8 heads, 128 rows 115 / 190, 192 164 / 222; 2 of 2000, 192 rows 38 / 57.
+// kv head.  Row blocks / unpacked, us: 32 requests of 4850 keys, 4 heads, 128 rows 246 / 320, 192 362 / 346, 256
+// 473 / 373; 8 of 4000, 8 heads, 192 rows 164 / 225, 256 213 / 236, 320 262 / 225; 2 of 2000, 256 rows 45 / 57, 384
+// 61 / 77: between what many requests and few would have.
 constexpr int64_t kU4PromptRows = 256;
 struct U4PromptPlan {
   bool eligible;

@@ -22,11 +22,12 @@
 // the smaller group's bits from a ratio of 2^14, all of them at 2^26.)
 //
 // The floor of a decode step is HBM: 144 bytes a key and kv head (D = 128).  64 requests of 2K-16K keys, 32/8
-// heads, take 128 us, 0.80 of a copy's rate (48 of 4K-12K, 64/8 heads, f16: 96 us, 0.71).  What bounds it is
-// the latency of the instructions: about 450 a tile of 32 keys and warp (unpacking 160, weights and sums
-// 180, matrix instructions 36, copies 60), 16 warps an SM at 127 registers, issue slots 54 % busy.  Twelve
-// warps took 145 us; twenty spill.  Tiles come by 16-byte asynchronous copies, a ring to each warp, so that no
-// warp waits for another inside a unit; a third or fourth stage gained nothing (137, 145 us).
+// heads, take 129 us, 0.78 of a copy's rate (48 of 4K-12K, 64/8 heads, f16: 96 us, 0.71), in a graph of a dozen
+// calls; in runs of hundreds, where the power limit lowers the clocks, 139 to 142 (101).  The variants below are
+// compared in such runs.  What bounds it is the latency of the instructions: about 500 a tile of 32 keys and warp
+// (unpacking 160, weights, their references and sums 230, matrix instructions 36, copies 60), 12 warps an SM at 168
+// registers, issue slots 51 % busy.  Tiles come by 16-byte asynchronous copies, a ring to each warp, so that no
+// warp waits for another inside a unit.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,15 +37,16 @@
 namespace nvm {
 namespace {
 
-constexpr int kWarps = 4;    // 2 or 8: one request 13.6 or 11.3 us for 11.3, 64 requests 132 or 146 for 136
+constexpr int kWarps = 4;    // 2: a long context 43 us for 33; 8: 64 requests 148 us for 139, 5 tokens 113 for 103
 constexpr int kTile = 32;    // keys of a stage, one page lookup a lane
 constexpr int kStages = 2;   // of each warp's own ring: one tile is copied while one is worked on
 // Blocks an SM holds.  One tile of rows: of 64 elements four at 124 registers (three: 30.7 us for 28.7); of 128
-// three, whose 168 registers hold what four spill (64 requests 140 us for 147).  Two tiles: two.
+// three, whose 168 registers hold what four spill (64 requests 139 us, four 146, two 162).  Two tiles: two
+// (5 tokens 103 us, three 108).
 constexpr int blocks_of(int64_t D, int tiles) { return tiles == 2 ? 2 : D == 128 ? 3 : 4; }
 constexpr int kStep = kWarps * kTile;  // keys that a block takes at a time, the unit that work is dealt in
-constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of (0: 64 requests 136 us for 126; 6: 129)
-constexpr int kFan = 16;     // partial results that are joined at a time (one request of 90K-130K keys: 8 31, 16 29.5, 40 33 us)
+constexpr int kUnitCost = 3;  // steps that beginning and ending a unit takes the time of (0: 64 requests 146 us for 139, 5 tokens 125 for 103; 6: 142, 100)
+constexpr int kFan = 16;     // partial results that are joined at a time (8: one request 14.4 us for 13.0; 40: one of 90K-130K keys 35.0 for 33.0)
 constexpr float kSlack = 1024.0f;   // how far a weight may pass 2^M, and a weight times a scale its unit
 constexpr float kLeast = 0x1p-100f;  // least scale that a key's values count as
 constexpr float kNoKeys = -0x1p127f;  // M of a row that has seen no key

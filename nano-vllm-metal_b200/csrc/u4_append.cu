@@ -7,9 +7,9 @@
 // vectors), so a warp works on 256 / D rows at once: a group's extremes are three or four shuffles away and
 // a lane's codes of a half are 16 bits.  A warp walks rows of one kind of one token, all q, all k or all v,
 // with the loads of the next kAhead steps in flight; few tokens are spread over more warps, down to one
-// step each.  Bound by HBM (22 KB a token, 32/8 heads) as far as issue allows: 8192 tokens, bf16, 47.5 us
-// without a norm (3.8 TB/s, issue slots 71 % busy) and 57 with one; one token 3.1 us.  In qk_prep.cu's
-// layout (a row over 32 lanes, eight rows unrolled) the same took 68, 86 and 6.1 us.
+// step each.  Bound by HBM (22 KB a token, 32/8 heads) as far as issue allows: 8192 tokens, bf16, 49 us
+// without a norm (3.7 TB/s, issue slots 71 % busy) and 59 with one; one token 3.1 us.  In qk_prep.cu's
+// layout (a row over 32 lanes, eight rows unrolled) the same took 1.4 and 1.5 times as long, one token twice.
 #include <algorithm>
 
 #include "nvm_internal.h"
@@ -19,8 +19,8 @@ namespace nvm {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kBlocks = 4;  // of an SM (3: 56 us, 5: 52, which spills)
-constexpr int kMost = 8;   // steps of a warp (4: 55 us, 16: 60)
+constexpr int kBlocks = 4;  // of an SM (8192 f16 tokens appended and read back, 59.4 us: 3 67.0; 5, which spills, 62.8)
+constexpr int kMost = 8;   // steps of a warp (the same: 4 59.5, 16 69.9)
 constexpr int kAhead = 4;  // steps whose loads are in flight
 
 struct AppendParams {

@@ -3,8 +3,8 @@
 //
 // A row block of paged_u4.cu unpacks the keys that it sees for itself, which costs it more than the
 // matrix instructions do once a kv head has many blocks; here a key is unpacked once for all of them and
-// the tensor cores run from TMA tiles: 4 x 512 tokens against 2K-8K keys, 32/8 heads, take 247 us, 200 of
-// them the tcgen05 kernel's (885 us in row blocks).  Calls of fewer rows a kv head stay with the row blocks
+// the tensor cores run from TMA tiles: 4 x 512 tokens against 2K-8K keys, 32/8 heads, take 243 us, about 205
+// of them the tcgen05 kernel's (pages of 24 tokens, in row blocks, 3.4 times as long).  Calls of fewer rows a kv head stay with the row blocks
 // (kU4PromptRows has both sides).
 // f16 rounds values and queries of bfloat16 range to 11 bits, eight times finer than bfloat16 would, as long
 // as they lie in its range.  Fixed powers of two bring ordinary ones into its middle (Held; the queries' makes
@@ -12,7 +12,7 @@
 // the data: a power of two from all keys of a request lets a key change rows that do not see it.  What f16
 // cannot hold (larger, far smaller, NaN) is left out of the unpacked pages and noted: the rows that see such a
 // key, or are themselves too large, are computed by the row blocks in a second step, which ends at once
-// where there are none (3 us).  So a row depends on what it sees only, bit for bit.
+// where there are none (3 us).  So which kernel computes a row, and from what, depends on what the row sees only.
 // The unpacking is bound by HBM (144 bytes in, 512 out a key) and its result mostly stays in L2 for the
 // attention.
 #include <algorithm>
