@@ -408,3 +408,58 @@ def test_values_without_a_span(cuda, L, sdt, value, groups):
     x[4][..., groups] = torch.tensor([0.0, value] * 2, device="cuda")[groups].to(sdt)
     want, rows, prompts = attention(*x, 16)
     close(_call(x, out_dtype=FF), want, torch.maximum(rows, prompts) if L == 70 else rows)
+
+
+# ---------------------------------------------------------------------------
+# prompts in company
+# ---------------------------------------------------------------------------
+def test_prompts_without_a_workspace(cuda):
+    """The entry without a workspace gives what the other one does, keys left out of the unpacked pages among them."""
+    gen = torch.Generator().manual_seed(47)
+    x = _problem(gen, [900, 130], 70, BF)
+    for far in (False, True):
+        if far:
+            _far_keys(x, gen, 16, 2, [0, 1])
+        q, kp, vp, ks, vs, bt, cl = x
+        out = torch.empty_like(q)
+        nv.check(nv.lib().nvm_paged_attention_noalloc(
+            q.data_ptr(), 2, kp.data_ptr(), vp.data_ptr(), nv.NVM_U4, ks.data_ptr(), vs.data_ptr(), 2, bt.data_ptr(),
+            cl.data_ptr(), out.data_ptr(), 2, 2, 8, 2, 70, 128, kp.shape[0], 16, bt.shape[1], 128 ** -0.5, 1, nv.stream_ptr(cuda)))
+        assert torch.equal(out, _call(x, out_dtype=BF))
+
+
+@pytest.mark.parametrize("sdt", [BF, HF])
+def test_nan_queries_of_a_prompt_stay_in_their_rows(cuda, sdt):
+    gen = torch.Generator().manual_seed(48)
+    x = _problem(gen, [300, 90], 70, sdt)
+    clean = _call(x, out_dtype=FF)
+    bad = torch.zeros(2, 8, 70, dtype=torch.bool, device="cuda")
+    for b, h, row, value in ((0, 2, 0, "nan"), (0, 5, 69, "inf"), (1, 7, 33, "-inf"), (1, 0, 64, "nan")):
+        x[0][b, h, row, 5 * h] = float(value)
+        bad[b, h, row] = True
+    got = _call(x, out_dtype=FF)
+    assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+
+
+def test_prompts_of_both_kinds_take_turns(cuda):
+    """Calls with and without keys left out, of other shapes and page types, over one workspace."""
+    gen = torch.Generator().manual_seed(49)
+    problems = [_problem(gen, [700, 90, 200], 70), _problem(gen, [2500], 300), _problem(gen, [1500, 64], 64, HF), _problem(gen, [400], 5)]
+    _far_keys(problems[0], gen, 16, 3, [0, 2])
+    _far_keys(problems[1], gen, 16, 1, [0])
+    k16, v16 = (torch.randn(problems[0][1].shape[0], 2, 16, 128, generator=gen).to(BF).cuda() for _ in range(2))
+    calls = [lambda x=x: _call(x, out_dtype=FF) for x in problems]
+    calls.append(lambda: lib.paged_attention(problems[0][0], k16, v16, *problems[0][5:], 16, mask="causal"))
+    alone = [c() for c in calls]
+    for _ in range(4):
+        for i in torch.randperm(len(calls), generator=gen).tolist():
+            assert torch.equal(calls[i](), alone[i])
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        outs = []
+        for s, c in zip(streams, calls):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append(c())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
