@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_of(D, kTiles)) paged_u4_ke
             const float was = kap[j][i];
             kap[j][i] = __uint_as_float(__float_as_uint(was) & 0xff800000u);
             M[j][i] *= __fdiv_rn(kap[j][i], was);
-            top = fabsf(kap[j][i]) * most;
+            top = fmaxf(M[j][i], fabsf(kap[j][i]) * most);
           }
 #pragma unroll
           for (int g = 0; g < G; ++g) product[g] = kNoKeys;

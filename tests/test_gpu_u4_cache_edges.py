@@ -463,3 +463,23 @@ def test_prompts_of_both_kinds_take_turns(cuda):
                 outs.append(c())
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+
+
+def test_large_value_behind_a_far_score(cuda):
+    """Scores of 2^28: a key 96 below the first, with values 2^120 times finer held before it, takes nothing from it."""
+    B, D, ps = 300, 128, 16
+    kp = torch.zeros(9, 1, ps, D // 2, dtype=torch.uint8, device="cuda")
+    vp = kp.clone()
+    ks = torch.zeros(9, 1, ps, 4, dtype=BF, device="cuda")
+    vs = ks.clone()
+    for page in (0, 8):  # keys 0 and 128, which one warp meets one after the other
+        ks[page, 0, 0] = torch.tensor([1.0, 2.0 ** 21] * 2, device="cuda")
+        vp[page, 0, 0] = 0x88
+        vs[page, 0, 0] = torch.tensor([2.0 ** (-60 if page == 0 else 60), 2.0 ** 40 if page == 0 else 0.0] * 2, device="cuda")
+    kp[0, 0, 0, :32] = 0x21  # 32 times 1 and 2
+    bt = torch.arange(9, dtype=torch.int32, device="cuda").expand(B, -1)
+    cl = torch.full((B,), 129, dtype=torch.int32, device="cuda")
+    for L in (1, 5):
+        q = torch.ones(B, 2, L, D, dtype=BF, device="cuda")
+        got = lib.paged_attention(q, kp, vp, bt, cl, ps, ks, vs, scale=0.6931472, mask=None, out_dtype=FF)
+        assert (got == 2.0 ** 40).all()
