@@ -8,9 +8,9 @@ their terms' sizes, |scale| sum |q| (s code + |z|); the exponential and its argu
 their sum are then off by a factor of e^d each, the output by less than 2.1 d sum p |v| while d is below 0.05.
 
 Row blocks: queries as they are (those of 32 bits to 11 bits), elements far below the row's largest to 2^-34 of
-it.  The weight times s is rounded to 11 bits and multiplies code - 8; below 2^-14 of the largest such product of
-its row and group (the reference may lag 2^10 behind it, never pass it) it is off by 2^-25 of that, for each of n
-keys.  Everything else is fp32: a sum of n / 16 terms and 64 more takes (n / 16 + 64) 2^-24 of its terms.
+it.  The weight times s is rounded to 11 bits and multiplies code - 8, at most 8; below 2^-14 of its unit it is off by
+2^-25 of that.  The unit is a power of two, at most twice the largest such product of the row and group (it may lag
+2^10 behind it): 8 * 2^-24 of the largest product, for each of n keys.  Everything else is fp32: a sum of n / 16 terms and 64 more takes (n / 16 + 64) 2^-24 of its terms.
 
 Prompts: K times 16 and V times 64 are held in 16 bits (where the scales are float16, as they are), the queries
 times 2^8 and the scale's power of two; K and V are off by 2^-11 and 2^-29 or 2^-31, queries by 2^-32 of a score
@@ -65,7 +65,7 @@ def attention(q, kp, vp, ks, vs, bt, cl, ps, scale=None, causal=True):
                 d = d.masked_fill(~seen, 0).amax(-1, keepdim=True)
                 sums = (n / 16 + 64) * 2.0 ** -24
                 held_to = torch.einsum("ln,nd->lnd", p, sv).amax(1)
-                rows[b, hq] = (2.1 * d + sums) * (p @ off_v) + 2.0 ** -11 * (p @ (v - zv - 8 * sv).abs()) + 2.0 ** -22 * n * held_to
+                rows[b, hq] = (2.1 * d + sums) * (p @ off_v) + 2.0 ** -11 * (p @ (v - zv - 8 * sv).abs()) + 2.0 ** -21 * n * held_to
                 d = common + thin + 2.0 ** -11 * plain + 2.0 ** -29 * abs(scale) * x.abs().sum(-1, keepdim=True) + 2.0 ** -32 * k.abs().sum(-1)
                 d = d.masked_fill(~seen, 0).amax(-1, keepdim=True)
                 lost = 2.0 ** -25 * (seen.double() @ v.abs()) + 2.0 ** -31
